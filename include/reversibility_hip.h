@@ -358,6 +358,43 @@ int rv_head_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int6
                int64_t padded, void* dw, int dw_dtype, int accumulate, void* workspace,
                int64_t workspace_bytes, void* stream);
 
+/* Log-probabilities of the labels under the tied head, without the logits in
+ * memory: z = x head^T with fp32 sums, lse[r] = log sum_{j < vocab} exp(z[r, j]),
+ * logp[r] = z[r, labels[r]] - lse[r]; 0 for label == ignore_index, NaN for
+ * another label outside [0, vocab).  x [rows, d] and head [>= vocab, d] of dtype
+ * RV_F16 or RV_BF16, 16-byte aligned, d a multiple of 8; labels int64 [rows];
+ * logp, lse fp32 [rows]. */
+int64_t rv_head_logp_workspace_bytes(int64_t rows, int64_t d, int64_t vocab);
+int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                     int dtype, const int64_t* labels, int64_t ignore_index, float* logp,
+                     float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its backward for the gradient grad[rows] of logp, in three steps over a chunk
+ * of rows that share a scale (scale[0] a power of two that brings the largest
+ * |grad| of a row with a label to [2^14, 2^15), scale[1] its inverse):
+ *   scale    scale[0], scale[1] from grad
+ *   dlogits  dlogits[rows, padded] of dtype: scale[0] grad[r] ([j == labels[r]] -
+ *            exp(z[r, j] - lse[r])), computed from x and head again; columns from
+ *            vocab on zero; ignored rows zero (their grad is not read), a row of
+ *            another label outside [0, vocab) NaN
+ *   dx       dx[rows, d] of dtype = scale[1] dlogits head
+ *   dw       dw[vocab, d] = scale[1] dlogits^T x, of dtype, or fp32 (added to dw
+ *            with accumulate)
+ * padded, a multiple of 64, is the row count of head. */
+int rv_head_logp_scale(const float* grad, const int64_t* labels, int64_t rows,
+                       int64_t ignore_index, float* scale, void* stream);
+int rv_head_logp_dlogits(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                         int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,
+                         const float* lse, const float* grad, const float* scale, void* dlogits,
+                         void* stream);
+int64_t rv_head_logp_grad_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded);
+int rv_head_logp_dx(const void* dlogits, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                    int64_t padded, int dtype, const float* scale, void* dx, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+int rv_head_logp_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int64_t vocab,
+                    int64_t padded, int dtype, const float* scale, void* dw, int dw_dtype,
+                    int accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Two layers' weight gradients over the same rows in one launch: dw_a[out_a,
  * in_a] (+)= fp32(fp16(dy_a^T x_a)) and dw_b likewise (x_a, x_b contiguous). */
 int64_t rv_linear_dw_pair_workspace_bytes(int64_t rows, int64_t in_a, int64_t out_a,
@@ -422,6 +459,23 @@ int rv_adamw_step_clipped(int count, float* const* params, const float* const* g
                           const float* found_inf, const float* inv_scale,
                           const float* clip_coef, void* stream);
 
+/* The same update with both moments in 8 bits: e4m3 values with one scale byte b
+ * per rv_adamw8_block() consecutive elements of a tensor (value = e4m3 *
+ * 2^(b - 127); ceil(numel / block) bytes, all zero at the start).  p takes the fp32
+ * moments; what is stored is rounded, the first moment to nearest, the second at
+ * random (its expectation kept) with bits that follow from seed, the tensor's
+ * ordinal, *step and the element's index alone.  Multiplies and adds are rounded
+ * one by one (no fused multiply-add). */
+int rv_adamw8_max_tensors(void);
+int rv_adamw8_block(void);
+int rv_adamw8_step(int count, float* const* params, const float* const* grads,
+                   uint8_t* const* exp_avg, uint8_t* const* exp_avg_scale,
+                   uint8_t* const* exp_avg_sq, uint8_t* const* exp_avg_sq_scale,
+                   const int64_t* numel, const uint32_t* ordinal, uint32_t seed, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, const float* step,
+                   const float* found_inf, const float* inv_scale, const float* clip_coef,
+                   void* stream);
+
 /* GradScaler.unscale_ followed by torch.nn.utils.clip_grad_norm_(params,
  * max_norm) (norm type 2; scripts/train_baseline.py:278-280) without writing
  * the gradients: rv_grad_sq_partials stores, for each 16384-element chunk of
@@ -474,6 +528,50 @@ int rv_ce_fused(const void* logits, int dtype, int64_t ld, const int64_t* labels
                 int64_t rows, int64_t cols, int64_t ignore_index, const float* grad,
                 float* row_max, float* row_lse, float* loss, void* dlogits,
                 void* stream);
+
+/* ------------------------------------------------------------------------
+ * Losses on token log-probabilities (fp32 [sequences, tokens], row strides in
+ * elements; mask: one byte per token, nonzero where the token counts, NULL =
+ * every token; a masked token is never used, whatever it holds).  Sums are
+ * held in fp64 and taken in a fixed order.
+ */
+
+/* Preference loss over pairs (row i against row pairs + i of 2 pairs rows):
+ *   s_i = sum_t (logp - ref) (average: over the row's counted tokens, 0 without any)
+ *   m_i = beta (s_i - s_{pairs + i})
+ *   loss = mean_i -(1 - smoothing) log sigmoid(m_i) - smoothing log sigmoid(-m_i)
+ * reward[2 pairs] = beta s; coef[2 pairs] = d loss / d logp of a row's counted
+ * tokens.  tokens may be 0. */
+int64_t rv_pref_loss_workspace_bytes(int64_t pairs, int64_t tokens);
+int rv_pref_loss(const float* logp, int64_t ld_logp, const float* ref, int64_t ld_ref,
+                 const uint8_t* mask, int64_t ld_mask, int64_t pairs, int64_t tokens, double beta,
+                 double smoothing, int average, float* loss, float* reward, float* coef,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dlogp[seqs, tokens] = coef[row] * *grad where the mask counts the token, else 0. */
+int rv_pref_grad(const float* coef, const uint8_t* mask, int64_t ld_mask, const float* grad,
+                 int64_t seqs, int64_t tokens, float* dlogp, void* stream);
+
+/* Clipped policy loss with a KL term.  Per counted token, r = exp(logp - old):
+ *   -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k,
+ *   k = exp(ref - logp) - (ref - logp) - 1       (ref NULL: no such term)
+ * loss: the sum over the counted tokens divided by their number (per_sequence ==
+ * 0), or the mean over all sequences of each one's mean (0 without tokens).
+ * adv[s * adv_row + t * adv_col].  stats[3] = mean k, share of tokens whose ratio
+ * is clipped (both over all counted tokens), and the factor that rv_policy_grad
+ * applies.  slope (nullable) [seqs, tokens], contiguous: the
+ * tokens' d loss / d logp but for that factor, 0 where masked. */
+int64_t rv_policy_loss_workspace_bytes(int64_t seqs, int64_t tokens, int per_sequence);
+int rv_policy_loss(const float* logp, int64_t ld_logp, const float* old_logp, int64_t ld_old,
+                   const float* ref, int64_t ld_ref, const float* adv, int64_t adv_row,
+                   int64_t adv_col, const uint8_t* mask, int64_t ld_mask, int64_t seqs,
+                   int64_t tokens, double clip_low, double clip_high, double kl_coef,
+                   int per_sequence, float* loss, float* stats, float* slope, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* dlogp[i] = slope[i] * (*factor * *grad), i < n. */
+int rv_policy_grad(const float* slope, const float* factor, const float* grad, int64_t n,
+                   float* dlogp, void* stream);
 
 /* ------------------------------------------------------------------------
  * Causal self-attention (F.scaled_dot_product_attention(q, k, v,

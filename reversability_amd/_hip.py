@@ -64,6 +64,14 @@ SIGNATURES = {
     "rv_head_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "rv_head_dx": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "rv_head_dw": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _I, _I, _P, _I64, _P]),
+    "rv_head_logp_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "rv_head_logp_fwd": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _P, _I64, _P]),
+    "rv_head_logp_scale": (_I, [_P, _P, _I64, _I64, _P, _P]),
+    "rv_head_logp_dlogits": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _P, _P,
+                                  _P]),
+    "rv_head_logp_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "rv_head_logp_dx": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
+    "rv_head_logp_dw": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _I, _I, _P, _I64, _P]),
     "rv_linear_dw_pair_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "rv_linear_dw_pair": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _I, _P, _I64,
                                _P]),
@@ -74,6 +82,10 @@ SIGNATURES = {
     "rv_adamw_step": (_I, [_I, _P, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _P, _P, _P]),
     "rv_adamw_step_clipped": (_I, [_I, _P, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _P, _P, _P,
                                    _P]),
+    "rv_adamw8_max_tensors": (_I, []),
+    "rv_adamw8_block": (_I, []),
+    "rv_adamw8_step": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_uint32, _D, _D, _D, _D,
+                            _D, _P, _P, _P, _P, _P]),
     "rv_grad_chunks": (_I, [_P, _I]),
     "rv_grad_sq_partials": (_I, [_I, _P, _P, _P, _P, _P, _I, _P]),
     "rv_grad_clip_coef": (_I, [_P, _P, _I, _D, _P, _P, _P, _P]),
@@ -95,6 +107,14 @@ SIGNATURES = {
     "rv_mlp_dx": (_I, [_P, _P, _I64, _I64, _I64, _P, _P]),
     "rv_mlp_wgrad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "rv_mlp_wgrad": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I, _P, _I64, _P]),
+    "rv_pref_loss_workspace_bytes": (_I64, [_I64, _I64]),
+    "rv_pref_loss": (_I, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _D, _D, _I, _P, _P, _P, _P,
+                          _I64, _P]),
+    "rv_pref_grad": (_I, [_P, _P, _I64, _P, _I64, _I64, _P, _P]),
+    "rv_policy_loss_workspace_bytes": (_I64, [_I64, _I64, _I]),
+    "rv_policy_loss": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64,
+                            _D, _D, _D, _I, _P, _P, _P, _P, _I64, _P]),
+    "rv_policy_grad": (_I, [_P, _P, _P, _I64, _P, _P]),
     "rv_attn_fwd": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P]),
     "rv_attn_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "rv_attn_bwd": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),

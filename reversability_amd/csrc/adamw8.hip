@@ -1,0 +1,292 @@
+// AdamW over many fp32 tensors with its moments in 8 bits, for gfx950.
+//
+// The update is adamw.hip's (torch.optim.AdamW, driven through GradScaler, the
+// step count and the overflow flag on the device); m and v are held between steps
+// as e4m3 values with one power-of-two scale per 32 consecutive elements of a
+// tensor (the last block of a tensor may be short), the layout of the OCP
+// microscaling formats: value = e4m3 * 2^(byte - 127).  A block's byte brings its
+// largest magnitude to [2^7, 2^8), below the largest e4m3 value (448).
+//
+//     m  = b1 m + (1 - b1) g
+//     v  = b2 v + (1 - b2) g g
+//     p  = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// The parameter takes the fp32 m and v of this step; only what the next step
+// starts from is rounded.  m goes to the nearest value (2^-4 of it: it is replaced
+// within 1 / (1 - b1) steps).  v moves by (1 - b2) of itself a step, less than half
+// a step of e4m3: to the nearest it would stand still, or climb only, so it is
+// rounded up or down at random with the fractions as probabilities, which keeps its
+// expectation.  The random bits are MurmurHash3's 32-bit finalizer (A. Appleby) of
+// the element's index plus a key of seed, tensor and step: the same call gives the
+// same bits.  A v > 0 stays > 0: a zero v under an m that is not would make the next
+// update as large as 1 / eps.
+//
+// Memory-bound: 16.125 bytes a parameter (p 8, g 4, codes 4, scales 4 / 32) against
+// about 100 VALU instructions, 28 bytes with fp32 moments.
+
+#include <cmath>
+
+#include "rv_device.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTensors = 48;
+constexpr int kBlock = 32;                        // elements per scale: 8 lanes of 4
+constexpr int64_t kChunk = kThreads * 4;          // elements per workgroup
+constexpr int kGridRow = 1 << 22;                 // a launch dimension holds < 2^32 threads
+
+struct Table {
+  float* p[kMaxTensors];
+  const float* g[kMaxTensors];
+  uint8_t* m[kMaxTensors];
+  uint8_t* ms[kMaxTensors];
+  uint8_t* v[kMaxTensors];
+  uint8_t* vs[kMaxTensors];
+  int64_t n[kMaxTensors];
+  uint32_t key[kMaxTensors];
+  int chunk_start[kMaxTensors + 1];
+  int count;
+};
+
+struct Hyper {
+  float beta1, beta2, eps, decay, w1, w2;  // decay = 1 - lr wd, w = 1 - beta
+  double lr, log2_beta1, log2_beta2;
+  const float* step;       // t after this update (already advanced)
+  const float* found_inf;  // nullable
+  const float* inv_scale;  // nullable
+  const float* clip;       // nullable
+};
+
+__device__ __forceinline__ uint32_t mix(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
+  h = (h ^ (h >> 13)) * 0xC2B2AE35u;
+  return h ^ (h >> 16);
+}
+
+// Largest of the 8 lanes that hold a block.
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
+  auto take = [](uint32_t a, int b) { return a > (uint32_t)b ? a : (uint32_t)b; };
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, false));   // lane ^ 1
+  x = take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, false));   // lane ^ 2
+  return take(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, false));  // 7 - lane
+}
+
+// A finite value's magnitude as ordered bits; 0 for the others, which have codes of
+// their own and leave their block's scale alone.
+__device__ __forceinline__ uint32_t magnitude(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// The scale byte of a block whose largest magnitude has these bits.
+__device__ __forceinline__ int scale_byte(uint32_t bits) {
+  const int e = (int)(bits >> 23) - 7;
+  return e > 0 ? e : 0;
+}
+
+__device__ __forceinline__ void decode(uint32_t codes, int scale, float (&x)[4]) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  x[0] = __builtin_ldexpf(lo[0], scale - 127);
+  x[1] = __builtin_ldexpf(lo[1], scale - 127);
+  x[2] = __builtin_ldexpf(hi[0], scale - 127);
+  x[3] = __builtin_ldexpf(hi[1], scale - 127);
+}
+
+// e4m3 codes of x at the scale, to nearest even (NaN and infinities: NaN).
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], int scale) {
+  float q[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    q[e] = __builtin_ldexpf(x[e], 127 - scale);
+    if (fabsf(q[e]) > 448.f) q[e] = NAN;  // an infinity: finite ones are below 2^8
+  }
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+  return (uint32_t)w;
+}
+
+// e4m3 code of v >= 0 at the scale, up with probability `noise` 2^-20 against the
+// fraction that is cut off; at least the smallest value for v > 0.
+__device__ __forceinline__ uint32_t encode_random(float v, int scale, uint32_t noise) {
+  const float q = __builtin_ldexpf(v, 127 - scale);
+  if (!(q < 512.f)) return 0x7f;  // infinity or NaN
+  // 3 of 23 mantissa bits stay; fp32's exponent 120 is e4m3's 0 (values below 2^-6,
+  // in steps of 2^-9)
+  const uint32_t normal = ((__float_as_uint(q) + noise) >> 20) - 960u;
+  const uint32_t tiny = (uint32_t)(q * 512.f + (float)noise * 0x1p-20f);
+  const uint32_t code = q < 0x1p-6f ? tiny : normal;
+  return code == 0 && v > 0.f ? 1u : code;
+}
+
+__device__ __forceinline__ int tensor_of(const int* chunk_start, int count, int block) {
+  int t = 0, above = count;
+  while (above - t > 1) {
+    const int mid = (t + above) >> 1;
+    if (chunk_start[mid] <= block) t = mid;
+    else above = mid;
+  }
+  return t;
+}
+
+__global__ __launch_bounds__(kThreads)
+void adamw8_k(Table tab, Hyper h) {
+  if (h.found_inf != nullptr && *h.found_inf != 0.0f) return;  // uniform skip
+  const int64_t block = (int64_t)blockIdx.y * kGridRow + blockIdx.x;
+  if (block >= tab.chunk_start[tab.count]) return;  // past the last row's end
+  const int t = tensor_of(tab.chunk_start, tab.count, (int)block);
+  const int64_t n = tab.n[t];
+  const int64_t i = (block - tab.chunk_start[t]) * kChunk + threadIdx.x * 4;
+  const int64_t at = i / kBlock;
+  float* p = tab.p[t] + i;
+  const float* g = tab.g[t] + i;
+  uint8_t* mc = tab.m[t] + i;
+  uint8_t* vc = tab.v[t] + i;
+  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(mc) | reinterpret_cast<uintptr_t>(vc)) & 3) == 0;
+  const bool full = vec && i + 4 <= n;
+  const int here = i >= n ? 0 : i + 4 <= n ? 4 : (int)(n - i);  // elements of this thread
+  float pp[4] = {}, gg[4] = {};
+  uint32_t mw = 0, vw = 0;
+  int ms = 0, vs = 0;
+  if (full) {
+    const float4 a = rv::ld_f4(p), b = rv::ld_f4(g);
+    mw = *reinterpret_cast<const uint32_t*>(mc);
+    vw = *reinterpret_cast<const uint32_t*>(vc);
+    pp[0] = a.x; pp[1] = a.y; pp[2] = a.z; pp[3] = a.w;
+    gg[0] = b.x; gg[1] = b.y; gg[2] = b.z; gg[3] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < here) {
+        pp[e] = p[e];
+        gg[e] = g[e];
+        mw |= (uint32_t)mc[e] << (8 * e);
+        vw |= (uint32_t)vc[e] << (8 * e);
+      }
+  }
+  if (here > 0) {
+    ms = tab.ms[t][at];
+    vs = tab.vs[t][at];
+  }
+  const double step = (double)*h.step;
+  const float step_size = (float)(h.lr / (1.0 - exp2(step * h.log2_beta1)));
+  const float bc2_sqrt = (float)sqrt(1.0 - exp2(step * h.log2_beta2));
+  const float inv = h.inv_scale != nullptr ? *h.inv_scale : 1.0f;
+  const float clip = h.clip != nullptr ? *h.clip : 1.0f;
+  const uint32_t key = mix(tab.key[t] + (uint32_t)*h.step);
+
+  float m[4], v[4];
+  decode(mw, ms, m);
+  decode(vw, vs, v);
+  uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float u = gg[e] * inv * clip;  // unscale_'s multiply, then clip_grad_norm_'s
+    m[e] = m[e] * h.beta1 + u * h.w1;
+    v[e] = v[e] * h.beta2 + u * h.w2 * u;
+    const float denom = sqrtf(v[e]) / bc2_sqrt + h.eps;
+    pp[e] = pp[e] * h.decay - step_size * (m[e] / denom);
+    if (e < here) {
+      const uint32_t a = magnitude(m[e]), b = magnitude(v[e]);
+      mtop = a > mtop ? a : mtop;
+      vtop = b > vtop ? b : vtop;
+    }
+  }
+  ms = scale_byte(block_max(mtop));
+  vs = scale_byte(block_max(vtop));
+  mw = encode(m, ms);
+  vw = 0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t bits = mix((uint32_t)(i >> 1) + half + key);  // 16 for each of two elements
+    vw |= encode_random(v[2 * half], vs, (bits & 0xffffu) << 4 | 8u) << (16 * half);
+    vw |= encode_random(v[2 * half + 1], vs, bits >> 16 << 4 | 8u) << (16 * half + 8);
+  }
+  if (full) {
+    rv::st_f4(p, make_float4(pp[0], pp[1], pp[2], pp[3]));
+    *reinterpret_cast<uint32_t*>(mc) = mw;
+    *reinterpret_cast<uint32_t*>(vc) = vw;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < here) {
+        p[e] = pp[e];
+        mc[e] = (uint8_t)(mw >> (8 * e));
+        vc[e] = (uint8_t)(vw >> (8 * e));
+      }
+  }
+  if ((threadIdx.x & 7) == 0 && here > 0) {
+    tab.ms[t][at] = (uint8_t)ms;
+    tab.vs[t][at] = (uint8_t)vs;
+  }
+}
+
+uint32_t host_mix(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
+  h = (h ^ (h >> 13)) * 0xC2B2AE35u;
+  return h ^ (h >> 16);
+}
+
+}  // namespace
+
+extern "C" {
+
+int rv_adamw8_max_tensors(void) { return kMaxTensors; }
+int rv_adamw8_block(void) { return kBlock; }
+
+int rv_adamw8_step(int count, float* const* params, const float* const* grads,
+                   uint8_t* const* exp_avg, uint8_t* const* exp_avg_scale,
+                   uint8_t* const* exp_avg_sq, uint8_t* const* exp_avg_sq_scale,
+                   const int64_t* numel, const uint32_t* ordinal, uint32_t seed, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, const float* step,
+                   const float* found_inf, const float* inv_scale, const float* clip_coef,
+                   void* stream) {
+  if (count <= 0) return count == 0 ? RV_OK : RV_ERR_BAD_SIZE;
+  if (count > kMaxTensors) return RV_ERR_UNSUPPORTED;
+  if (!params || !grads || !exp_avg || !exp_avg_scale || !exp_avg_sq || !exp_avg_sq_scale ||
+      !numel || !ordinal || !step)
+    return RV_ERR_NULL_POINTER;
+  Table tab{};
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (!params[i] || !grads[i] || !exp_avg[i] || !exp_avg_scale[i] || !exp_avg_sq[i] ||
+        !exp_avg_sq_scale[i])
+      return RV_ERR_NULL_POINTER;
+    if (numel[i] <= 0) return RV_ERR_BAD_SIZE;
+    tab.p[i] = params[i];
+    tab.g[i] = grads[i];
+    tab.m[i] = exp_avg[i];
+    tab.ms[i] = exp_avg_scale[i];
+    tab.v[i] = exp_avg_sq[i];
+    tab.vs[i] = exp_avg_sq_scale[i];
+    tab.n[i] = numel[i];
+    tab.key[i] = host_mix(seed + 0x9E3779B9u * (ordinal[i] + 1u));
+    tab.chunk_start[i] = (int)chunks;
+    chunks += (numel[i] + kChunk - 1) / kChunk;
+    if (chunks > 0x7fffffff) return RV_ERR_UNSUPPORTED;
+  }
+  tab.chunk_start[count] = (int)chunks;
+  tab.count = count;
+  Hyper h{};
+  h.beta1 = (float)beta1;
+  h.beta2 = (float)beta2;
+  h.eps = (float)eps;
+  h.decay = (float)(1.0 - lr * weight_decay);
+  h.w1 = (float)(1.0 - beta1);
+  h.w2 = (float)(1.0 - beta2);
+  h.lr = lr;
+  h.log2_beta1 = std::log2(beta1);  // beta 0: -inf, and 2^-inf = 0 = beta^t for t >= 1
+  h.log2_beta2 = std::log2(beta2);
+  h.step = step;
+  h.found_inf = found_inf;
+  h.inv_scale = inv_scale;
+  h.clip = clip_coef;
+  const dim3 grid((unsigned)(chunks < kGridRow ? chunks : kGridRow),
+                  (unsigned)((chunks + kGridRow - 1) / kGridRow));
+  hipLaunchKernelGGL(adamw8_k, grid, dim3(kThreads), 0, (hipStream_t)stream, tab, h);
+  return rv_host::check_launch();
+}
+
+}  // extern "C"

@@ -73,6 +73,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));  // 16-byte staging word
 #define RV_LDS __attribute__((address_space(3)))
 
@@ -316,6 +317,38 @@ enum class Epi {
   StoreF32OfF16,  // c fp32 = fp32(fp16(acc))
   AccF32OfF16,    // c fp32 (+)= fp32(fp16(acc))
   PartialF32,     // c fp32 partial [split][m][n] = acc
+  // the tied head's log-probabilities (HeadLogp):
+  LogProb,        // c = float2 [tile column][m]: a row's maximum and sum of exp over the tile
+  LogProbGrad,    // c 16-bit [m][n] = scaled gradient of the logits
+  StoreScaled,    // c 16-bit = acc * *scale
+  AccF32Scaled,   // c fp32 (+)= acc * *scale
+  PartialRagged,  // PartialF32 whose tiles may pass column n
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Two fp32 values rounded to nearest even to the 16-bit operand type.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// What the tied head's log-probability epilogues read and write beside the
+// product (rows and labels of the chunk at hand).
+struct HeadLogp {
+  const int64_t* labels;   // [m]
+  int64_t ignore, vocab;   // rows with this label have no log-probability; columns in use
+  float* label_logit;      // LogProb, [m]: a row's logit at its label
+  const float* lse;        // LogProbGrad, [m]: log sum exp of the row
+  const float* grad;       // LogProbGrad, [m]: gradient of the row's log-probability
+  const float* scale;      // LogProbGrad: *scale multiplies the gradient; Scaled: the result
 };
 
 constexpr int kSplitStep = 64;  // weight gradients: granularity of a split's token range
@@ -332,6 +365,7 @@ struct GemmArgs {
   int accumulate;          // AccF32OfF16
   int64_t group = 8;       // M tiles per group of the tile order (tile_of)
   int64_t valid;           // StoreF16: columns valid .. n - 1 are written as zero (0: none)
+  HeadLogp head;
 };
 
 // Workgroups are dispatched to the 8 XCDs round robin.  Tiles are numbered in
@@ -361,7 +395,8 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-template <int SHAPE, bool A_RC, bool B_RC, Epi EPI>
+// BF: the operands (and 16-bit results) are bf16 instead of fp16.
+template <int SHAPE, bool A_RC, bool B_RC, Epi EPI, bool BF = false>
 __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) {
   constexpr int BM = kShapes[SHAPE].bm, BN = kShapes[SHAPE].bn, WAVES = kShapes[SHAPE].waves;
   constexpr int BK = kShapes[SHAPE].bk, RA = kShapes[SHAPE].ra, RB = kShapes[SHAPE].rb;
@@ -501,7 +536,12 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
         if constexpr (i == 0) after_wait(fb[S][j]);
         if constexpr (j == 0) after_wait(fa[S][i]);
       }
-      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[S][j], fa[S][i], acc[i][j], 0, 0, 0);
+      if constexpr (BF)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, fb[S][j]), __builtin_bit_cast(bf16x8, fa[S][i]), acc[i][j],
+            0, 0, 0);
+      else
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[S][j], fa[S][i], acc[i][j], 0, 0, 0);
       static_for<kF>([&](auto fc) {
         constexpr int f = decltype(fc)::value;
         if constexpr (f * kM / kF == q)
@@ -576,8 +616,78 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
   // its 32x32 tile and, for q = 0..3, the 4 consecutive columns
   // q*8 + (lane/32)*4 + 0..3 (accumulator values 4q..4q+3).
   const int cq = (lane >> 5) * 4;
-  if constexpr (EPI == Epi::PartialF32 || EPI == Epi::StoreF32OfF16 ||
-                EPI == Epi::AccF32OfF16) {
+  if constexpr (EPI == Epi::LogProb) {
+    // A row's maximum and sum of exp(z - maximum) over the tile's columns, from
+    // the fp32 accumulators: the logits are neither rounded nor stored.  A lane
+    // holds half of its row's columns of the wave's block, its partner (lane ^ 32)
+    // the other half; the wave columns meet in LDS.
+    float2* red = reinterpret_cast<float2*>(lds);  // [WCOLS][BM]
+    const int64_t col0 = n0 + wn * WN;
+    const int64_t left = args.head.vocab - col0;
+    const int nv = left < 0 ? 0 : left < WN ? (int)left : WN;  // columns in use
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int r = wm * WM + i * 32 + (lane & 31);
+      const int64_t row = m0 + r;
+      if (nv < WN) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (j * 32 + (e >> 2) * 8 + cq + (e & 3) >= nv) acc[i][j][e] = -INFINITY;
+      }
+      float top = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      // exp(z - top) = exp2(z log2e + shift) in one multiply-add and one v_exp; shift's
+      // rounding (a factor 1 +- 2^-24 |top|) is taken back from the sum
+      const float shift = top == -INFINITY ? 0.f : -top * kLog2e;  // no column in use
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, shift));
+      sum += __shfl_xor(sum, 32, 64);
+      if (top != -INFINITY) sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(top, kLog2e, shift));
+      if (lane < 32) red[wn * BM + r] = make_float2(top, sum);
+      // the label's logit, where the label is one of the wave's columns
+      const int64_t label = row < args.m ? args.head.labels[row] : -1;
+      const int64_t c = label - col0;
+      const bool mine = c >= 0 && c < nv && ((int)c & 4) == cq;
+      if (__any(mine)) {
+        const int at = ((int)c >> 5) * 16 + (((int)c >> 3) & 3) * 4 + ((int)c & 3);
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (at == j * 16 + e) z = acc[i][j][e];
+        if (mine) args.head.label_logit[row] = z;
+      }
+    }
+    __syncthreads();
+    float2* out = static_cast<float2*>(args.c) + tn * args.m + m0;
+    for (int r = threadIdx.x; r < BM; r += WAVES * 64) {
+      if (m0 + r >= args.m) break;
+      float2 v = red[r];
+#pragma unroll
+      for (int w = 1; w < WCOLS; ++w) {
+        const float2 u = red[w * BM + r];
+        const float top = fmaxf(v.x, u.x);
+        if (u.x != -INFINITY)
+          v.y = v.y * __builtin_amdgcn_exp2f((v.x - top) * kLog2e) +
+                u.y * __builtin_amdgcn_exp2f((u.x - top) * kLog2e);
+        v.x = top;
+      }
+      out[r] = v;
+    }
+  } else if constexpr (EPI == Epi::PartialF32 || EPI == Epi::StoreF32OfF16 ||
+                       EPI == Epi::AccF32OfF16 || EPI == Epi::AccF32Scaled ||
+                       EPI == Epi::PartialRagged) {
     // fp32 outputs: each wave passes its block through LDS 32 rows at a time
     // (row stride WN + 4 floats: conflict free both ways), so that a store
     // instruction covers whole rows (512 or 256 contiguous bytes) instead of
@@ -586,7 +696,12 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
     float* stage = reinterpret_cast<float*>(lds) + wave * (32 * S);
     const int c = lane % CPR * 4;
     float* out = static_cast<float*>(args.c) + n0 + wn * WN + c;
-    if constexpr (EPI == Epi::PartialF32) out += split * args.m * args.ldc;
+    if constexpr (EPI == Epi::PartialF32 || EPI == Epi::PartialRagged)
+      out += split * args.m * args.ldc;
+    constexpr bool kRagged = EPI == Epi::PartialRagged || EPI == Epi::AccF32Scaled;
+    const bool outside = kRagged && n0 + wn * WN + c >= args.n;
+    float scale = 1.f;
+    if constexpr (EPI == Epi::AccF32Scaled) scale = *args.head.scale;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -603,9 +718,15 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
       for (int r = lane / CPR; r < 32; r += RPP) {
         const int64_t row = row0 + r;
         float4 v = *reinterpret_cast<const float4*>(stage + r * S + c);
-        if (row >= args.m) continue;
+        if (row >= args.m || outside) continue;
         float4* dst = reinterpret_cast<float4*>(out + row * args.ldc);
-        if constexpr (EPI != Epi::PartialF32) {
+        if constexpr (EPI == Epi::AccF32Scaled) {
+          v = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+          if (args.accumulate) {
+            const float4 p = *dst;
+            v = make_float4(p.x + v.x, p.y + v.y, p.z + v.z, p.w + v.w);
+          }
+        } else if constexpr (EPI != Epi::PartialF32 && EPI != Epi::PartialRagged) {
           v = make_float4(rv::round_to<__half>(v.x), rv::round_to<__half>(v.y),
                           rv::round_to<__half>(v.z), rv::round_to<__half>(v.w));
           if constexpr (EPI == Epi::AccF32OfF16) {
@@ -628,17 +749,55 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
     // per training step of the two decoders, consumers included.
     constexpr int S = WN + 8;
     _Float16* stage = lds + wave * (WM * S);
+    if constexpr (EPI == Epi::LogProbGrad) {
+      // acc = s ([j == label] - exp(z - lse)), s = the row's gradient times *scale
+      const float scale = *args.head.scale;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int64_t row = m0 + wm * WM + i * 32 + (lane & 31);
+        const bool in = row < args.m;
+        const int64_t label = in ? args.head.labels[row] : args.head.ignore;
+        const bool ignored = label == args.head.ignore;
+        const bool bad = !ignored && (label < 0 || label >= args.head.vocab);
+        const float s = ignored ? 0.f : bad ? NAN : args.head.grad[row] * scale;
+        const float lse = ignored ? INFINITY : args.head.lse[row];
+        const float shift = -lse * kLog2e;  // its rounding is taken back in t
+        const float t = ignored ? 0.f : -s * __builtin_amdgcn_exp2f(-__builtin_fmaf(lse, kLog2e, shift));
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, shift)) * t;
+        const int64_t c = label - (n0 + wn * WN);
+        const bool mine = !ignored && c >= 0 && c < WN && ((int)c & 4) == cq;
+        if (__any(mine)) {
+          const int at = mine ? ((int)c >> 5) * 16 + (((int)c >> 3) & 3) * 4 + ((int)c & 3) : -1;
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (at == j * 16 + e) acc[i][j][e] += s;
+        }
+      }
+    }
+    if constexpr (EPI == Epi::StoreScaled) {
+      const float scale = *args.head.scale;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] *= scale;
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const __half2 h01 = __floats2half2_rn(acc[i][j][q * 4], acc[i][j][q * 4 + 1]);
-          const __half2 h23 = __floats2half2_rn(acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]);
           uint2 p;
-          p.x = *reinterpret_cast<const uint32_t*>(&h01);
-          p.y = *reinterpret_cast<const uint32_t*>(&h23);
+          p.x = pack2<BF>(acc[i][j][q * 4], acc[i][j][q * 4 + 1]);
+          p.y = pack2<BF>(acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]);
           *reinterpret_cast<uint2*>(stage + (i * 32 + (lane & 31)) * S + j * 32 + q * 8 + cq) = p;
         }
     // each wave reads back only its own staged block: a wave-local wait
@@ -677,7 +836,7 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
           __builtin_nontemporal_store(vw, reinterpret_cast<u32x4*>(u + row * args.ldu + args.f + col));
         }
       }
-    } else if constexpr (EPI == Epi::StoreF16) {
+    } else if constexpr (EPI != Epi::SwiGLUBwd) {  // StoreF16, LogProbGrad, StoreScaled
       constexpr int CPR = WN / 8, RPP = 64 / CPR;
       const int c = lane % CPR;
       const int64_t col = n0 + wn * WN + c * 8;
@@ -749,11 +908,11 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
   }
 }
 
-template <int SHAPE, bool A_RC, bool B_RC, Epi EPI>
+template <int SHAPE, bool A_RC, bool B_RC, Epi EPI, bool BF = false>
 __global__ __launch_bounds__(kShapes[SHAPE].waves * 64,
                              kShapes[SHAPE].per_cu * kShapes[SHAPE].waves / 4)
 void gemm_kernel(GemmArgs args) {
-  gemm_block<SHAPE, A_RC, B_RC, EPI>(args, blockIdx.x);
+  gemm_block<SHAPE, A_RC, B_RC, EPI, BF>(args, blockIdx.x);
 }
 
 // Two independent GEMMs in one launch: workgroups [0, first) run g[0], the rest
@@ -798,6 +957,24 @@ RV_ACT_KERNELS(0) RV_ACT_KERNELS(1) RV_ACT_KERNELS(2) RV_ACT_KERNELS(3)
 RV_ACT_KERNELS(4) RV_ACT_KERNELS(5) RV_ACT_KERNELS(6)
 RV_WGRAD_KERNELS(0) RV_WGRAD_KERNELS(1) RV_WGRAD_KERNELS(2) RV_WGRAD_KERNELS(3)
 static_assert(kNumShapes == 7 && kRuleShapes == 4, "instantiations above");
+
+// The tied head's log-probabilities, both operand types: the tile shapes that
+// head_logits_shape, head_dx_shape and plan_wgrad choose from.
+#define RV_LOGP_KERNELS(BF)                                                                    \
+  RV_LOGP_Z(1, BF) RV_LOGP_Z(2, BF) RV_LOGP_Z(3, BF) RV_LOGP_Z(4, BF)                          \
+  RV_LOGP_DX(0, BF) RV_LOGP_DX(1, BF) RV_LOGP_DX(2, BF) RV_LOGP_DX(3, BF) RV_LOGP_DX(5, BF)    \
+  RV_LOGP_DW(0, BF) RV_LOGP_DW(1, BF) RV_LOGP_DW(2, BF) RV_LOGP_DW(3, BF)
+#define RV_LOGP_Z(SHAPE, BF)                                                                \
+  template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProb, BF>(GemmArgs);     \
+  template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProbGrad, BF>(GemmArgs);
+#define RV_LOGP_DX(SHAPE, BF)                                                               \
+  template __global__ void gemm_kernel<SHAPE, false, true, Epi::StoreScaled, BF>(GemmArgs);  \
+  template __global__ void gemm_kernel<SHAPE, false, true, Epi::PartialRagged, BF>(GemmArgs);
+#define RV_LOGP_DW(SHAPE, BF)                                                               \
+  template __global__ void gemm_kernel<SHAPE, true, true, Epi::StoreScaled, BF>(GemmArgs);   \
+  template __global__ void gemm_kernel<SHAPE, true, true, Epi::AccF32Scaled, BF>(GemmArgs);  \
+  template __global__ void gemm_kernel<SHAPE, true, true, Epi::PartialRagged, BF>(GemmArgs);
+RV_LOGP_KERNELS(false) RV_LOGP_KERNELS(true)
 
 // acc[i] (+)= fp32(fp16(sum_s part[s][i])), splits summed in order.  This is
 // autocast's weight gradient: the fp16 GEMM result, cast to the fp32 weight
@@ -882,6 +1059,119 @@ void act_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t n, 
     v.y = *reinterpret_cast<const uint32_t*>(&hi);
     *reinterpret_cast<uint2*>(out + i) = v;
   }
+}
+
+// The split reductions of the tied head's log-probability gradients: out[i] (+)=
+// *scale * sum_s part[s][i], splits summed in order; T fp32, fp16 or bf16 (added
+// to the fp32 result only).  n % 4 == 0.
+template <typename T>
+__global__ __launch_bounds__(256)
+void scaled_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t n, int splits,
+                   const float* __restrict__ scale, int accumulate) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 s = *reinterpret_cast<const float4*>(part + i);
+  int k = 1;
+  for (; k + 4 <= splits; k += 4) {  // four splits' loads in flight, added in order
+    float4 t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      t[j] = *reinterpret_cast<const float4*>(part + (int64_t)(k + j) * n + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s.x = s.x + t[j].x; s.y = s.y + t[j].y; s.z = s.z + t[j].z; s.w = s.w + t[j].w;
+    }
+  }
+  for (; k < splits; ++k) {
+    const float4 t = *reinterpret_cast<const float4*>(part + (int64_t)k * n + i);
+    s.x = s.x + t.x; s.y = s.y + t.y; s.z = s.z + t.z; s.w = s.w + t.w;
+  }
+  const float f = *scale;
+  s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+  if constexpr (std::is_same<T, float>::value) {
+    float4* o = reinterpret_cast<float4*>(out + i);
+    if (accumulate) {
+      const float4 p = *o;
+      s = make_float4(p.x + s.x, p.y + s.y, p.z + s.z, p.w + s.w);
+    }
+    *o = s;
+  } else {
+    constexpr bool BF = std::is_same<T, __hip_bfloat16>::value;
+    *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<BF>(s.x, s.y), pack2<BF>(s.z, s.w));
+  }
+}
+
+// A row's log-probability from its tiles' maxima and sums (Epi::LogProb):
+// lse = M + log sum_t s_t exp(m_t - M), logp = z_label - lse; 0 for an ignored
+// label, NaN for one outside the vocabulary.  A workgroup owns R rows, 256 / R
+// threads each, which take the tiles in turn and meet in LDS in a fixed order.
+template <int R>
+__global__ __launch_bounds__(256)
+void logprob_rows(const float2* __restrict__ part, const float* __restrict__ label_logit,
+                  const int64_t* __restrict__ labels, int64_t rows, int tiles, int64_t vocab,
+                  int64_t ignore, float* __restrict__ logp, float* __restrict__ lse) {
+  constexpr int kSlices = 256 / R;
+  const int r = threadIdx.x % R, slice = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
+  float top = -INFINITY, sum = 0.f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int t = slice; t < tiles; t += kSlices) {
+      const float2 v = part[(int64_t)t * rows + row];
+      const float n = fmaxf(top, v.x);
+      if (n != -INFINITY)
+        sum = sum * __builtin_amdgcn_exp2f((top - n) * kLog2e) +
+              v.y * __builtin_amdgcn_exp2f((v.x - n) * kLog2e);
+      else
+        sum += v.y;  // NaN where every logit is
+      top = n;
+    }
+  }
+  __shared__ float2 red[256];
+  red[threadIdx.x] = make_float2(top, sum);
+  __syncthreads();
+  if (slice != 0 || row >= rows) return;
+  for (int k = 1; k < kSlices; ++k) {
+    const float2 v = red[k * R + r];
+    const float n = fmaxf(top, v.x);
+    if (n != -INFINITY)
+      sum = sum * __builtin_amdgcn_exp2f((top - n) * kLog2e) +
+            v.y * __builtin_amdgcn_exp2f((v.x - n) * kLog2e);
+    else
+      sum += v.y;
+    top = n;
+  }
+  const int64_t label = labels[row];
+  const float l = logf(sum);
+  lse[row] = top + l;
+  logp[row] = label == ignore ? 0.f
+              : label < 0 || label >= vocab ? NAN
+                                            : (label_logit[row] - top) - l;
+}
+
+// The power of two that brings the largest gradient of a row that counts to
+// [2^14, 2^15), and its inverse: the gradients of the logits are held in 16 bits,
+// where fp16 has no room for small ones (p g < 2^-24), and no logit's exceeds
+// its row's.  1 where none is finite and nonzero.  One workgroup.
+__global__ __launch_bounds__(1024)
+void logprob_scale(const float* __restrict__ grad, const int64_t* __restrict__ labels,
+                   int64_t rows, int64_t ignore, float* __restrict__ scale) {
+  float top = 0.f;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    const float g = fabsf(grad[r]);
+    if (labels[r] != ignore && g < INFINITY) top = fmaxf(top, g);
+  }
+  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  __shared__ float red[16];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w]);
+  int e = top > 0.f ? 14 - ilogbf(top) : 0;
+  e = e > 100 ? 100 : e < -100 ? -100 : e;  // both factors normal numbers
+  scale[0] = ldexpf(1.f, e);
+  scale[1] = ldexpf(1.f, -e);
 }
 
 // dst = fp16(src), round to nearest even; 8 elements per thread.
@@ -1473,6 +1763,81 @@ int head_check(int64_t rows, int64_t d, int64_t vocab, int64_t padded) {
   return RV_OK;
 }
 
+// The tied head's log-probabilities: launches of one tile shape.
+template <bool A_RC, bool B_RC, Epi EPI, bool BF>
+int launch_logp(int shape, GemmArgs a, hipStream_t s) {
+  const TileShape t = kShapes[shape];
+  a.tiles_m = (a.m + t.bm - 1) / t.bm;
+  a.tiles_n = (a.n + t.bn - 1) / t.bn;
+  const int64_t blocks = a.tiles_m * a.tiles_n * ((a.k + a.k_chunk - 1) / a.k_chunk);
+  if (blocks * t.waves * 64 >= (int64_t)1 << 32) return RV_ERR_UNSUPPORTED;  // threads a launch holds
+  const dim3 grid((unsigned)blocks), block(t.waves * 64);
+#define RV_LAUNCH(SHAPE) \
+  hipLaunchKernelGGL((gemm_kernel<SHAPE, A_RC, B_RC, EPI, BF>), grid, block, 0, s, a)
+  constexpr bool kZ = EPI == Epi::LogProb || EPI == Epi::LogProbGrad;
+  switch (shape) {
+    case 1: RV_LAUNCH(1); break;
+    case 2: RV_LAUNCH(2); break;
+    case 3: RV_LAUNCH(3); break;
+    case 0:
+      if constexpr (kZ) return RV_ERR_UNSUPPORTED;
+      else RV_LAUNCH(0);
+      break;
+    case 4:
+      if constexpr (!kZ) return RV_ERR_UNSUPPORTED;
+      else RV_LAUNCH(4);
+      break;
+    case 5:
+      if constexpr (kZ || A_RC) return RV_ERR_UNSUPPORTED;
+      else RV_LAUNCH(5);
+      break;
+    default: return RV_ERR_UNSUPPORTED;
+  }
+#undef RV_LAUNCH
+  return rv_host::check_launch();
+}
+
+template <typename T>
+int launch_scaled_reduce(const float* part, void* out, int64_t n, int64_t splits,
+                         const float* scale, int accumulate, hipStream_t s) {
+  hipLaunchKernelGGL(scaled_reduce<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, part,
+                     static_cast<T*>(out), n, (int)splits, scale, accumulate);
+  return rv_host::check_launch();
+}
+int launch_scaled_reduce(int dtype, const float* part, void* out, int64_t n, int64_t splits,
+                         const float* scale, int accumulate, hipStream_t s) {
+  if (dtype == RV_F32)
+    return launch_scaled_reduce<float>(part, out, n, splits, scale, accumulate, s);
+  if (dtype == RV_BF16)
+    return launch_scaled_reduce<__hip_bfloat16>(part, out, n, splits, scale, 0, s);
+  return launch_scaled_reduce<__half>(part, out, n, splits, scale, 0, s);
+}
+
+// Widths as the tile choices above take them: whole tiles of 128 columns.
+int64_t up128(int64_t n) { return (n + 127) / 128 * 128; }
+
+int logp_check(int64_t rows, int64_t d, int64_t vocab, int64_t padded, int dtype) {
+  if (rows <= 0 || d <= 0 || vocab <= 0 || padded < vocab) return RV_ERR_BAD_SIZE;
+  if (dtype != RV_F16 && dtype != RV_BF16) return RV_ERR_UNSUPPORTED;
+  if (d % 8 || padded % 64 || !span32(padded) || !span32(d)) return RV_ERR_UNSUPPORTED;
+  return RV_OK;
+}
+
+// The logits' product: x[rows, d] head[vocab, d]^T.
+GemmArgs logp_args(const void* x, const void* head, int64_t rows, int64_t d, int64_t n,
+                   const int64_t* labels, int64_t ignore, int64_t vocab) {
+  GemmArgs a{};
+  a.a = static_cast<const __half*>(x); a.lda = d; a.a_bytes = rows * d * 2;
+  a.b = static_cast<const __half*>(head); a.ldb = d; a.b_bytes = n * d * 2;
+  a.m = rows; a.n = n; a.k = d; a.k_chunk = d;
+  a.head.labels = labels; a.head.ignore = ignore; a.head.vocab = vocab;
+  return a;
+}
+
+int logp_z_shape(int64_t rows, int64_t d, int64_t padded) {
+  return head_logits_shape(rows, d, padded);
+}
+
 // Buffer loads address an operand with 32-bit byte offsets.
 bool fits32(int64_t elems) { return elems > 0 && elems * 2 <= (int64_t)INT32_MAX - (int64_t)(1 << 24); }
 
@@ -1771,6 +2136,144 @@ int rv_head_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int6
   hipLaunchKernelGGL(act_reduce<__half>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s,
                      part, static_cast<__half*>(dw), n, (int)p.splits);
   return rv_host::check_launch();
+}
+
+int64_t rv_head_logp_workspace_bytes(int64_t rows, int64_t d, int64_t vocab) {
+  const int bad = logp_check(rows, d, vocab, up128(vocab), RV_F16);
+  if (bad) return -(int64_t)bad;
+  const int64_t bn = kShapes[logp_z_shape(rows, d, vocab)].bn;
+  return (vocab + bn - 1) / bn * rows * 8 + rows * 4;
+}
+
+int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                     int dtype, const int64_t* labels, int64_t ignore_index, float* logp,
+                     float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!x || !head || !labels || !logp || !lse) return RV_ERR_NULL_POINTER;
+  const int bad = logp_check(rows, d, vocab, up128(vocab), dtype);
+  if (bad) return bad;
+  if (!ok16(x) || !ok16(head)) return RV_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < rv_head_logp_workspace_bytes(rows, d, vocab) ||
+      !ok16(workspace))
+    return RV_ERR_WORKSPACE;
+  const int shape = logp_z_shape(rows, d, vocab);
+  const int64_t tiles = (vocab + kShapes[shape].bn - 1) / kShapes[shape].bn;
+  float2* part = static_cast<float2*>(workspace);
+  float* label_logit = reinterpret_cast<float*>(part + tiles * rows);
+  GemmArgs a = logp_args(x, head, rows, d, vocab, labels, ignore_index, vocab);
+  a.c = part;
+  a.head.label_logit = label_logit;
+  const hipStream_t s = (hipStream_t)stream;
+  const int st = dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProb, true>(shape, a, s)
+                                  : launch_logp<false, false, Epi::LogProb, false>(shape, a, s);
+  if (st != RV_OK) return st;
+  if (rows >= 32 * kCUs)
+    hipLaunchKernelGGL(logprob_rows<32>, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, part,
+                       label_logit, labels, rows, (int)tiles, vocab, ignore_index, logp, lse);
+  else
+    hipLaunchKernelGGL(logprob_rows<4>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, part,
+                       label_logit, labels, rows, (int)tiles, vocab, ignore_index, logp, lse);
+  return rv_host::check_launch();
+}
+
+int rv_head_logp_scale(const float* grad, const int64_t* labels, int64_t rows,
+                       int64_t ignore_index, float* scale, void* stream) {
+  if (!grad || !labels || !scale) return RV_ERR_NULL_POINTER;
+  if (rows <= 0) return RV_ERR_BAD_SIZE;
+  hipLaunchKernelGGL(logprob_scale, dim3(1), dim3(1024), 0, (hipStream_t)stream, grad, labels,
+                     rows, ignore_index, scale);
+  return rv_host::check_launch();
+}
+
+int rv_head_logp_dlogits(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                         int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,
+                         const float* lse, const float* grad, const float* scale, void* dlogits,
+                         void* stream) {
+  if (!x || !head || !labels || !lse || !grad || !scale || !dlogits) return RV_ERR_NULL_POINTER;
+  const int bad = logp_check(rows, d, vocab, padded, dtype);
+  if (bad) return bad;
+  if (!ok16(x) || !ok16(head) || !ok16(dlogits)) return RV_ERR_UNSUPPORTED;
+  GemmArgs a = logp_args(x, head, rows, d, padded, labels, ignore_index, vocab);
+  a.c = dlogits; a.ldc = padded; a.valid = vocab;
+  a.head.lse = lse; a.head.grad = grad; a.head.scale = scale;
+  const int shape = logp_z_shape(rows, d, padded);
+  const hipStream_t s = (hipStream_t)stream;
+  return dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProbGrad, true>(shape, a, s)
+                          : launch_logp<false, false, Epi::LogProbGrad, false>(shape, a, s);
+}
+
+int64_t rv_head_logp_grad_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded) {
+  const int bad = logp_check(rows, d, vocab, padded, RV_F16);
+  if (bad) return -(int64_t)bad;
+  const WgradPlan p = plan_wgrad(rows, vocab, up128(d), true);
+  if (p.shape < 0) return -(int64_t)RV_ERR_UNSUPPORTED;
+  const int64_t dx = head_dx_bytes(rows, up128(d), padded), dw = part_bytes(p, vocab, up128(d));
+  return dx > dw ? dx : dw;
+}
+
+int rv_head_logp_dx(const void* dlogits, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                    int64_t padded, int dtype, const float* scale, void* dx, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+  if (!dlogits || !head || !scale || !dx) return RV_ERR_NULL_POINTER;
+  const int bad = logp_check(rows, d, vocab, padded, dtype);
+  if (bad) return bad;
+  if (!ok16(dlogits) || !ok16(head) || !ok16(dx)) return RV_ERR_UNSUPPORTED;
+  GemmArgs a{};
+  a.a = static_cast<const __half*>(dlogits); a.lda = padded; a.a_bytes = rows * padded * 2;
+  a.b = static_cast<const __half*>(head); a.ldb = d;  // B(d, v) = head[v][d]: RC
+  a.b_bytes = vocab * d * 2;  // the operand ends here: the pad rows read as zero
+  a.m = rows; a.n = d; a.k = padded; a.k_chunk = head_chunk(rows, up128(d), padded);
+  a.ldc = d; a.head.scale = scale;
+  const hipStream_t s = (hipStream_t)stream;
+  const int64_t splits = (padded + a.k_chunk - 1) / a.k_chunk;
+  const int shape = head_dx_shape(rows, up128(d), padded);
+  if (splits == 1) {
+    a.c = dx;
+    return dtype == RV_BF16 ? launch_logp<false, true, Epi::StoreScaled, true>(shape, a, s)
+                            : launch_logp<false, true, Epi::StoreScaled, false>(shape, a, s);
+  }
+  if (!workspace || workspace_bytes < splits * rows * d * (int64_t)sizeof(float) ||
+      !ok16(workspace))
+    return RV_ERR_WORKSPACE;
+  a.c = workspace;
+  const int st = dtype == RV_BF16 ? launch_logp<false, true, Epi::PartialRagged, true>(shape, a, s)
+                                  : launch_logp<false, true, Epi::PartialRagged, false>(shape, a, s);
+  if (st != RV_OK) return st;
+  return launch_scaled_reduce(dtype, static_cast<const float*>(workspace), dx, rows * d, splits,
+                              scale, 0, s);
+}
+
+int rv_head_logp_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int64_t vocab,
+                    int64_t padded, int dtype, const float* scale, void* dw, int dw_dtype,
+                    int accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!dlogits || !x || !scale || !dw) return RV_ERR_NULL_POINTER;
+  const int bad = logp_check(rows, d, vocab, padded, dtype);
+  if (bad) return bad;
+  if (dw_dtype != RV_F32 && (dw_dtype != dtype || accumulate)) return RV_ERR_UNSUPPORTED;
+  if (!ok16(dlogits) || !ok16(x) || !ok16(dw)) return RV_ERR_UNSUPPORTED;
+  const WgradPlan p = plan_wgrad(rows, vocab, up128(d), true);
+  if (p.shape < 0) return RV_ERR_UNSUPPORTED;
+  if (p.splits > 1 &&
+      (!workspace || workspace_bytes < part_bytes(p, vocab, up128(d)) || !ok16(workspace)))
+    return RV_ERR_WORKSPACE;
+  // dW[v][d] = sum_m dlogits[m][v] x[m][d]; rows from vocab on are not written
+  WgradJob j = plan_job(p, static_cast<const __half*>(dlogits), padded,
+                        static_cast<const __half*>(x), d, rows, vocab, d, static_cast<float*>(dw),
+                        accumulate, static_cast<float*>(workspace));
+  j.g.head.scale = scale;
+  const hipStream_t s = (hipStream_t)stream;
+  if (p.splits == 1) {
+    if (dw_dtype == RV_F32)
+      return dtype == RV_BF16 ? launch_logp<true, true, Epi::AccF32Scaled, true>(p.shape, j.g, s)
+                              : launch_logp<true, true, Epi::AccF32Scaled, false>(p.shape, j.g, s);
+    return dtype == RV_BF16 ? launch_logp<true, true, Epi::StoreScaled, true>(p.shape, j.g, s)
+                            : launch_logp<true, true, Epi::StoreScaled, false>(p.shape, j.g, s);
+  }
+  const int st = dtype == RV_BF16
+                     ? launch_logp<true, true, Epi::PartialRagged, true>(p.shape, j.g, s)
+                     : launch_logp<true, true, Epi::PartialRagged, false>(p.shape, j.g, s);
+  if (st != RV_OK) return st;
+  return launch_scaled_reduce(dw_dtype, static_cast<const float*>(workspace), dw, vocab * d,
+                              p.splits, scale, accumulate, s);
 }
 
 int64_t rv_linear_dw_pair_workspace_bytes(int64_t rows, int64_t in_a, int64_t out_a, int64_t in_b,

@@ -25,6 +25,9 @@ with the scaler as ``unscale_`` does, and leaves both multiplies to the next
 ``step()``, which applies them as it reads each gradient
 (``rv_adamw_step_clipped``) -- the values the two passes would have written.
 Between the two calls ``p.grad`` still holds the scaled, unclipped gradient.
+
+``FusedAdamW8bit`` is the same optimizer with the moments of large tensors in 8
+bits (no counterpart in the reference).
 """
 from __future__ import annotations
 
@@ -69,10 +72,18 @@ class FusedAdamW(Optimizer):
         for p in params:
             st = self.state[p]
             if "exp_avg" not in st:
-                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                st.update(self._new_moments(p))
             st["step"] = step
         return step, params
+
+    def _new_moments(self, p):
+        return {k: torch.zeros_like(p, memory_format=torch.preserve_format)
+                for k in ("exp_avg", "exp_avg_sq")}
+
+    def load_state_dict(self, state_dict):
+        if any("exp_avg_scale" in st for st in state_dict["state"].values()):
+            raise ValueError("these moments are in 8 bits: load them into FusedAdamW8bit")
+        super().load_state_dict(state_dict)
 
     @torch.no_grad()
     def unscale_clip_(self, scaler, max_norm: float) -> torch.Tensor:
@@ -151,24 +162,134 @@ class FusedAdamW(Optimizer):
                    if grad_scale is not None else pending_inv)
             _check(lib.rv_adamw_advance(step.data_ptr(), fi.data_ptr() if fi is not None else None,
                                         stream), "rv_adamw_advance")
-            beta1, beta2 = group["betas"]
-            limit = lib.rv_adamw_max_tensors()
-            for start in range(0, len(params), limit):
-                chunk = params[start:start + limit]
-                n = len(chunk)
-                for p in chunk:
-                    if not (p.is_contiguous() and p.grad.is_contiguous()):
-                        raise ValueError("FusedAdamW requires contiguous parameters and gradients")
-                P = ctypes.c_void_p * n
-                ptrs = [P(*[t.data_ptr() for t in ts]) for ts in (
-                    chunk, [p.grad for p in chunk], [self.state[p]["exp_avg"] for p in chunk],
-                    [self.state[p]["exp_avg_sq"] for p in chunk])]
-                numel = (ctypes.c_int64 * n)(*[p.numel() for p in chunk])
-                _check(lib.rv_adamw_step_clipped(
-                    n, ptrs[0], ptrs[1], ptrs[2], ptrs[3], numel, float(group["lr"]),
-                    float(beta1), float(beta2), float(group["eps"]), float(group["weight_decay"]),
-                    step.data_ptr(), fi.data_ptr() if fi is not None else None,
-                    inv.data_ptr() if inv is not None else None,
-                    clip.data_ptr() if clip is not None else None, stream),
-                    "rv_adamw_step_clipped")
+            device = (step.data_ptr(), *(t.data_ptr() if t is not None else None
+                                         for t in (fi, inv, clip)), stream)
+            self._update(lib, group, params, device)
         return loss
+
+    def _update(self, lib, group, params, device):
+        """One update of a group's ``params`` (step count, overflow flag, inverse scale
+        and clip coefficient on the device, stream: ``device``)."""
+        beta1, beta2 = group["betas"]
+        limit = lib.rv_adamw_max_tensors()
+        for start in range(0, len(params), limit):
+            chunk = params[start:start + limit]
+            n = len(chunk)
+            for p in chunk:
+                if not (p.is_contiguous() and p.grad.is_contiguous()):
+                    raise ValueError("FusedAdamW requires contiguous parameters and gradients")
+            P = ctypes.c_void_p * n
+            ptrs = [P(*[t.data_ptr() for t in ts]) for ts in (
+                chunk, [p.grad for p in chunk], [self.state[p]["exp_avg"] for p in chunk],
+                [self.state[p]["exp_avg_sq"] for p in chunk])]
+            numel = (ctypes.c_int64 * n)(*[p.numel() for p in chunk])
+            _check(lib.rv_adamw_step_clipped(
+                n, ptrs[0], ptrs[1], ptrs[2], ptrs[3], numel, float(group["lr"]),
+                float(beta1), float(beta2), float(group["eps"]), float(group["weight_decay"]),
+                *device), "rv_adamw_step_clipped")
+
+
+# A moment held in 8 bits: its e4m3 values and, under this name, its scale bytes.
+_SCALES = {"exp_avg": "exp_avg_scale", "exp_avg_sq": "exp_avg_sq_scale"}
+
+
+class FusedAdamW8bit(FusedAdamW):
+    """``FusedAdamW`` with the moments of large tensors in 8 bits: 2.06 bytes of state
+    per parameter instead of 8 (``rv_adamw8_step``).
+
+    A tensor of at least ``min_8bit_numel`` elements keeps ``exp_avg`` and
+    ``exp_avg_sq`` as torch.float8_e4m3fn of the parameter's shape with one power of
+    two per 32 consecutive elements (``exp_avg_scale``, ``exp_avg_sq_scale``: uint8,
+    value = e4m3 * 2^(byte - 127)); smaller ones (norm weights) keep them in fp32.
+    The update uses the fp32 moments of its step; what is stored is rounded to
+    nearest (``exp_avg``) or at random with its expectation kept (``exp_avg_sq``,
+    whose change per step is below half a step of e4m3).  The random bits follow
+    from ``seed``, the parameter's place, the step count and the element: a run
+    repeats bit for bit.  GradScaler, ``unscale_clip_``, the device-side step count
+    and graph capture work as in ``FusedAdamW``; ``moments(p)`` returns a
+    parameter's moments in fp32.  A checkpoint of ``FusedAdamW`` can be loaded (its
+    moments stay in fp32), not the other way round.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 amsgrad=False, *, min_8bit_numel=4096, seed=0, maximize=False, foreach=None,
+                 capturable=False, differentiable=False, fused=None):
+        if min_8bit_numel < 1:
+            raise ValueError("min_8bit_numel must be positive")
+        if not 0 <= seed < 1 << 32:
+            raise ValueError("seed must be an unsigned 32-bit number")
+        self.min_8bit_numel = min_8bit_numel
+        super().__init__(params, lr, betas, eps, weight_decay, amsgrad, maximize=maximize,
+                         foreach=foreach, capturable=capturable, differentiable=differentiable,
+                         fused=fused)
+        self.defaults["seed"] = seed  # saved with the groups: a resumed run goes on alike
+        for group in self.param_groups:
+            group.setdefault("seed", seed)
+
+    def _new_moments(self, p):
+        if p.numel() < self.min_8bit_numel:
+            return super()._new_moments(p)
+        if not p.is_contiguous():
+            raise ValueError("FusedAdamW8bit requires contiguous parameters")
+        blocks = -(-p.numel() // library().rv_adamw8_block())
+        st = {}
+        for name, scale in _SCALES.items():
+            codes = torch.zeros(p.shape, device=p.device, dtype=torch.uint8)
+            st[name] = codes.view(torch.float8_e4m3fn)
+            st[scale] = torch.zeros(blocks, device=p.device, dtype=torch.uint8)
+        return st
+
+    def _update(self, lib, group, params, device):
+        ordinal = {p: i for i, p in enumerate(q for g in self.param_groups for q in g["params"])}
+        small = [p for p in params if "exp_avg_scale" not in self.state[p]]
+        large = [p for p in params if "exp_avg_scale" in self.state[p]]
+        if small:
+            super()._update(lib, group, small, device)
+        beta1, beta2 = group["betas"]
+        limit = lib.rv_adamw8_max_tensors()
+        for start in range(0, len(large), limit):
+            chunk = large[start:start + limit]
+            n = len(chunk)
+            for p in chunk:
+                if not (p.is_contiguous() and p.grad.is_contiguous()):
+                    raise ValueError("FusedAdamW8bit requires contiguous parameters and gradients")
+            P = ctypes.c_void_p * n
+            states = [self.state[p] for p in chunk]
+            ptrs = [P(*[t.data_ptr() for t in ts]) for ts in (
+                chunk, [p.grad for p in chunk],
+                *([st[k] for st in states] for k in ("exp_avg", "exp_avg_scale", "exp_avg_sq",
+                                                     "exp_avg_sq_scale")))]
+            numel = (ctypes.c_int64 * n)(*[p.numel() for p in chunk])
+            places = (ctypes.c_uint32 * n)(*[ordinal[p] for p in chunk])
+            _check(lib.rv_adamw8_step(
+                n, *ptrs, numel, places, group["seed"], float(group["lr"]), float(beta1),
+                float(beta2), float(group["eps"]), float(group["weight_decay"]), *device),
+                "rv_adamw8_step")
+
+    @torch.no_grad()
+    def moments(self, p) -> tuple:
+        """fp32 (exp_avg, exp_avg_sq) of a parameter that has taken a step."""
+        st, out = self.state[p], []
+        for name, scale in _SCALES.items():
+            value = st[name].float()
+            if scale in st:
+                block = library().rv_adamw8_block()
+                # ldexp in two factors: 2^(byte - 127) alone may be no normal number
+                exponent = st[scale].double().repeat_interleave(block)[:p.numel()] - 127
+                value = (value.double() * exponent.exp2().view(p.shape)).float()
+            out.append(value)
+        return tuple(out)
+
+    def load_state_dict(self, state_dict):
+        """As torch's, which casts every floating or parameter-like state to the
+        parameter's type; the 8-bit moments keep theirs."""
+        Optimizer.load_state_dict(self, state_dict)
+        saved = state_dict["state"]
+        places = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(places, (q for g in self.param_groups for q in g["params"])):
+            for name, scale in _SCALES.items():
+                if scale in saved.get(i, {}):
+                    for key in (name, scale):
+                        t = saved[i][key]
+                        bits = t.contiguous().view(torch.uint8).to(p.device, copy=True)
+                        self.state[p][key] = bits.view(t.dtype)
