@@ -935,6 +935,8 @@ void wgrad_pair_kernel(GemmPair pair) {
   gemm_block<SHAPE, true, true, EPI>(pair.g[second], blockIdx.x - (second ? pair.first : 0));
 }
 
+#include "head_stream.h"
+
 // Explicit instantiations of every (tile shape, operand layout, epilogue) the
 // host dispatch can launch.  Without them this compiler emits the host-side
 // launch stubs of only some of the kernels reached through the dispatch
@@ -975,6 +977,12 @@ static_assert(kNumShapes == 7 && kRuleShapes == 4, "instantiations above");
   template __global__ void gemm_kernel<SHAPE, true, true, Epi::AccF32Scaled, BF>(GemmArgs);  \
   template __global__ void gemm_kernel<SHAPE, true, true, Epi::PartialRagged, BF>(GemmArgs);
 RV_LOGP_KERNELS(false) RV_LOGP_KERNELS(true)
+#define RV_STREAM_KERNELS(KS)                                       \
+  template __global__ void head_stream_k<KS, false, false>(StreamArgs); \
+  template __global__ void head_stream_k<KS, false, true>(StreamArgs);  \
+  template __global__ void head_stream_k<KS, true, false>(StreamArgs);  \
+  template __global__ void head_stream_k<KS, true, true>(StreamArgs);
+RV_STREAM_KERNELS(8) RV_STREAM_KERNELS(16)
 
 // acc[i] (+)= fp32(fp16(sum_s part[s][i])), splits summed in order.  This is
 // autocast's weight gradient: the fp16 GEMM result, cast to the fp32 weight
@@ -1101,52 +1109,54 @@ void scaled_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t 
   }
 }
 
-// A row's log-probability from its tiles' maxima and sums (Epi::LogProb):
-// lse = M + log sum_t s_t exp(m_t - M), logp = z_label - lse; 0 for an ignored
-// label, NaN for one outside the vocabulary.  A workgroup owns R rows, 256 / R
-// threads each, which take the tiles in turn and meet in LDS in a fixed order.
+// Joins two (maximum, sum of exp(z - maximum)) of the same row; a maximum of -inf
+// comes with a sum of 0 (or NaN, which stays).
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  if (top == -INFINITY) return make_float2(top, a.y + b.y);
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - top) * kLog2e) +
+                              b.y * __builtin_amdgcn_exp2f((b.x - top) * kLog2e));
+}
+
+// A row's log-probability from its tiles' maxima and sums: lse = M + log sum_t s_t
+// exp(m_t - M), logp = z_label - lse; 0 for an ignored label, NaN for one outside the
+// vocabulary.  A workgroup owns R rows, 256 / R threads each, which take the tiles in
+// turn, four loads at a time, and meet by lane swaps and in LDS in a fixed order (51
+// rows of 197 tiles: 9.6 us with one join after the other, see the launch).
 template <int R>
 __global__ __launch_bounds__(256)
 void logprob_rows(const float2* __restrict__ part, const float* __restrict__ label_logit,
                   const int64_t* __restrict__ labels, int64_t rows, int tiles, int64_t vocab,
                   int64_t ignore, float* __restrict__ logp, float* __restrict__ lse) {
-  constexpr int kSlices = 256 / R;
+  constexpr int kSlices = 256 / R, kAhead = 4;
   const int r = threadIdx.x % R, slice = threadIdx.x / R;
   const int64_t row = (int64_t)blockIdx.x * R + r;
-  float top = -INFINITY, sum = 0.f;
-  if (row < rows) {
-#pragma unroll 4
-    for (int t = slice; t < tiles; t += kSlices) {
-      const float2 v = part[(int64_t)t * rows + row];
-      const float n = fmaxf(top, v.x);
-      if (n != -INFINITY)
-        sum = sum * __builtin_amdgcn_exp2f((top - n) * kLog2e) +
-              v.y * __builtin_amdgcn_exp2f((v.x - n) * kLog2e);
-      else
-        sum += v.y;  // NaN where every logit is
-      top = n;
+  float2 all = make_float2(-INFINITY, 0.f);
+  for (int t = slice; t < tiles; t += kSlices * kAhead) {
+    float2 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = t + k * kSlices;
+      v[k] = at < tiles && row < rows ? part[(int64_t)at * rows + row] : make_float2(-INFINITY, 0.f);
     }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) all = join(all, v[k]);
   }
-  __shared__ float2 red[256];
-  red[threadIdx.x] = make_float2(top, sum);
+#pragma unroll
+  for (int o = R; o < 64; o <<= 1)
+    all = join(all, make_float2(__shfl_xor(all.x, o, 64), __shfl_xor(all.y, o, 64)));
+  __shared__ float2 red[4][R];
+  if ((threadIdx.x & 63) < R) red[threadIdx.x >> 6][r] = all;
   __syncthreads();
-  if (slice != 0 || row >= rows) return;
-  for (int k = 1; k < kSlices; ++k) {
-    const float2 v = red[k * R + r];
-    const float n = fmaxf(top, v.x);
-    if (n != -INFINITY)
-      sum = sum * __builtin_amdgcn_exp2f((top - n) * kLog2e) +
-            v.y * __builtin_amdgcn_exp2f((v.x - n) * kLog2e);
-    else
-      sum += v.y;
-    top = n;
-  }
+  if (threadIdx.x >= R || row >= rows) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) all = join(all, red[w][r]);
   const int64_t label = labels[row];
-  const float l = logf(sum);
-  lse[row] = top + l;
+  const float l = logf(all.y);
+  lse[row] = all.x + l;
   logp[row] = label == ignore ? 0.f
               : label < 0 || label >= vocab ? NAN
-                                            : (label_logit[row] - top) - l;
+                                            : (label_logit[row] - all.x) - l;
 }
 
 // The power of two that brings the largest gradient of a row that counts to
@@ -1838,6 +1848,52 @@ int logp_z_shape(int64_t rows, int64_t d, int64_t padded) {
   return head_logits_shape(rows, d, padded);
 }
 
+// The streamed logits of narrow models (head_stream_k): stages of 64 columns per
+// workgroup.  Two workgroups a CU run at a time; a workgroup's start (its rows of
+// x, the first stage) costs about three stages.
+bool stream_takes(int64_t d) { return d <= 256; }
+int64_t stream_chunk(int64_t rows, int64_t n) {
+  const int64_t stages = (n + 63) / 64, tiles_m = (rows + 255) / 256, places = 2 * kCUs;
+  int64_t best = stages, least = 0;
+  for (int64_t rounds = 1; rounds <= 8; ++rounds) {
+    int64_t splits = rounds * places / tiles_m;
+    if (splits < 1) splits = 1;
+    if (splits > stages) splits = stages;
+    const int64_t chunk = (stages + splits - 1) / splits;
+    const int64_t tiles = tiles_m * ((stages + chunk - 1) / chunk);
+    const int64_t cost = (tiles + places - 1) / places * (chunk + 3);
+    if (least == 0 || cost < least) best = chunk, least = cost;
+  }
+  return best;
+}
+template <bool GRAD>
+int launch_stream(StreamArgs a, int dtype, hipStream_t s) {
+  a.stages = (a.n + 63) / 64;
+  a.chunk = stream_chunk(a.m, a.n);
+  a.tiles_m = (a.m + 255) / 256;
+  a.tiles = a.tiles_m * ((a.stages + a.chunk - 1) / a.chunk);
+  const int64_t blocks = (a.tiles + 7) / 8 * 8;
+  if (blocks * 256 >= (int64_t)1 << 32) return RV_ERR_UNSUPPORTED;  // threads a launch holds
+  const dim3 grid((unsigned)blocks), block(256);
+#define RV_LAUNCH(KS, BF) hipLaunchKernelGGL((head_stream_k<KS, BF, GRAD>), grid, block, 0, s, a)
+  if (a.d <= 128) {
+    if (dtype == RV_BF16) RV_LAUNCH(8, true);
+    else RV_LAUNCH(8, false);
+  } else {
+    if (dtype == RV_BF16) RV_LAUNCH(16, true);
+    else RV_LAUNCH(16, false);
+  }
+#undef RV_LAUNCH
+  return rv_host::check_launch();
+}
+
+// Tiles of columns that the forward's statistics come in.
+int64_t logp_parts(int64_t rows, int64_t d, int64_t vocab) {
+  const int64_t cols = stream_takes(d) ? 64 * stream_chunk(rows, vocab)
+                                       : kShapes[logp_z_shape(rows, d, vocab)].bn;
+  return (vocab + cols - 1) / cols;
+}
+
 // Buffer loads address an operand with 32-bit byte offsets.
 bool fits32(int64_t elems) { return elems > 0 && elems * 2 <= (int64_t)INT32_MAX - (int64_t)(1 << 24); }
 
@@ -2141,8 +2197,7 @@ int rv_head_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int6
 int64_t rv_head_logp_workspace_bytes(int64_t rows, int64_t d, int64_t vocab) {
   const int bad = logp_check(rows, d, vocab, up128(vocab), RV_F16);
   if (bad) return -(int64_t)bad;
-  const int64_t bn = kShapes[logp_z_shape(rows, d, vocab)].bn;
-  return (vocab + bn - 1) / bn * rows * 8 + rows * 4;
+  return logp_parts(rows, d, vocab) * rows * 8 + rows * 4;
 }
 
 int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
@@ -2155,16 +2210,22 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
   if (!workspace || workspace_bytes < rv_head_logp_workspace_bytes(rows, d, vocab) ||
       !ok16(workspace))
     return RV_ERR_WORKSPACE;
-  const int shape = logp_z_shape(rows, d, vocab);
-  const int64_t tiles = (vocab + kShapes[shape].bn - 1) / kShapes[shape].bn;
+  const int64_t tiles = logp_parts(rows, d, vocab);
   float2* part = static_cast<float2*>(workspace);
   float* label_logit = reinterpret_cast<float*>(part + tiles * rows);
   GemmArgs a = logp_args(x, head, rows, d, vocab, labels, ignore_index, vocab);
   a.c = part;
   a.head.label_logit = label_logit;
   const hipStream_t s = (hipStream_t)stream;
-  const int st = dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProb, true>(shape, a, s)
-                                  : launch_logp<false, false, Epi::LogProb, false>(shape, a, s);
+  int st;
+  if (stream_takes(d)) {
+    st = launch_stream<false>({a.a, a.b, rows, vocab, d, 0, 0, 0, 0, part, nullptr, a.head}, dtype,
+                              s);
+  } else {
+    const int shape = logp_z_shape(rows, d, vocab);
+    st = dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProb, true>(shape, a, s)
+                          : launch_logp<false, false, Epi::LogProb, false>(shape, a, s);
+  }
   if (st != RV_OK) return st;
   if (rows >= 32 * kCUs)
     hipLaunchKernelGGL(logprob_rows<32>, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, s, part,
@@ -2197,6 +2258,9 @@ int rv_head_logp_dlogits(const void* x, const void* head, int64_t rows, int64_t 
   a.head.lse = lse; a.head.grad = grad; a.head.scale = scale;
   const int shape = logp_z_shape(rows, d, padded);
   const hipStream_t s = (hipStream_t)stream;
+  if (stream_takes(d))
+    return launch_stream<true>({a.a, a.b, rows, padded, d, 0, 0, 0, 0, nullptr,
+                                static_cast<__half*>(dlogits), a.head}, dtype, s);
   return dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProbGrad, true>(shape, a, s)
                           : launch_logp<false, false, Epi::LogProbGrad, false>(shape, a, s);
 }

@@ -198,12 +198,15 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
 # ---------------------------------------------------------------------------
 # losses on token log-probabilities
 # ---------------------------------------------------------------------------
-def _tokens(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
+def _rows(t: torch.Tensor) -> torch.Tensor:
     """A [sequences, tokens] operand with dense rows."""
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _tokens(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
     if t.dtype != torch.float32 or t.shape != like.shape or t.device != like.device:
         raise ValueError(f"{what} must be fp32, of logp's shape and on its device")
-    t = t.detach()
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+    return _rows(t)
 
 
 def _mask(mask, like: torch.Tensor):
@@ -211,7 +214,7 @@ def _mask(mask, like: torch.Tensor):
         return None
     if mask.dtype != torch.bool or mask.shape != like.shape or mask.device != like.device:
         raise ValueError("mask must be a bool tensor of logp's shape on its device")
-    return mask if mask.stride(1) == 1 or mask.shape[1] <= 1 else mask.contiguous()
+    return _rows(mask)
 
 
 def _check_logp(logp: torch.Tensor, what: str) -> None:
@@ -220,12 +223,18 @@ def _check_logp(logp: torch.Tensor, what: str) -> None:
                          "no silent fallback")
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _at(t) -> tuple:
+    """(address, row stride) of an optional [sequences, tokens] operand."""
+    return (None, 0) if t is None else (t.data_ptr(), t.stride(0))
 
 
-def _ld(t):
-    return 0 if t is None else t.stride(0)
+# The two Functions below are called on small batches too, where the host's work is
+# what they take: few allocations (outputs and workspace cut from one) and no zeros
+# made for the outputs without a gradient.  fp32 values of the workspace's share:
+def _floats(nbytes: int, what: str) -> int:
+    if nbytes < 0:
+        _check(-nbytes, what)
+    return -(-nbytes // 4)
 
 
 class PreferenceLoss(torch.autograd.Function):
@@ -234,33 +243,34 @@ class PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, ref, mask, beta, smoothing, average):
         seqs, tokens = logp.shape
-        lib, pairs = library(), seqs // 2
-        loss = torch.empty((), device=logp.device, dtype=torch.float32)
-        reward, coef = torch.empty(2, seqs, device=logp.device, dtype=torch.float32).unbind()
-        rows = _tokens(logp, logp, "logp")
+        lib, pairs, dev = library(), seqs // 2, logp.device
+        rows = _rows(logp)
         with _DeviceGuard(logp):
             nbytes = lib.rv_pref_loss_workspace_bytes(pairs, tokens)
-            ws = _workspace(nbytes, logp, "rv_pref_loss_workspace_bytes")
+            # the workspace first: its fp64 sums need the allocation's alignment
+            sizes = (_floats(nbytes, "rv_pref_loss_workspace_bytes"), seqs, pairs, pairs)
+            ws, coef, chosen, rejected = torch.empty(
+                sum(sizes), device=dev, dtype=torch.float32).split(sizes)
+            loss = torch.empty((), device=dev, dtype=torch.float32)
             _check(lib.rv_pref_loss(
-                _ptr(rows), _ld(rows), _ptr(ref), _ld(ref), _ptr(mask), _ld(mask), pairs, tokens,
-                beta, smoothing, int(average), loss.data_ptr(), reward.data_ptr(),
-                coef.data_ptr(), ws.data_ptr(), nbytes, _stream(logp)), "rv_pref_loss")
+                rows.data_ptr(), rows.stride(0), *_at(ref), *_at(mask), pairs, tokens, beta,
+                smoothing, average, loss.data_ptr(), chosen.data_ptr(), coef.data_ptr(),
+                ws.data_ptr(), nbytes, _stream(logp)), "rv_pref_loss")
         ctx.save_for_backward(coef, mask)
         ctx.shape = (seqs, tokens)
-        chosen, rejected = reward[:pairs], reward[pairs:]
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(chosen, rejected)
         return loss, chosen, rejected
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gradient, *_):
+        if gradient is None:
+            return None, None, None, None, None, None
         coef, mask = ctx.saved_tensors
         dlogp = torch.empty(ctx.shape, device=coef.device, dtype=torch.float32)
-        gradient = gradient.to(torch.float32)
-        with _DeviceGuard(coef):
-            _check(library().rv_pref_grad(coef.data_ptr(), _ptr(mask), _ld(mask),
-                                          gradient.data_ptr(), *ctx.shape, dlogp.data_ptr(),
-                                          _stream(coef)), "rv_pref_grad")
+        _check(library().rv_pref_grad(coef.data_ptr(), *_at(mask), gradient.data_ptr(), *ctx.shape,
+                                      dlogp.data_ptr(), _stream(coef)), "rv_pref_grad")
         return dlogp, None, None, None, None, None
 
 
@@ -288,8 +298,8 @@ def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor, beta: float = 0.
     if not 0.0 <= label_smoothing <= 0.5:
         raise ValueError("label_smoothing must be in [0, 0.5]")
     return PreferenceResult(*PreferenceLoss.apply(
-        logp, _tokens(ref_logp, logp, "ref_logp"), _mask(mask, logp), float(beta),
-        float(label_smoothing), bool(average)))
+        logp, _tokens(ref_logp, logp, "ref_logp"), _mask(mask, logp), beta, label_smoothing,
+        bool(average)))
 
 
 class PolicyLoss(torch.autograd.Function):
@@ -298,35 +308,39 @@ class PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, old, ref, adv, mask, clip, kl_coef, per_sequence):
         seqs, tokens = logp.shape
-        lib = library()
-        rows = _tokens(logp, logp, "logp")
-        loss = torch.empty((), device=logp.device, dtype=torch.float32)
-        stats = torch.empty(3, device=logp.device, dtype=torch.float32)
-        slope = (torch.empty(seqs, tokens, device=logp.device, dtype=torch.float32)
+        lib, dev = library(), logp.device
+        rows = _rows(logp)
+        slope = (torch.empty(seqs, tokens, device=dev, dtype=torch.float32)
                  if ctx.needs_input_grad[0] else None)
         with _DeviceGuard(logp):
             nbytes = lib.rv_policy_loss_workspace_bytes(seqs, tokens, per_sequence)
-            ws = _workspace(nbytes, logp, "rv_policy_loss_workspace_bytes")
+            # the workspace first: its fp64 sums need the allocation's alignment
+            sizes = (_floats(nbytes, "rv_policy_loss_workspace_bytes"), 1, 1, 1)
+            ws, kl, clipped, factor = torch.empty(
+                sum(sizes), device=dev, dtype=torch.float32).split(sizes)
+            loss = torch.empty((), device=dev, dtype=torch.float32)
             _check(lib.rv_policy_loss(
-                _ptr(rows), _ld(rows), _ptr(old), _ld(old), _ptr(ref), _ld(ref), _ptr(adv),
-                adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, _ptr(mask), _ld(mask), seqs,
-                tokens, *clip, kl_coef, per_sequence, loss.data_ptr(), stats.data_ptr(),
-                _ptr(slope), ws.data_ptr(), nbytes, _stream(logp)), "rv_policy_loss")
-        ctx.save_for_backward(slope, stats)
-        kl, clipped = stats[0], stats[1]
+                rows.data_ptr(), rows.stride(0), *_at(old), *_at(ref), adv.data_ptr(),
+                adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, *_at(mask), seqs, tokens,
+                *clip, kl_coef, per_sequence, loss.data_ptr(), kl.data_ptr(),
+                slope.data_ptr() if slope is not None else None, ws.data_ptr(), nbytes,
+                _stream(logp)), "rv_policy_loss")
+        ctx.save_for_backward(slope, factor)
+        ctx.set_materialize_grads(False)
+        kl, clipped = kl.reshape(()), clipped.reshape(())
         ctx.mark_non_differentiable(kl, clipped)
         return loss, kl, clipped
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gradient, *_):
-        slope, stats = ctx.saved_tensors
+        if gradient is None:
+            return None, None, None, None, None, None, None, None
+        slope, factor = ctx.saved_tensors
         dlogp = torch.empty_like(slope)
-        gradient = gradient.to(torch.float32)
-        with _DeviceGuard(slope):
-            _check(library().rv_policy_grad(slope.data_ptr(), stats.data_ptr() + 8,
-                                            gradient.data_ptr(), slope.numel(), dlogp.data_ptr(),
-                                            _stream(slope)), "rv_policy_grad")
+        _check(library().rv_policy_grad(slope.data_ptr(), factor.data_ptr(), gradient.data_ptr(),
+                                        slope.numel(), dlogp.data_ptr(), _stream(slope)),
+               "rv_policy_grad")
         return dlogp, None, None, None, None, None, None, None
 
 
@@ -365,8 +379,8 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Te
         raise ValueError("a KL term needs ref_logp")
     ref = None if ref_logp is None else _tokens(ref_logp, logp, "ref_logp")
     return PolicyResult(*PolicyLoss.apply(
-        logp, _tokens(old_logp, logp, "old_logp"), ref, advantages.detach(), _mask(mask, logp),
-        (low, high), float(kl_coef), int(reduction == "sequence")))
+        logp, _tokens(old_logp, logp, "old_logp"), ref, advantages, _mask(mask, logp), (low, high),
+        kl_coef, reduction == "sequence"))
 
 
 # ---------------------------------------------------------------------------
