@@ -21,8 +21,12 @@
 // same bits.  A v > 0 stays > 0: a zero v under an m that is not would make the next
 // update as large as 1 / eps.
 //
-// Memory-bound: 16.125 bytes a parameter (p 8, g 4, codes 4, scales 4 / 32) against
-// about 100 VALU instructions, 28 bytes with fp32 moments.
+// Memory-bound: 16.125 bytes a parameter (p 8, g 4, codes 4, scales 4 / 32; 28 with fp32
+// moments) against about 85 VALU instructions.  93.2 M parameters in 6 tensors,
+// operands evicted: 291 us, 5.2 TB/s (fp32 moments 498 us); 355 us with one unit of four
+// elements a thread and correctly rounded divisions, 312 with one unit, 311 with four
+// (the bias corrections, in fp64, and the tensor's search are paid per thread; four
+// units leave fewer waves); streaming hints on the parameters 294 -> 291, left out.
 
 #include <cmath>
 
@@ -33,7 +37,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 48;
 constexpr int kBlock = 32;                        // elements per scale: 8 lanes of 4
-constexpr int64_t kChunk = kThreads * 4;          // elements per workgroup
+constexpr int kUnits = 2;                         // of four elements per thread
+constexpr int64_t kChunk = kThreads * 4 * kUnits;  // elements per workgroup
 constexpr int kGridRow = 1 << 22;                 // a launch dimension holds < 2^32 threads
 
 struct Table {
@@ -130,6 +135,99 @@ __device__ __forceinline__ int tensor_of(const int* chunk_start, int count, int 
   return t;
 }
 
+struct Scalars {
+  float step_size, inv_bc2, inv, clip;
+  uint32_t key;
+};
+
+// Four elements of a thread: where they are and what was loaded.
+struct Four {
+  float* p;
+  uint8_t *m, *v, *ms, *vs;   // codes of the four, scales of their block
+  int here;                   // elements inside the tensor
+  bool full;                  // all four, on vector boundaries
+  float pp[4], gg[4];
+  uint32_t mw, vw;
+  int mscale, vscale;
+};
+
+__device__ __forceinline__ void load(Four& f, const float* g) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f.pp[e] = f.gg[e] = 0.f;
+  f.mw = f.vw = 0;
+  f.mscale = f.vscale = 0;
+  if (f.full) {
+    const float4 a = rv::ld_f4(f.p), b = rv::ld_f4(g);
+    f.mw = *reinterpret_cast<const uint32_t*>(f.m);
+    f.vw = *reinterpret_cast<const uint32_t*>(f.v);
+    f.pp[0] = a.x; f.pp[1] = a.y; f.pp[2] = a.z; f.pp[3] = a.w;
+    f.gg[0] = b.x; f.gg[1] = b.y; f.gg[2] = b.z; f.gg[3] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < f.here) {
+        f.pp[e] = f.p[e];
+        f.gg[e] = g[e];
+        f.mw |= (uint32_t)f.m[e] << (8 * e);
+        f.vw |= (uint32_t)f.v[e] << (8 * e);
+      }
+  }
+  if (f.here > 0) {
+    f.mscale = *f.ms;
+    f.vscale = *f.vs;
+  }
+}
+
+// The update and the stores; every lane of a block takes part.  `pair`: the counter
+// of the first two elements' random bits.
+__device__ __forceinline__ void update(Four& f, const Hyper& h, const Scalars& s, uint32_t pair) {
+  float m[4], v[4];
+  decode(f.mw, f.mscale, m);
+  decode(f.vw, f.vscale, v);
+  uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float u = f.gg[e] * s.inv * s.clip;  // unscale_'s multiply, then clip_grad_norm_'s
+    m[e] = m[e] * h.beta1 + u * h.w1;
+    v[e] = v[e] * h.beta2 + u * h.w2 * u;
+    // v_rcp_f32 (1 ulp) instead of a division: the quotient is off by 2 ulps at most,
+    // and is added to p after a multiplication by the learning rate
+    const float denom = sqrtf(v[e]) * s.inv_bc2 + h.eps;
+    f.pp[e] = f.pp[e] * h.decay - s.step_size * (m[e] * __builtin_amdgcn_rcpf(denom));
+    if (e < f.here) {
+      const uint32_t a = magnitude(m[e]), b = magnitude(v[e]);
+      mtop = a > mtop ? a : mtop;
+      vtop = b > vtop ? b : vtop;
+    }
+  }
+  const int ms = scale_byte(block_max(mtop)), vs = scale_byte(block_max(vtop));
+  const uint32_t mw = encode(m, ms);
+  uint32_t vw = 0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t bits = mix(pair + half + s.key);  // 16 for each of two elements
+    vw |= encode_random(v[2 * half], vs, (bits & 0xffffu) << 4 | 8u) << (16 * half);
+    vw |= encode_random(v[2 * half + 1], vs, bits >> 16 << 4 | 8u) << (16 * half + 8);
+  }
+  if (f.full) {
+    rv::st_f4(f.p, make_float4(f.pp[0], f.pp[1], f.pp[2], f.pp[3]));
+    *reinterpret_cast<uint32_t*>(f.m) = mw;
+    *reinterpret_cast<uint32_t*>(f.v) = vw;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < f.here) {
+        f.p[e] = f.pp[e];
+        f.m[e] = (uint8_t)(mw >> (8 * e));
+        f.v[e] = (uint8_t)(vw >> (8 * e));
+      }
+  }
+  if ((threadIdx.x & 7) == 0 && f.here > 0) {
+    *f.ms = (uint8_t)ms;
+    *f.vs = (uint8_t)vs;
+  }
+}
+
 __global__ __launch_bounds__(kThreads)
 void adamw8_k(Table tab, Hyper h) {
   if (h.found_inf != nullptr && *h.found_inf != 0.0f) return;  // uniform skip
@@ -137,90 +235,35 @@ void adamw8_k(Table tab, Hyper h) {
   if (block >= tab.chunk_start[tab.count]) return;  // past the last row's end
   const int t = tensor_of(tab.chunk_start, tab.count, (int)block);
   const int64_t n = tab.n[t];
-  const int64_t i = (block - tab.chunk_start[t]) * kChunk + threadIdx.x * 4;
-  const int64_t at = i / kBlock;
-  float* p = tab.p[t] + i;
-  const float* g = tab.g[t] + i;
-  uint8_t* mc = tab.m[t] + i;
-  uint8_t* vc = tab.v[t] + i;
-  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(mc) | reinterpret_cast<uintptr_t>(vc)) & 3) == 0;
-  const bool full = vec && i + 4 <= n;
-  const int here = i >= n ? 0 : i + 4 <= n ? 4 : (int)(n - i);  // elements of this thread
-  float pp[4] = {}, gg[4] = {};
-  uint32_t mw = 0, vw = 0;
-  int ms = 0, vs = 0;
-  if (full) {
-    const float4 a = rv::ld_f4(p), b = rv::ld_f4(g);
-    mw = *reinterpret_cast<const uint32_t*>(mc);
-    vw = *reinterpret_cast<const uint32_t*>(vc);
-    pp[0] = a.x; pp[1] = a.y; pp[2] = a.z; pp[3] = a.w;
-    gg[0] = b.x; gg[1] = b.y; gg[2] = b.z; gg[3] = b.w;
-  } else {
+  const int64_t first = (block - tab.chunk_start[t]) * kChunk + threadIdx.x * 4;
+  const bool vec = ((reinterpret_cast<uintptr_t>(tab.p[t]) | reinterpret_cast<uintptr_t>(tab.g[t])) &
+                    15) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(tab.m[t]) | reinterpret_cast<uintptr_t>(tab.v[t])) &
+                    3) == 0;
+  Four f[kUnits];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < here) {
-        pp[e] = p[e];
-        gg[e] = g[e];
-        mw |= (uint32_t)mc[e] << (8 * e);
-        vw |= (uint32_t)vc[e] << (8 * e);
-      }
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t i = first + u * (kThreads * 4), at = i / kBlock;
+    f[u].here = i >= n ? 0 : i + 4 <= n ? 4 : (int)(n - i);
+    f[u].full = vec && i + 4 <= n;
+    f[u].p = tab.p[t] + i;
+    f[u].m = tab.m[t] + i;
+    f[u].v = tab.v[t] + i;
+    f[u].ms = tab.ms[t] + at;
+    f[u].vs = tab.vs[t] + at;
+    load(f[u], tab.g[t] + i);
   }
-  if (here > 0) {
-    ms = tab.ms[t][at];
-    vs = tab.vs[t][at];
-  }
+  __builtin_amdgcn_sched_barrier(0);
   const double step = (double)*h.step;
-  const float step_size = (float)(h.lr / (1.0 - exp2(step * h.log2_beta1)));
-  const float bc2_sqrt = (float)sqrt(1.0 - exp2(step * h.log2_beta2));
-  const float inv = h.inv_scale != nullptr ? *h.inv_scale : 1.0f;
-  const float clip = h.clip != nullptr ? *h.clip : 1.0f;
-  const uint32_t key = mix(tab.key[t] + (uint32_t)*h.step);
-
-  float m[4], v[4];
-  decode(mw, ms, m);
-  decode(vw, vs, v);
-  uint32_t mtop = 0, vtop = 0;
+  Scalars s;
+  s.step_size = (float)(h.lr / (1.0 - exp2(step * h.log2_beta1)));
+  s.inv_bc2 = (float)(1.0 / sqrt(1.0 - exp2(step * h.log2_beta2)));
+  s.inv = h.inv_scale != nullptr ? *h.inv_scale : 1.0f;
+  s.clip = h.clip != nullptr ? *h.clip : 1.0f;
+  s.key = mix(tab.key[t] + (uint32_t)*h.step);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float u = gg[e] * inv * clip;  // unscale_'s multiply, then clip_grad_norm_'s
-    m[e] = m[e] * h.beta1 + u * h.w1;
-    v[e] = v[e] * h.beta2 + u * h.w2 * u;
-    const float denom = sqrtf(v[e]) / bc2_sqrt + h.eps;
-    pp[e] = pp[e] * h.decay - step_size * (m[e] / denom);
-    if (e < here) {
-      const uint32_t a = magnitude(m[e]), b = magnitude(v[e]);
-      mtop = a > mtop ? a : mtop;
-      vtop = b > vtop ? b : vtop;
-    }
-  }
-  ms = scale_byte(block_max(mtop));
-  vs = scale_byte(block_max(vtop));
-  mw = encode(m, ms);
-  vw = 0;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const uint32_t bits = mix((uint32_t)(i >> 1) + half + key);  // 16 for each of two elements
-    vw |= encode_random(v[2 * half], vs, (bits & 0xffffu) << 4 | 8u) << (16 * half);
-    vw |= encode_random(v[2 * half + 1], vs, bits >> 16 << 4 | 8u) << (16 * half + 8);
-  }
-  if (full) {
-    rv::st_f4(p, make_float4(pp[0], pp[1], pp[2], pp[3]));
-    *reinterpret_cast<uint32_t*>(mc) = mw;
-    *reinterpret_cast<uint32_t*>(vc) = vw;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < here) {
-        p[e] = pp[e];
-        mc[e] = (uint8_t)(mw >> (8 * e));
-        vc[e] = (uint8_t)(vw >> (8 * e));
-      }
-  }
-  if ((threadIdx.x & 7) == 0 && here > 0) {
-    tab.ms[t][at] = (uint8_t)ms;
-    tab.vs[t][at] = (uint8_t)vs;
-  }
+  for (int u = 0; u < kUnits; ++u)
+    update(f[u], h, s, (uint32_t)((first + u * (kThreads * 4)) >> 1));
 }
 
 uint32_t host_mix(uint32_t h) {

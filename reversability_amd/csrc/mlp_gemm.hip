@@ -961,10 +961,10 @@ RV_WGRAD_KERNELS(0) RV_WGRAD_KERNELS(1) RV_WGRAD_KERNELS(2) RV_WGRAD_KERNELS(3)
 static_assert(kNumShapes == 7 && kRuleShapes == 4, "instantiations above");
 
 // The tied head's log-probabilities, both operand types: the tile shapes that
-// head_logits_shape, head_dx_shape and plan_wgrad choose from.
+// logp_z_shape, logp_dx_plan and plan_wgrad choose from.
 #define RV_LOGP_KERNELS(BF)                                                                    \
   RV_LOGP_Z(1, BF) RV_LOGP_Z(2, BF) RV_LOGP_Z(3, BF) RV_LOGP_Z(4, BF)                          \
-  RV_LOGP_DX(0, BF) RV_LOGP_DX(1, BF) RV_LOGP_DX(2, BF) RV_LOGP_DX(3, BF) RV_LOGP_DX(5, BF)    \
+  RV_LOGP_DX(0, BF) RV_LOGP_DX(2, BF) RV_LOGP_DX(3, BF)                                        \
   RV_LOGP_DW(0, BF) RV_LOGP_DW(1, BF) RV_LOGP_DW(2, BF) RV_LOGP_DW(3, BF)
 #define RV_LOGP_Z(SHAPE, BF)                                                                \
   template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProb, BF>(GemmArgs);     \
@@ -1122,7 +1122,7 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 // exp(m_t - M), logp = z_label - lse; 0 for an ignored label, NaN for one outside the
 // vocabulary.  A workgroup owns R rows, 256 / R threads each, which take the tiles in
 // turn, four loads at a time, and meet by lane swaps and in LDS in a fixed order (51
-// rows of 197 tiles: 9.6 us with one join after the other, see the launch).
+// rows of 393 tiles 3.9 us; a thread that joins the slices one by one 9.6 at 197).
 template <int R>
 __global__ __launch_bounds__(256)
 void logprob_rows(const float2* __restrict__ part, const float* __restrict__ label_logit,
@@ -1784,22 +1784,21 @@ int launch_logp(int shape, GemmArgs a, hipStream_t s) {
   const dim3 grid((unsigned)blocks), block(t.waves * 64);
 #define RV_LAUNCH(SHAPE) \
   hipLaunchKernelGGL((gemm_kernel<SHAPE, A_RC, B_RC, EPI, BF>), grid, block, 0, s, a)
-  constexpr bool kZ = EPI == Epi::LogProb || EPI == Epi::LogProbGrad;
+  constexpr bool kZ = !B_RC, kDx = !A_RC && B_RC;  // the logits, dx; else dw
   switch (shape) {
-    case 1: RV_LAUNCH(1); break;
-    case 2: RV_LAUNCH(2); break;
-    case 3: RV_LAUNCH(3); break;
     case 0:
       if constexpr (kZ) return RV_ERR_UNSUPPORTED;
       else RV_LAUNCH(0);
       break;
+    case 1:
+      if constexpr (kDx) return RV_ERR_UNSUPPORTED;
+      else RV_LAUNCH(1);
+      break;
+    case 2: RV_LAUNCH(2); break;
+    case 3: RV_LAUNCH(3); break;
     case 4:
       if constexpr (!kZ) return RV_ERR_UNSUPPORTED;
       else RV_LAUNCH(4);
-      break;
-    case 5:
-      if constexpr (kZ || A_RC) return RV_ERR_UNSUPPORTED;
-      else RV_LAUNCH(5);
       break;
     default: return RV_ERR_UNSUPPORTED;
   }
@@ -1844,8 +1843,59 @@ GemmArgs logp_args(const void* x, const void* head, int64_t rows, int64_t d, int
   return a;
 }
 
+// Their tile shape above the widths that are streamed: head_logits_shape's, but 2 and 3
+// wherever the 256 x 256 tiles fill less than one and a half rounds (us, shapes 2 / 3 / 4:
+// 51 x 512 over 50257 31.4 / 29.9 / 34.1, 700 x 640 over 10000 25.0 / 32.8 / 30.8, 300 x 1024
+// over 50257 75.0 / 85.5 / 75.5): nothing is stored, so the XCDs' shares matter less.
 int logp_z_shape(int64_t rows, int64_t d, int64_t padded) {
-  return head_logits_shape(rows, d, padded);
+  const int64_t wide = (rows + 255) / 256 * ((padded + 255) / 256);
+  if (wide >= 3 * kCUs / 2) return head_logits_shape(rows, d, padded);
+  return rows <= 64 || (rows + 127) / 128 * ((padded + 127) / 128) < kCUs ? 3 : 2;
+}
+
+// Tile shape and splits of their input gradient (rows x d reduced over the padded
+// vocabulary), by the time they are expected to take.  A workgroup takes `start` us
+// and `stage` us per 64 of its reduction alone on its CU, `full` with two there; a
+// split one's partial sums 8 bytes each at 5 TB/s and 4.5 us.  The constants are fitted
+// to 1,100 timings at 37 sizes (64 .. 20000 rows, widths 64 .. 1024, vocabularies
+// 1000 .. 50257, all shapes, 1 .. 64 splits, operands evicted): the plan it picks takes
+// 1.5% more than the best one measured on average (18% at worst), where head_dx_shape's
+// lines and head_chunk took 17% more (74%); 1554 x 512 over 32000 167 -> 95 us.
+struct DxPlan {
+  int shape;
+  int64_t chunk, splits;
+};
+DxPlan logp_dx_plan(int64_t rows, int64_t d, int64_t k) {
+  static const struct {
+    int shape;
+    double stage, full, start;
+  } fit[] = {{0, 1.58, 1.58, 6.2}, {2, 0.98, 1.35, 2.2}, {3, 0.55, 1.01, 1.6}};
+  static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  DxPlan best{0, k, 1};
+  double least = 0;
+  for (const auto& f : fit) {
+    const TileShape t = kShapes[f.shape];
+    const int64_t tiles = (rows + t.bm - 1) / t.bm * ((d + t.bn - 1) / t.bn);
+    const int64_t places = (int64_t)kCUs * t.per_cu;
+    for (const int want : splits) {
+      if (want > 1 && k / want < 4 * kSplitStep) break;
+      const int64_t chunk = ((k + want - 1) / want + kSplitStep - 1) / kSplitStep * kSplitStep;
+      const int64_t n = (k + chunk - 1) / chunk, rest = tiles * n % places;
+      const double stages = (double)chunk / kSplitStep;
+      double us = (double)(tiles * n / places) * (stages * f.full + f.start);
+      if (rest > 0) us += stages * (rest <= kCUs ? f.stage : f.full) + f.start;
+      if (n > 1) us += 4.5 + 8.0 * n * rows * d / 5e6;
+      if (least == 0 || us < least) {
+        best = DxPlan{f.shape, chunk, n};
+        least = us;
+      }
+    }
+  }
+  return best;
+}
+int64_t logp_dx_bytes(int64_t rows, int64_t d, int64_t k) {
+  const DxPlan p = logp_dx_plan(rows, d, k);
+  return p.splits > 1 ? p.splits * rows * d * (int64_t)sizeof(float) : 0;
 }
 
 // The streamed logits of narrow models (head_stream_k): stages of 64 columns per
@@ -2270,7 +2320,7 @@ int64_t rv_head_logp_grad_workspace_bytes(int64_t rows, int64_t d, int64_t vocab
   if (bad) return -(int64_t)bad;
   const WgradPlan p = plan_wgrad(rows, vocab, up128(d), true);
   if (p.shape < 0) return -(int64_t)RV_ERR_UNSUPPORTED;
-  const int64_t dx = head_dx_bytes(rows, up128(d), padded), dw = part_bytes(p, vocab, up128(d));
+  const int64_t dx = logp_dx_bytes(rows, d, padded), dw = part_bytes(p, vocab, up128(d));
   return dx > dw ? dx : dw;
 }
 
@@ -2285,18 +2335,18 @@ int rv_head_logp_dx(const void* dlogits, const void* head, int64_t rows, int64_t
   a.a = static_cast<const __half*>(dlogits); a.lda = padded; a.a_bytes = rows * padded * 2;
   a.b = static_cast<const __half*>(head); a.ldb = d;  // B(d, v) = head[v][d]: RC
   a.b_bytes = vocab * d * 2;  // the operand ends here: the pad rows read as zero
-  a.m = rows; a.n = d; a.k = padded; a.k_chunk = head_chunk(rows, up128(d), padded);
+  const DxPlan p = logp_dx_plan(rows, d, padded);
+  a.m = rows; a.n = d; a.k = padded; a.k_chunk = p.chunk;
   a.ldc = d; a.head.scale = scale;
   const hipStream_t s = (hipStream_t)stream;
-  const int64_t splits = (padded + a.k_chunk - 1) / a.k_chunk;
-  const int shape = head_dx_shape(rows, up128(d), padded);
+  const int64_t splits = p.splits;
+  const int shape = p.shape;
   if (splits == 1) {
     a.c = dx;
     return dtype == RV_BF16 ? launch_logp<false, true, Epi::StoreScaled, true>(shape, a, s)
                             : launch_logp<false, true, Epi::StoreScaled, false>(shape, a, s);
   }
-  if (!workspace || workspace_bytes < splits * rows * d * (int64_t)sizeof(float) ||
-      !ok16(workspace))
+  if (!workspace || workspace_bytes < logp_dx_bytes(rows, d, padded) || !ok16(workspace))
     return RV_ERR_WORKSPACE;
   a.c = workspace;
   const int st = dtype == RV_BF16 ? launch_logp<false, true, Epi::PartialRagged, true>(shape, a, s)

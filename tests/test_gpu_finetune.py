@@ -103,6 +103,7 @@ def test_preference_update_matches_plain_torch(cuda_device, method, wired, preci
     margin = s[:3] - s[3:]
     loss = -(0.9 * F.logsigmoid(margin) + 0.1 * F.logsigmoid(-margin)).mean()
     (loss * 256).backward()
+    loss = loss.detach()
     assert abs(float(out.loss - loss)) <= 2e-3 * scale * (1 + float(loss))
     assert rel(torch.cat([out.chosen, out.rejected]), s.detach()) <= 2e-2 * scale
     compare(model, plain, 2e-2 * scale)
@@ -133,7 +134,9 @@ def test_policy_update_matches_plain_torch(cuda_device, method, wired, reduction
     else:
         loss = (term.sum(1) / mask.sum(1).clamp_min(1)).mean()
     loss.backward()
+    loss = loss.detach()
     assert abs(float(out.loss - loss)) <= 2e-3 * (1 + abs(float(loss)))
+    r = r.detach()
     clipped = ((a > 0) & (r > 1.3) | (a < 0) & (r < 0.8)) & mask
     assert abs(float(out.clipped) - float(clipped.sum() / mask.sum())) <= 1e-6
     compare(model, plain, 2e-2)
