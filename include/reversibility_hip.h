@@ -369,31 +369,21 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
                      int dtype, const int64_t* labels, int64_t ignore_index, float* logp,
                      float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Its backward for the gradient grad[rows] of logp, in three steps over a chunk
- * of rows that share a scale (scale[0] a power of two that brings the largest
- * |grad| of a row with a label to [2^14, 2^15), scale[1] its inverse):
- *   scale    scale[0], scale[1] from grad
- *   dlogits  dlogits[rows, padded] of dtype: scale[0] grad[r] ([j == labels[r]] -
- *            exp(z[r, j] - lse[r])), computed from x and head again; columns from
- *            vocab on zero; ignored rows zero (their grad is not read), a row of
- *            another label outside [0, vocab) NaN
- *   dx       dx[rows, d] of dtype = scale[1] dlogits head
- *   dw       dw[vocab, d] = scale[1] dlogits^T x, of dtype, or fp32 (added to dw
- *            with accumulate)
- * padded, a multiple of 64, is the row count of head. */
-int rv_head_logp_scale(const float* grad, const int64_t* labels, int64_t rows,
-                       int64_t ignore_index, float* scale, void* stream);
-int rv_head_logp_dlogits(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
-                         int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,
-                         const float* lse, const float* grad, const float* scale, void* dlogits,
-                         void* stream);
-int64_t rv_head_logp_grad_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded);
-int rv_head_logp_dx(const void* dlogits, const void* head, int64_t rows, int64_t d, int64_t vocab,
-                    int64_t padded, int dtype, const float* scale, void* dx, void* workspace,
-                    int64_t workspace_bytes, void* stream);
-int rv_head_logp_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int64_t vocab,
-                    int64_t padded, int dtype, const float* scale, void* dw, int dw_dtype,
-                    int accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+/* Its backward for the gradient grad[rows] of logp: with the logits' gradient
+ * dz[r, j] = grad[r] ([j == labels[r]] - exp(z[r, j] - lse[r])), z computed again,
+ *   dx[rows, d] = dz head         of dtype
+ *   dw[dw_rows, d] = dz^T x       of dtype, or fp32 (added to dw with accumulate)
+ * either may be NULL.  Ignored rows have none (their grad is not read), a row of
+ * another label outside [0, vocab) NaN.  padded, a multiple of 64, is the row count
+ * of head; dw_rows is vocab or padded (pad rows: sums of zeros).  dz is held in dtype
+ * in the workspace, times a power of two that brings the largest |grad| of a row
+ * with a label to [2^14, 2^15).  rows <= 2^22. */
+int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded);
+int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                     int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,
+                     const float* lse, const float* grad, void* dx, void* dw, int64_t dw_rows,
+                     int dw_dtype, int accumulate, void* workspace, int64_t workspace_bytes,
+                     void* stream);
 
 /* Two layers' weight gradients over the same rows in one launch: dw_a[out_a,
  * in_a] (+)= fp32(fp16(dy_a^T x_a)) and dw_b likewise (x_a, x_b contiguous). */

@@ -66,12 +66,9 @@ SIGNATURES = {
     "rv_head_dw": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _I, _I, _P, _I64, _P]),
     "rv_head_logp_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "rv_head_logp_fwd": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _P, _I64, _P]),
-    "rv_head_logp_scale": (_I, [_P, _P, _I64, _I64, _P, _P]),
-    "rv_head_logp_dlogits": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _P, _P,
-                                  _P]),
-    "rv_head_logp_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
-    "rv_head_logp_dx": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
-    "rv_head_logp_dw": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _I, _I, _P, _I64, _P]),
+    "rv_head_logp_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "rv_head_logp_bwd": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _P, _P, _P, _I64,
+                              _I, _I, _P, _I64, _P]),
     "rv_linear_dw_pair_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "rv_linear_dw_pair": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _I, _P, _I64,
                                _P]),

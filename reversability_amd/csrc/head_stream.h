@@ -24,7 +24,7 @@ struct StreamArgs {
   int64_t stages, chunk;  // stages of 64 columns in all, and per workgroup
   int64_t tiles_m, tiles; // workgroups: 256 rows x chunk stages, tiles_m fastest
   float2* part;           // forward: [tile column][m]
-  __half* out;            // backward: [m][n]
+  __half* out;            // backward: panels [n / 64][m][64]
   HeadLogp head_logp;
 };
 
@@ -122,12 +122,11 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
       ref[i] = top[i] * kLog2e;
     }
   }
-  // backward: rows past the end are past the resource
-  const int64_t rows_here = a.m - m0 < 64 ? (a.m - m0 < 0 ? 0 : a.m - m0) : 64;
-  const auto out_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      reinterpret_cast<char*>(uniform(reinterpret_cast<int64_t>(a.out + (GRAD ? m0 * a.n : 0)))), 0,
-      GRAD ? (int)uniform(rows_here * a.n * 2) : 0, kRsrcWord3);
-  const uint32_t out_off = (uint32_t)((lane & 15) * a.n * 2 + (lane >> 4 & 1) * 32 + (lane >> 5) * 16);
+  // backward: the wave's 64 rows of a panel (64 columns: a stage); rows past the end are
+  // past the resource
+  const int rows_here = (int)uniform(a.m - m0 < 64 ? (a.m - m0 < 0 ? 0 : a.m - m0) : 64);
+  const int64_t out0 = uniform(reinterpret_cast<int64_t>(a.out) + (first * a.m + m0) * 128);
+  const uint32_t out_off = (uint32_t)((lane & 15) * 128 + (lane >> 4 & 1) * 32 + (lane >> 5) * 16);
 
   const uint32_t lds0 = (uint32_t)(size_t)(RV_LDS void*)lds;
   const uint32_t at = (lane & 31) * kRow + (((lane >> 5) ^ (lane & 15)) << 4);
@@ -212,11 +211,12 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
         const u32x4 v = {w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]};
         // all of the offset in the vector register: with a scalar part the compiler
         // leaves no wait state between a 16-byte store and the next write of its data
-        // registers, and lanes 12 .. 15 of each 16 stored what came after
+        // registers, and lanes 12 .. 15 of each 16 stored what came after.  Streaming.
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            reinterpret_cast<char*>(out0 + (int64_t)(col >> 6) * a.m * 128), 0, rows_here * 128,
+            kRsrcWord3);
         __builtin_amdgcn_raw_buffer_store_b128(
-            v, out_rsrc,
-            (int)(out_off + (uint32_t)((i * 32 + r * 16) * a.n * 2) + (uint32_t)((col0 + col) * 2)),
-            0, 2);  // streaming (nt)
+            v, rsrc, (int)(out_off + (uint32_t)((i * 32 + r * 16) * 128 + (col & 63) * 2)), 0, 2);
       }
     }
   };

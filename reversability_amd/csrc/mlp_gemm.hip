@@ -212,6 +212,41 @@ struct Dma {
       off[it] = (uint32_t)((krow * ld + chunk * 8) * 2);
     }
   }
+  // Panels (the tied head's logit gradients): [columns / 64][rows][64], so that what a
+  // workgroup writes or reads of 64 columns is contiguous.  `panel` elements each.
+  // As a KC source (k = the columns, BK = 64) a stage is one panel.
+  template <class Map>
+  __device__ __forceinline__ void init_kc_panel(const __half* p, int64_t bytes, int64_t panel,
+                                                const Map& map, int64_t kbeg, int wave, int lane) {
+    static_assert(RC || BK == 64, "a stage is a panel");
+    const int64_t first = map.origin() * 64 + kbeg / 64 * panel;
+    base = uniform(reinterpret_cast<int64_t>(p + first));
+    left = uniform(bytes - first * 2);
+    kstep = panel * 2;
+#pragma unroll
+    for (int it = 0; it < kPerWave; ++it) {
+      const int row = (it * WAVES + wave) * kRows + lane / kChunks;
+      off[it] = (uint32_t)((map(row) * 64 + ((lane % kChunks) ^ f_kc<BK>(row)) * 8) * 2);
+    }
+  }
+  // As an RC source (k = the rows): a tile's columns row0 .. are ROWS / 64 panels of
+  // `panels`.  Rows past the end read the next panel (the other operand's are zero).
+  __device__ __forceinline__ void init_rc_panel(const __half* p, int64_t bytes, int64_t panel,
+                                                int64_t panels, int64_t row0, int64_t kbeg,
+                                                int wave, int lane) {
+    const int64_t first = row0 / 64 * panel + kbeg * 64;
+    base = uniform(reinterpret_cast<int64_t>(p + first));
+    left = uniform(bytes - first * 2);
+    kstep = BK * 64 * 2;
+#pragma unroll
+    for (int it = 0; it < kPerWave; ++it) {
+      const int b = (it * WAVES + wave) * 1024 + lane * 16;
+      const int krow = b / (ROWS * 2), chunk = ((b % (ROWS * 2)) >> 4) ^ f_rc<ROWS>(krow);
+      off[it] = row0 / 64 + chunk / 8 < panels
+                    ? (uint32_t)((chunk / 8 * panel + krow * 64 + chunk % 8 * 8) * 2)
+                    : 0x80000000u;  // past the columns: zeros
+    }
+  }
   // A KC row's last stage holds `valid` < BK values of the reduction: chunks
   // at or past it are sent out of the resource's range and read as zero (stage()
   // gives it at most INT32_MAX bytes, whatever the operand's size).
@@ -319,10 +354,10 @@ enum class Epi {
   PartialF32,     // c fp32 partial [split][m][n] = acc
   // the tied head's log-probabilities (HeadLogp):
   LogProb,        // c = float2 [tile column][m]: a row's maximum and sum of exp over the tile
-  LogProbGrad,    // c 16-bit [m][n] = scaled gradient of the logits
-  StoreScaled,    // c 16-bit = acc * *scale
-  AccF32Scaled,   // c fp32 (+)= acc * *scale
-  PartialRagged,  // PartialF32 whose tiles may pass column n
+  LogProbGrad,    // c 16-bit, panels = scaled gradient of the logits
+  StoreScaled,    // c 16-bit = acc * *scale, a in panels
+  AccF32Scaled,   // c fp32 (+)= acc * *scale, a in panels
+  PartialRagged,  // PartialF32 whose tiles may pass column n, a in panels
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -365,6 +400,7 @@ struct GemmArgs {
   int accumulate;          // AccF32OfF16
   int64_t group = 8;       // M tiles per group of the tile order (tile_of)
   int64_t valid;           // StoreF16: columns valid .. n - 1 are written as zero (0: none)
+  int64_t panel, panels;   // the logits' gradients (LogProbGrad's c, the Scaled products' a)
   HeadLogp head;
 };
 
@@ -428,7 +464,13 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
 
   Dma<A_RC, BM, BK, WAVES> da;
   Dma<B_RC, BN, BK, WAVES> db;
-  if constexpr (A_RC) da.init_rc(args.a, args.a_bytes, args.lda, m0, kbeg, wave, lane);
+  constexpr bool kPanels =
+      EPI == Epi::StoreScaled || EPI == Epi::AccF32Scaled || EPI == Epi::PartialRagged;
+  if constexpr (kPanels && A_RC)
+    da.init_rc_panel(args.a, args.a_bytes, args.panel, args.panels, m0, kbeg, wave, lane);
+  else if constexpr (kPanels)
+    da.init_kc_panel(args.a, args.a_bytes, args.panel, MapDirect{m0, args.m}, kbeg, wave, lane);
+  else if constexpr (A_RC) da.init_rc(args.a, args.a_bytes, args.lda, m0, kbeg, wave, lane);
   else da.init_kc(args.a, args.a_bytes, args.lda, MapDirect{m0, args.m}, kbeg, wave, lane);
   if constexpr (B_RC) db.init_rc(args.b, args.b_bytes, args.ldb, n0, kbeg, wave, lane);
   else if constexpr (EPI == Epi::SwiGLU)
@@ -851,7 +893,9 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
             if (col + e >= args.valid)
               dw[e >> 1] = (e & 1) ? dw[e >> 1] & 0xffffu : dw[e >> 1] & 0xffff0000u;
         }
-        __builtin_nontemporal_store(dw, reinterpret_cast<u32x4*>(static_cast<__half*>(args.c) + row * args.ldc + col));
+        const int64_t to = EPI == Epi::LogProbGrad ? col / 64 * args.panel + row * 64 + col % 64
+                                                   : row * args.ldc + col;
+        __builtin_nontemporal_store(dw, reinterpret_cast<u32x4*>(static_cast<__half*>(args.c) + to));
       }
     } else {
       // SwiGLUBwd: du from u = [gate | value] and d_o = fp16(acc).  The u
@@ -1162,15 +1206,20 @@ void logprob_rows(const float2* __restrict__ part, const float* __restrict__ lab
 // The power of two that brings the largest gradient of a row that counts to
 // [2^14, 2^15), and its inverse: the gradients of the logits are held in 16 bits,
 // where fp16 has no room for small ones (p g < 2^-24), and no logit's exceeds
-// its row's.  1 where none is finite and nonzero.  One workgroup.
+// its row's.  1 where none is finite and nonzero.  One workgroup over the rows (labels
+// given), or over what several such left in `tops` (FINISH).
+constexpr int kScaleTops = 256;           // workgroups of the first pass over many rows
+constexpr int64_t kScaleRows = 1 << 14;   // rows that one workgroup takes alone
+template <bool FINISH>
 __global__ __launch_bounds__(1024)
 void logprob_scale(const float* __restrict__ grad, const int64_t* __restrict__ labels,
-                   int64_t rows, int64_t ignore, float* __restrict__ scale) {
+                   int64_t rows, int64_t ignore, float* __restrict__ tops,
+                   float* __restrict__ scale) {
   float top = 0.f;
 #pragma unroll 4
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+  for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows; r += gridDim.x * 1024) {
     const float g = fabsf(grad[r]);
-    if (labels[r] != ignore && g < INFINITY) top = fmaxf(top, g);
+    if ((labels == nullptr || labels[r] != ignore) && g < INFINITY) top = fmaxf(top, g);
   }
   for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   __shared__ float red[16];
@@ -1178,10 +1227,14 @@ void logprob_scale(const float* __restrict__ grad, const int64_t* __restrict__ l
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w]);
-  int e = top > 0.f ? 14 - ilogbf(top) : 0;
-  e = e > 100 ? 100 : e < -100 ? -100 : e;  // both factors normal numbers
-  scale[0] = ldexpf(1.f, e);
-  scale[1] = ldexpf(1.f, -e);
+  if constexpr (!FINISH) {
+    tops[blockIdx.x] = top;
+  } else {
+    int e = top > 0.f ? 14 - ilogbf(top) : 0;
+    e = e > 100 ? 100 : e < -100 ? -100 : e;  // both factors normal numbers
+    scale[0] = ldexpf(1.f, e);
+    scale[1] = ldexpf(1.f, -e);
+  }
 }
 
 // dst = fp16(src), round to nearest even; 8 elements per thread.
@@ -2286,108 +2339,106 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
   return rv_host::check_launch();
 }
 
-int rv_head_logp_scale(const float* grad, const int64_t* labels, int64_t rows,
-                       int64_t ignore_index, float* scale, void* stream) {
-  if (!grad || !labels || !scale) return RV_ERR_NULL_POINTER;
-  if (rows <= 0) return RV_ERR_BAD_SIZE;
-  hipLaunchKernelGGL(logprob_scale, dim3(1), dim3(1024), 0, (hipStream_t)stream, grad, labels,
-                     rows, ignore_index, scale);
-  return rv_host::check_launch();
-}
+// The backward's workspace starts with the scale, its inverse and the rows' tops.
+constexpr int64_t kLogpHeader = 256 + kScaleTops * sizeof(float);
 
-int rv_head_logp_dlogits(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
-                         int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,
-                         const float* lse, const float* grad, const float* scale, void* dlogits,
-                         void* stream) {
-  if (!x || !head || !labels || !lse || !grad || !scale || !dlogits) return RV_ERR_NULL_POINTER;
-  const int bad = logp_check(rows, d, vocab, padded, dtype);
-  if (bad) return bad;
-  if (!ok16(x) || !ok16(head) || !ok16(dlogits)) return RV_ERR_UNSUPPORTED;
-  GemmArgs a = logp_args(x, head, rows, d, padded, labels, ignore_index, vocab);
-  a.c = dlogits; a.ldc = padded; a.valid = vocab;
-  a.head.lse = lse; a.head.grad = grad; a.head.scale = scale;
-  const int shape = logp_z_shape(rows, d, padded);
-  const hipStream_t s = (hipStream_t)stream;
-  if (stream_takes(d))
-    return launch_stream<true>({a.a, a.b, rows, padded, d, 0, 0, 0, 0, nullptr,
-                                static_cast<__half*>(dlogits), a.head}, dtype, s);
-  return dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProbGrad, true>(shape, a, s)
-                          : launch_logp<false, false, Epi::LogProbGrad, false>(shape, a, s);
-}
-
-int64_t rv_head_logp_grad_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded) {
+int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded) {
   const int bad = logp_check(rows, d, vocab, padded, RV_F16);
   if (bad) return -(int64_t)bad;
-  const WgradPlan p = plan_wgrad(rows, vocab, up128(d), true);
+  // a tile's panels stay within 32-bit offsets
+  if (rows > (int64_t)1 << 22) return -(int64_t)RV_ERR_UNSUPPORTED;
+  const WgradPlan p = plan_wgrad(rows, padded, up128(d), true);
   if (p.shape < 0) return -(int64_t)RV_ERR_UNSUPPORTED;
-  const int64_t dx = logp_dx_bytes(rows, d, padded), dw = part_bytes(p, vocab, up128(d));
-  return dx > dw ? dx : dw;
+  const int64_t dx = logp_dx_bytes(rows, d, padded), dw = part_bytes(p, padded, up128(d));
+  return kLogpHeader + align256(rows * padded * 2) + (dx > dw ? dx : dw);
 }
 
-int rv_head_logp_dx(const void* dlogits, const void* head, int64_t rows, int64_t d, int64_t vocab,
-                    int64_t padded, int dtype, const float* scale, void* dx, void* workspace,
-                    int64_t workspace_bytes, void* stream) {
-  if (!dlogits || !head || !scale || !dx) return RV_ERR_NULL_POINTER;
+int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
+                     int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,
+                     const float* lse, const float* grad, void* dx, void* dw, int64_t dw_rows,
+                     int dw_dtype, int accumulate, void* workspace, int64_t workspace_bytes,
+                     void* stream) {
+  if (!x || !head || !labels || !lse || !grad) return RV_ERR_NULL_POINTER;
   const int bad = logp_check(rows, d, vocab, padded, dtype);
   if (bad) return bad;
-  if (!ok16(dlogits) || !ok16(head) || !ok16(dx)) return RV_ERR_UNSUPPORTED;
-  GemmArgs a{};
-  a.a = static_cast<const __half*>(dlogits); a.lda = padded; a.a_bytes = rows * padded * 2;
-  a.b = static_cast<const __half*>(head); a.ldb = d;  // B(d, v) = head[v][d]: RC
-  a.b_bytes = vocab * d * 2;  // the operand ends here: the pad rows read as zero
-  const DxPlan p = logp_dx_plan(rows, d, padded);
-  a.m = rows; a.n = d; a.k = padded; a.k_chunk = p.chunk;
-  a.ldc = d; a.head.scale = scale;
+  if (!ok16(x) || !ok16(head) || (dx && !ok16(dx)) || (dw && !ok16(dw))) return RV_ERR_UNSUPPORTED;
+  if (dw && dw_dtype != RV_F32 && (dw_dtype != dtype || accumulate)) return RV_ERR_UNSUPPORTED;
+  if (dw && dw_rows != vocab && dw_rows != padded) return RV_ERR_BAD_SIZE;
+  const int64_t need = rv_head_logp_bwd_workspace_bytes(rows, d, vocab, padded);
+  if (need < 0) return (int)-need;
+  if (!workspace || workspace_bytes < need || !ok16(workspace)) return RV_ERR_WORKSPACE;
   const hipStream_t s = (hipStream_t)stream;
-  const int64_t splits = p.splits;
-  const int shape = p.shape;
-  if (splits == 1) {
-    a.c = dx;
-    return dtype == RV_BF16 ? launch_logp<false, true, Epi::StoreScaled, true>(shape, a, s)
-                            : launch_logp<false, true, Epi::StoreScaled, false>(shape, a, s);
+  const bool bf = dtype == RV_BF16;
+  // workspace: the scale and its inverse, the logits' gradients in panels, the
+  // products' partial sums
+  float* scale = static_cast<float*>(workspace);
+  float* tops = scale + 64;
+  __half* dlogits = reinterpret_cast<__half*>(static_cast<char*>(workspace) + kLogpHeader);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kLogpHeader +
+                                         align256(rows * padded * 2));
+  if (rows <= kScaleRows) {
+    hipLaunchKernelGGL(logprob_scale<true>, dim3(1), dim3(1024), 0, s, grad, labels, rows,
+                       ignore_index, tops, scale);
+  } else {
+    const int wgs = (int)std::min<int64_t>(kScaleTops, (rows + 4095) / 4096);
+    hipLaunchKernelGGL(logprob_scale<false>, dim3(wgs), dim3(1024), 0, s, grad, labels, rows,
+                       ignore_index, tops, scale);
+    hipLaunchKernelGGL(logprob_scale<true>, dim3(1), dim3(1024), 0, s, tops,
+                       (const int64_t*)nullptr, (int64_t)wgs, ignore_index, tops, scale);
   }
-  if (!workspace || workspace_bytes < logp_dx_bytes(rows, d, padded) || !ok16(workspace))
-    return RV_ERR_WORKSPACE;
-  a.c = workspace;
-  const int st = dtype == RV_BF16 ? launch_logp<false, true, Epi::PartialRagged, true>(shape, a, s)
-                                  : launch_logp<false, true, Epi::PartialRagged, false>(shape, a, s);
-  if (st != RV_OK) return st;
-  return launch_scaled_reduce(dtype, static_cast<const float*>(workspace), dx, rows * d, splits,
-                              scale, 0, s);
-}
-
-int rv_head_logp_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int64_t vocab,
-                    int64_t padded, int dtype, const float* scale, void* dw, int dw_dtype,
-                    int accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (!dlogits || !x || !scale || !dw) return RV_ERR_NULL_POINTER;
-  const int bad = logp_check(rows, d, vocab, padded, dtype);
-  if (bad) return bad;
-  if (dw_dtype != RV_F32 && (dw_dtype != dtype || accumulate)) return RV_ERR_UNSUPPORTED;
-  if (!ok16(dlogits) || !ok16(x) || !ok16(dw)) return RV_ERR_UNSUPPORTED;
-  const WgradPlan p = plan_wgrad(rows, vocab, up128(d), true);
-  if (p.shape < 0) return RV_ERR_UNSUPPORTED;
-  if (p.splits > 1 &&
-      (!workspace || workspace_bytes < part_bytes(p, vocab, up128(d)) || !ok16(workspace)))
-    return RV_ERR_WORKSPACE;
-  // dW[v][d] = sum_m dlogits[m][v] x[m][d]; rows from vocab on are not written
-  WgradJob j = plan_job(p, static_cast<const __half*>(dlogits), padded,
-                        static_cast<const __half*>(x), d, rows, vocab, d, static_cast<float*>(dw),
-                        accumulate, static_cast<float*>(workspace));
-  j.g.head.scale = scale;
-  const hipStream_t s = (hipStream_t)stream;
-  if (p.splits == 1) {
-    if (dw_dtype == RV_F32)
-      return dtype == RV_BF16 ? launch_logp<true, true, Epi::AccF32Scaled, true>(p.shape, j.g, s)
-                              : launch_logp<true, true, Epi::AccF32Scaled, false>(p.shape, j.g, s);
-    return dtype == RV_BF16 ? launch_logp<true, true, Epi::StoreScaled, true>(p.shape, j.g, s)
-                            : launch_logp<true, true, Epi::StoreScaled, false>(p.shape, j.g, s);
+  GemmArgs z = logp_args(x, head, rows, d, padded, labels, ignore_index, vocab);
+  z.c = dlogits; z.valid = vocab; z.panel = rows * 64; z.panels = padded / 64;
+  z.head.lse = lse; z.head.grad = grad; z.head.scale = scale;
+  int st;
+  if (stream_takes(d)) {
+    st = launch_stream<true>({z.a, z.b, rows, padded, d, 0, 0, 0, 0, nullptr, dlogits, z.head},
+                             dtype, s);
+  } else {
+    const int shape = logp_z_shape(rows, d, padded);
+    st = bf ? launch_logp<false, false, Epi::LogProbGrad, true>(shape, z, s)
+            : launch_logp<false, false, Epi::LogProbGrad, false>(shape, z, s);
   }
-  const int st = dtype == RV_BF16
-                     ? launch_logp<true, true, Epi::PartialRagged, true>(p.shape, j.g, s)
-                     : launch_logp<true, true, Epi::PartialRagged, false>(p.shape, j.g, s);
   if (st != RV_OK) return st;
-  return launch_scaled_reduce(dw_dtype, static_cast<const float*>(workspace), dw, vocab * d,
-                              p.splits, scale, accumulate, s);
+  if (dx) {
+    const DxPlan p = logp_dx_plan(rows, d, padded);
+    GemmArgs a{};
+    a.a = dlogits; a.a_bytes = rows * padded * 2; a.panel = z.panel; a.panels = z.panels;
+    a.b = static_cast<const __half*>(head); a.ldb = d;  // B(d, v) = head[v][d]: RC
+    a.b_bytes = vocab * d * 2;  // the operand ends here: the pad rows read as zero
+    a.m = rows; a.n = d; a.k = padded; a.k_chunk = p.chunk;
+    a.ldc = d; a.head.scale = scale + 1;
+    if (p.splits == 1) {
+      a.c = dx;
+      st = bf ? launch_logp<false, true, Epi::StoreScaled, true>(p.shape, a, s)
+              : launch_logp<false, true, Epi::StoreScaled, false>(p.shape, a, s);
+    } else {
+      a.c = part;
+      st = bf ? launch_logp<false, true, Epi::PartialRagged, true>(p.shape, a, s)
+              : launch_logp<false, true, Epi::PartialRagged, false>(p.shape, a, s);
+      if (st == RV_OK)
+        st = launch_scaled_reduce(dtype, part, dx, rows * d, p.splits, scale + 1, 0, s);
+    }
+    if (st != RV_OK) return st;
+  }
+  if (dw) {
+    // dW[v][d] = sum_m dlogits[m][v] x[m][d]; of the pad rows the sum of zeros
+    const WgradPlan p = plan_wgrad(rows, padded, up128(d), true);
+    WgradJob j = plan_job(p, dlogits, padded, static_cast<const __half*>(x), d, rows, dw_rows, d,
+                          static_cast<float*>(dw), accumulate, part);
+    j.g.panel = z.panel; j.g.panels = z.panels; j.g.head.scale = scale + 1;
+    if (p.splits == 1) {
+      if (dw_dtype == RV_F32)
+        return bf ? launch_logp<true, true, Epi::AccF32Scaled, true>(p.shape, j.g, s)
+                  : launch_logp<true, true, Epi::AccF32Scaled, false>(p.shape, j.g, s);
+      return bf ? launch_logp<true, true, Epi::StoreScaled, true>(p.shape, j.g, s)
+                : launch_logp<true, true, Epi::StoreScaled, false>(p.shape, j.g, s);
+    }
+    st = bf ? launch_logp<true, true, Epi::PartialRagged, true>(p.shape, j.g, s)
+            : launch_logp<true, true, Epi::PartialRagged, false>(p.shape, j.g, s);
+    if (st == RV_OK)
+      st = launch_scaled_reduce(dw_dtype, part, dw, dw_rows * d, p.splits, scale + 1, accumulate, s);
+  }
+  return st;
 }
 
 int64_t rv_linear_dw_pair_workspace_bytes(int64_t rows, int64_t in_a, int64_t out_a, int64_t in_b,

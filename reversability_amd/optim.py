@@ -36,7 +36,7 @@ import ctypes
 import torch
 from torch.optim import Optimizer
 
-from ._hip import _check, _stream, library
+from ._hip import _check, _DeviceGuard, _stream, library
 
 
 class FusedAdamW(Optimizer):
@@ -156,15 +156,17 @@ class FusedAdamW(Optimizer):
             if not params:
                 continue
             dev = params[0].device
-            stream = _stream(params[0])
-            fi = found_inf.to(dev, torch.float32) if found_inf is not None else None
-            inv = (grad_scale.to(dev, torch.float64).reciprocal().to(torch.float32)
-                   if grad_scale is not None else pending_inv)
-            _check(lib.rv_adamw_advance(step.data_ptr(), fi.data_ptr() if fi is not None else None,
-                                        stream), "rv_adamw_advance")
-            device = (step.data_ptr(), *(t.data_ptr() if t is not None else None
-                                         for t in (fi, inv, clip)), stream)
-            self._update(lib, group, params, device)
+            with _DeviceGuard(params[0]):
+                stream = _stream(params[0])
+                fi = found_inf.to(dev, torch.float32) if found_inf is not None else None
+                inv = (grad_scale.to(dev, torch.float64).reciprocal().to(torch.float32)
+                       if grad_scale is not None else pending_inv)
+                _check(lib.rv_adamw_advance(step.data_ptr(),
+                                            fi.data_ptr() if fi is not None else None, stream),
+                       "rv_adamw_advance")
+                device = (step.data_ptr(), *(t.data_ptr() if t is not None else None
+                                             for t in (fi, inv, clip)), stream)
+                self._update(lib, group, params, device)
         return loss
 
     def _update(self, lib, group, params, device):
@@ -226,11 +228,18 @@ class FusedAdamW8bit(FusedAdamW):
         for group in self.param_groups:
             group.setdefault("seed", seed)
 
+    def _group_state(self, group):
+        # before anything of the step is launched
+        params = [p for p in group["params"] if p.grad is not None]
+        if any(p.device != params[0].device or not (p.is_contiguous() and p.grad.is_contiguous())
+               for p in params):
+            raise ValueError("FusedAdamW8bit requires contiguous parameters and gradients, a "
+                             "group's on one device")
+        return super()._group_state(group)
+
     def _new_moments(self, p):
         if p.numel() < self.min_8bit_numel:
             return super()._new_moments(p)
-        if not p.is_contiguous():
-            raise ValueError("FusedAdamW8bit requires contiguous parameters")
         blocks = -(-p.numel() // library().rv_adamw8_block())
         st = {}
         for name, scale in _SCALES.items():
@@ -250,9 +259,6 @@ class FusedAdamW8bit(FusedAdamW):
         for start in range(0, len(large), limit):
             chunk = large[start:start + limit]
             n = len(chunk)
-            for p in chunk:
-                if not (p.is_contiguous() and p.grad.is_contiguous()):
-                    raise ValueError("FusedAdamW8bit requires contiguous parameters and gradients")
             P = ctypes.c_void_p * n
             states = [self.state[p] for p in chunk]
             ptrs = [P(*[t.data_ptr() for t in ts]) for ts in (

@@ -86,45 +86,35 @@ def _logp_forward(x, head, vocab, labels):
 def _logp_backward(x, head, vocab, labels, lse, grad, dx=None, dw=None, accumulate=False,
                    chunk_tokens=None):
     """Gradients for ``grad`` (fp32 [rows]) into dx [rows, d] of x's type and dw
-    [>= vocab, d] of x's type or fp32 (added to it with ``accumulate``); either may
-    be None.  ``dw`` of x's type takes one chunk only.  All dense."""
+    [vocab or padded, d] of x's type or fp32 (added to it with ``accumulate``); either
+    may be None.  ``dw`` of x's type takes one chunk only.  All dense."""
     rows, d = x.shape
     padded = head.shape[0]
     lib, code = library(), _CODES[x.dtype]
     step = min(rows, chunk_tokens or max_chunk(padded))
-    size = x.element_size()
-    dlogits = torch.empty(step, padded, device=x.device, dtype=x.dtype)
-    scale = torch.empty(2, device=x.device, dtype=torch.float32)
-    inverse = scale.data_ptr() + 4
+    out = (None, vocab, code) if dw is None else (
+        dw.data_ptr(), dw.shape[0], RV_F32 if dw.dtype == torch.float32 else code)
     with _DeviceGuard(x):
-        st = _stream(x)
+        nbytes = lib.rv_head_logp_bwd_workspace_bytes(step, d, vocab, padded)
+        ws = _workspace(nbytes, x, "rv_head_logp_bwd_workspace_bytes")
         for at in range(0, rows, step):
             n = min(step, rows - at)
-            xp, lp = x.data_ptr() + at * d * size, labels.data_ptr() + at * 8
-            gp = grad.data_ptr() + at * 4
-            _check(lib.rv_head_logp_scale(gp, lp, n, IGNORE_INDEX, scale.data_ptr(), st),
-                   "rv_head_logp_scale")
-            _check(lib.rv_head_logp_dlogits(
-                xp, head.data_ptr(), n, d, vocab, padded, code, lp, IGNORE_INDEX,
-                lse.data_ptr() + at * 4, gp, scale.data_ptr(), dlogits.data_ptr(), st),
-                "rv_head_logp_dlogits")
-            nbytes = lib.rv_head_logp_grad_workspace_bytes(n, d, vocab, padded)
-            ws = _workspace(nbytes, x, "rv_head_logp_grad_workspace_bytes")
-            wp = ws.data_ptr() if ws is not None else None
-            if dx is not None:
-                _check(lib.rv_head_logp_dx(
-                    dlogits.data_ptr(), head.data_ptr(), n, d, vocab, padded, code, inverse,
-                    dx.data_ptr() + at * d * size, wp, nbytes, st), "rv_head_logp_dx")
-            if dw is not None:
-                _check(lib.rv_head_logp_dw(
-                    dlogits.data_ptr(), xp, n, d, vocab, padded, code, inverse, dw.data_ptr(),
-                    RV_F32 if dw.dtype == torch.float32 else code,
-                    int(accumulate or at > 0), wp, nbytes, st), "rv_head_logp_dw")
+            if n < step:  # a short last chunk has a plan of its own
+                nbytes = lib.rv_head_logp_bwd_workspace_bytes(n, d, vocab, padded)
+                if nbytes > ws.numel():
+                    ws = _workspace(nbytes, x, "rv_head_logp_bwd_workspace_bytes")
+            _check(lib.rv_head_logp_bwd(
+                x.data_ptr() + at * d * 2, head.data_ptr(), n, d, vocab, padded, code,
+                labels.data_ptr() + at * 8, IGNORE_INDEX, lse.data_ptr() + at * 4,
+                grad.data_ptr() + at * 4, dx.data_ptr() + at * d * 2 if dx is not None else None,
+                *out, accumulate or at > 0, ws.data_ptr(), ws.numel(), _stream(x)),
+                "rv_head_logp_bwd")
 
 
 def max_chunk(padded: int) -> int:
-    """Tokens whose 16-bit logit gradients over ``padded`` columns fill GRADIENT_BYTES."""
-    return max(256, GRADIENT_BYTES // (2 * padded) // 256 * 256)
+    """Tokens whose 16-bit logit gradients over ``padded`` columns fill GRADIENT_BYTES
+    (at most 2^22, what one call takes)."""
+    return min(1 << 22, max(256, GRADIENT_BYTES // (2 * padded) // 256 * 256))
 
 
 class TiedHeadLogProbs(torch.autograd.Function):
@@ -149,17 +139,18 @@ class TiedHeadLogProbs(torch.autograd.Function):
             return (torch.zeros_like(x) if need_x else None,
                     torch.zeros_like(head) if need_head else None, None, None, None)
         width, padded = ctx.width, head.shape[0]
-        grad = gradient.to(torch.float32).contiguous()
+        grad = gradient.contiguous()
         dx = x.new_empty(rows, width) if need_x else None
         one = rows <= (ctx.chunk_tokens or max_chunk(padded))
         dw = (torch.empty(padded, width, device=x.device,
                           dtype=head.dtype if one else torch.float32) if need_head else None)
         _logp_backward(_rows16(x, width), _rows16(head, width), ctx.vocab, labels, lse, grad, dx,
                        dw, chunk_tokens=ctx.chunk_tokens)
-        if need_head:
-            dw[ctx.vocab:].zero_()
-            dw = dw.to(head.dtype)[:, :d]
-        return dx[:, :d] if need_x else None, dw, None, None, None
+        if need_head and not one:
+            dw = dw.to(head.dtype)
+        if width != d:
+            dx, dw = (t if t is None else t[:, :d] for t in (dx, dw))
+        return dx, dw, None, None, None
 
 
 def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labels: torch.Tensor,
@@ -187,8 +178,8 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
                          "[padded, d] of the same type and int64 labels [...]")
     if head16.device != x16.device or labels.device != x16.device:
         raise ValueError("tied_head_logprobs needs its head and labels on x's device")
-    if chunk_tokens is not None and chunk_tokens < 1:
-        raise ValueError("tied_head_logprobs needs a positive chunk_tokens")
+    if chunk_tokens is not None and not 1 <= chunk_tokens <= 1 << 22:
+        raise ValueError("tied_head_logprobs needs chunk_tokens in [1, 2^22]")
     paths.took("tied_head_logprobs", "mfma")
     flat = x16.reshape(-1, x16.shape[-1])
     return TiedHeadLogProbs.apply(flat, head16, vocab, labels.reshape(-1),
@@ -418,9 +409,12 @@ def sequence_logprobs(model, ids: torch.Tensor, labels: torch.Tensor,
                       precision: str = "fp16") -> torch.Tensor:
     """fp32 [batch, tokens] log-probabilities of ``labels`` (0 where -100) under
     ``model``, without a graph: a reference or behaviour policy's score of a batch."""
+    from .optimized_v3 import castable_weights
     dtype = _compute_dtype(model, ids, precision)
     targets = _labels(ids, labels)
     with weight_cast_cache(), amp_context(ids.device, precision):
+        if precision == "fp16":
+            prefetch_casts(castable_weights(model))
         hidden = hidden_states(model, ids)
     weight = model.lm_head.weight
     head = _head16(weight, dtype)
@@ -436,8 +430,8 @@ def _loss_backward(model, ids, labels, loss_of, chunk_tokens, scaler, precision)
     from .optimized_v3 import castable_weights
     dtype = _compute_dtype(model, ids, precision)
     targets = _labels(ids, labels)
-    if chunk_tokens is not None and chunk_tokens < 1:
-        raise ValueError("Positive chunk size required")
+    if chunk_tokens is not None and not 1 <= chunk_tokens <= 1 << 22:
+        raise ValueError("chunk size in [1, 2^22] required")
     with weight_cast_cache():  # weights are constant until the optimizer step
         if precision == "fp16":
             prefetch_casts(castable_weights(model))

@@ -377,3 +377,20 @@ def test_another_stream(cuda_device):
     torch.cuda.current_stream().wait_stream(side)
     plain.update(grads)
     same_state(opt, params, plain)
+
+
+def test_refused_before_anything_changes(cuda_device):
+    p, q = (torch.zeros(64, 80, device=cuda_device, requires_grad=True) for _ in range(2))
+    opt = FusedAdamW8bit([p, q], lr=LR, min_8bit_numel=1)
+    p.grad = torch.ones_like(p)
+    q.grad = torch.ones(80, 64, device=cuda_device).t()
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    assert not p.detach().any() and not opt.state[p]
+    q.grad = torch.ones_like(q)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 1 and bool(p.detach().all())
+    with pytest.raises(ValueError, match="contiguous"):
+        r = torch.zeros(64, 80, device=cuda_device).t().requires_grad_(True)
+        r.grad = torch.ones_like(r)
+        FusedAdamW8bit([r], min_8bit_numel=1).step()

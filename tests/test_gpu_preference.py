@@ -90,7 +90,8 @@ def within(got, ref, bound):
 
 SIZES = [(1, 8, 1), (1, 128, 50257), (3, 64, 2), (7, 72, 64), (51, 256, 1000), (130, 128, 4097),
          (257, 100, 3001), (300, 200, 777), (64, 1, 300), (1000, 384, 4097), (2331, 512, 5000),
-         (700, 640, 50257), (5000, 128, 20011), (66, 2048, 130)]
+         (700, 640, 50257), (5000, 128, 20011), (66, 2048, 130), (20000, 264, 500),
+         (70000, 32, 90)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])

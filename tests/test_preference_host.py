@@ -65,32 +65,21 @@ def test_head_logp_argument_checks():
     assert fwd(ws=None) == fwd(nbytes=need - 1) == fwd(ws=ODD) == WORKSPACE
     assert lib.rv_head_logp_workspace_bytes(0, 256, 10) == -BAD_SIZE
     assert lib.rv_head_logp_workspace_bytes(5, 4, 10) == -UNSUPPORTED
-    assert lib.rv_head_logp_scale(None, FAKE, 4, -100, FAKE, None) == NULL
-    assert lib.rv_head_logp_scale(FAKE, FAKE, 0, -100, FAKE, None) == BAD_SIZE
+    ws = lib.rv_head_logp_bwd_workspace_bytes(51, 256, 50257, 50304)
+    assert ws > 51 * 50304 * 2
+    assert lib.rv_head_logp_bwd_workspace_bytes(51, 256, 50257, 50240) == -BAD_SIZE
+    assert lib.rv_head_logp_bwd_workspace_bytes((1 << 22) + 1, 256, 64, 64) == -UNSUPPORTED
 
-    def dlogits(vocab=1000, padded=1024, d=256, dtype=bf16, out=FAKE, lse=FAKE):
-        return lib.rv_head_logp_dlogits(FAKE, FAKE, 51, d, vocab, padded, dtype, FAKE, -100, lse,
-                                        FAKE, FAKE, out, None)
-    assert dlogits(lse=None) == dlogits(out=None) == NULL
-    assert dlogits(padded=960) == BAD_SIZE
-    assert dlogits(padded=1000) == dlogits(d=4) == dlogits(out=ODD) == UNSUPPORTED
-    assert dlogits(padded=1 << 23) == UNSUPPORTED  # a tile's rows pass 32-bit offsets
-    ws = lib.rv_head_logp_grad_workspace_bytes(51, 256, 50257, 50304)
-    assert ws > 0
-
-    def dx(out=FAKE, space=FAKE, nbytes=ws):
-        return lib.rv_head_logp_dx(FAKE, FAKE, 51, 256, 50257, 50304, f16, FAKE, out, space,
-                                   nbytes, None)
-    assert dx(out=None) == NULL and dx(out=ODD) == UNSUPPORTED
-    assert dx(space=None) == dx(nbytes=16) == WORKSPACE
-    need_dw = lib.rv_head_logp_grad_workspace_bytes(32768, 128, 256, 256)
-    assert need_dw > 0
-
-    def dw(dtype=f16, out_dtype=f16, accumulate=0, nbytes=need_dw):
-        return lib.rv_head_logp_dw(FAKE, FAKE, 32768, 128, 256, 256, dtype, FAKE, FAKE, out_dtype,
-                                   accumulate, FAKE, nbytes, None)
-    assert dw(accumulate=1) == dw(out_dtype=bf16) == dw(dtype=f32, out_dtype=f32) == UNSUPPORTED
-    assert dw(nbytes=0) == WORKSPACE
+    def bwd(d=256, padded=50304, dtype=f16, lse=FAKE, grad=FAKE, dx=FAKE, dw=FAKE, dw_rows=50257,
+            dw_dtype=f16, accumulate=0, space=FAKE, nbytes=ws):
+        return lib.rv_head_logp_bwd(FAKE, FAKE, 51, d, 50257, padded, dtype, FAKE, -100, lse, grad,
+                                    dx, dw, dw_rows, dw_dtype, accumulate, space, nbytes, None)
+    assert bwd(lse=None) == bwd(grad=None) == NULL
+    assert bwd(padded=50240) == bwd(dw_rows=50258) == BAD_SIZE
+    assert bwd(padded=50300) == bwd(d=4) == bwd(dx=ODD) == bwd(dw=ODD) == UNSUPPORTED
+    assert bwd(padded=1 << 23) == UNSUPPORTED  # a tile's rows pass 32-bit offsets
+    assert bwd(accumulate=1) == bwd(dw_dtype=bf16) == bwd(dtype=f32, dw_dtype=f32) == UNSUPPORTED
+    assert bwd(space=None) == bwd(nbytes=ws - 1) == WORKSPACE
 
 
 def test_loss_argument_checks():
