@@ -128,6 +128,8 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
   const int64_t out0 = uniform(reinterpret_cast<int64_t>(a.out) + (first * a.m + m0) * 128);
   const uint32_t out_off = (uint32_t)((lane & 15) * 128 + (lane >> 4 & 1) * 32 + (lane >> 5) * 16);
 
+  fill(1);  // both buffers are free at the start
+
   const uint32_t lds0 = (uint32_t)(size_t)(RV_LDS void*)lds;
   const uint32_t at = (lane & 31) * kRow + (((lane >> 5) ^ (lane & 15)) << 4);
   f32x16 acc[2][2];  // [block of the pair][row block]
@@ -271,11 +273,12 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
     // this wave's loads of the stage have to have landed.  Newer than them are, in the
     // backward, the stores of two blocks (of one in the second stage), four a block,
     // always issued in full
-    if (GRAD && live && st > 1) wait_vmcnt<8>();
-    else if (GRAD && live && st > 0) wait_vmcnt<4>();
+    if constexpr (!decltype(begun)::value) wait_vmcnt<kDma>();  // the next stage's
+    else if (GRAD && live && st > 1) wait_vmcnt<8>();
+    else if (GRAD && live) wait_vmcnt<4>();
     else wait_vmcnt<0>();
     lds_barrier();  // every wave's loads have landed, and none reads the stage before
-    fill(st + 1);
+    if constexpr (decltype(begun)::value) fill(st + 1);
     if (!live) return;
     const uint32_t tile = lds0 + (st & 1) * kStage;
     static_for<D>([&](auto rc) __attribute__((always_inline)) { read(rc, tile); });

@@ -181,9 +181,14 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     if chunk_tokens is not None and not 1 <= chunk_tokens <= 1 << 22:
         raise ValueError("tied_head_logprobs needs chunk_tokens in [1, 2^22]")
     paths.took("tied_head_logprobs", "mfma")
-    flat = x16.reshape(-1, x16.shape[-1])
-    return TiedHeadLogProbs.apply(flat, head16, vocab, labels.reshape(-1),
-                                  chunk_tokens).reshape(labels.shape)
+    flat, targets = x16.reshape(-1, x16.shape[-1]), labels.reshape(-1)
+    if torch.is_grad_enabled() and (x16.requires_grad or head16.requires_grad):
+        logp = TiedHeadLogProbs.apply(flat, head16, vocab, targets, chunk_tokens)
+    else:
+        width = -(-flat.shape[1] // 8) * 8
+        logp, _ = _logp_forward(_rows16(flat, width), _rows16(head16, width), vocab,
+                                targets.contiguous())
+    return logp.reshape(labels.shape)
 
 
 # ---------------------------------------------------------------------------
