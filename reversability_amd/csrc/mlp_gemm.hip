@@ -1953,18 +1953,21 @@ int64_t logp_dx_bytes(int64_t rows, int64_t d, int64_t k) {
 
 // The streamed logits of narrow models (head_stream_k): stages of 64 columns per
 // workgroup.  Two workgroups a CU run at a time; a workgroup's start (its rows of
-// x, the first stage) costs about three stages.
+// x, the first stage) costs about three stages, and a workgroup alone on its CU takes
+// 0.65 of the time it takes beside another (512 x 256 over 50257: 226 workgroups of 7
+// stages 29.9 us, 394 of 4 33.3; 4096 rows: 256 of 50 116 us, 512 of 25 108).
 bool stream_takes(int64_t d) { return d <= 256; }
 int64_t stream_chunk(int64_t rows, int64_t n) {
   const int64_t stages = (n + 63) / 64, tiles_m = (rows + 255) / 256, places = 2 * kCUs;
   int64_t best = stages, least = 0;
-  for (int64_t rounds = 1; rounds <= 8; ++rounds) {
-    int64_t splits = rounds * places / tiles_m;
+  for (int64_t halves = 1; halves <= 16; ++halves) {
+    int64_t splits = halves * kCUs / tiles_m;
     if (splits < 1) splits = 1;
     if (splits > stages) splits = stages;
     const int64_t chunk = (stages + splits - 1) / splits;
     const int64_t tiles = tiles_m * ((stages + chunk - 1) / chunk);
-    const int64_t cost = (tiles + places - 1) / places * (chunk + 3);
+    const int64_t rest = tiles % places, last = rest == 0 ? 0 : rest <= kCUs ? 13 : 20;
+    const int64_t cost = (tiles / places * 20 + last) * (chunk + 3);
     if (least == 0 || cost < least) best = chunk, least = cost;
   }
   return best;
