@@ -226,7 +226,10 @@ def _at(t) -> tuple:
 
 # The two Functions below are called on small batches too, where the host's work is
 # what they take: few allocations (outputs and workspace cut from one) and no zeros
-# made for the outputs without a gradient.  fp32 values of the workspace's share:
+# made for the outputs without a gradient.  Pieces of one allocation share its version
+# count, so none is handed to save_for_backward: a caller may change the returned
+# statistics in place (an all-reduce) before the backward pass.  fp32 values of the
+# workspace's share:
 def _floats(nbytes: int, what: str) -> int:
     if nbytes < 0:
         _check(-nbytes, what)
@@ -244,9 +247,10 @@ class PreferenceLoss(torch.autograd.Function):
         with _DeviceGuard(logp):
             nbytes = lib.rv_pref_loss_workspace_bytes(pairs, tokens)
             # the workspace first: its fp64 sums need the allocation's alignment
-            sizes = (_floats(nbytes, "rv_pref_loss_workspace_bytes"), seqs, pairs, pairs)
-            ws, coef, chosen, rejected = torch.empty(
+            sizes = (_floats(nbytes, "rv_pref_loss_workspace_bytes"), pairs, pairs)
+            ws, chosen, rejected = torch.empty(
                 sum(sizes), device=dev, dtype=torch.float32).split(sizes)
+            coef = torch.empty(seqs, device=dev, dtype=torch.float32)
             loss = torch.empty((), device=dev, dtype=torch.float32)
             _check(lib.rv_pref_loss(
                 rows.data_ptr(), rows.stride(0), *_at(ref), *_at(mask), pairs, tokens, beta,
@@ -321,7 +325,8 @@ class PolicyLoss(torch.autograd.Function):
                 *clip, kl_coef, per_sequence, loss.data_ptr(), kl.data_ptr(),
                 slope.data_ptr() if slope is not None else None, ws.data_ptr(), nbytes,
                 _stream(logp)), "rv_policy_loss")
-        ctx.save_for_backward(slope, factor)
+        ctx.save_for_backward(slope)
+        ctx.factor = factor
         ctx.set_materialize_grads(False)
         kl, clipped = kl.reshape(()), clipped.reshape(())
         ctx.mark_non_differentiable(kl, clipped)
@@ -332,9 +337,9 @@ class PolicyLoss(torch.autograd.Function):
     def backward(ctx, gradient, *_):
         if gradient is None:
             return None, None, None, None, None, None, None, None
-        slope, factor = ctx.saved_tensors
+        slope, = ctx.saved_tensors
         dlogp = torch.empty_like(slope)
-        _check(library().rv_policy_grad(slope.data_ptr(), factor.data_ptr(), gradient.data_ptr(),
+        _check(library().rv_policy_grad(slope.data_ptr(), ctx.factor.data_ptr(), gradient.data_ptr(),
                                         slope.numel(), dlogp.data_ptr(), _stream(slope)),
                "rv_policy_grad")
         return dlogp, None, None, None, None, None, None, None

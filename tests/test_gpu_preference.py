@@ -577,3 +577,19 @@ def test_losses_captured_and_on_another_stream(cuda_device):
         there = step()
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(x, y) for x, y in zip(out, there))
+
+
+def test_statistics_may_change_before_the_backward(cuda_device):
+    """An in-place change of a returned statistic (as an all-reduce makes it) leaves the
+    backward as it is."""
+    old, ref, logp = (-torch.rand(4, 30, device="cuda") for _ in range(3))
+    adv = torch.randn(4, device="cuda")
+    logp.requires_grad_(True)
+    for call in (lambda: preference_loss(logp, ref),
+                 lambda: policy_loss(logp, old, adv, ref_logp=ref, kl_coef=0.1)):
+        plain, = torch.autograd.grad(call().loss, logp)
+        out = call()
+        for t in out[1:]:
+            t.mul_(0.5)
+        changed, = torch.autograd.grad(out.loss, logp)
+        assert torch.equal(changed, plain) and plain.any()
