@@ -597,7 +597,7 @@ int rv_policy_loss(const float* logp, int64_t ld_logp, const float* old_logp, in
   if (per_sequence) {
     float* weight = reinterpret_cast<float*>(a.part + blocks * 4);
     a.weight = weight;
-    const int64_t chunks = mask ? count_chunks(tokens) : 0;
+    const int64_t chunks = mask && seqs > 0 ? count_chunks(tokens) : 0;
     const int lanes = lanes_of(tokens / 4);
     const int64_t wgs = chunks ? seqs * chunks : (seqs * lanes + kThreads - 1) / kThreads;
     if (wgs * kThreads >= (int64_t)1 << 32) return RV_ERR_UNSUPPORTED;  // threads a launch holds

@@ -579,6 +579,18 @@ def test_losses_captured_and_on_another_stream(cuda_device):
     assert all(torch.equal(x, y) for x, y in zip(out, there))
 
 
+@pytest.mark.parametrize("tokens", [0, 40, 9000])
+def test_policy_without_sequences(cuda_device, tokens):
+    logp = torch.zeros(0, tokens, device="cuda", requires_grad=True)
+    for mask in (None, torch.ones(0, tokens, device="cuda", dtype=torch.bool)):
+        for reduction in ("token", "sequence"):
+            out = policy_loss(logp, logp.detach(), torch.zeros(0, device="cuda"), mask=mask,
+                              reduction=reduction)
+            dlogp, = torch.autograd.grad(out.loss, logp)
+            assert [float(t.detach()) for t in out] == [0.0, 0.0, 0.0]
+            assert dlogp.shape == (0, tokens)
+
+
 def test_statistics_may_change_before_the_backward(cuda_device):
     """An in-place change of a returned statistic (as an all-reduce makes it) leaves the
     backward as it is."""
