@@ -579,6 +579,32 @@ def test_losses_captured_and_on_another_stream(cuda_device):
     assert all(torch.equal(x, y) for x, y in zip(out, there))
 
 
+@pytest.mark.parametrize("shift", [1e-6, 1e-3, 0.1, 0.9, 1.5])
+def test_policy_kl_of_close_models(cuda_device, shift):
+    """exp(s) - s - 1 and its gradient keep their digits where they are small."""
+    g = gen(17)
+    # multiples of 2^-22 up to 2: sums and differences are exact
+    grid = lambda t: (t * 2.0 ** 22).round() * 2.0 ** -22
+    logp = grid(-0.5 * torch.rand(6, 500, generator=g, device="cuda"))
+    ref = logp + grid(shift * torch.randn(6, 500, generator=g, device="cuda").clamp(-1, 1))
+    s = ref.double() - logp.double()
+    assert torch.equal((ref - logp).double(), s)
+    leaf = logp.clone().requires_grad_(True)
+    out = policy_loss(leaf, logp, torch.zeros(6, device="cuda"), ref_logp=ref, kl_coef=1.0)
+    dlogp, = torch.autograd.grad(out.loss, leaf)
+    k = torch.expm1(s) - s
+    # relative, in units of 2^-24: the series 1.5 (its last step and coefficient; the
+    # terms before shrink), the square and the product 2, its end 2^-3, the mean's rounding
+    # 1; from 1 on exp's 2 of up to 4.5 and two roundings, of a value of 0.37 (s = -1) or
+    # 0.72 (s = 1) and more: 16
+    within(out.kl, k.mean(), 16 * 2.0 ** -24 * k.mean())
+    within(out.loss.detach(), k.mean(), 17 * 2.0 ** -24 * k.mean())
+    # k and s add to exp(s) - 1: at s = -1, where they cancel most, 0.37 and 1 leave 0.63, so
+    # a relative error of 16 of k is 10 of the sum; its rounding, 1 / n and the products 4
+    grad = -torch.expm1(s) / s.numel()
+    within(dlogp, grad, 14 * 2.0 ** -24 * grad.abs())
+
+
 @pytest.mark.parametrize("tokens", [0, 40, 9000])
 def test_policy_without_sequences(cuda_device, tokens):
     logp = torch.zeros(0, tokens, device="cuda", requires_grad=True)
