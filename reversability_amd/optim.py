@@ -288,11 +288,24 @@ class FusedAdamW8bit(FusedAdamW):
 
     def load_state_dict(self, state_dict):
         """As torch's, which casts every floating or parameter-like state to the
-        parameter's type; the 8-bit moments keep theirs."""
-        Optimizer.load_state_dict(self, state_dict)
+        parameter's type; the 8-bit moments keep theirs.  Moments of another size than
+        the parameter's are refused: the kernel would read past them."""
         saved = state_dict["state"]
         places = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(places, (q for g in self.param_groups for q in g["params"])):
+        params = [p for g in self.param_groups for p in g["params"]]
+        block = library().rv_adamw8_block()
+        for i, p in zip(places, params):
+            st = saved.get(i, {})
+            for name, scale in _SCALES.items():
+                if name in st and st[name].shape != p.shape:
+                    raise ValueError(f"{name} of shape {tuple(st[name].shape)} for a parameter "
+                                     f"of shape {tuple(p.shape)}")
+                if (scale in st) != (_SCALES["exp_avg"] in st) or scale in st and (
+                        st[name].dtype != torch.float8_e4m3fn or st[scale].dtype != torch.uint8
+                        or st[scale].numel() != -(-p.numel() // block)):
+                    raise ValueError(f"{name} is not the 8-bit moment of its parameter")
+        Optimizer.load_state_dict(self, state_dict)
+        for i, p in zip(places, params):
             for name, scale in _SCALES.items():
                 if scale in saved.get(i, {}):
                     for key in (name, scale):

@@ -343,6 +343,29 @@ def test_state_dict_round_trip(cuda_device):
     assert all(resumed.state[q]["exp_avg"].dtype == torch.float32 for q in twins)
 
 
+def test_moments_of_another_size_are_refused(cuda_device):
+    """Such a checkpoint (another width or vocabulary) changes nothing."""
+    def made(shape):
+        p = torch.ones(shape, device=cuda_device, requires_grad=True)
+        p.grad = torch.ones_like(p)
+        return p, FusedAdamW8bit([p], lr=LR, min_8bit_numel=64)
+    small, source = made((40, 64))
+    source.step()
+    plain = FusedAdamW([small])
+    plain.step()
+    for state in (source.state_dict(), plain.state_dict()):
+        p, opt = made((80, 64))
+        with pytest.raises(ValueError, match="shape"):
+            opt.load_state_dict(state)
+        assert not opt.state[p]
+    for key, wrong in (("exp_avg_scale", torch.zeros(79, dtype=torch.uint8)),
+                       ("exp_avg_sq", torch.zeros(40, 64))):
+        state = copy.deepcopy(source.state_dict())
+        state["state"][0][key] = wrong.to(cuda_device)
+        with pytest.raises(ValueError, match="8-bit"):
+            made((40, 64))[1].load_state_dict(state)
+
+
 def test_captured_updates_equal_eager_ones(cuda_device):
     """Replays advance the device's step count, and with it the random bits."""
     runs = []
