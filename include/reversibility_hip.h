@@ -452,8 +452,8 @@ int rv_adamw_step_clipped(int count, float* const* params, const float* const* g
 /* The same update with both moments in 8 bits: e4m3 values with one scale byte b
  * per rv_adamw8_block() consecutive elements of a tensor (value = e4m3 *
  * 2^(b - 127); ceil(numel / block) bytes, all zero at the start).  p takes the fp32
- * moments; what is stored is rounded, the first moment to nearest, the second at
- * random (its expectation kept) with bits that follow from seed, the tensor's
+ * moments; what is stored is rounded, the second moment at random (its expectation
+ * kept), the first to nearest where 1 - beta1 >= 2^-4 and else at random too, with bits that follow from seed, the tensor's
  * ordinal, *step and the element's index alone.  Multiplies and adds are rounded
  * one by one (no fused multiply-add). */
 int rv_adamw8_max_tensors(void);

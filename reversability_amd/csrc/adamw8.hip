@@ -12,11 +12,13 @@
 //     p  = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // The parameter takes the fp32 m and v of this step; only what the next step
-// starts from is rounded.  m goes to the nearest value (2^-4 of it: it is replaced
-// within 1 / (1 - b1) steps).  v moves by (1 - b2) of itself a step, less than half
+// starts from is rounded.  v moves by (1 - b2) of itself a step, less than half
 // a step of e4m3: to the nearest it would stand still, or climb only, so it is
 // rounded up or down at random with the fractions as probabilities, which keeps its
-// expectation.  The random bits are MurmurHash3's 32-bit finalizer (A. Appleby) of
+// expectation.  m goes to the nearest value where 1 - b1 is at least 2^-4, the largest
+// half step (2^-4 of it: it is replaced within 1 / (1 - b1) steps, and a zero gradient
+// takes every value to a smaller one); with a slower b1 it would stand still like v, and is
+// rounded at random too (303 us where the nearest takes 293, below).  The random bits are MurmurHash3's 32-bit finalizer (A. Appleby) of
 // the element's index plus a key of seed, tensor and step: the same call gives the
 // same bits.  A v > 0 stays > 0: a zero v under an m that is not would make the next
 // update as large as 1 / eps.
@@ -113,16 +115,33 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], int scale) {
 }
 
 // e4m3 code of v >= 0 at the scale, up with probability `noise` 2^-20 against the
-// fraction that is cut off; at least the smallest value for v > 0.
-__device__ __forceinline__ uint32_t encode_random(float v, int scale, uint32_t noise) {
+// fraction that is cut off.
+__device__ __forceinline__ uint32_t round_random(float v, int scale, uint32_t noise) {
   const float q = __builtin_ldexpf(v, 127 - scale);
   if (!(q < 512.f)) return 0x7f;  // infinity or NaN
   // 3 of 23 mantissa bits stay; fp32's exponent 120 is e4m3's 0 (values below 2^-6,
   // in steps of 2^-9)
   const uint32_t normal = ((__float_as_uint(q) + noise) >> 20) - 960u;
   const uint32_t tiny = (uint32_t)(q * 512.f + (float)noise * 0x1p-20f);
-  const uint32_t code = q < 0x1p-6f ? tiny : normal;
-  return code == 0 && v > 0.f ? 1u : code;
+  return q < 0x1p-6f ? tiny : normal;
+}
+
+// e4m3 codes of x at the scale, rounded at random with 16 bits an element; POSITIVE:
+// x >= 0, and at least the smallest value for x > 0.
+template <bool POSITIVE>
+__device__ __forceinline__ uint32_t encode_random(const float (&x)[4], int scale, uint32_t first,
+                                                  uint32_t key) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t bits = mix(first + e / 2 + key);  // of two elements
+    const uint32_t noise = (e & 1 ? bits >> 16 : bits & 0xffffu) << 4 | 8u;
+    uint32_t code = round_random(POSITIVE ? x[e] : fabsf(x[e]), scale, noise);
+    if (POSITIVE) code = code == 0 && x[e] > 0.f ? 1u : code;
+    else code |= __float_as_uint(x[e]) >> 31 << 7;
+    w |= code << (8 * e);
+  }
+  return w;
 }
 
 __device__ __forceinline__ int tensor_of(const int* chunk_start, int count, int block) {
@@ -137,7 +156,7 @@ __device__ __forceinline__ int tensor_of(const int* chunk_start, int count, int 
 
 struct Scalars {
   float step_size, inv_bc2, inv, clip;
-  uint32_t key;
+  uint32_t key, m_key;
 };
 
 // Four elements of a thread: where they are and what was loaded.
@@ -179,7 +198,8 @@ __device__ __forceinline__ void load(Four& f, const float* g) {
 }
 
 // The update and the stores; every lane of a block takes part.  `pair`: the counter
-// of the first two elements' random bits.
+// of the first two elements' random bits.  RANDOM_M: m is rounded at random too.
+template <bool RANDOM_M>
 __device__ __forceinline__ void update(Four& f, const Hyper& h, const Scalars& s, uint32_t pair) {
   float m[4], v[4];
   decode(f.mw, f.mscale, m);
@@ -201,14 +221,10 @@ __device__ __forceinline__ void update(Four& f, const Hyper& h, const Scalars& s
     }
   }
   const int ms = scale_byte(block_max(mtop)), vs = scale_byte(block_max(vtop));
-  const uint32_t mw = encode(m, ms);
-  uint32_t vw = 0;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const uint32_t bits = mix(pair + half + s.key);  // 16 for each of two elements
-    vw |= encode_random(v[2 * half], vs, (bits & 0xffffu) << 4 | 8u) << (16 * half);
-    vw |= encode_random(v[2 * half + 1], vs, bits >> 16 << 4 | 8u) << (16 * half + 8);
-  }
+  const uint32_t vw = encode_random<true>(v, vs, pair, s.key);
+  uint32_t mw;
+  if constexpr (RANDOM_M) mw = encode_random<false>(m, ms, pair, s.m_key);
+  else mw = encode(m, ms);
   if (f.full) {
     rv::st_f4(f.p, make_float4(f.pp[0], f.pp[1], f.pp[2], f.pp[3]));
     *reinterpret_cast<uint32_t*>(f.m) = mw;
@@ -228,6 +244,7 @@ __device__ __forceinline__ void update(Four& f, const Hyper& h, const Scalars& s
   }
 }
 
+template <bool RANDOM_M>
 __global__ __launch_bounds__(kThreads)
 void adamw8_k(Table tab, Hyper h) {
   if (h.found_inf != nullptr && *h.found_inf != 0.0f) return;  // uniform skip
@@ -261,9 +278,10 @@ void adamw8_k(Table tab, Hyper h) {
   s.inv = h.inv_scale != nullptr ? *h.inv_scale : 1.0f;
   s.clip = h.clip != nullptr ? *h.clip : 1.0f;
   s.key = mix(tab.key[t] + (uint32_t)*h.step);
+  s.m_key = RANDOM_M ? mix(s.key + 0x9E3779B9u) : 0u;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u)
-    update(f[u], h, s, (uint32_t)((first + u * (kThreads * 4)) >> 1));
+    update<RANDOM_M>(f[u], h, s, (uint32_t)((first + u * (kThreads * 4)) >> 1));
 }
 
 uint32_t host_mix(uint32_t h) {
@@ -328,7 +346,10 @@ int rv_adamw8_step(int count, float* const* params, const float* const* grads,
   h.clip = clip_coef;
   const dim3 grid((unsigned)(chunks < kGridRow ? chunks : kGridRow),
                   (unsigned)((chunks + kGridRow - 1) / kGridRow));
-  hipLaunchKernelGGL(adamw8_k, grid, dim3(kThreads), 0, (hipStream_t)stream, tab, h);
+  if (1.0 - beta1 < 0x1p-4)
+    hipLaunchKernelGGL(adamw8_k<true>, grid, dim3(kThreads), 0, (hipStream_t)stream, tab, h);
+  else
+    hipLaunchKernelGGL(adamw8_k<false>, grid, dim3(kThreads), 0, (hipStream_t)stream, tab, h);
   return rv_host::check_launch();
 }
 

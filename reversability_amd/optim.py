@@ -204,8 +204,9 @@ class FusedAdamW8bit(FusedAdamW):
     two per 32 consecutive elements (``exp_avg_scale``, ``exp_avg_sq_scale``: uint8,
     value = e4m3 * 2^(byte - 127)); smaller ones (norm weights) keep them in fp32.
     The update uses the fp32 moments of its step; what is stored is rounded to
-    nearest (``exp_avg``) or at random with its expectation kept (``exp_avg_sq``,
-    whose change per step is below half a step of e4m3).  The random bits follow
+    nearest (``exp_avg`` where beta1 <= 0.9375) or at random with its expectation kept
+    (``exp_avg_sq``, and ``exp_avg`` of a larger beta1, whose change per step is below
+    half a step of e4m3).  The random bits follow
     from ``seed``, the parameter's place, the step count and the element: a run
     repeats bit for bit.  GradScaler, ``unscale_clip_``, the device-side step count
     and graph capture work as in ``FusedAdamW``; ``moments(p)`` returns a
