@@ -363,7 +363,7 @@ int rv_head_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int6
  * logp[r] = z[r, labels[r]] - lse[r]; 0 for label == ignore_index, NaN for
  * another label outside [0, vocab).  x [rows, d] and head [>= vocab, d] of dtype
  * RV_F16 or RV_BF16, 16-byte aligned, d a multiple of 8; labels int64 [rows];
- * logp, lse fp32 [rows]. */
+ * logp, lse (may be NULL: scoring alone) fp32 [rows]. */
 int64_t rv_head_logp_workspace_bytes(int64_t rows, int64_t d, int64_t vocab);
 int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
                      int dtype, const int64_t* labels, int64_t ignore_index, float* logp,
@@ -373,7 +373,7 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
  * dz[r, j] = grad[r] ([j == labels[r]] - exp(z[r, j] - lse[r])), z computed again,
  *   dx[rows, d] = dz head         of dtype
  *   dw[dw_rows, d] = dz^T x       of dtype, or fp32 (added to dw with accumulate)
- * either may be NULL.  Ignored rows have none (their grad is not read), a row of
+ * either may be NULL.  Ignored rows have none (their grad is not used), a row of
  * another label outside [0, vocab) NaN.  padded, a multiple of 64, is the row count
  * of head; dw_rows is vocab or padded (pad rows: sums of zeros).  dz is held in dtype
  * in the workspace, times a power of two that brings the largest |grad| of a row

@@ -1197,7 +1197,7 @@ void logprob_rows(const float2* __restrict__ part, const float* __restrict__ lab
   for (int w = 1; w < 4; ++w) all = join(all, red[w][r]);
   const int64_t label = labels[row];
   const float l = logf(all.y);
-  lse[row] = all.x + l;
+  if (lse != nullptr) lse[row] = all.x + l;
   logp[row] = label == ignore ? 0.f
               : label < 0 || label >= vocab ? NAN
                                             : (label_logit[row] - all.x) - l;
@@ -2309,7 +2309,7 @@ int64_t rv_head_logp_workspace_bytes(int64_t rows, int64_t d, int64_t vocab) {
 int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
                      int dtype, const int64_t* labels, int64_t ignore_index, float* logp,
                      float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (!x || !head || !labels || !logp || !lse) return RV_ERR_NULL_POINTER;
+  if (!x || !head || !labels || !logp) return RV_ERR_NULL_POINTER;
   const int bad = logp_check(rows, d, vocab, up128(vocab), dtype);
   if (bad) return bad;
   if (!ok16(x) || !ok16(head)) return RV_ERR_UNSUPPORTED;

@@ -40,8 +40,8 @@ from .mlp import prefetch_casts, weight_cast_cache
 from .optimized import _AMP_DTYPES, amp_context, hidden_states
 
 _CODES = {torch.float16: RV_F16, torch.bfloat16: RV_BF16}
-# tokens per launch of the forward (its partial statistics: 8 bytes per token and
-# 128 or 256 columns) and bytes of one chunk's logit gradients in the backward
+# tokens per launch of the forward (its partial statistics: 8 bytes per token and tile of
+# columns, of 64 to the whole vocabulary) and bytes of one chunk's logit gradients in the backward
 FORWARD_TOKENS = 1 << 16
 GRADIENT_BYTES = 1 << 32
 
@@ -50,11 +50,12 @@ GRADIENT_BYTES = 1 << 32
 # log-probabilities of the tied head
 # ---------------------------------------------------------------------------
 def _rows16(t: torch.Tensor, width: int) -> torch.Tensor:
-    """``t`` as the kernels read it: dense rows of ``width`` (zeros behind t's own
-    columns), 16-byte aligned."""
-    if t.shape[1] != width:
-        out = t.new_zeros(t.shape[0], width)
-        out[:, :t.shape[1]] = t
+    """``t`` [..., d] as the kernels read it: dense rows of ``width`` (zeros behind t's
+    own columns), 16-byte aligned."""
+    d = t.shape[-1]
+    if d != width:
+        out = t.new_zeros(*t.shape[:-1], width)
+        out[..., :d] = t
         return out
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -66,11 +67,12 @@ def _workspace(nbytes: int, like: torch.Tensor, what: str):
     return torch.empty(nbytes, device=like.device, dtype=torch.uint8) if nbytes else None
 
 
-def _logp_forward(x, head, vocab, labels):
-    """(logp, lse), fp32 [rows], of dense operands."""
-    rows, d = x.shape
+def _logp_forward(x, head, vocab, labels, want_lse=True):
+    """(logp, lse or None), fp32 of the labels' shape, of dense operands."""
+    rows, d = labels.numel(), x.shape[-1]
     lib, code = library(), _CODES[x.dtype]
-    logp, lse = (torch.empty(rows, device=x.device, dtype=torch.float32) for _ in range(2))
+    logp = torch.empty(labels.shape, device=x.device, dtype=torch.float32)
+    lse = torch.empty_like(logp) if want_lse else None
     with _DeviceGuard(x):
         for at in range(0, rows, FORWARD_TOKENS):
             n = min(FORWARD_TOKENS, rows - at)
@@ -79,7 +81,7 @@ def _logp_forward(x, head, vocab, labels):
             _check(lib.rv_head_logp_fwd(
                 x.data_ptr() + at * d * 2, head.data_ptr(), n, d, vocab, code,
                 labels.data_ptr() + at * 8, IGNORE_INDEX, logp.data_ptr() + at * 4,
-                lse.data_ptr() + at * 4, ws.data_ptr(), nbytes, _stream(x)), "rv_head_logp_fwd")
+                lse.data_ptr() + at * 4 if want_lse else None, ws.data_ptr(), nbytes, _stream(x)), "rv_head_logp_fwd")
     return logp, lse
 
 
@@ -170,10 +172,11 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     a NaN or an infinity in an unscored token's row of ``x16`` reaches the gradient of
     the head.
     """
-    if (x16.dtype not in _CODES or head16.dtype != x16.dtype or x16.ndim < 1 or head16.ndim != 2
-            or not x16.is_cuda or x16.shape[-1] != head16.shape[1] or not x16.shape[-1]
-            or head16.shape[0] % VOCAB_ALIGN or not 0 < vocab <= head16.shape[0]
-            or labels.dtype != torch.int64 or labels.shape != x16.shape[:-1]):
+    shape, table = x16.shape, head16.shape
+    if (x16.dtype not in _CODES or head16.dtype != x16.dtype or len(shape) < 1 or len(table) != 2
+            or not x16.is_cuda or shape[-1] != table[1] or not table[1]
+            or table[0] % VOCAB_ALIGN or not 0 < vocab <= table[0]
+            or labels.dtype != torch.int64 or labels.shape != shape[:-1]):
         raise ValueError("tied_head_logprobs needs CUDA fp16 or bf16 x [..., d], a padded head "
                          "[padded, d] of the same type and int64 labels [...]")
     if head16.device != x16.device or labels.device != x16.device:
@@ -181,14 +184,12 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     if chunk_tokens is not None and not 1 <= chunk_tokens <= 1 << 22:
         raise ValueError("tied_head_logprobs needs chunk_tokens in [1, 2^22]")
     paths.took("tied_head_logprobs", "mfma")
-    flat, targets = x16.reshape(-1, x16.shape[-1]), labels.reshape(-1)
     if torch.is_grad_enabled() and (x16.requires_grad or head16.requires_grad):
-        logp = TiedHeadLogProbs.apply(flat, head16, vocab, targets, chunk_tokens)
-    else:
-        width = -(-flat.shape[1] // 8) * 8
-        logp, _ = _logp_forward(_rows16(flat, width), _rows16(head16, width), vocab,
-                                targets.contiguous())
-    return logp.reshape(labels.shape)
+        return TiedHeadLogProbs.apply(x16.reshape(-1, table[1]), head16, vocab,
+                                      labels.reshape(-1), chunk_tokens).reshape(labels.shape)
+    width = -(-table[1] // 8) * 8
+    return _logp_forward(_rows16(x16, width), _rows16(head16, width), vocab, labels.contiguous(),
+                         want_lse=False)[0]
 
 
 # ---------------------------------------------------------------------------
@@ -430,7 +431,7 @@ def sequence_logprobs(model, ids: torch.Tensor, labels: torch.Tensor,
     head = _head16(weight, dtype)
     x = _rows16(hidden.reshape(-1, hidden.shape[-1]).to(dtype), head.shape[1])
     paths.took("tied_head_logprobs", "mfma")
-    return _logp_forward(x, head, weight.shape[0], targets)[0].reshape(ids.shape)
+    return _logp_forward(x, head, weight.shape[0], targets, want_lse=False)[0].reshape(ids.shape)
 
 
 def _loss_backward(model, ids, labels, loss_of, chunk_tokens, scaler, precision):
