@@ -660,7 +660,9 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
   const int cq = (lane >> 5) * 4;
   if constexpr (EPI == Epi::LogProb) {
     // A row's maximum and sum of exp(z - maximum) over the tile's columns, from
-    // the fp32 accumulators: the logits are neither rounded nor stored.  A lane
+    // the fp32 accumulators: the logits are neither rounded nor stored.  Per tile about
+    // three VALU operations and a v_exp a value behind the MFMAs (32768 x 1024 over 50257
+    // 3.16 ms, 1070 TFLOP/s; 1554 x 512 over 32000 79 us, 645, of 3.4 rounds of tiles).  A lane
     // holds half of its row's columns of the wave's block, its partner (lane ^ 32)
     // the other half; the wave columns meet in LDS.
     float2* red = reinterpret_cast<float2*>(lds);  // [WCOLS][BM]
@@ -792,7 +794,8 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
     constexpr int S = WN + 8;
     _Float16* stage = lds + wave * (WM * S);
     if constexpr (EPI == Epi::LogProbGrad) {
-      // acc = s ([j == label] - exp(z - lse)), s = the row's gradient times *scale
+      // acc = s ([j == label] - exp(z - lse)), s = the row's gradient times *scale (32768 x
+      // 1024 over 50257 3.44 ms with 3.3 GB of stores, 980 TFLOP/s)
       const float scale = *args.head.scale;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {

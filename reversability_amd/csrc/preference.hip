@@ -13,6 +13,11 @@
 // kernel joins.  The gradient is one coefficient a row, written by a third.
 // Policy: elementwise, four tokens a thread; the mean over a sequence needs its
 // token count before the gradient, so a pass over the mask alone makes it.
+//
+// 4096 x 2048 tokens: preference 16.6 us forward (76 MB, 4.5 TB/s), policy 33.2 us (176 MB
+// with per-token advantages and the slopes, 5.3 TB/s), its gradient 10.9 us (67 MB, from the Infinity Cache); 64 x
+// 512: 8.8 + 2.7 + 3.1 us.  The kernels of a call take 7 to 50 us; a call with its backward
+// 58 to 100, the host's time through autograd's device thread.
 
 #include <cmath>
 
@@ -209,7 +214,7 @@ void pref_total_k(const double* __restrict__ part, int64_t n, int64_t pairs,
 // dlogp = coef[row] * *grad where counted: four consecutive tokens a thread, of
 // the contiguous output (they may belong to two rows or more).
 // FLAT: the mask is contiguous on a 4-byte boundary, one word a thread (4096 x 2048 tokens
-// 15.4 -> 12.6 us).
+// 15.4 -> 11.6 us; 42 MB, inside the Infinity Cache).
 template <bool FLAT>
 __global__ __launch_bounds__(kThreads)
 void pref_grad_k(const float* __restrict__ coef, const uint8_t* __restrict__ mask,
