@@ -15,11 +15,12 @@
 // (forward) or lse log2e (backward).
 //
 // 16896 x 256 over 50257, fp16 (435 GFLOP): forward 390-440 us, 990-1115 TFLOP/s (the
-// 256 x 256 tiles of gemm_kernel with the LogProb epilogue 626), backward 485-560 us with
-// its 1.7 GB of stores (846); width 128 forward 244 us (417), backward 457 us (640 with
-// the gradients row by row instead of in panels).  Bound by the matrix cores' power: at
-// 1.8 GHz they are busy 66% (forward) and 51% (backward) of the time, and a wave waits
-// 0.4 of its own.  A few rows are bound by the first bytes' way from HBM and the join (51
+// 256 x 256 tiles of gemm_kernel with the LogProb epilogue 626), backward 440-510 us with
+// its 1.7 GB of stores (846; 485-560 in panels of 64 columns, where a store instruction
+// wrote halves of 16 rows' 128 bytes instead of a whole KB; without its stores it would take
+// about as long as the forward); width 128 forward 244 us (417), backward 355 us (457 in
+// panels of 64 columns, 640 row by row).  Bound by the matrix cores' power: at 1.7 GHz they
+// are busy 66% of the forward's time, and a wave waits 0.4 of its own.  A few rows are bound by the first bytes' way from HBM and the join (51
 // rows 12 + 4 us; 64 rows to a workgroup, so that no wave idles, 22.0 -> 21.6 us of a
 // call: left out).  Wider than 256 the rows' fragments no longer fit beside the
 // accumulators of 64 rows, and with 32 rows a wave every MFMA would read 1 KB of LDS, all
@@ -35,7 +36,7 @@ struct StreamArgs {
   int64_t stages, chunk;  // stages of 64 columns in all, and per workgroup
   int64_t tiles_m, tiles; // workgroups: 256 rows x chunk stages, tiles_m fastest
   float2* part;           // forward: [tile column][m]
-  __half* out;            // backward: panels [n / 64][m][64]
+  __half* out;            // backward: panels [n / 32][m][32]
   HeadLogp head_logp;
 };
 
@@ -133,11 +134,11 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
       ref[i] = top[i] * kLog2e;
     }
   }
-  // backward: the wave's 64 rows of a panel (64 columns: a stage); rows past the end are
+  // backward: the wave's 64 rows of a panel (32 columns: a block); rows past the end are
   // past the resource
   const int rows_here = (int)uniform(a.m - m0 < 64 ? (a.m - m0 < 0 ? 0 : a.m - m0) : 64);
-  const int64_t out0 = uniform(reinterpret_cast<int64_t>(a.out) + (first * a.m + m0) * 128);
-  const uint32_t out_off = (uint32_t)((lane & 15) * 128 + (lane >> 4 & 1) * 32 + (lane >> 5) * 16);
+  const int64_t out0 = uniform(reinterpret_cast<int64_t>(a.out) + (first * 2 * a.m + m0) * 64);
+  const uint32_t out_off = (uint32_t)((lane & 15) * 64 + (lane >> 4 & 1) * 32 + (lane >> 5) * 16);
 
   fill(1);  // both buffers are free at the start
 
@@ -212,7 +213,7 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
           w[k + 2 + u] = t[1];
         }
       // rows: store r covers rows 16 r + lane % 16, columns 16 (lane / 16 % 2) + 8 (lane /
-      // 32) .., 64 consecutive bytes of each row
+      // 32) ..: 1 KB of a panel
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const auto t = __builtin_amdgcn_permlane16_swap(w[k], w[k + 4], false, false);
@@ -226,10 +227,10 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
         // leaves no wait state between a 16-byte store and the next write of its data
         // registers, and lanes 12 .. 15 of each 16 stored what came after.  Streaming.
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            reinterpret_cast<char*>(out0 + (int64_t)(col >> 6) * a.m * 128), 0, rows_here * 128,
+            reinterpret_cast<char*>(out0 + (int64_t)(col >> 5) * a.m * 64), 0, rows_here * 64,
             kRsrcWord3);
         __builtin_amdgcn_raw_buffer_store_b128(
-            v, rsrc, (int)(out_off + (uint32_t)((i * 32 + r * 16) * 128 + (col & 63) * 2)), 0, 2);
+            v, rsrc, (int)(out_off + (uint32_t)((i * 32 + r * 16) * 64)), 0, 2);
       }
     }
   };

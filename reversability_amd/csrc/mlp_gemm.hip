@@ -212,38 +212,40 @@ struct Dma {
       off[it] = (uint32_t)((krow * ld + chunk * 8) * 2);
     }
   }
-  // Panels (the tied head's logit gradients): [columns / 64][rows][64], so that what a
-  // workgroup writes or reads of 64 columns is contiguous.  `panel` elements each.
-  // As a KC source (k = the columns, BK = 64) a stage is one panel.
+  // Panels (the tied head's logit gradients): [columns / 32][rows][32], so that what a
+  // store instruction of head_stream_k writes (16 rows of a 32-column block) is one
+  // contiguous KB and what a load here reads is at least 128 bytes of a panel.  `panel`
+  // elements each.  As a KC source (k = the columns, BK = 64) a stage is two panels.
   template <class Map>
   __device__ __forceinline__ void init_kc_panel(const __half* p, int64_t bytes, int64_t panel,
                                                 const Map& map, int64_t kbeg, int wave, int lane) {
-    static_assert(RC || BK == 64, "a stage is a panel");
-    const int64_t first = map.origin() * 64 + kbeg / 64 * panel;
+    static_assert(RC || BK == 64, "a stage is two panels");
+    const int64_t first = map.origin() * 32 + kbeg / 32 * panel;
     base = uniform(reinterpret_cast<int64_t>(p + first));
     left = uniform(bytes - first * 2);
-    kstep = panel * 2;
+    kstep = panel * 4;
 #pragma unroll
     for (int it = 0; it < kPerWave; ++it) {
       const int row = (it * WAVES + wave) * kRows + lane / kChunks;
-      off[it] = (uint32_t)((map(row) * 64 + ((lane % kChunks) ^ f_kc<BK>(row)) * 8) * 2);
+      const int chunk = (lane % kChunks) ^ f_kc<BK>(row);
+      off[it] = (uint32_t)((chunk / 4 * panel + map(row) * 32 + chunk % 4 * 8) * 2);
     }
   }
-  // As an RC source (k = the rows): a tile's columns row0 .. are ROWS / 64 panels of
+  // As an RC source (k = the rows): a tile's columns row0 .. are ROWS / 32 panels of
   // `panels`.  Rows past the end read the next panel (the other operand's are zero).
   __device__ __forceinline__ void init_rc_panel(const __half* p, int64_t bytes, int64_t panel,
                                                 int64_t panels, int64_t row0, int64_t kbeg,
                                                 int wave, int lane) {
-    const int64_t first = row0 / 64 * panel + kbeg * 64;
+    const int64_t first = row0 / 32 * panel + kbeg * 32;
     base = uniform(reinterpret_cast<int64_t>(p + first));
     left = uniform(bytes - first * 2);
-    kstep = BK * 64 * 2;
+    kstep = BK * 32 * 2;
 #pragma unroll
     for (int it = 0; it < kPerWave; ++it) {
       const int b = (it * WAVES + wave) * 1024 + lane * 16;
       const int krow = b / (ROWS * 2), chunk = ((b % (ROWS * 2)) >> 4) ^ f_rc<ROWS>(krow);
-      off[it] = row0 / 64 + chunk / 8 < panels
-                    ? (uint32_t)((chunk / 8 * panel + krow * 64 + chunk % 8 * 8) * 2)
+      off[it] = row0 / 32 + chunk / 4 < panels
+                    ? (uint32_t)((chunk / 4 * panel + krow * 32 + chunk % 4 * 8) * 2)
                     : 0x80000000u;  // past the columns: zeros
     }
   }
@@ -896,7 +898,7 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
             if (col + e >= args.valid)
               dw[e >> 1] = (e & 1) ? dw[e >> 1] & 0xffffu : dw[e >> 1] & 0xffff0000u;
         }
-        const int64_t to = EPI == Epi::LogProbGrad ? col / 64 * args.panel + row * 64 + col % 64
+        const int64_t to = EPI == Epi::LogProbGrad ? col / 32 * args.panel + row * 32 + col % 32
                                                    : row * args.ldc + col;
         __builtin_nontemporal_store(dw, reinterpret_cast<u32x4*>(static_cast<__half*>(args.c) + to));
       }
@@ -2393,7 +2395,7 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
                        (const int64_t*)nullptr, (int64_t)wgs, ignore_index, tops, scale);
   }
   GemmArgs z = logp_args(x, head, rows, d, padded, labels, ignore_index, vocab);
-  z.c = dlogits; z.valid = vocab; z.panel = rows * 64; z.panels = padded / 64;
+  z.c = dlogits; z.valid = vocab; z.panel = rows * 32; z.panels = padded / 32;
   z.head.lse = lse; z.head.grad = grad; z.head.scale = scale;
   int st;
   if (stream_takes(d)) {
