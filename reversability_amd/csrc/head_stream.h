@@ -200,6 +200,12 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
         for (int e = 0; e < 16; ++e)
           if (e == e0) z[i][e] += g[i];
       }
+      if (col0 + col + 32 > a.head_logp.vocab) {  // pad columns: zero, whatever the row's g
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (col0 + col + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3) >= a.head_logp.vocab)
+            z[i][e] = 0.f;
+      }
       uint32_t w[8];  // pairs of columns; word 2 q + k: columns 8 q + cq + 2 k
 #pragma unroll
       for (int k = 0; k < 8; ++k) w[k] = pack2<BF>(z[i][2 * k], z[i][2 * k + 1]);

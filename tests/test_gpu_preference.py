@@ -209,6 +209,23 @@ def test_logprobs_special_labels_and_values(cuda_device):
     assert bool(((same + math.log(1000)).abs() <= 2.0 ** -15 + 2.0 ** -23 * 7).all())
 
 
+@pytest.mark.parametrize("d", [64, 256, 512])
+def test_pad_rows_of_the_head_get_zeros(cuda_device, d):
+    """Whatever they hold, and beside rows whose gradients are NaN."""
+    x, head, labels, grad = head_inputs(40, d, 70, torch.float16, pad=192)
+    with torch.no_grad():
+        head[70:] = math.nan
+    labels[3] = 70
+    x.requires_grad_(True)
+    head.requires_grad_(True)
+    logp = tied_head_logprobs(x, head, 70, labels)
+    dx, dhead = torch.autograd.grad(logp, (x, head), grad)
+    assert torch.isnan(logp[3]) and torch.isnan(dx[3]).all() and torch.isnan(dhead[:70]).all()
+    assert not torch.isnan(torch.cat([logp[:3], logp[4:]])).any()
+    assert not torch.isnan(torch.cat([dx[:3], dx[4:]])).any()
+    assert not dhead[70:].any() and not torch.isnan(dhead[70:]).any()
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e-5, 1.0, 1e4])
 def test_logprobs_gradients_of_any_size(cuda_device, scale):
     """Small gradients do not vanish in the 16-bit logit gradients (bf16 operands hold
