@@ -17,7 +17,10 @@ and bias corrections live on the device), gradients set to ``None`` at the
 start of the step (so the captured backward writes them rather than adding
 to stale ones), and no ``hipMemsetAsync`` inside (none of this library's entry
 points records one; the embedding backward's rocPRIM sort takes its
-memset-free merge path up to 2^20 tokens).  The GEMM tile-shape tuner never
+memset-free merge path up to 2^20 tokens).  While it is captured, no graph of
+an eager call on the same leaves may be alive (a loss that was kept, not
+detached): its gradient accumulation belongs to the eager stream, and a backward
+pass that reaches it from the captured one ends the process.  The GEMM tile-shape tuner never
 runs during capture: captured calls use the shapes the warm-up calls chose.
 
 Everything the graph touches must outlive it: the step's parameters,
