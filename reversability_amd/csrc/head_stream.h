@@ -29,6 +29,10 @@
 // Included by mlp_gemm.hip, whose staging, LDS and epilogue helpers it uses.
 #pragma once
 
+// What the kernel leaves behind: log-probabilities' statistics, the logits' gradients in 16
+// bits, or those and what the 16 bits left out.
+enum class Stream { Logp, Grad, GradLow };
+
 struct StreamArgs {
   const __half* x;        // [m][d]
   const __half* head;     // [n][d]
@@ -36,15 +40,17 @@ struct StreamArgs {
   int64_t stages, chunk;  // stages of 64 columns in all, and per workgroup
   int64_t tiles_m, tiles; // workgroups: 256 rows x chunk stages, tiles_m fastest
   float2* part;           // forward: [tile column][m]
-  __half* out;            // backward: panels [n / 32][m][32]
+  __half* out;            // backward: panels [n / 32][panel_rows][32]
   HeadLogp head_logp;
+  int64_t panel_rows;     // m, or 2 m with the rows' remainders behind them
 };
 
 // One lane's 16-byte chunk address in a stage: column (row of the head) c, 16-byte
 // chunk q is at c * 32 KS + ((q ^ (c & 15)) * 16): the columns' reads of one chunk
 // fall on different banks.
-template <int KS, bool BF, bool GRAD>
+template <int KS, bool BF, Stream MODE>
 __device__ __forceinline__ void head_stream(const StreamArgs& a) {
+  constexpr bool GRAD = MODE != Stream::Logp;
   constexpr int kRow = KS * 32;              // bytes of a column in LDS
   constexpr int kStage = 64 * kRow;          // bytes of a stage
   constexpr int kDma = kStage / 1024 / 4;    // loads per wave and stage
@@ -137,7 +143,7 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
   // backward: the wave's 64 rows of a panel (32 columns: a block); rows past the end are
   // past the resource
   const int rows_here = (int)uniform(a.m - m0 < 64 ? (a.m - m0 < 0 ? 0 : a.m - m0) : 64);
-  const int64_t out0 = uniform(reinterpret_cast<int64_t>(a.out) + (first * 2 * a.m + m0) * 64);
+  const int64_t out0 = uniform(reinterpret_cast<int64_t>(a.out) + (first * 2 * a.panel_rows + m0) * 64);
   const uint32_t out_off = (uint32_t)((lane & 15) * 64 + (lane >> 4 & 1) * 32 + (lane >> 5) * 16);
 
   fill(1);  // both buffers are free at the start
@@ -187,9 +193,44 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
       asm volatile("" : "+v"(sum[i]));
     }
   };
-  // After its values: the label's part, the 16-bit results and their stores.  A lane
+  // The 16-bit results of row block i and their stores to the panels at `to`.  A lane
   // holds 4 consecutive columns of each 8; the swap of the halves' odd and even
   // groups leaves it 8 consecutive ones of each 16.
+  auto put = [&](const f32x16 (&z)[2], int i, int col, int64_t to) __attribute__((always_inline)) {
+    uint32_t w[8];  // pairs of columns; word 2 q + k: columns 8 q + cq + 2 k
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = pack2<BF>(z[i][2 * k], z[i][2 * k + 1]);
+    // halves: word 4 h + k holds columns 16 h + 8 (lane / 32) + 2 k of its row
+#pragma unroll
+    for (int k = 0; k < 8; k += 4)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const auto t = __builtin_amdgcn_permlane32_swap(w[k + u], w[k + 2 + u], false, false);
+        w[k + u] = t[0];
+        w[k + 2 + u] = t[1];
+      }
+    // rows: store r covers rows 16 r + lane % 16, columns 16 (lane / 16 % 2) + 8 (lane /
+    // 32) ..: 1 KB of a panel
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const auto t = __builtin_amdgcn_permlane16_swap(w[k], w[k + 4], false, false);
+      w[k] = t[0];
+      w[k + 4] = t[1];
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const u32x4 v = {w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]};
+      // all of the offset in the vector register: with a scalar part the compiler
+      // leaves no wait state between a 16-byte store and the next write of its data
+      // registers, and lanes 12 .. 15 of each 16 stored what came after.  Streaming.
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          reinterpret_cast<char*>(to + (int64_t)(col >> 5) * a.panel_rows * 64), 0, rows_here * 64,
+          kRsrcWord3);
+      __builtin_amdgcn_raw_buffer_store_b128(
+          v, rsrc, (int)(out_off + (uint32_t)((i * 32 + r * 16) * 64)), 0, 2);
+    }
+  };
+  // After its values: the label's part and the results.
   auto close = [&](f32x16 (&z)[2], int i, int col) __attribute__((always_inline)) {
     if constexpr (GRAD) {
       const int c = label[i] - col;
@@ -206,37 +247,11 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
           if (col0 + col + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3) >= a.head_logp.vocab)
             z[i][e] = 0.f;
       }
-      uint32_t w[8];  // pairs of columns; word 2 q + k: columns 8 q + cq + 2 k
+      put(z, i, col, out0);
+      if constexpr (MODE == Stream::GradLow) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = pack2<BF>(z[i][2 * k], z[i][2 * k + 1]);
-      // halves: word 4 h + k holds columns 16 h + 8 (lane / 32) + 2 k of its row
-#pragma unroll
-      for (int k = 0; k < 8; k += 4)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const auto t = __builtin_amdgcn_permlane32_swap(w[k + u], w[k + 2 + u], false, false);
-          w[k + u] = t[0];
-          w[k + 2 + u] = t[1];
-        }
-      // rows: store r covers rows 16 r + lane % 16, columns 16 (lane / 16 % 2) + 8 (lane /
-      // 32) ..: 1 KB of a panel
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const auto t = __builtin_amdgcn_permlane16_swap(w[k], w[k + 4], false, false);
-        w[k] = t[0];
-        w[k + 4] = t[1];
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const u32x4 v = {w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]};
-        // all of the offset in the vector register: with a scalar part the compiler
-        // leaves no wait state between a 16-byte store and the next write of its data
-        // registers, and lanes 12 .. 15 of each 16 stored what came after.  Streaming.
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            reinterpret_cast<char*>(out0 + (int64_t)(col >> 5) * a.m * 64), 0, rows_here * 64,
-            kRsrcWord3);
-        __builtin_amdgcn_raw_buffer_store_b128(
-            v, rsrc, (int)(out_off + (uint32_t)((i * 32 + r * 16) * 64)), 0, 2);
+        for (int e = 0; e < 16; ++e) z[i][e] -= round16<BF>(z[i][e]);
+        put(z, i, col, out0 + a.head_logp.low * 64);
       }
     }
   };
@@ -289,8 +304,8 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
   // Stage st: `begun` once a block is waiting for its exponentials.
   auto stage = [&](int st, auto begun) __attribute__((always_inline)) {
     // this wave's loads of the stage have to have landed.  Newer than them are, in the
-    // backward, the stores of two blocks (of one in the second stage), four a block,
-    // always issued in full
+    // backward, the stores of two blocks (of one in the second stage), four a block or
+    // eight (then the wait is for some of them too), always issued in full
     if constexpr (!decltype(begun)::value) wait_vmcnt<kDma>();  // the next stage's
     else if (GRAD && live && st > 1) wait_vmcnt<8>();
     else if (GRAD && live) wait_vmcnt<4>();
@@ -329,8 +344,8 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
   }
 }
 
-template <int KS, bool BF, bool GRAD>
+template <int KS, bool BF, Stream MODE>
 __global__ __launch_bounds__(256, 2)
 void head_stream_k(StreamArgs a) {
-  head_stream<KS, BF, GRAD>(a);
+  head_stream<KS, BF, MODE>(a);
 }

@@ -357,6 +357,7 @@ enum class Epi {
   // the tied head's log-probabilities (HeadLogp):
   LogProb,        // c = float2 [tile column][m]: a row's maximum and sum of exp over the tile
   LogProbGrad,    // c 16-bit, panels = scaled gradient of the logits
+  LogProbLow,     // what LogProbGrad's 16 bits leave out, in 16 bits
   StoreScaled,    // c 16-bit = acc * *scale, a in panels
   AccF32Scaled,   // c fp32 (+)= acc * *scale, a in panels
   PartialRagged,  // PartialF32 whose tiles may pass column n, a in panels
@@ -377,6 +378,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// A value as pack2 rounds it.
+template <bool BF>
+__device__ __forceinline__ float round16(float v) {
+  if constexpr (BF) return (float)(__bf16)v;
+  else return __half2float(__float2half_rn(v));
+}
+
 // What the tied head's log-probability epilogues read and write beside the
 // product (rows and labels of the chunk at hand).
 struct HeadLogp {
@@ -386,6 +394,7 @@ struct HeadLogp {
   const float* lse;        // LogProbGrad, [m]: log sum exp of the row
   const float* grad;       // LogProbGrad, [m]: gradient of the row's log-probability
   const float* scale;      // LogProbGrad: *scale multiplies the gradient; Scaled: the result
+  int64_t low;             // head_stream_k: what a row's 16 bits leave out goes to row + low
 };
 
 constexpr int kSplitStep = 64;  // weight gradients: granularity of a split's token range
@@ -795,7 +804,10 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
     // per training step of the two decoders, consumers included.
     constexpr int S = WN + 8;
     _Float16* stage = lds + wave * (WM * S);
-    if constexpr (EPI == Epi::LogProbGrad) {
+    constexpr bool kLogits = EPI == Epi::LogProbGrad || EPI == Epi::LogProbLow;
+    if constexpr (kLogits) {
+      // (LogProbLow is a launch of its own: both halves in one epilogue spilled the
+      // accumulators, 1554 x 512 over 32000 94 -> 330 us.)
       // acc = s ([j == label] - exp(z - lse)), s = the row's gradient times *scale (32768 x
       // 1024 over 50257 3.44 ms with 3.3 GB of stores, 980 TFLOP/s)
       const float scale = *args.head.scale;
@@ -824,6 +836,12 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               if (at == j * 16 + e) acc[i][j][e] += s;
+        }
+        if constexpr (EPI == Epi::LogProbLow) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] -= round16<BF>(acc[i][j][e]);
         }
       }
     }
@@ -898,8 +916,8 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
             if (col + e >= args.valid)
               dw[e >> 1] = (e & 1) ? dw[e >> 1] & 0xffffu : dw[e >> 1] & 0xffff0000u;
         }
-        const int64_t to = EPI == Epi::LogProbGrad ? col / 32 * args.panel + row * 32 + col % 32
-                                                   : row * args.ldc + col;
+        const int64_t to = kLogits ? col / 32 * args.panel + row * 32 + col % 32
+                                   : row * args.ldc + col;
         __builtin_nontemporal_store(dw, reinterpret_cast<u32x4*>(static_cast<__half*>(args.c) + to));
       }
     } else {
@@ -1017,7 +1035,8 @@ static_assert(kNumShapes == 7 && kRuleShapes == 4, "instantiations above");
   RV_LOGP_DW(0, BF) RV_LOGP_DW(1, BF) RV_LOGP_DW(2, BF) RV_LOGP_DW(3, BF)
 #define RV_LOGP_Z(SHAPE, BF)                                                                \
   template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProb, BF>(GemmArgs);     \
-  template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProbGrad, BF>(GemmArgs);
+  template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProbGrad, BF>(GemmArgs); \
+  template __global__ void gemm_kernel<SHAPE, false, false, Epi::LogProbLow, BF>(GemmArgs);
 #define RV_LOGP_DX(SHAPE, BF)                                                               \
   template __global__ void gemm_kernel<SHAPE, false, true, Epi::StoreScaled, BF>(GemmArgs);  \
   template __global__ void gemm_kernel<SHAPE, false, true, Epi::PartialRagged, BF>(GemmArgs);
@@ -1026,12 +1045,11 @@ static_assert(kNumShapes == 7 && kRuleShapes == 4, "instantiations above");
   template __global__ void gemm_kernel<SHAPE, true, true, Epi::AccF32Scaled, BF>(GemmArgs);  \
   template __global__ void gemm_kernel<SHAPE, true, true, Epi::PartialRagged, BF>(GemmArgs);
 RV_LOGP_KERNELS(false) RV_LOGP_KERNELS(true)
-#define RV_STREAM_KERNELS(KS)                                       \
-  template __global__ void head_stream_k<KS, false, false>(StreamArgs); \
-  template __global__ void head_stream_k<KS, false, true>(StreamArgs);  \
-  template __global__ void head_stream_k<KS, true, false>(StreamArgs);  \
-  template __global__ void head_stream_k<KS, true, true>(StreamArgs);
-RV_STREAM_KERNELS(8) RV_STREAM_KERNELS(16)
+#define RV_STREAM_KERNELS(KS, MODE)                                           \
+  template __global__ void head_stream_k<KS, false, Stream::MODE>(StreamArgs); \
+  template __global__ void head_stream_k<KS, true, Stream::MODE>(StreamArgs);
+RV_STREAM_KERNELS(8, Logp) RV_STREAM_KERNELS(8, Grad) RV_STREAM_KERNELS(8, GradLow)
+RV_STREAM_KERNELS(16, Logp) RV_STREAM_KERNELS(16, Grad) RV_STREAM_KERNELS(16, GradLow)
 
 // acc[i] (+)= fp32(fp16(sum_s part[s][i])), splits summed in order.  This is
 // autocast's weight gradient: the fp16 GEMM result, cast to the fp32 weight
@@ -1977,7 +1995,7 @@ int64_t stream_chunk(int64_t rows, int64_t n) {
   }
   return best;
 }
-template <bool GRAD>
+template <Stream MODE>
 int launch_stream(StreamArgs a, int dtype, hipStream_t s) {
   a.stages = (a.n + 63) / 64;
   a.chunk = stream_chunk(a.m, a.n);
@@ -1986,7 +2004,7 @@ int launch_stream(StreamArgs a, int dtype, hipStream_t s) {
   const int64_t blocks = (a.tiles + 7) / 8 * 8;
   if (blocks * 256 >= (int64_t)1 << 32) return RV_ERR_UNSUPPORTED;  // threads a launch holds
   const dim3 grid((unsigned)blocks), block(256);
-#define RV_LAUNCH(KS, BF) hipLaunchKernelGGL((head_stream_k<KS, BF, GRAD>), grid, block, 0, s, a)
+#define RV_LAUNCH(KS, BF) hipLaunchKernelGGL((head_stream_k<KS, BF, MODE>), grid, block, 0, s, a)
   if (a.d <= 128) {
     if (dtype == RV_BF16) RV_LAUNCH(8, true);
     else RV_LAUNCH(8, false);
@@ -2330,7 +2348,7 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
   const hipStream_t s = (hipStream_t)stream;
   int st;
   if (stream_takes(d)) {
-    st = launch_stream<false>({a.a, a.b, rows, vocab, d, 0, 0, 0, 0, part, nullptr, a.head}, dtype,
+    st = launch_stream<Stream::Logp>({a.a, a.b, rows, vocab, d, 0, 0, 0, 0, part, nullptr, a.head, 0}, dtype,
                               s);
   } else {
     const int shape = logp_z_shape(rows, d, vocab);
@@ -2350,15 +2368,38 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
 // The backward's workspace starts with the scale, its inverse and the rows' tops.
 constexpr int64_t kLogpHeader = 256 + kScaleTops * sizeof(float);
 
+// Rows whose logits' gradients are held as two 16-bit numbers, the rounded value and what
+// it left out: a row's gradients are mostly its label's, one rounding, as large as the
+// results' own.  Over many rows that adds up to 1.4 times the error of gradients in fp32;
+// over few it may be far more of theirs.  The remainders are rows of their own behind
+// the others in both products (51 x 256 over 50257 fp16: error 4e-4 -> 2e-4).
+constexpr int64_t kFineRows = 1024;
+bool logp_fine(int64_t rows) { return rows <= kFineRows; }
+
+// x twice, for the remainders' share of dw.  n % 8 == 0 elements.
+__global__ __launch_bounds__(256)
+void twice_k(const uint4* __restrict__ x, int64_t vecs, uint4* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= vecs) return;
+  const uint4 v = x[i];
+  out[i] = v;
+  out[vecs + i] = v;
+}
+
 int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded) {
   const int bad = logp_check(rows, d, vocab, padded, RV_F16);
   if (bad) return -(int64_t)bad;
   // a tile's panels stay within 32-bit offsets
   if (rows > (int64_t)1 << 22) return -(int64_t)RV_ERR_UNSUPPORTED;
-  const WgradPlan p = plan_wgrad(rows, padded, up128(d), true);
+  const bool fine = logp_fine(rows);
+  const int64_t k = fine ? 2 * rows : rows;
+  const WgradPlan p = plan_wgrad(k, padded, up128(d), true);
   if (p.shape < 0) return -(int64_t)RV_ERR_UNSUPPORTED;
-  const int64_t dx = logp_dx_bytes(rows, d, padded), dw = part_bytes(p, padded, up128(d));
-  return kLogpHeader + align256(rows * padded * 2) + (dx > dw ? dx : dw);
+  const int64_t dx = fine ? logp_dx_plan(k, d, padded).splits * k * d * 4
+                          : logp_dx_bytes(rows, d, padded);
+  const int64_t dw = part_bytes(p, padded, up128(d));
+  return kLogpHeader + align256(k * padded * 2) + (fine ? align256(k * d * 2) : 0) +
+         (dx > dw ? dx : dw);
 }
 
 int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
@@ -2377,13 +2418,17 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
   if (!workspace || workspace_bytes < need || !ok16(workspace)) return RV_ERR_WORKSPACE;
   const hipStream_t s = (hipStream_t)stream;
   const bool bf = dtype == RV_BF16;
-  // workspace: the scale and its inverse, the logits' gradients in panels, the
-  // products' partial sums
+  // workspace: the scale and its inverse, the logits' gradients in panels (k rows), x
+  // twice if they have remainders, the products' partial sums
+  const bool fine = logp_fine(rows);
+  const int64_t k = fine ? 2 * rows : rows;
   float* scale = static_cast<float*>(workspace);
   float* tops = scale + 64;
   __half* dlogits = reinterpret_cast<__half*>(static_cast<char*>(workspace) + kLogpHeader);
-  float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kLogpHeader +
-                                         align256(rows * padded * 2));
+  __half* x2 = reinterpret_cast<__half*>(static_cast<char*>(workspace) + kLogpHeader +
+                                         align256(k * padded * 2));
+  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(x2) +
+                                         (fine ? align256(k * d * 2) : 0));
   if (rows <= kScaleRows) {
     hipLaunchKernelGGL(logprob_scale<true>, dim3(1), dim3(1024), 0, s, grad, labels, rows,
                        ignore_index, tops, scale);
@@ -2395,27 +2440,32 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
                        (const int64_t*)nullptr, (int64_t)wgs, ignore_index, tops, scale);
   }
   GemmArgs z = logp_args(x, head, rows, d, padded, labels, ignore_index, vocab);
-  z.c = dlogits; z.valid = vocab; z.panel = rows * 32; z.panels = padded / 32;
-  z.head.lse = lse; z.head.grad = grad; z.head.scale = scale;
+  z.c = dlogits; z.valid = vocab; z.panel = k * 32; z.panels = padded / 32;
+  z.head.lse = lse; z.head.grad = grad; z.head.scale = scale; z.head.low = fine ? rows : 0;
   int st;
   if (stream_takes(d)) {
-    st = launch_stream<true>({z.a, z.b, rows, padded, d, 0, 0, 0, 0, nullptr, dlogits, z.head},
-                             dtype, s);
+    const StreamArgs t{z.a, z.b, rows, padded, d, 0, 0, 0, 0, nullptr, dlogits, z.head, k};
+    st = fine ? launch_stream<Stream::GradLow>(t, dtype, s) : launch_stream<Stream::Grad>(t, dtype, s);
   } else {
     const int shape = logp_z_shape(rows, d, padded);
     st = bf ? launch_logp<false, false, Epi::LogProbGrad, true>(shape, z, s)
             : launch_logp<false, false, Epi::LogProbGrad, false>(shape, z, s);
+    if (fine && st == RV_OK) {  // the remainders, of the same product again
+      z.c = dlogits + rows * 32;
+      st = bf ? launch_logp<false, false, Epi::LogProbLow, true>(shape, z, s)
+              : launch_logp<false, false, Epi::LogProbLow, false>(shape, z, s);
+    }
   }
   if (st != RV_OK) return st;
   if (dx) {
-    const DxPlan p = logp_dx_plan(rows, d, padded);
+    const DxPlan p = logp_dx_plan(k, d, padded);
     GemmArgs a{};
-    a.a = dlogits; a.a_bytes = rows * padded * 2; a.panel = z.panel; a.panels = z.panels;
+    a.a = dlogits; a.a_bytes = k * padded * 2; a.panel = z.panel; a.panels = z.panels;
     a.b = static_cast<const __half*>(head); a.ldb = d;  // B(d, v) = head[v][d]: RC
     a.b_bytes = vocab * d * 2;  // the operand ends here: the pad rows read as zero
-    a.m = rows; a.n = d; a.k = padded; a.k_chunk = p.chunk;
+    a.m = k; a.n = d; a.k = padded; a.k_chunk = p.chunk;
     a.ldc = d; a.head.scale = scale + 1;
-    if (p.splits == 1) {
+    if (p.splits == 1 && !fine) {
       a.c = dx;
       st = bf ? launch_logp<false, true, Epi::StoreScaled, true>(p.shape, a, s)
               : launch_logp<false, true, Epi::StoreScaled, false>(p.shape, a, s);
@@ -2424,14 +2474,22 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
       st = bf ? launch_logp<false, true, Epi::PartialRagged, true>(p.shape, a, s)
               : launch_logp<false, true, Epi::PartialRagged, false>(p.shape, a, s);
       if (st == RV_OK)
-        st = launch_scaled_reduce(dtype, part, dx, rows * d, p.splits, scale + 1, 0, s);
+        // the remainders' sums follow the rows' own in each split
+        st = launch_scaled_reduce(dtype, part, dx, rows * d, p.splits * (fine ? 2 : 1), scale + 1,
+                                  0, s);
     }
     if (st != RV_OK) return st;
   }
   if (dw) {
     // dW[v][d] = sum_m dlogits[m][v] x[m][d]; of the pad rows the sum of zeros
-    const WgradPlan p = plan_wgrad(rows, padded, up128(d), true);
-    WgradJob j = plan_job(p, dlogits, padded, static_cast<const __half*>(x), d, rows, dw_rows, d,
+    const WgradPlan p = plan_wgrad(k, padded, up128(d), true);
+    if (fine) {
+      const int64_t vecs = rows * d / 8;
+      hipLaunchKernelGGL(twice_k, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s,
+                         static_cast<const uint4*>(x), vecs, reinterpret_cast<uint4*>(x2));
+    }
+    WgradJob j = plan_job(p, dlogits, padded, fine ? x2 : static_cast<const __half*>(x), d, k,
+                          dw_rows, d,
                           static_cast<float*>(dw), accumulate, part);
     j.g.panel = z.panel; j.g.panels = z.panels; j.g.head.scale = scale + 1;
     if (p.splits == 1) {

@@ -50,9 +50,11 @@ def head_inputs(rows, d, vocab, dtype, seed=0, pad=0, spread=2.0, scale=1.0):
     return x, head, labels, grad
 
 
-def exact_logp(x, head, vocab, labels, grad=None):
-    """(logp, bound, dx, dx bound, dhead, dhead bound) in 64 bits."""
+def exact_logp(x, head, vocab, labels, grad=None, held=None):
+    """(logp, bound, dx, dx bound, dhead, dhead bound) in 64 bits; ``held``: how far the
+    logits' gradients are off as they are held (None: their type's rounding)."""
     u = U[x.dtype]
+    held = held or u
     x, w = x.double(), head[:vocab].double()
     valid = labels != -100
     z = x @ w.t()
@@ -71,7 +73,7 @@ def exact_logp(x, head, vocab, labels, grad=None):
     dz.scatter_add_(1, labels.clamp_min(0)[:, None], g)
     # the error of a logit gradient
     floor = g.abs().max() * 2.0 ** -39
-    ddz = dz.abs() * u + (p * g.abs()) * (bound + 2.0 ** -22)[:, None] + floor * valid[:, None]
+    ddz = dz.abs() * held + (p * g.abs()) * (bound + 2.0 ** -22)[:, None] + floor * valid[:, None]
     dx, dhead = dz @ w, torch.zeros(head.shape, device="cuda", dtype=torch.float64)
     dhead[:vocab] = dz.t() @ x
     bx = ddz @ w.abs() + vocab * 2.0 ** -24 * (dz.abs() @ w.abs()) + u * dx.abs() + 1e-30
@@ -112,6 +114,27 @@ def test_logprobs_and_gradients(cuda_device, rows, d, vocab, dtype):
         assert torch.equal(tied_head_logprobs(x, head, vocab, labels), logp)
     again = torch.autograd.grad(tied_head_logprobs(x, head, vocab, labels), (x, head), grad)
     assert torch.equal(again[0], dx) and torch.equal(again[1], dhead)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,d,vocab", [(1, 64, 777), (3, 256, 5000), (51, 512, 5000), (51, 96, 64),
+                                          (700, 640, 20000), (1024, 256, 20000), (513, 8, 300)])
+def test_few_rows_hold_their_gradients_twice_as_long(cuda_device, rows, d, vocab, dtype):
+    """Up to 1024 rows a logit's gradient is a 16-bit number and the 16-bit number of
+    what that left out: off by u^2, so that the results are off by their own rounding."""
+    x, head, labels, grad = head_inputs(rows, d, vocab, dtype, seed=rows)
+    x.requires_grad_(True)
+    head.requires_grad_(True)
+    dx, dhead = torch.autograd.grad(tied_head_logprobs(x, head, vocab, labels), (x, head), grad)
+    _, _, rx, bx, rh, bh = exact_logp(x.detach(), head.detach(), vocab, labels, grad,
+                                      held=U[dtype] ** 2)
+    within(dx, rx, bx)
+    within(dhead, rh, bh)
+    # the whole of it: a rounding's error is at most u and 0.58 of it on average (a uniform
+    # one), where one of the gradient and one of the result make 0.82
+    for got, ref in ((dx, rx), (dhead, rh)):
+        if rows >= 51:
+            assert float((got.double() - ref).norm()) <= 0.6 * U[dtype] * float(ref.norm())
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
