@@ -377,7 +377,7 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
  * another label outside [0, vocab) NaN.  padded, a multiple of 64, is the row count
  * of head; dw_rows is vocab or padded (pad rows: sums of zeros).  dz is held in dtype
  * in the workspace, times a power of two that brings the largest |grad| of a row
- * with a label to [2^14, 2^15); up to 1024 rows as two such numbers, the rounded one
+ * with a label to [2^14, 2^15); up to 512 rows as two such numbers, the rounded one
  * and what it left out.  rows <= 2^22. */
 int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded);
 int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,

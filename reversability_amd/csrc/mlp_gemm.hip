@@ -2370,10 +2370,11 @@ constexpr int64_t kLogpHeader = 256 + kScaleTops * sizeof(float);
 
 // Rows whose logits' gradients are held as two 16-bit numbers, the rounded value and what
 // it left out: a row's gradients are mostly its label's, one rounding, as large as the
-// results' own.  Over many rows that adds up to 1.4 times the error of gradients in fp32;
-// over few it may be far more of theirs.  The remainders are rows of their own behind
-// the others in both products (51 x 256 over 50257 fp16: error 4e-4 -> 2e-4).
-constexpr int64_t kFineRows = 1024;
+// results' own.  Over many rows that adds up to 1.4 times the error of gradients in fp32
+// (1.33 to 1.41 where measured); over few it varies with their labels' (1.6 seen).  The remainders are rows of their own behind the others in both
+// products: logits, dx and dw of 300 x 256 over 50257 118 -> 146 us, 512 x 512 over 32000 140
+// -> 202, 1024 x 1024 over 50257 534 -> 823, so only where they are needed.
+constexpr int64_t kFineRows = 512;
 bool logp_fine(int64_t rows) { return rows <= kFineRows; }
 
 // x twice, for the remainders' share of dw.  n % 8 == 0 elements.

@@ -168,7 +168,7 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     gradients too).  Products are summed in fp32 and the logits never rounded.  The
     backward holds ``chunk_tokens`` tokens' logit gradients in 16 bits at a time
     (default: as many as fill GRADIENT_BYTES), scaled by a power of two so that small
-    gradients survive (up to 1024 tokens as two 16-bit numbers each); gradients come in the operands' type.  As in any product,
+    gradients survive (up to 512 tokens as two 16-bit numbers each); gradients come in the operands' type.  As in any product,
     a NaN or an infinity in an unscored token's row of ``x16`` reaches the gradient of
     the head.
     """

@@ -118,9 +118,9 @@ def test_logprobs_and_gradients(cuda_device, rows, d, vocab, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows,d,vocab", [(1, 64, 777), (3, 256, 5000), (51, 512, 5000), (51, 96, 64),
-                                          (700, 640, 20000), (1024, 256, 20000), (513, 8, 300)])
+                                          (400, 640, 20000), (512, 256, 20000), (511, 8, 300)])
 def test_few_rows_hold_their_gradients_twice_as_long(cuda_device, rows, d, vocab, dtype):
-    """Up to 1024 rows a logit's gradient is a 16-bit number and the 16-bit number of
+    """Up to 512 rows a logit's gradient is a 16-bit number and the 16-bit number of
     what that left out: off by u^2, so that the results are off by their own rounding."""
     x, head, labels, grad = head_inputs(rows, d, vocab, dtype, seed=rows)
     x.requires_grad_(True)
