@@ -61,20 +61,38 @@ class FusedAdamW(Optimizer):
                 raise ValueError("FusedAdamW requires dense CUDA (ROCm device) FP32 parameters")
         if not params:
             return None, []
-        step = None
+        step, dev = None, params[0].device
         for p in group["params"]:
             st = self.state[p]
             if "step" in st:
                 step = st["step"]
                 break
         if step is None:
-            step = torch.zeros((), device=params[0].device, dtype=torch.float32)
+            step = torch.zeros((), device=dev, dtype=torch.float32)
+        # the kernels read these through their addresses
+        elif not torch.is_tensor(step) or step.dtype != torch.float32 or step.device != dev:
+            raise ValueError("FusedAdamW's state needs its step count as an fp32 tensor on the "
+                             "parameters' device")
         for p in params:
             st = self.state[p]
             if "exp_avg" not in st:
                 st.update(self._new_moments(p))
+            elif st["exp_avg"].device != p.device or st["exp_avg_sq"].device != p.device:
+                raise ValueError("FusedAdamW's state must be on its parameter's device")
             st["step"] = step
         return step, params
+
+    def _place_steps(self):
+        """One step count per group after loading: fp32, on the parameters' device and apart
+        from the checkpoint's (torch leaves it where and as that had it)."""
+        for group in self.param_groups:
+            step = None
+            for p in group["params"]:
+                if "step" in self.state.get(p, ()):
+                    if step is None:
+                        step = torch.as_tensor(self.state[p]["step"]).to(
+                            p.device, torch.float32, copy=True).reshape(())
+                    self.state[p]["step"] = step
 
     def _new_moments(self, p):
         return {k: torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -84,6 +102,7 @@ class FusedAdamW(Optimizer):
         if any("exp_avg_scale" in st for st in state_dict["state"].values()):
             raise ValueError("these moments are in 8 bits: load them into FusedAdamW8bit")
         super().load_state_dict(state_dict)
+        self._place_steps()
 
     @torch.no_grad()
     def unscale_clip_(self, scaler, max_norm: float) -> torch.Tensor:
@@ -306,6 +325,7 @@ class FusedAdamW8bit(FusedAdamW):
                         or st[scale].numel() != -(-p.numel() // block)):
                     raise ValueError(f"{name} is not the 8-bit moment of its parameter")
         Optimizer.load_state_dict(self, state_dict)
+        self._place_steps()
         for i, p in zip(places, params):
             for name, scale in _SCALES.items():
                 if scale in saved.get(i, {}):

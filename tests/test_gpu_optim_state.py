@@ -1,0 +1,45 @@
+"""Resuming FusedAdamW and FusedAdamW8bit on the GPU from checkpoints of several kinds: the
+resumed run takes the steps that the first one would have taken, bit for bit."""
+from __future__ import annotations
+
+import io
+
+import pytest
+import torch
+
+from reversability_amd.optim import FusedAdamW, FusedAdamW8bit
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(33,), (64, 96), (1031, 7)]
+
+
+def made(kind, device, start=None):
+    g = torch.Generator().manual_seed(5)
+    base = [0.02 * torch.randn(s, generator=g) for s in SHAPES] if start is None else start
+    params = [t.detach().to(device).clone().requires_grad_(True) for t in base]
+    return params, kind(params, lr=1e-2)
+
+
+def steps(params, opt, seeds):
+    for seed in seeds:
+        g = torch.Generator().manual_seed(seed)
+        for p in params:
+            p.grad = 0.01 * torch.randn(p.shape, generator=g).to(p.device)
+        opt.step()
+
+
+@pytest.mark.parametrize("kind", [FusedAdamW, FusedAdamW8bit])
+def test_resumed_from_a_checkpoint_on_the_cpu(cuda_device, kind):
+    params, opt = made(kind, cuda_device)
+    steps(params, opt, range(3))
+    file = io.BytesIO()
+    torch.save(opt.state_dict(), file)
+    file.seek(0)
+    twins, other = made(kind, cuda_device, params)
+    other.load_state_dict(torch.load(file, map_location="cpu", weights_only=True))
+    steps(params, opt, range(3, 5))
+    steps(twins, other, range(3, 5))
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q)
+        assert float(other.state[q]["step"]) == 5.0

@@ -1,0 +1,63 @@
+"""State of FusedAdamW and FusedAdamW8bit on the CPU: what a checkpoint leaves, and what a
+step refuses before it launches anything (fake CUDA tensors: no kernel is launched)."""
+from __future__ import annotations
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from reversability_amd.optim import FusedAdamW, FusedAdamW8bit
+
+KINDS = [FusedAdamW, FusedAdamW8bit]
+SHAPES = [(128, 64), (16,)]
+
+
+def checkpoint(kind, step, shapes=SHAPES):
+    """A state dict on the CPU after one step of ``kind``."""
+    opt = kind([torch.zeros(s, requires_grad=True) for s in shapes])
+    for p in opt.param_groups[0]["params"]:
+        opt.state[p].update(opt._new_moments(p), step=step)
+    return opt.state_dict()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("step", [torch.tensor(3.0), torch.tensor(3), torch.tensor([3.0]), 3])
+def test_checkpoint_lands_on_the_parameters_device(kind, step):
+    params = [torch.zeros(s, device="meta", requires_grad=True) for s in SHAPES]
+    opt = kind(params)
+    opt.load_state_dict(checkpoint(kind, step))
+    for p in params:
+        assert all(t.device == p.device for t in opt.state[p].values())
+        assert opt.state[p]["step"].dtype == torch.float32 and opt.state[p]["step"].shape == ()
+    assert opt.state[params[0]]["step"] is opt.state[params[1]]["step"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_loaded_step_count_is_the_optimizers_own(kind):
+    state = checkpoint(kind, torch.tensor(3.0))
+    opt = kind([torch.zeros(s, requires_grad=True) for s in SHAPES])
+    opt.load_state_dict(state)
+    p = opt.param_groups[0]["params"][0]
+    opt.state[p]["step"].add_(1)
+    assert float(state["state"][0]["step"]) == 3.0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("key", ["step", "exp_avg", "exp_avg_sq", "dtype"])
+def test_state_elsewhere_is_refused(kind, key):
+    """Moments or a step count that the kernels would read on another device."""
+    with FakeTensorMode():
+        params = [torch.zeros(s, device="cuda:0", requires_grad=True) for s in SHAPES]
+        opt = kind(params)
+        for p in params:
+            p.grad = torch.ones_like(p)
+            moments = {k: torch.zeros_like(p) for k in ("exp_avg", "exp_avg_sq")}
+            opt.state[p].update(moments, step=torch.zeros((), device="cuda:0"))
+        opt._group_state(opt.param_groups[0])
+        for p in params:
+            if key == "dtype":
+                opt.state[p]["step"] = opt.state[p]["step"].double()
+            else:
+                opt.state[p][key] = opt.state[p][key].cpu()
+        with pytest.raises(ValueError, match="state"):
+            opt.step()
