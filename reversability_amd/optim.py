@@ -324,7 +324,10 @@ class FusedAdamW8bit(FusedAdamW):
                         st[name].dtype != torch.float8_e4m3fn or st[scale].dtype != torch.uint8
                         or st[scale].numel() != -(-p.numel() // block)):
                     raise ValueError(f"{name} is not the 8-bit moment of its parameter")
+        seeds = [g["seed"] for g in self.param_groups]
         Optimizer.load_state_dict(self, state_dict)
+        for group, seed in zip(self.param_groups, seeds):
+            group.setdefault("seed", seed)  # a plain checkpoint's groups have none
         self._place_steps()
         for i, p in zip(places, params):
             for name, scale in _SCALES.items():

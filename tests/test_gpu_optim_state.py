@@ -43,3 +43,20 @@ def test_resumed_from_a_checkpoint_on_the_cpu(cuda_device, kind):
     for p, q in zip(params, twins):
         assert torch.equal(p, q)
         assert float(other.state[q]["step"]) == 5.0
+
+
+def test_8_bit_moments_made_after_a_plain_checkpoint(cuda_device):
+    """A run that was saved before one of its large parameters had moments: the
+    parameter gets 8-bit ones, as in a run that never stopped."""
+    params, opt = made(FusedAdamW, cuda_device)
+    params[2].requires_grad_(False)  # frozen so far
+    for p in params[:2]:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    twins, other = made(FusedAdamW8bit, cuda_device, params)
+    other.load_state_dict(opt.state_dict())
+    steps(twins, other, [1])
+    assert "exp_avg_scale" not in other.state[twins[1]]
+    assert other.state[twins[2]]["exp_avg_scale"].dtype == torch.uint8
+    assert float(other.state[twins[2]]["step"]) == 2.0
+    assert not torch.equal(twins[2], params[2])

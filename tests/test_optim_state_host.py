@@ -61,3 +61,21 @@ def test_state_elsewhere_is_refused(kind, key):
                 opt.state[p][key] = opt.state[p][key].cpu()
         with pytest.raises(ValueError, match="state"):
             opt.step()
+
+
+@pytest.mark.parametrize("source", [FusedAdamW, torch.optim.AdamW])
+def test_plain_checkpoint_keeps_the_seed(source):
+    """A checkpoint without 8-bit moments has no seed in its groups; parameters that it
+    holds no moments for get 8-bit ones later."""
+    params = [torch.zeros(s, requires_grad=True) for s in SHAPES]
+    opt = FusedAdamW8bit(params, seed=7)
+    opt.add_param_group({"params": [torch.zeros(3, requires_grad=True)], "lr": 2.0})
+    other = source([torch.zeros(s, requires_grad=True) for s in SHAPES])
+    other.add_param_group({"params": [torch.zeros(3, requires_grad=True)], "lr": 3.0})
+    opt.load_state_dict(other.state_dict())
+    assert [g["seed"] for g in opt.param_groups] == [7, 7]
+    assert opt.param_groups[1]["lr"] == 3.0
+    saved = FusedAdamW8bit([torch.zeros(s, requires_grad=True) for s in SHAPES], seed=9)
+    opt = FusedAdamW8bit(params, seed=7)
+    opt.load_state_dict(saved.state_dict())
+    assert opt.param_groups[0]["seed"] == 9
