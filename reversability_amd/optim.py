@@ -54,33 +54,49 @@ class FusedAdamW(Optimizer):
             raise ValueError(f"Invalid betas: {betas}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
-    def _group_state(self, group):
+    def _group_params(self, group):
+        """A group's parameters with a gradient; raises for what the kernels do not take
+        (they read everything through its address) and changes nothing."""
         params = [p for p in group["params"] if p.grad is not None]
-        for p in params:
-            if p.dtype != torch.float32 or not p.is_cuda or p.grad.is_sparse:
-                raise ValueError("FusedAdamW requires dense CUDA (ROCm device) FP32 parameters")
         if not params:
-            return None, []
-        step, dev = None, params[0].device
-        for p in group["params"]:
-            st = self.state[p]
-            if "step" in st:
-                step = st["step"]
-                break
-        if step is None:
-            step = torch.zeros((), device=dev, dtype=torch.float32)
-        # the kernels read these through their addresses
-        elif not torch.is_tensor(step) or step.dtype != torch.float32 or step.device != dev:
+            return params
+        dev = params[0].device
+        for p in params:
+            g = p.grad
+            if p.dtype != torch.float32 or not p.is_cuda or g.is_sparse:
+                raise ValueError("FusedAdamW requires dense CUDA (ROCm device) FP32 parameters")
+            if p.device != dev or not (p.is_contiguous() and g.is_contiguous()):
+                raise ValueError("FusedAdamW requires contiguous parameters and gradients, a "
+                                 "group's on one device")
+            st = self.state.get(p)
+            if st and "exp_avg" in st and (st["exp_avg"].device != dev
+                                           or st["exp_avg_sq"].device != dev):
+                raise ValueError("FusedAdamW's state must be on its parameter's device")
+        step = self._step_count(group)
+        if step is not None and not (torch.is_tensor(step) and step.dtype == torch.float32
+                                     and step.device == dev):
             raise ValueError("FusedAdamW's state needs its step count as an fp32 tensor on the "
                              "parameters' device")
+        return params
+
+    def _step_count(self, group):
+        for p in group["params"]:
+            st = self.state.get(p)
+            if st and "step" in st:
+                return st["step"]
+        return None
+
+    def _group_state(self, group, params):
+        """The group's step count; makes the state that ``params`` lack."""
+        step = self._step_count(group)
+        if step is None:
+            step = torch.zeros((), device=params[0].device, dtype=torch.float32)
         for p in params:
             st = self.state[p]
             if "exp_avg" not in st:
                 st.update(self._new_moments(p))
-            elif st["exp_avg"].device != p.device or st["exp_avg_sq"].device != p.device:
-                raise ValueError("FusedAdamW's state must be on its parameter's device")
             st["step"] = step
-        return step, params
+        return step
 
     def _place_steps(self):
         """One step count per group after loading: fp32, on the parameters' device and apart
@@ -168,12 +184,14 @@ class FusedAdamW(Optimizer):
         lib = library()
         found_inf = getattr(self, "found_inf", None)
         grad_scale = getattr(self, "grad_scale", None)
+        # every refusal comes before anything is launched or forgotten
+        work = [(group, self._group_params(group)) for group in self.param_groups]
         pending_inv, clip = getattr(self, "_pending", (None, None))
         self._pending = (None, None)
-        for group in self.param_groups:
-            step, params = self._group_state(group)
+        for group, params in work:
             if not params:
                 continue
+            step = self._group_state(group, params)
             dev = params[0].device
             with _DeviceGuard(params[0]):
                 stream = _stream(params[0])
@@ -196,9 +214,6 @@ class FusedAdamW(Optimizer):
         for start in range(0, len(params), limit):
             chunk = params[start:start + limit]
             n = len(chunk)
-            for p in chunk:
-                if not (p.is_contiguous() and p.grad.is_contiguous()):
-                    raise ValueError("FusedAdamW requires contiguous parameters and gradients")
             P = ctypes.c_void_p * n
             ptrs = [P(*[t.data_ptr() for t in ts]) for ts in (
                 chunk, [p.grad for p in chunk], [self.state[p]["exp_avg"] for p in chunk],
@@ -247,15 +262,6 @@ class FusedAdamW8bit(FusedAdamW):
         self.defaults["seed"] = seed  # saved with the groups: a resumed run goes on alike
         for group in self.param_groups:
             group.setdefault("seed", seed)
-
-    def _group_state(self, group):
-        # before anything of the step is launched
-        params = [p for p in group["params"] if p.grad is not None]
-        if any(p.device != params[0].device or not (p.is_contiguous() and p.grad.is_contiguous())
-               for p in params):
-            raise ValueError("FusedAdamW8bit requires contiguous parameters and gradients, a "
-                             "group's on one device")
-        return super()._group_state(group)
 
     def _new_moments(self, p):
         if p.numel() < self.min_8bit_numel:

@@ -60,3 +60,32 @@ def test_8_bit_moments_made_after_a_plain_checkpoint(cuda_device):
     assert other.state[twins[2]]["exp_avg_scale"].dtype == torch.uint8
     assert float(other.state[twins[2]]["step"]) == 2.0
     assert not torch.equal(twins[2], params[2])
+
+
+@pytest.mark.parametrize("kind", [FusedAdamW, FusedAdamW8bit])
+def test_a_refused_step_can_be_taken_again(cuda_device, kind):
+    """A gradient of the second group that is refused after unscale_clip_: nothing has
+    changed, and the step that follows still unscales and clips."""
+    params, opt = made(kind, cuda_device)
+    twins, other = made(kind, cuda_device)
+    for o, (a, b, c) in ((opt, params), (other, twins)):
+        del o.param_groups[0]["params"][1:]
+        o.add_param_group({"params": [b, c]})
+    before = [p.detach().clone() for p in params]
+    for p, q in zip(params, twins):
+        p.grad = q.grad = torch.full_like(p, 3.0) * 1024
+    scalers = [torch.amp.GradScaler("cuda", init_scale=1024.0) for _ in range(2)]
+    for o, s in zip((opt, other), scalers):
+        s.scale(torch.ones((), device=cuda_device))
+        o.unscale_clip_(s, 0.5)
+    right = params[1].grad
+    params[1].grad = right.t().contiguous().t()
+    with pytest.raises(ValueError, match="contiguous"):
+        scalers[0].step(opt)
+    assert all(torch.equal(p, b) for p, b in zip(params, before)) and not opt.state
+    params[1].grad = right
+    opt.step()
+    scalers[1].step(other)
+    for p, q, b in zip(params, twins, before):
+        assert torch.equal(p, q) and not torch.equal(p, b)
+        assert torch.equal(opt.state[p]["exp_avg"].float(), other.state[q]["exp_avg"].float())

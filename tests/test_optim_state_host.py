@@ -53,7 +53,7 @@ def test_state_elsewhere_is_refused(kind, key):
             p.grad = torch.ones_like(p)
             moments = {k: torch.zeros_like(p) for k in ("exp_avg", "exp_avg_sq")}
             opt.state[p].update(moments, step=torch.zeros((), device="cuda:0"))
-        opt._group_state(opt.param_groups[0])
+        assert len(opt._group_params(opt.param_groups[0])) == 2
         for p in params:
             if key == "dtype":
                 opt.state[p]["step"] = opt.state[p]["step"].double()
@@ -79,3 +79,29 @@ def test_plain_checkpoint_keeps_the_seed(source):
     opt = FusedAdamW8bit(params, seed=7)
     opt.load_state_dict(saved.state_dict())
     assert opt.param_groups[0]["seed"] == 9
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bad", ["gradient", "parameter", "device", "type", "step"])
+def test_a_refusal_in_the_second_group_comes_first(kind, bad, monkeypatch):
+    """Nothing is launched, no state is made and unscale_clip_'s factors wait for the
+    step that is taken."""
+    with FakeTensorMode():
+        devices = ["cuda:0", {"device": "cuda:1", "type": "cpu"}.get(bad, "cuda:0")]
+        first = [torch.zeros(s, device="cuda:0", requires_grad=True) for s in SHAPES]
+        p, q = (torch.zeros(s, device=d, requires_grad=True) for s, d in zip(SHAPES, devices))
+        for t in (*first, p, q):
+            t.grad = torch.ones_like(t)
+        opt = kind([{"params": first}, {"params": [p, q]}])
+        if bad == "gradient":
+            p.grad = torch.ones(64, 128, device="cuda:0").t()
+        elif bad == "parameter":
+            p.data = torch.zeros(64, 128, device="cuda:0").t()
+        elif bad == "step":
+            opt.state[p]["step"] = torch.zeros(())
+        waiting = opt._pending = (torch.ones(1), torch.ones(1))
+        monkeypatch.setattr(kind, "_update", lambda *_: pytest.fail("launched"))
+        with pytest.raises(ValueError, match="FusedAdamW"):
+            opt.step()
+        assert opt._pending is waiting
+        assert not any("exp_avg" in st for st in opt.state.values())
