@@ -55,9 +55,9 @@ class FusedAdamW(Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def _group_params(self, group):
-        """A group's parameters with a gradient; raises for what the kernels do not take
+        """A group's parameters with elements and a gradient; raises for what the kernels do not take
         (they read everything through its address) and changes nothing."""
-        params = [p for p in group["params"] if p.grad is not None]
+        params = [p for p in group["params"] if p.grad is not None and p.numel()]
         if not params:
             return params
         dev = params[0].device
@@ -128,7 +128,8 @@ class FusedAdamW(Optimizer):
         only)."""
         from torch.amp.grad_scaler import OptState
         lib = library()
-        params = [p for group in self.param_groups for p in group["params"] if p.grad is not None]
+        params = [p for group in self.param_groups for p in group["params"]
+                  if p.grad is not None and p.numel()]
         if not params:
             return torch.zeros(())
         dev = params[0].device

@@ -89,3 +89,27 @@ def test_a_refused_step_can_be_taken_again(cuda_device, kind):
     for p, q, b in zip(params, twins, before):
         assert torch.equal(p, q) and not torch.equal(p, b)
         assert torch.equal(opt.state[p]["exp_avg"].float(), other.state[q]["exp_avg"].float())
+
+
+@pytest.mark.parametrize("kind", [FusedAdamW, FusedAdamW8bit])
+def test_empty_parameters_are_passed_over(cuda_device, kind):
+    """A parameter without elements beside others, in a group of its own, and alone."""
+    params, opt = made(kind, cuda_device)
+    twins, other = made(kind, cuda_device)
+    empty = [torch.empty(0, 7, device=cuda_device, requires_grad=True) for _ in range(2)]
+    other.param_groups[0]["params"].insert(1, empty[0])
+    other.add_param_group({"params": [empty[1]]})
+    for p, q in zip(params, twins):
+        p.grad = torch.full_like(p, 3.0)
+        q.grad = p.grad.clone()
+    for e in empty:
+        e.grad = torch.empty_like(e)
+    for o in (opt, other):
+        o.unscale_clip_(None, 0.5)
+        o.step()
+    assert float(other.state[twins[0]]["step"]) == 1.0
+    # the random bits follow a parameter's place: only the moments' codes may differ
+    assert all(torch.equal(p, q) for p, q in zip(params, twins))
+    alone = kind([empty[0]])
+    assert float(alone.unscale_clip_(None, 1.0)) == 0.0
+    alone.step()

@@ -105,3 +105,12 @@ def test_a_refusal_in_the_second_group_comes_first(kind, bad, monkeypatch):
             opt.step()
         assert opt._pending is waiting
         assert not any("exp_avg" in st for st in opt.state.values())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_empty_parameters_are_no_work(kind):
+    with FakeTensorMode():
+        full, empty = (torch.zeros(s, device="cuda:0", requires_grad=True) for s in ((5,), (0, 7)))
+        full.grad, empty.grad = torch.ones_like(full), torch.ones_like(empty)
+        opt = kind([full, empty])
+        assert opt._group_params(opt.param_groups[0]) == [full]
