@@ -158,18 +158,19 @@ class FusedAdamW(Optimizer):
         partials, flags = work[:total_chunks], work[total_chunks:2 * total_chunks]
         total, coef, found = (work[2 * total_chunks + i:2 * total_chunks + i + 1]
                               for i in range(3))
-        stream = _stream(params[0])
-        first = 0
-        for g, n, c in zip(groups, numels, counts):
-            ptrs = (ctypes.c_void_p * len(g))(*[p.grad.data_ptr() for p in g])
-            _check(lib.rv_grad_sq_partials(len(g), ptrs, n,
-                                           inv.data_ptr() if inv is not None else None,
-                                           partials.data_ptr(), flags.data_ptr(), first, stream),
-                   "rv_grad_sq_partials")
-            first += c
-        _check(lib.rv_grad_clip_coef(partials.data_ptr(), flags.data_ptr(), total_chunks,
-                                     float(max_norm), total.data_ptr(), coef.data_ptr(),
-                                     found.data_ptr(), stream), "rv_grad_clip_coef")
+        with _DeviceGuard(params[0]):
+            stream = _stream(params[0])
+            first = 0
+            for g, n, c in zip(groups, numels, counts):
+                ptrs = (ctypes.c_void_p * len(g))(*[p.grad.data_ptr() for p in g])
+                _check(lib.rv_grad_sq_partials(len(g), ptrs, n,
+                                               inv.data_ptr() if inv is not None else None,
+                                               partials.data_ptr(), flags.data_ptr(), first, stream),
+                       "rv_grad_sq_partials")
+                first += c
+            _check(lib.rv_grad_clip_coef(partials.data_ptr(), flags.data_ptr(), total_chunks,
+                                         float(max_norm), total.data_ptr(), coef.data_ptr(),
+                                         found.data_ptr(), stream), "rv_grad_clip_coef")
         if state is not None:
             state["found_inf_per_device"] = {dev: found.reshape(())}
             state["stage"] = OptState.UNSCALED

@@ -6,6 +6,7 @@ import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
+from reversability_amd import optim
 from reversability_amd.optim import FusedAdamW, FusedAdamW8bit
 
 KINDS = [FusedAdamW, FusedAdamW8bit]
@@ -114,3 +115,35 @@ def test_empty_parameters_are_no_work(kind):
         full.grad, empty.grad = torch.ones_like(full), torch.ones_like(empty)
         opt = kind([full, empty])
         assert opt._group_params(opt.param_groups[0]) == [full]
+
+
+def test_unscale_clip_launches_on_the_gradients_device(monkeypatch):
+    """Every launch is made with the gradients' device current."""
+    inside, launches = [], []
+
+    class Guard:
+        def __init__(self, t):
+            self.device = t.device
+
+        def __enter__(self):
+            inside.append(self.device)
+
+        def __exit__(self, *exc):
+            inside.pop()
+
+    class Library:
+        rv_adamw_max_tensors = staticmethod(lambda: 1)
+        rv_grad_chunks = staticmethod(lambda *_: 1)
+
+        def __getattr__(self, name):
+            return lambda *_: launches.append((name, list(inside))) or 0
+
+    p = [torch.zeros(5, requires_grad=True) for _ in range(2)]
+    for t in p:
+        t.grad = torch.ones_like(t)
+    monkeypatch.setattr(optim, "library", Library)
+    monkeypatch.setattr(optim, "_DeviceGuard", Guard)
+    monkeypatch.setattr(optim, "_stream", lambda t: 0)
+    FusedAdamW(p).unscale_clip_(None, 1.0)
+    assert [name for name, _ in launches] == ["rv_grad_sq_partials"] * 2 + ["rv_grad_clip_coef"]
+    assert all(devices == [p[0].device] for _, devices in launches)
