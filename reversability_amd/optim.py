@@ -265,6 +265,9 @@ class FusedAdamW8bit(FusedAdamW):
         for group in self.param_groups:
             group.setdefault("seed", seed)
 
+    def __getstate__(self):  # of copies and pickles: torch keeps defaults, groups and state
+        return {**super().__getstate__(), "min_8bit_numel": self.min_8bit_numel}
+
     def _new_moments(self, p):
         if p.numel() < self.min_8bit_numel:
             return super()._new_moments(p)

@@ -2,6 +2,9 @@
 step refuses before it launches anything (fake CUDA tensors: no kernel is launched)."""
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -147,3 +150,15 @@ def test_unscale_clip_launches_on_the_gradients_device(monkeypatch):
     FusedAdamW(p).unscale_clip_(None, 1.0)
     assert [name for name, _ in launches] == ["rv_grad_sq_partials"] * 2 + ["rv_grad_clip_coef"]
     assert all(devices == [p[0].device] for _, devices in launches)
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_keep_their_options(copied):
+    params = [torch.zeros(s, requires_grad=True) for s in SHAPES]
+    twin = copied(FusedAdamW8bit(params, lr=0.5, min_8bit_numel=10, seed=3))
+    assert (twin.min_8bit_numel, twin.defaults["seed"]) == (10, 3)
+    assert twin.param_groups[0]["seed"] == 3 and twin.param_groups[0]["lr"] == 0.5
+    small = twin.param_groups[0]["params"][1]
+    assert twin._new_moments(small)["exp_avg"].dtype == torch.float8_e4m3fn
+    twin.load_state_dict(FusedAdamW8bit(params, min_8bit_numel=99).state_dict())
+    assert twin.min_8bit_numel == 10
