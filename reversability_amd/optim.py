@@ -98,6 +98,21 @@ class FusedAdamW(Optimizer):
             st["step"] = step
         return step
 
+    def _check_shapes(self, state_dict):
+        """Moments of another size than the parameter's are refused: the kernels would
+        read past them."""
+        for p, st in self._saved(state_dict):
+            for name in ("exp_avg", "exp_avg_sq"):
+                if name in st and st[name].shape != p.shape:
+                    raise ValueError(f"{name} of shape {tuple(st[name].shape)} for a parameter "
+                                     f"of shape {tuple(p.shape)}")
+
+    def _saved(self, state_dict):
+        """Each parameter and what the checkpoint holds for it."""
+        places = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        return [(p, state_dict["state"].get(i, {})) for i, p in zip(places, params)]
+
     def _place_steps(self):
         """One step count per group after loading: fp32, on the parameters' device and apart
         from the checkpoint's (torch leaves it where and as that had it)."""
@@ -117,6 +132,7 @@ class FusedAdamW(Optimizer):
     def load_state_dict(self, state_dict):
         if any("exp_avg_scale" in st for st in state_dict["state"].values()):
             raise ValueError("these moments are in 8 bits: load them into FusedAdamW8bit")
+        self._check_shapes(state_dict)
         super().load_state_dict(state_dict)
         self._place_steps()
 
@@ -319,18 +335,12 @@ class FusedAdamW8bit(FusedAdamW):
 
     def load_state_dict(self, state_dict):
         """As torch's, which casts every floating or parameter-like state to the
-        parameter's type; the 8-bit moments keep theirs.  Moments of another size than
-        the parameter's are refused: the kernel would read past them."""
-        saved = state_dict["state"]
-        places = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
+        parameter's type; the 8-bit moments keep theirs."""
+        self._check_shapes(state_dict)
+        saved = self._saved(state_dict)
         block = library().rv_adamw8_block()
-        for i, p in zip(places, params):
-            st = saved.get(i, {})
+        for p, st in saved:
             for name, scale in _SCALES.items():
-                if name in st and st[name].shape != p.shape:
-                    raise ValueError(f"{name} of shape {tuple(st[name].shape)} for a parameter "
-                                     f"of shape {tuple(p.shape)}")
                 if (scale in st) != (_SCALES["exp_avg"] in st) or scale in st and (
                         st[name].dtype != torch.float8_e4m3fn or st[scale].dtype != torch.uint8
                         or st[scale].numel() != -(-p.numel() // block)):
@@ -340,10 +350,10 @@ class FusedAdamW8bit(FusedAdamW):
         for group, seed in zip(self.param_groups, seeds):
             group.setdefault("seed", seed)  # a plain checkpoint's groups have none
         self._place_steps()
-        for i, p in zip(places, params):
+        for p, st in saved:
             for name, scale in _SCALES.items():
-                if scale in saved.get(i, {}):
+                if scale in st:
                     for key in (name, scale):
-                        t = saved[i][key]
+                        t = st[key]
                         bits = t.contiguous().view(torch.uint8).to(p.device, copy=True)
                         self.state[p][key] = bits.view(t.dtype)

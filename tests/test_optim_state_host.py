@@ -162,3 +162,13 @@ def test_copies_keep_their_options(copied):
     assert twin._new_moments(small)["exp_avg"].dtype == torch.float8_e4m3fn
     twin.load_state_dict(FusedAdamW8bit(params, min_8bit_numel=99).state_dict())
     assert twin.min_8bit_numel == 10
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_moments_of_another_shape_are_refused(kind):
+    """The kernels would read past them; nothing is loaded."""
+    opt = kind([torch.zeros(s, requires_grad=True) for s in [(128, 65), (16,)]])
+    for state in (checkpoint(kind, torch.tensor(1.0)), checkpoint(FusedAdamW, torch.tensor(1.0))):
+        with pytest.raises(ValueError, match="shape"):
+            opt.load_state_dict(state)
+        assert not opt.state
