@@ -113,17 +113,22 @@ class FusedAdamW(Optimizer):
         params = [p for g in self.param_groups for p in g["params"]]
         return [(p, state_dict["state"].get(i, {})) for i, p in zip(places, params)]
 
-    def _place_steps(self):
-        """One step count per group after loading: fp32, on the parameters' device and apart
-        from the checkpoint's (torch leaves it where and as that had it)."""
+    def _place_state(self):
+        """What the kernels read through its address, after loading (torch leaves it as the
+        checkpoint had it): one step count per group, fp32, on the parameters' device
+        and apart from the checkpoint's; moments in the order of their elements."""
         for group in self.param_groups:
             step = None
             for p in group["params"]:
-                if "step" in self.state.get(p, ()):
+                st = self.state.get(p, {})
+                if "step" in st:
                     if step is None:
-                        step = torch.as_tensor(self.state[p]["step"]).to(
-                            p.device, torch.float32, copy=True).reshape(())
-                    self.state[p]["step"] = step
+                        step = torch.as_tensor(st["step"]).to(p.device, torch.float32,
+                                                              copy=True).reshape(())
+                    st["step"] = step
+                for name in ("exp_avg", "exp_avg_sq"):
+                    if name in st:
+                        st[name] = st[name].contiguous()
 
     def _new_moments(self, p):
         return {k: torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -134,7 +139,7 @@ class FusedAdamW(Optimizer):
             raise ValueError("these moments are in 8 bits: load them into FusedAdamW8bit")
         self._check_shapes(state_dict)
         super().load_state_dict(state_dict)
-        self._place_steps()
+        self._place_state()
 
     @torch.no_grad()
     def unscale_clip_(self, scaler, max_norm: float) -> torch.Tensor:
@@ -349,7 +354,7 @@ class FusedAdamW8bit(FusedAdamW):
         Optimizer.load_state_dict(self, state_dict)
         for group, seed in zip(self.param_groups, seeds):
             group.setdefault("seed", seed)  # a plain checkpoint's groups have none
-        self._place_steps()
+        self._place_state()
         for p, st in saved:
             for name, scale in _SCALES.items():
                 if scale in st:

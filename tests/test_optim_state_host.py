@@ -172,3 +172,16 @@ def test_moments_of_another_shape_are_refused(kind):
         with pytest.raises(ValueError, match="shape"):
             opt.load_state_dict(state)
         assert not opt.state
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_transposed_moments_keep_their_elements(kind):
+    """Moments saved with other strides (of a transposed parameter): the kernels pair
+    them with the parameter's elements by their place in memory."""
+    state = checkpoint(FusedAdamW, torch.tensor(1.0))
+    moment = torch.randn(64, 128).t()
+    state["state"][0]["exp_avg"] = moment
+    opt = kind([torch.zeros(s, requires_grad=True) for s in SHAPES])
+    opt.load_state_dict(state)
+    loaded = opt.state[opt.param_groups[0]["params"][0]]["exp_avg"]
+    assert torch.equal(loaded, moment) and loaded.is_contiguous()
