@@ -385,6 +385,15 @@ __device__ __forceinline__ float round16(float v) {
   else return __half2float(__float2half_rn(v));
 }
 
+// Joins two (maximum, sum of exp(z - maximum)) of the same row; a maximum of -inf
+// comes with a sum of 0 (or NaN, which stays).
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  if (top == -INFINITY) return make_float2(top, a.y + b.y);
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - top) * kLog2e) +
+                              b.y * __builtin_amdgcn_exp2f((b.x - top) * kLog2e));
+}
+
 // What the tied head's log-probability epilogues read and write beside the
 // product (rows and labels of the chunk at hand).
 struct HeadLogp {
@@ -730,14 +739,7 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
       if (m0 + r >= args.m) break;
       float2 v = red[r];
 #pragma unroll
-      for (int w = 1; w < WCOLS; ++w) {
-        const float2 u = red[w * BM + r];
-        const float top = fmaxf(v.x, u.x);
-        if (u.x != -INFINITY)
-          v.y = v.y * __builtin_amdgcn_exp2f((v.x - top) * kLog2e) +
-                u.y * __builtin_amdgcn_exp2f((u.x - top) * kLog2e);
-        v.x = top;
-      }
+      for (int w = 1; w < WCOLS; ++w) v = join(v, red[w * BM + r]);
       out[r] = v;
     }
   } else if constexpr (EPI == Epi::PartialF32 || EPI == Epi::StoreF32OfF16 ||
@@ -1174,15 +1176,6 @@ void scaled_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t 
     constexpr bool BF = std::is_same<T, __hip_bfloat16>::value;
     *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<BF>(s.x, s.y), pack2<BF>(s.z, s.w));
   }
-}
-
-// Joins two (maximum, sum of exp(z - maximum)) of the same row; a maximum of -inf
-// comes with a sum of 0 (or NaN, which stays).
-__device__ __forceinline__ float2 join(float2 a, float2 b) {
-  const float top = fmaxf(a.x, b.x);
-  if (top == -INFINITY) return make_float2(top, a.y + b.y);
-  return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - top) * kLog2e) +
-                              b.y * __builtin_amdgcn_exp2f((b.x - top) * kLog2e));
 }
 
 // A row's log-probability from its tiles' maxima and sums: lse = M + log sum_t s_t

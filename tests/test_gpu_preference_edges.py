@@ -1,0 +1,71 @@
+"""Edges of the log-probabilities and the policy loss: not-a-numbers and infinities in the
+head, against 64 bits."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from reversability_amd.preference import tied_head_logprobs
+
+pytestmark = pytest.mark.gpu
+
+
+def operands(rows, d, vocab, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    head = torch.zeros(-(-vocab // 64) * 64, d, device="cuda", dtype=dtype)
+    head[:vocab] = (torch.randn(vocab, d, generator=g, device="cuda") / math.sqrt(d)).to(dtype)
+    x = torch.randn(rows, d, generator=g, device="cuda").to(dtype)
+    labels = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    if rows > 2:
+        labels[2] = -100
+    return x, head, labels
+
+
+# both sides of width 256, of 64 and 128 rows, and enough tiles for 256 x 256 ones
+NAN_SIZES = [(5, 512, 321), (100, 512, 321), (700, 264, 321), (9, 1024, 50257),
+             (300, 512, 50257), (2100, 512, 12305), (5, 256, 321), (300, 64, 12305)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,d,vocab", NAN_SIZES)
+def test_nan_in_a_row_of_the_head_reaches_every_token(cuda_device, rows, d, vocab, dtype):
+    """A logit that is no number leaves no log-probability of its row a number: in the
+    first columns, the last whole block of them, and alone among padding."""
+    x, head, labels = operands(rows, d, vocab, dtype)
+    assert bool(tied_head_logprobs(x, head, vocab, labels).isfinite().all())
+    scored = labels != -100
+    for first, last in ((0, 1), (vocab // 2, vocab // 2 + 1), (vocab - 1, vocab),
+                        (vocab - 17, vocab), (0, vocab)):
+        broken = head.clone()
+        broken[first:last] = math.nan
+        logp = tied_head_logprobs(x, broken, vocab, labels)
+        assert bool(logp[scored].isnan().all()) and not logp[~scored].any(), (first, last)
+    # behind the vocabulary it reaches nothing
+    broken = head.clone()
+    broken[vocab:] = math.nan
+    assert torch.equal(tied_head_logprobs(x, broken, vocab, labels),
+                       tied_head_logprobs(x, head, vocab, labels))
+
+
+@pytest.mark.parametrize("rows,d,vocab", NAN_SIZES)
+def test_infinite_logits(cuda_device, rows, d, vocab):
+    """A head row of an infinity: a logit of -inf counts for nothing, one of +inf leaves
+    its row without a log-probability."""
+    x, head, labels = operands(rows, d, vocab, torch.bfloat16, seed=1)
+    at = min(vocab - 1, 320)
+    head[at] = 0
+    head[at, 3] = math.inf
+    head[vocab - 1, 5] = -math.inf
+    x[:, 3] = x[:, 3].abs() + 1
+    x[::2, 3] *= -1
+    x[:, 5] = x[:, 5].abs() + 1
+    logp = tied_head_logprobs(x, head, vocab, labels).double()
+    z = x.double() @ head[:vocab].double().t()
+    ref = z.log_softmax(1).gather(1, labels.clamp_min(0)[:, None])[:, 0]
+    ref = torch.where(labels == -100, 0.0, ref)
+    assert torch.equal(logp.isnan(), ref.isnan())
+    assert torch.equal(logp.isinf(), ref.isinf())
+    ok = ref.isfinite()
+    assert bool(((logp - ref)[ok].abs() <= 1e-3).all())  # fp32 sums of d products: below 1e-4
