@@ -334,17 +334,24 @@ void policy_join_k(const int* __restrict__ part, int64_t seqs, int64_t chunks,
   if ((threadIdx.x & 63) == 0) weight[s] = weight_of(count, seqs);
 }
 
-// exp(s) - s - 1: the differences would leave nothing of a small s (s^2 / 2), where a model
-// close to its reference spends its time.  Below 1 the series s^2 sum_k s^k / (k + 2)!, to
-// k = 9 (the rest is below 2^-27 of it).
-__device__ __forceinline__ float kl_term(float s) {
-  if (fabsf(s) >= 1.f) return expf(s) - s - 1.f;
+// k = exp(s) - s - 1 and its derivative exp(s) - 1: the differences would leave nothing of
+// a small s (k = s^2 / 2), where a model close to its reference spends its time.  Below 1
+// the series k = s^2 sum_i s^i / (i + 2)!, to i = 9 (the rest is below 2^-27 of it), and
+// k + s; above, k and -s are large where exp(s) - 1 is not.
+__device__ __forceinline__ void kl_term(float s, float& k, float& slope) {
+  if (fabsf(s) >= 1.f) {
+    const float e = expf(s);
+    k = e - s - 1.f;
+    slope = e - 1.f;
+    return;
+  }
   constexpr float c[] = {1.f / 39916800, 1.f / 3628800, 1.f / 362880, 1.f / 40320, 1.f / 5040,
                          1.f / 720,      1.f / 120,     1.f / 24,     1.f / 6,     1.f / 2};
   float p = c[0];
 #pragma unroll
   for (int i = 1; i < 10; ++i) p = __builtin_fmaf(p, s, c[i]);
-  return s * s * p;
+  k = s * s * p;
+  slope = k + s;
 }
 
 // One token: its loss, KL term, whether its ratio is clipped, and d loss / d logp.
@@ -361,10 +368,10 @@ __device__ __forceinline__ void policy_token(const PolicyArgs& a, float logp, fl
   slope = clipped ? 0.f : -ratio * adv;
   k = 0.f;
   if (a.ref) {
-    const float shift = ref - logp;
-    k = kl_term(shift);
+    float away;
+    kl_term(ref - logp, k, away);
     loss += a.kl * k;
-    slope -= a.kl * (k + shift);  // exp(shift) - 1
+    slope -= a.kl * away;
   }
 }
 

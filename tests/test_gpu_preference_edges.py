@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from reversability_amd.preference import tied_head_logprobs
+from reversability_amd.preference import policy_loss, tied_head_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,33 @@ def test_infinite_logits(cuda_device, rows, d, vocab):
     assert torch.equal(logp.isinf(), ref.isinf())
     ok = ref.isfinite()
     assert bool(((logp - ref)[ok].abs() <= 1e-3).all())  # fp32 sums of d products: below 1e-4
+
+
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_kl_gradient_of_tokens_far_from_the_reference(cuda_device, sign):
+    """d/dlogp of exp(s) - s - 1, s = ref - logp, is 1 - exp(s): no difference of large
+    numbers.  In units of 2^-24 of it: expf 2 of exp(s), which is at most 0.59 (s <= -1)
+    or 1.59 (s >= 1) times the value; the subtraction, 1 / n, its product and the
+    coefficient's 1 each: 7.2 at most."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    # multiples of 2^-16 up to 128: sums and differences are exact
+    grid = lambda t: (t * 2.0 ** 16).round() * 2.0 ** -16
+    logp = grid(-40 * torch.rand(6, 500, generator=g, device="cuda"))
+    ref = logp + sign * grid(1 + 39 * torch.rand(6, 500, generator=g, device="cuda"))
+    s = ref.double() - logp.double()
+    assert torch.equal((ref - logp).double(), s)
+    leaf = logp.clone().requires_grad_(True)
+    out = policy_loss(leaf, logp, torch.zeros(6, device="cuda"), ref_logp=ref, kl_coef=1.0)
+    dlogp, = torch.autograd.grad(out.loss, leaf)
+    grad = -torch.expm1(s) / s.numel()
+    assert bool(((dlogp.double() - grad).abs() <= 8 * 2.0 ** -24 * grad.abs()).all())
+
+
+def test_kl_gradient_of_an_impossible_reference(cuda_device):
+    """A reference probability of 0: an infinite term whose gradient is the coefficient."""
+    logp = torch.tensor([[-1.0, -2.0]], device="cuda", requires_grad=True)
+    out = policy_loss(logp, logp.detach(), torch.zeros(1, device="cuda"), kl_coef=0.5,
+                      ref_logp=torch.tensor([[-math.inf, -2.0]], device="cuda"))
+    out.loss.backward()
+    assert float(out.loss.detach()) == float(out.kl) == math.inf
+    assert logp.grad.tolist() == [[0.25, 0.0]]
