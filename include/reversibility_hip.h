@@ -545,7 +545,7 @@ int rv_pref_grad(const float* coef, const uint8_t* mask, int64_t ld_mask, const 
 
 /* Clipped policy loss with a KL term.  Per counted token, r = exp(logp - old):
  *   -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k,
- *   k = exp(ref - logp) - (ref - logp) - 1       (ref NULL: no such term)
+ *   k = exp(ref - logp) - (ref - logp) - 1       (ref NULL or kl_coef 0: no such term)
  * loss: the sum over the counted tokens divided by their number (per_sequence ==
  * 0), or the mean over all sequences of each one's mean (0 without tokens).
  * adv[s * adv_row + t * adv_col].  stats[3] = mean k, share of tokens whose ratio

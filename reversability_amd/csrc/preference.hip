@@ -370,8 +370,10 @@ __device__ __forceinline__ void policy_token(const PolicyArgs& a, float logp, fl
   if (a.ref) {
     float away;
     kl_term(ref - logp, k, away);
-    loss += a.kl * k;
-    slope -= a.kl * away;
+    if (a.kl != 0.f) {  // 0: the statistic alone, which may be infinite
+      loss += a.kl * k;
+      slope -= a.kl * away;
+    }
   }
 }
 

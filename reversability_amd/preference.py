@@ -362,9 +362,10 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Te
     one that sampled the answers, ``advantages`` fp32 [sequences] or [sequences,
     tokens], ``mask`` the tokens that count (None: all).  With r = exp(logp - old_logp)
     a token's loss is -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A), plus kl_coef
-    (exp(d) - d - 1), d = ref_logp - logp, if ``ref_logp`` is given.  ``reduction``
-    "token": the mean over all counted tokens; "sequence": the mean over all sequences
-    of each one's mean.  Nothing counted gives 0.  Where the ratio is clipped the
+    (exp(d) - d - 1), d = ref_logp - logp, if ``ref_logp`` is given (kl_coef 0: its
+    mean is returned, the loss has no such term).  ``reduction`` "token": the mean over
+    all counted tokens; "sequence": the mean over all sequences of each one's mean.
+    Nothing counted gives 0.  Where the ratio is clipped the
     first term has no gradient (at the border itself it has).  The gradient reaches
     ``logp`` alone.  Sums in fp64, deterministic."""
     _check_logp(logp, "policy_loss")

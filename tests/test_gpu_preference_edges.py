@@ -99,3 +99,22 @@ def test_kl_gradient_of_an_impossible_reference(cuda_device):
     out.loss.backward()
     assert float(out.loss.detach()) == float(out.kl) == math.inf
     assert logp.grad.tolist() == [[0.25, 0.0]]
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_kl_as_a_statistic_alone(cuda_device, reduction):
+    """A reference with a coefficient of 0: its KL estimate is returned, and an infinite
+    one (s = 100) leaves the loss and its gradient as they are without it."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    old = -torch.rand(3, 50, generator=g, device="cuda")
+    old[1, 7] = -101.0
+    ref = old.clone()
+    ref[1, 7] = -1.0
+    adv = torch.randn(3, generator=g, device="cuda")
+    logp, plain = (old.clone().requires_grad_(True) for _ in range(2))
+    out = policy_loss(logp, old, adv, ref_logp=ref, reduction=reduction)
+    bare = policy_loss(plain, old, adv, reduction=reduction)
+    assert float(out.kl) == math.inf and torch.equal(out.loss, bare.loss)
+    out.loss.backward()
+    bare.loss.backward()
+    assert torch.equal(logp.grad, plain.grad) and bool(logp.grad.isfinite().all())
