@@ -31,6 +31,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import paths
@@ -173,6 +174,9 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     the head.
     """
     shape, table = x16.shape, head16.shape
+    # a dual tensor requires no gradient: without an autograd node its tangent would vanish
+    if unpack_dual(x16).tangent is not None or unpack_dual(head16).tangent is not None:
+        raise NotImplementedError("tied_head_logprobs has no forward-mode derivative")
     if (x16.dtype not in _CODES or head16.dtype != x16.dtype or len(shape) < 1 or len(table) != 2
             or not x16.is_cuda or shape[-1] != table[1] or not table[1]
             or table[0] % VOCAB_ALIGN or not 0 < vocab <= table[0]
