@@ -1253,6 +1253,16 @@ void logprob_scale(const float* __restrict__ grad, const int64_t* __restrict__ l
   }
 }
 
+// x twice, for the remainders' share of dw.  n % 8 == 0 elements.
+__global__ __launch_bounds__(256)
+void twice_k(const uint4* __restrict__ x, int64_t vecs, uint4* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= vecs) return;
+  const uint4 v = x[i];
+  out[i] = v;
+  out[vecs + i] = v;
+}
+
 // dst = fp16(src), round to nearest even; 8 elements per thread.
 __global__ __launch_bounds__(256)
 void cast_f32_f16(const float* __restrict__ src, __half* __restrict__ dst, int64_t n) {
@@ -2009,6 +2019,18 @@ int launch_stream(StreamArgs a, int dtype, hipStream_t s) {
   return rv_host::check_launch();
 }
 
+// The backward's workspace starts with the scale, its inverse and the rows' tops.
+constexpr int64_t kLogpHeader = 256 + kScaleTops * sizeof(float);
+
+// Rows whose logits' gradients are held as two 16-bit numbers, the rounded value and what
+// it left out: a row's gradients are mostly its label's, one rounding, as large as the
+// results' own.  Over many rows that adds up to 1.4 times the error of gradients in fp32
+// (1.33 to 1.41 where measured); over few it varies with their labels' (1.6 seen).  The remainders are rows of their own behind the others in both
+// products: logits, dx and dw of 300 x 256 over 50257 118 -> 146 us, 512 x 512 over 32000 140
+// -> 202, 1024 x 1024 over 50257 534 -> 823, so only where they are needed.
+constexpr int64_t kFineRows = 512;
+bool logp_fine(int64_t rows) { return rows <= kFineRows; }
+
 // Tiles of columns that the forward's statistics come in.
 int64_t logp_parts(int64_t rows, int64_t d, int64_t vocab) {
   const int64_t cols = stream_takes(d) ? 64 * stream_chunk(rows, vocab)
@@ -2356,28 +2378,6 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
     hipLaunchKernelGGL(logprob_rows<4>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, part,
                        label_logit, labels, rows, (int)tiles, vocab, ignore_index, logp, lse);
   return rv_host::check_launch();
-}
-
-// The backward's workspace starts with the scale, its inverse and the rows' tops.
-constexpr int64_t kLogpHeader = 256 + kScaleTops * sizeof(float);
-
-// Rows whose logits' gradients are held as two 16-bit numbers, the rounded value and what
-// it left out: a row's gradients are mostly its label's, one rounding, as large as the
-// results' own.  Over many rows that adds up to 1.4 times the error of gradients in fp32
-// (1.33 to 1.41 where measured); over few it varies with their labels' (1.6 seen).  The remainders are rows of their own behind the others in both
-// products: logits, dx and dw of 300 x 256 over 50257 118 -> 146 us, 512 x 512 over 32000 140
-// -> 202, 1024 x 1024 over 50257 534 -> 823, so only where they are needed.
-constexpr int64_t kFineRows = 512;
-bool logp_fine(int64_t rows) { return rows <= kFineRows; }
-
-// x twice, for the remainders' share of dw.  n % 8 == 0 elements.
-__global__ __launch_bounds__(256)
-void twice_k(const uint4* __restrict__ x, int64_t vecs, uint4* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= vecs) return;
-  const uint4 v = x[i];
-  out[i] = v;
-  out[vecs + i] = v;
 }
 
 int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded) {

@@ -2,7 +2,7 @@
 // of sequences and the clipped policy loss with a KL term, forward and backward.
 //
 // Inputs are fp32 [sequences][tokens] with row strides and a byte mask.  Both
-// are bandwidth-bound where they are large (9 to 17 bytes and about twenty
+// are bandwidth-bound where they are large (9 to 21 bytes and about twenty
 // operations a token) and bound by launches where they are small.  Differences
 // of log-probabilities are small against their sums over a sequence and cancel
 // between a pair's sequences, so all sums are fp64, in a fixed order.
