@@ -376,9 +376,10 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
  * either may be NULL.  Ignored rows have none (their grad is not used), a row of
  * another label outside [0, vocab) NaN.  padded, a multiple of 64, is the row count
  * of head; dw_rows is vocab or padded (pad rows: sums of zeros).  dz is held in dtype
- * in the workspace, times a power of two that brings the largest |grad| of a row
- * with a label to [2^14, 2^15); up to 512 rows as two such numbers, the rounded one
- * and what it left out.  rows <= 2^22. */
+ * in the workspace, times a power of two that brings a row's |grad| (fp16: each row's
+ * own, bf16: the largest of a row with a label) to [2^14, 2^15); up to 512 rows as two
+ * such numbers, the rounded one and what it left out.  dw's product takes x times powers
+ * of two that make up for the rows' (fp16).  rows <= 2^22, rows d < 2^34. */
 int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab, int64_t padded);
 int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
                      int64_t padded, int dtype, const int64_t* labels, int64_t ignore_index,

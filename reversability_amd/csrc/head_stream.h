@@ -129,7 +129,8 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
     const int64_t c = y - col0;
     label[i] = !ignored && !bad && c >= 0 && c < (int64_t)stages * 64 ? (int)c : -1;
     if constexpr (GRAD) {
-      g[i] = ignored ? 0.f : bad ? NAN : a.head_logp.grad[row] * *a.head_logp.scale;
+      g[i] = ignored ? 0.f : bad ? NAN
+             : a.head_logp.grad[row] * a.head_logp.scale[row * a.head_logp.scale_step];
       const float lse = ignored ? INFINITY : a.head_logp.lse[row];
       ref[i] = lse * kLog2e;  // its rounding is taken back in sum
       sum[i] = ignored ? 0.f

@@ -358,7 +358,7 @@ enum class Epi {
   LogProb,        // c = float2 [tile column][m]: a row's maximum and sum of exp over the tile
   LogProbGrad,    // c 16-bit, panels = scaled gradient of the logits
   LogProbLow,     // what LogProbGrad's 16 bits leave out, in 16 bits
-  StoreScaled,    // c 16-bit = acc * *scale, a in panels
+  StoreScaled,    // c 16-bit = acc * its row's scale, a in panels
   AccF32Scaled,   // c fp32 (+)= acc * *scale, a in panels
   PartialRagged,  // PartialF32 whose tiles may pass column n, a in panels
 };
@@ -402,7 +402,8 @@ struct HeadLogp {
   float* label_logit;      // LogProb, [m]: a row's logit at its label
   const float* lse;        // LogProbGrad, [m]: log sum exp of the row
   const float* grad;       // LogProbGrad, [m]: gradient of the row's log-probability
-  const float* scale;      // LogProbGrad: *scale multiplies the gradient; Scaled: the result
+  const float* scale;      // LogProbGrad: multiplies a row's gradient; Scaled: the result's
+  int64_t scale_step;      // 1: one for each row of the result, 0: one for all
   int64_t low;             // head_stream_k: what a row's 16 bits leave out goes to row + low
 };
 
@@ -810,9 +811,8 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
     if constexpr (kLogits) {
       // (LogProbLow is a launch of its own: both halves in one epilogue spilled the
       // accumulators, 1554 x 512 over 32000 94 -> 330 us.)
-      // acc = s ([j == label] - exp(z - lse)), s = the row's gradient times *scale (32768 x
+      // acc = s ([j == label] - exp(z - lse)), s = the row's gradient times its scale (32768 x
       // 1024 over 50257 3.44 ms with 3.3 GB of stores, 980 TFLOP/s)
-      const float scale = *args.head.scale;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int64_t row = m0 + wm * WM + i * 32 + (lane & 31);
@@ -820,7 +820,8 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
         const int64_t label = in ? args.head.labels[row] : args.head.ignore;
         const bool ignored = label == args.head.ignore;
         const bool bad = !ignored && (label < 0 || label >= args.head.vocab);
-        const float s = ignored ? 0.f : bad ? NAN : args.head.grad[row] * scale;
+        const float s = ignored ? 0.f : bad ? NAN
+                        : args.head.grad[row] * args.head.scale[row * args.head.scale_step];
         const float lse = ignored ? INFINITY : args.head.lse[row];
         const float shift = -lse * kLog2e;  // its rounding is taken back in t
         const float t = ignored ? 0.f : -s * __builtin_amdgcn_exp2f(-__builtin_fmaf(lse, kLog2e, shift));
@@ -848,13 +849,15 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
       }
     }
     if constexpr (EPI == Epi::StoreScaled) {
-      const float scale = *args.head.scale;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i) {
+        const int64_t row = m0 + wm * WM + i * 32 + (lane & 31);
+        const float scale = args.head.scale[(row < args.m ? row : 0) * args.head.scale_step];
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[i][j][e] *= scale;
+      }
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -1139,12 +1142,12 @@ void act_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t n, 
 }
 
 // The split reductions of the tied head's log-probability gradients: out[i] (+)=
-// *scale * sum_s part[s][i], splits summed in order; T fp32, fp16 or bf16 (added
-// to the fp32 result only).  n % 4 == 0.
+// scale * sum_s part[s][i], splits summed in order; T fp32, fp16 or bf16 (added
+// to the fp32 result only).  n % 4 == 0.  d > 0: a scale for each row of d; 0: *scale.
 template <typename T>
 __global__ __launch_bounds__(256)
 void scaled_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t n, int splits,
-                   const float* __restrict__ scale, int accumulate) {
+                   const float* __restrict__ scale, int64_t d, int accumulate) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
   float4 s = *reinterpret_cast<const float4*>(part + i);
@@ -1163,7 +1166,7 @@ void scaled_reduce(const float* __restrict__ part, T* __restrict__ out, int64_t 
     const float4 t = *reinterpret_cast<const float4*>(part + (int64_t)k * n + i);
     s.x = s.x + t.x; s.y = s.y + t.y; s.z = s.z + t.z; s.w = s.w + t.w;
   }
-  const float f = *scale;
+  const float f = scale[d > 0 ? i / d : 0];
   s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
   if constexpr (std::is_same<T, float>::value) {
     float4* o = reinterpret_cast<float4*>(out + i);
@@ -1219,12 +1222,105 @@ void logprob_rows(const float2* __restrict__ part, const float* __restrict__ lab
                                             : (label_logit[row] - all.x) - l;
 }
 
-// The power of two that brings the largest gradient of a row that counts to
-// [2^14, 2^15), and its inverse: the gradients of the logits are held in 16 bits,
-// where fp16 has no room for small ones (p g < 2^-24), and no logit's exceeds
-// its row's.  1 where none is finite and nonzero.  One workgroup over the rows (labels
+// The gradients of the logits are held in 16 bits, scaled by powers of two that bring a
+// row's gradient, which none of its logits' exceeds, to [2^14, 2^15).
+//
+// fp16 has no room for the small ones (p g < 2^-24), so each row has its own scale 2^e: what
+// its input gradient is made of does not depend on the other rows'.  The head's gradient
+// is a sum over the rows and needs one scale 2^C for all, so it takes x 2^(C - e) for x:
+// C is the least e + 14 - exponent(max |x|), at which all of these are below 2^15.  Rows
+// that do not count (ignored, or a gradient that is zero or not finite) have scale 1.
+__device__ __forceinline__ bool token_exponent(float grad, bool ignored, int& e) {
+  const float g = fabsf(grad);
+  e = 0;
+  if (ignored || !(g > 0.f && g < INFINITY)) return false;
+  e = 14 - ilogbf(g);
+  if (e > 126) e = 126;  // its inverse a normal number
+  return true;
+}
+
+// scale[r] = 2^e and its inverse; in tops, each workgroup's least e + 14 - exponent(max
+// |x|).  A wave a row.
+constexpr int kScaleTops = 1024;  // workgroups at most
+constexpr int kNoTop = 1 << 20;
+__global__ __launch_bounds__(256)
+void token_scales(const __half* __restrict__ x, const float* __restrict__ grad,
+                  const int64_t* __restrict__ labels, int64_t rows, int64_t d, int64_t ignore,
+                  float* __restrict__ scale, float* __restrict__ inverse, int* __restrict__ tops) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int least = kNoTop;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)gridDim.x * 4) {
+    uint32_t top = 0;  // the largest finite |x|, as bits
+    for (int64_t c = lane * 8; c < d; c += 512) {
+      const uint4 v = *reinterpret_cast<const uint4*>(x + r * d + c);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t b = w[k / 2] >> (k & 1) * 16 & 0x7fffu;
+        if (b < 0x7c00u && b > top) top = b;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const uint32_t other = __shfl_xor(top, o, 64);
+      top = other > top ? other : top;
+    }
+    int e;
+    const bool counts = token_exponent(grad[r], labels[r] == ignore, e);
+    if (counts && top > 0) {
+      const int at = e + 14 - ilogbf(__half2float(__ushort_as_half((unsigned short)top)));
+      least = at < least ? at : least;
+    }
+    if (lane == 0) {
+      scale[r] = ldexpf(1.f, e);
+      inverse[r] = ldexpf(1.f, -e);
+    }
+  }
+  __shared__ int red[4];
+  if (lane == 0) red[wave] = least;
+  __syncthreads();
+  if (threadIdx.x == 0) tops[blockIdx.x] = min(min(red[0], red[1]), min(red[2], red[3]));
+}
+
+// out = x 2^(C - e), C the least of `count` tops, and *unscale = 2^-C; TWICE: two copies, the
+// second for the remainders' rows.
+template <bool TWICE>
+__global__ __launch_bounds__(256)
+void scaled_tokens(const uint4* __restrict__ x, const float* __restrict__ grad,
+                   const int64_t* __restrict__ labels, int64_t vecs, int64_t row_vecs,
+                   int64_t ignore, const int* __restrict__ tops, int count,
+                   uint4* __restrict__ out, float* __restrict__ unscale) {
+  int least = kNoTop;
+  for (int t = threadIdx.x; t < count; t += 256) least = min(least, tops[t]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
+  __shared__ int red[4];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = least;
+  __syncthreads();
+  least = min(min(red[0], red[1]), min(red[2], red[3]));
+  if (least == kNoTop) least = 0;
+  if (least > 126) least = 126;  // its inverse a normal number, as from the least C, -114, on
+  if (blockIdx.x == 0 && threadIdx.x == 0) *unscale = ldexpf(1.f, -least);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= vecs) return;
+  const int64_t r = i / row_vecs;
+  int e;
+  const int shift = token_exponent(grad[r], labels[r] == ignore, e) ? least - e : 0;
+  const uint4 v = x[i];
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    w[k] = pack2<false>(__builtin_ldexpf(f.x, shift), __builtin_ldexpf(f.y, shift));
+  }
+  const uint4 y = make_uint4(w[0], w[1], w[2], w[3]);
+  out[i] = y;
+  if (TWICE) out[vecs + i] = y;
+}
+
+// bf16 has fp32's exponents, and one scale for all rows is enough: the largest row's, and its
+// inverse; 1 where no gradient is finite and nonzero.  One workgroup over the rows (labels
 // given), or over what several such left in `tops` (FINISH).
-constexpr int kScaleTops = 256;           // workgroups of the first pass over many rows
 constexpr int64_t kScaleRows = 1 << 14;   // rows that one workgroup takes alone
 template <bool FINISH>
 __global__ __launch_bounds__(1024)
@@ -1887,18 +1983,18 @@ int launch_logp(int shape, GemmArgs a, hipStream_t s) {
 
 template <typename T>
 int launch_scaled_reduce(const float* part, void* out, int64_t n, int64_t splits,
-                         const float* scale, int accumulate, hipStream_t s) {
+                         const float* scale, int64_t d, int accumulate, hipStream_t s) {
   hipLaunchKernelGGL(scaled_reduce<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, part,
-                     static_cast<T*>(out), n, (int)splits, scale, accumulate);
+                     static_cast<T*>(out), n, (int)splits, scale, d, accumulate);
   return rv_host::check_launch();
 }
 int launch_scaled_reduce(int dtype, const float* part, void* out, int64_t n, int64_t splits,
-                         const float* scale, int accumulate, hipStream_t s) {
+                         const float* scale, int64_t d, int accumulate, hipStream_t s) {
   if (dtype == RV_F32)
-    return launch_scaled_reduce<float>(part, out, n, splits, scale, accumulate, s);
+    return launch_scaled_reduce<float>(part, out, n, splits, scale, d, accumulate, s);
   if (dtype == RV_BF16)
-    return launch_scaled_reduce<__hip_bfloat16>(part, out, n, splits, scale, 0, s);
-  return launch_scaled_reduce<__half>(part, out, n, splits, scale, 0, s);
+    return launch_scaled_reduce<__hip_bfloat16>(part, out, n, splits, scale, d, 0, s);
+  return launch_scaled_reduce<__half>(part, out, n, splits, scale, d, 0, s);
 }
 
 // Widths as the tile choices above take them: whole tiles of 128 columns.
@@ -2019,8 +2115,9 @@ int launch_stream(StreamArgs a, int dtype, hipStream_t s) {
   return rv_host::check_launch();
 }
 
-// The backward's workspace starts with the scale, its inverse and the rows' tops.
-constexpr int64_t kLogpHeader = 256 + kScaleTops * sizeof(float);
+// The backward's workspace starts with the scale of all rows and its inverse (or the head
+// gradient's), the tops, and the rows' scales and inverses.
+int64_t logp_header(int64_t rows) { return 256 + kScaleTops * 4 + align256(rows * 8); }
 
 // Rows whose logits' gradients are held as two 16-bit numbers, the rounded value and what
 // it left out: a row's gradients are mostly its label's, one rounding, as large as the
@@ -2385,6 +2482,8 @@ int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab,
   if (bad) return -(int64_t)bad;
   // a tile's panels stay within 32-bit offsets
   if (rows > (int64_t)1 << 22) return -(int64_t)RV_ERR_UNSUPPORTED;
+  // and the passes over x and dx, four elements a thread, within one launch
+  if (rows >= ((int64_t)1 << 34) / d) return -(int64_t)RV_ERR_UNSUPPORTED;
   const bool fine = logp_fine(rows);
   const int64_t k = fine ? 2 * rows : rows;
   const WgradPlan p = plan_wgrad(k, padded, up128(d), true);
@@ -2392,7 +2491,7 @@ int64_t rv_head_logp_bwd_workspace_bytes(int64_t rows, int64_t d, int64_t vocab,
   const int64_t dx = fine ? logp_dx_plan(k, d, padded).splits * k * d * 4
                           : logp_dx_bytes(rows, d, padded);
   const int64_t dw = part_bytes(p, padded, up128(d));
-  return kLogpHeader + align256(k * padded * 2) + (fine ? align256(k * d * 2) : 0) +
+  return logp_header(rows) + align256(k * padded * 2) + align256(k * d * 2) +
          (dx > dw ? dx : dw);
 }
 
@@ -2412,22 +2511,29 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
   if (!workspace || workspace_bytes < need || !ok16(workspace)) return RV_ERR_WORKSPACE;
   const hipStream_t s = (hipStream_t)stream;
   const bool bf = dtype == RV_BF16;
-  // workspace: the scale and its inverse, the logits' gradients in panels (k rows), x
-  // twice if they have remainders, the products' partial sums
+  // workspace: the scales, the logits' gradients in panels (k rows), what dw takes for x if
+  // that is another, the products' partial sums
   const bool fine = logp_fine(rows);
   const int64_t k = fine ? 2 * rows : rows;
+  char* ws = static_cast<char*>(workspace);
   float* scale = static_cast<float*>(workspace);
   float* tops = scale + 64;
-  __half* dlogits = reinterpret_cast<__half*>(static_cast<char*>(workspace) + kLogpHeader);
-  __half* x2 = reinterpret_cast<__half*>(static_cast<char*>(workspace) + kLogpHeader +
-                                         align256(k * padded * 2));
-  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(x2) +
-                                         (fine ? align256(k * d * 2) : 0));
-  if (rows <= kScaleRows) {
+  float* token_scale = tops + kScaleTops;
+  float* token_inverse = token_scale + rows;
+  __half* dlogits = reinterpret_cast<__half*>(ws + logp_header(rows));
+  __half* x2 = reinterpret_cast<__half*>(ws + logp_header(rows) + align256(k * padded * 2));
+  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(x2) + align256(k * d * 2));
+  const int64_t step = bf ? 0 : 1;  // of the scales
+  const int wgs_x = (int)std::min<int64_t>(kScaleTops, (rows + 3) / 4);
+  if (!bf) {
+    hipLaunchKernelGGL(token_scales, dim3(wgs_x), dim3(256), 0, s, static_cast<const __half*>(x),
+                       grad, labels, rows, d, ignore_index, token_scale, token_inverse,
+                       reinterpret_cast<int*>(tops));
+  } else if (rows <= kScaleRows) {
     hipLaunchKernelGGL(logprob_scale<true>, dim3(1), dim3(1024), 0, s, grad, labels, rows,
                        ignore_index, tops, scale);
   } else {
-    const int wgs = (int)std::min<int64_t>(kScaleTops, (rows + 4095) / 4096);
+    const int wgs = (int)std::min<int64_t>(256, (rows + 4095) / 4096);
     hipLaunchKernelGGL(logprob_scale<false>, dim3(wgs), dim3(1024), 0, s, grad, labels, rows,
                        ignore_index, tops, scale);
     hipLaunchKernelGGL(logprob_scale<true>, dim3(1), dim3(1024), 0, s, tops,
@@ -2435,7 +2541,8 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
   }
   GemmArgs z = logp_args(x, head, rows, d, padded, labels, ignore_index, vocab);
   z.c = dlogits; z.valid = vocab; z.panel = k * 32; z.panels = padded / 32;
-  z.head.lse = lse; z.head.grad = grad; z.head.scale = scale; z.head.low = fine ? rows : 0;
+  z.head.lse = lse; z.head.grad = grad; z.head.low = fine ? rows : 0;
+  z.head.scale = bf ? scale : token_scale; z.head.scale_step = step;
   int st;
   if (stream_takes(d)) {
     const StreamArgs t{z.a, z.b, rows, padded, d, 0, 0, 0, 0, nullptr, dlogits, z.head, k};
@@ -2458,7 +2565,7 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
     a.b = static_cast<const __half*>(head); a.ldb = d;  // B(d, v) = head[v][d]: RC
     a.b_bytes = vocab * d * 2;  // the operand ends here: the pad rows read as zero
     a.m = k; a.n = d; a.k = padded; a.k_chunk = p.chunk;
-    a.ldc = d; a.head.scale = scale + 1;
+    a.ldc = d; a.head.scale = bf ? scale + 1 : token_inverse; a.head.scale_step = step;
     if (p.splits == 1 && !fine) {
       a.c = dx;
       st = bf ? launch_logp<false, true, Epi::StoreScaled, true>(p.shape, a, s)
@@ -2469,23 +2576,31 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
               : launch_logp<false, true, Epi::PartialRagged, false>(p.shape, a, s);
       if (st == RV_OK)
         // the remainders' sums follow the rows' own in each split
-        st = launch_scaled_reduce(dtype, part, dx, rows * d, p.splits * (fine ? 2 : 1), scale + 1,
-                                  0, s);
+        st = launch_scaled_reduce(dtype, part, dx, rows * d, p.splits * (fine ? 2 : 1),
+                                  a.head.scale, bf ? 0 : d, 0, s);
     }
     if (st != RV_OK) return st;
   }
   if (dw) {
     // dW[v][d] = sum_m dlogits[m][v] x[m][d]; of the pad rows the sum of zeros
     const WgradPlan p = plan_wgrad(k, padded, up128(d), true);
-    if (fine) {
-      const int64_t vecs = rows * d / 8;
-      hipLaunchKernelGGL(twice_k, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s,
-                         static_cast<const uint4*>(x), vecs, reinterpret_cast<uint4*>(x2));
-    }
-    WgradJob j = plan_job(p, dlogits, padded, fine ? x2 : static_cast<const __half*>(x), d, k,
+    const int64_t vecs = rows * d / 8;
+    const uint4* from = static_cast<const uint4*>(x);
+    uint4* to = reinterpret_cast<uint4*>(x2);
+    const dim3 grid((unsigned)((vecs + 255) / 256)), block(256);
+    if (bf && fine)
+      hipLaunchKernelGGL(twice_k, grid, block, 0, s, from, vecs, to);
+    else if (fine)
+      hipLaunchKernelGGL(scaled_tokens<true>, grid, block, 0, s, from, grad, labels, vecs, d / 8,
+                         ignore_index, reinterpret_cast<int*>(tops), wgs_x, to, scale + 1);
+    else if (!bf)
+      hipLaunchKernelGGL(scaled_tokens<false>, grid, block, 0, s, from, grad, labels, vecs, d / 8,
+                         ignore_index, reinterpret_cast<int*>(tops), wgs_x, to, scale + 1);
+    WgradJob j = plan_job(p, dlogits, padded, bf && !fine ? static_cast<const __half*>(x) : x2, d, k,
                           dw_rows, d,
                           static_cast<float*>(dw), accumulate, part);
     j.g.panel = z.panel; j.g.panels = z.panels; j.g.head.scale = scale + 1;
+    j.g.head.scale_step = 0;
     if (p.splits == 1) {
       if (dw_dtype == RV_F32)
         return bf ? launch_logp<true, true, Epi::AccF32Scaled, true>(p.shape, j.g, s)
@@ -2496,7 +2611,7 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
     st = bf ? launch_logp<true, true, Epi::PartialRagged, true>(p.shape, j.g, s)
             : launch_logp<true, true, Epi::PartialRagged, false>(p.shape, j.g, s);
     if (st == RV_OK)
-      st = launch_scaled_reduce(dw_dtype, part, dw, dw_rows * d, p.splits, scale + 1, accumulate, s);
+      st = launch_scaled_reduce(dw_dtype, part, dw, dw_rows * d, p.splits, scale + 1, 0, accumulate, s);
   }
   return st;
 }

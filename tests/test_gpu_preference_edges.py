@@ -118,3 +118,57 @@ def test_kl_as_a_statistic_alone(cuda_device, reduction):
     out.loss.backward()
     bare.loss.backward()
     assert torch.equal(logp.grad, plain.grad) and bool(logp.grad.isfinite().all())
+
+
+# up to 512 rows and more, both sides of width 256, products in one piece and split
+APART_SIZES = [(9, 256, 5000), (300, 512, 5000), (600, 128, 20000), (700, 640, 8000),
+               (2100, 512, 12305), (20000, 64, 500)]
+
+
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("rows,d,vocab", APART_SIZES)
+def test_gradients_of_tokens_far_apart(cuda_device, rows, d, vocab, few):
+    """fp16, token gradients over 2^30: a small one's input gradient is its own, not what a
+    larger one's scale leaves of it (the softmax's part takes most of the label's away
+    here: the head's rows are much alike).  ``few``: one token is large, the others
+    2^-24 of it and less.
+
+    A logit's gradient is off by u of it and, in fp16's last range, by half a step at the scale
+    that brings its token's gradient to 2^14 or more: 2^-39 of that; by its exponential's
+    argument, d 2^-24 and a few more units of sum |x w|; the sums of n products by n
+    2^-24.  The head's gradient takes x at a scale of the token too: off by 2^-25 where the
+    largest |g| max|x| is at 2^28 or more, times a logit gradient of up to 2^15: by
+    2^-38 of that largest one, times dz / g."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    u = 2.0 ** -11
+    head = torch.zeros(-(-vocab // 64) * 64, d, device="cuda", dtype=torch.float16)
+    head[:vocab] = 0.25 + 0.05 * torch.randn(vocab, d, generator=g, device="cuda")
+    x = (torch.randn(rows, d, generator=g, device="cuda") / math.sqrt(d)).half()
+    labels = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    labels[rows // 2] = -100
+    low = 24 * torch.ones(rows, device="cuda") if few else torch.zeros(rows, device="cuda")
+    grad = 2.0 ** (15 - low - (6 if few else 30) * torch.rand(rows, generator=g, device="cuda"))
+    grad[0] = 2.0 ** 15
+    grad[rows // 2] = 2.0 ** 30  # not scored: not looked at
+    x.requires_grad_(True)
+    head.requires_grad_(True)
+    dx, dhead = torch.autograd.grad(tied_head_logprobs(x, head, vocab, labels), (x, head), grad)
+    xd, w = x.detach().double(), head.detach()[:vocab].double()
+    on = labels != -100
+    gd = (grad.double() * on)[:, None]
+    z = xd @ w.t()
+    p = z.softmax(1)
+    share = -p  # dz / g
+    share.scatter_add_(1, labels.clamp_min(0)[:, None], torch.ones_like(gd))
+    argument = (2 * d + 8) * 2.0 ** -24 * (xd.abs() @ w.abs().t()).amax(1, keepdim=True) + 2.0 ** -14
+    off = share.abs() * u + p * argument + 2.0 ** -39
+    rx = gd * (share @ w)
+    bx = gd.abs() * (off @ w.abs() + vocab * 2.0 ** -24 * (share.abs() @ w.abs()))
+    bx += u * rx.abs() + 2.0 ** -25
+    assert bool(((dx.double() - rx).abs() <= bx).all()), float(((dx.double() - rx).abs() / bx).max())
+    rh = (gd * share).t() @ xd
+    largest = float((gd[:, 0].abs() * xd.abs().amax(1)).max())
+    bh = (gd.abs() * off).t() @ xd.abs() + rows * 2.0 ** -24 * ((gd * share).abs().t() @ xd.abs())
+    bh += largest * 2.0 ** -38 * share[on].abs().sum(0)[:, None] + u * rh.abs() + 2.0 ** -25
+    assert bool(((dhead[:vocab].double() - rh).abs() <= bh).all())
+    assert not dx[rows // 2].any() and not dhead[vocab:].any()
