@@ -361,9 +361,10 @@ int rv_head_dw(const void* dlogits, const void* x, int64_t rows, int64_t d, int6
 /* Log-probabilities of the labels under the tied head, without the logits in
  * memory: z = x head^T with fp32 sums, lse[r] = log sum_{j < vocab} exp(z[r, j]),
  * logp[r] = z[r, labels[r]] - lse[r]; 0 for label == ignore_index, NaN for
- * another label outside [0, vocab).  x [rows, d] and head [>= vocab, d] of dtype
- * RV_F16 or RV_BF16, 16-byte aligned, d a multiple of 8; labels int64 [rows];
- * logp, lse (may be NULL: scoring alone) fp32 [rows]. */
+ * another label outside [0, vocab) and where the row's largest z is beyond 2^126 in
+ * magnitude (lower ones than -2^126 count for nothing).  x [rows, d] and head [>=
+ * vocab, d] of dtype RV_F16 or RV_BF16, 16-byte aligned, d a multiple of 8; labels int64
+ * [rows]; logp, lse (may be NULL: scoring alone) fp32 [rows]. */
 int64_t rv_head_logp_workspace_bytes(int64_t rows, int64_t d, int64_t vocab);
 int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, int64_t vocab,
                      int dtype, const int64_t* labels, int64_t ignore_index, float* logp,

@@ -137,7 +137,7 @@ __device__ __forceinline__ void head_stream(const StreamArgs& a) {
                        : -g[i] * __builtin_amdgcn_exp2f(-__builtin_fmaf(lse, kLog2e, -ref[i]));
     } else {
       g[i] = sum[i] = 0.f;
-      top[i] = -1e38f;  // finite: no logit is lower, and differences of it are numbers
+      top[i] = kLowest;  // finite: differences of it are numbers
       ref[i] = top[i] * kLog2e;
     }
   }

@@ -364,6 +364,9 @@ enum class Epi {
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
+// Logits below it count for nothing beside higher ones (times log2e they may overflow); a
+// row has no log-probabilities unless its largest is between it and its negative.
+constexpr float kLowest = -0x1p126f;
 
 // Two fp32 values rounded to nearest even to the 16-bit operand type.
 template <bool BF>
@@ -709,7 +712,9 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       // exp(z - top) = exp2(z log2e + shift) in one multiply-add and one v_exp; shift's
       // rounding (a factor 1 +- 2^-24 |top|) is taken back from the sum
-      const float shift = top == -INFINITY ? 0.f : -top * kLog2e;  // no column in use
+      // (columns masked by the type's lowest value, or none in use: exponentials of 0)
+      const bool low = top < kLowest;
+      const float shift = low ? 0.f : -top * kLog2e;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < TN; ++j)
@@ -717,7 +722,7 @@ __device__ __forceinline__ void gemm_block(const GemmArgs& args, int64_t block) 
         for (int e = 0; e < 16; ++e)
           sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, shift));
       sum += __shfl_xor(sum, 32, 64);
-      if (top != -INFINITY) sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(top, kLog2e, shift));
+      if (!low) sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(top, kLog2e, shift));
       if (lane < 32) red[wn * BM + r] = make_float2(top, sum);
       // the label's logit, where the label is one of the wave's columns
       const int64_t label = row < args.m ? args.head.labels[row] : -1;
@@ -1215,7 +1220,7 @@ void logprob_rows(const float2* __restrict__ part, const float* __restrict__ lab
 #pragma unroll
   for (int w = 1; w < 4; ++w) all = join(all, red[w][r]);
   const int64_t label = labels[row];
-  const float l = logf(all.y);
+  const float l = all.y > 0.f ? logf(all.y) : NAN;  // 0: the largest is out of range
   if (lse != nullptr) lse[row] = all.x + l;
   logp[row] = label == ignore ? 0.f
               : label < 0 || label >= vocab ? NAN

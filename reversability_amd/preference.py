@@ -172,7 +172,8 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     token, so that a small gradient of x16 does not depend on larger ones of other tokens
     (up to 512 tokens as two 16-bit numbers each); gradients come in the operands' type.
     As in any product, a NaN or an infinity in an unscored token's row of ``x16`` reaches
-    the gradient of the head.  Logits beyond 2^126 in magnitude have no defined result.
+    the gradient of the head.  A row whose largest logit is beyond 2^126 in magnitude has
+    no log-probability (NaN); lower logits than -2^126 count for nothing.
     """
     shape, table = x16.shape, head16.shape
     # a dual tensor requires no gradient: without an autograd node its tangent would vanish

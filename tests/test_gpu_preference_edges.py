@@ -172,3 +172,51 @@ def test_gradients_of_tokens_far_apart(cuda_device, rows, d, vocab, few):
     bh += largest * 2.0 ** -38 * share[on].abs().sum(0)[:, None] + u * rh.abs() + 2.0 ** -25
     assert bool(((dhead[:vocab].double() - rh).abs() <= bh).all())
     assert not dx[rows // 2].any() and not dhead[vocab:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,d,vocab", NAN_SIZES)
+def test_columns_masked_with_the_lowest_value(cuda_device, rows, d, vocab, dtype):
+    """A vocabulary whose first columns, and one in five of the others, are masked by the
+    type's lowest value (times a constant input): as if they were not there, also
+    for the gradients of the others, and a masked label's log-probability is as low."""
+    x, head, labels = operands(rows, d, vocab, dtype, seed=2)
+    masked = torch.rand(vocab, generator=torch.Generator().manual_seed(9)) < 0.2
+    masked[:min(256, vocab - 1)] = True
+    masked[vocab - 1] = False
+    masked = masked.cuda()
+    x[:, 1] = 1.0
+    head[:vocab, 1] = torch.where(masked, torch.finfo(dtype).min, 0.0).to(dtype)
+    kept = (~masked).nonzero()[:, 0]
+    place = torch.randint(0, len(kept), (rows,), device="cuda")
+    place[min(2, rows - 1)] = 0
+    small = -(-len(kept) // 64) * 64
+    other = torch.zeros(small, d, device="cuda", dtype=dtype)
+    other[:len(kept)] = head[kept]
+    a, b = ((t.clone().requires_grad_(True), u.clone().requires_grad_(True))
+            for t, u in ((x, head), (x, other)))
+    one = tied_head_logprobs(*a, vocab, kept[place])
+    two = tied_head_logprobs(*b, len(kept), place)
+    assert bool(((one - two).abs() <= 1e-4).all())  # other tiles: sums in another order
+    weight = torch.randn(rows, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    got = torch.autograd.grad(one, a, weight)
+    ref = torch.autograd.grad(two, b, weight)
+    # both sides are rounded twice, and another order moves a rounding: 2^-8 at the most in
+    # fp16 and 2^-6 in bf16 of the largest entry
+    near = {torch.float16: 2.0 ** -8, torch.bfloat16: 2.0 ** -6}[dtype]
+    assert float((got[0] - ref[0]).abs().max()) <= near * float(ref[0].abs().max())
+    assert float((got[1][kept] - ref[1][:len(kept)]).abs().max()) <= near * float(ref[1].abs().max())
+    assert not got[1][:vocab][masked].any()
+    labels[0] = 0
+    low = tied_head_logprobs(x, head, vocab, labels)
+    assert bool(low.isfinite().all()) and float(low[0]) < 0.99 * torch.finfo(dtype).min
+
+
+@pytest.mark.parametrize("lowest", [-1.0, 1.0])
+@pytest.mark.parametrize("rows,d,vocab", NAN_SIZES)
+def test_rows_out_of_range_have_no_log_probability(cuda_device, rows, d, vocab, lowest):
+    x, head, labels = operands(rows, d, vocab, torch.bfloat16, seed=2)
+    x[:, 1] = 1.0
+    head[:vocab, 1] = lowest * torch.finfo(torch.bfloat16).max
+    logp = tied_head_logprobs(x, head, vocab, labels)
+    assert bool(logp[labels != -100].isnan().all()) and not logp[labels == -100].any()
