@@ -446,6 +446,8 @@ def _loss_backward(model, ids, labels, loss_of, chunk_tokens, scaler, precision)
     returns a result whose first item is the loss.  Gradients are added to the
     parameters' ``.grad``."""
     from .optimized_v3 import castable_weights
+    if not torch.is_grad_enabled():
+        raise ValueError("an update needs gradients enabled")
     dtype = _compute_dtype(model, ids, precision)
     targets = _labels(ids, labels)
     if chunk_tokens is not None and not 1 <= chunk_tokens <= 1 << 22:
@@ -455,6 +457,8 @@ def _loss_backward(model, ids, labels, loss_of, chunk_tokens, scaler, precision)
             prefetch_casts(castable_weights(model))
         with amp_context(ids.device, precision):
             hidden = hidden_states(model, ids)
+        if not hidden.requires_grad:  # before the head's gradient is added
+            raise ValueError("an update needs gradients of the hidden states")
         weight = model.lm_head.weight
         vocab, d = weight.shape
         flat = hidden.detach().reshape(-1, d)
