@@ -26,6 +26,11 @@
 // accumulators of 64 rows, and with 32 rows a wave every MFMA would read 1 KB of LDS, all
 // that the LDS delivers.
 //
+// Registers: all 256 at widths 129 to 256.  Forward and backward keep 3 values in scratch and
+// read them after the loop or where a label falls; with remainders (GradLow) it is 17, a
+// fragment of x among them, which every block reads again behind a wait for all loads and
+// stores: 300 x 256 over 50257 37 us where the forward takes 22 (0.54 of 4 matrix cores busy).
+//
 // Included by mlp_gemm.hip, whose staging, LDS and epilogue helpers it uses.
 #pragma once
 

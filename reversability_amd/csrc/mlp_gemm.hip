@@ -2124,12 +2124,15 @@ int launch_stream(StreamArgs a, int dtype, hipStream_t s) {
 // gradient's), the tops, and the rows' scales and inverses.
 int64_t logp_header(int64_t rows) { return 256 + kScaleTops * 4 + align256(rows * 8); }
 
-// Rows whose logits' gradients are held as two 16-bit numbers, the rounded value and what
-// it left out: a row's gradients are mostly its label's, one rounding, as large as the
-// results' own.  Over many rows that adds up to 1.4 times the error of gradients in fp32
-// (1.33 to 1.41 where measured); over few it varies with their labels' (1.6 seen).  The remainders are rows of their own behind the others in both
-// products: logits, dx and dw of 300 x 256 over 50257 118 -> 146 us, 512 x 512 over 32000 140
-// -> 202, 1024 x 1024 over 50257 534 -> 823, so only where they are needed.
+// Up to this many rows the logits' gradients are held as two 16-bit numbers, the rounded value
+// and what it left out.  A row's gradients are mostly its label's, and one rounding of that
+// is as large as the results' own: with one number both gradients have 1.33 to 1.43 times
+// the error of fp32 ones (fp16 2.9e-4 against 2.1e-4, bf16 2.3e-3 against 1.7e-3), at
+// any size; over a few rows it varies with their labels (1.6 seen).  The line is where
+// the price of exact gradients was put, not where the error changes: the remainders are
+// rows of their own behind the others in both products, and a trained call takes 209 us for
+// 512 x 256 over 50257 where 513 rows take 164, 228 for 512 x 512 over 32000 where 513 take
+// 184 (1024 x 1024 over 50257, backward alone, 823 us with them and 540 without).
 constexpr int64_t kFineRows = 512;
 bool logp_fine(int64_t rows) { return rows <= kFineRows; }
 

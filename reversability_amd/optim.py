@@ -268,7 +268,8 @@ class FusedAdamW8bit(FusedAdamW):
     repeats bit for bit.  GradScaler, ``unscale_clip_``, the device-side step count
     and graph capture work as in ``FusedAdamW``; ``moments(p)`` returns a
     parameter's moments in fp32.  A checkpoint of ``FusedAdamW`` can be loaded (its
-    moments stay in fp32), not the other way round.
+    moments stay in fp32; a large parameter that it has none for gets 8-bit ones), not
+    the other way round.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
