@@ -94,7 +94,7 @@ def _logp_backward(x, head, vocab, labels, lse, grad, dx=None, dw=None, accumula
     rows, d = x.shape
     padded = head.shape[0]
     lib, code = library(), _CODES[x.dtype]
-    step = min(rows, chunk_tokens or max_chunk(padded))
+    step = min(rows, chunk_of(padded, d, chunk_tokens))
     out = (None, vocab, code) if dw is None else (
         dw.data_ptr(), dw.shape[0], RV_F32 if dw.dtype == torch.float32 else code)
     with _DeviceGuard(x):
@@ -118,6 +118,11 @@ def max_chunk(padded: int) -> int:
     """Tokens whose 16-bit logit gradients over ``padded`` columns fill GRADIENT_BYTES
     (at most 2^22, what one call takes)."""
     return min(1 << 22, max(256, GRADIENT_BYTES // (2 * padded) // 256 * 256))
+
+
+def chunk_of(padded: int, d: int, chunk_tokens: Optional[int]) -> int:
+    """Tokens that the backward takes at a time (one call: fewer than 2^34 elements of x)."""
+    return min(chunk_tokens or max_chunk(padded), ((1 << 34) - 1) // d)
 
 
 class TiedHeadLogProbs(torch.autograd.Function):
@@ -144,7 +149,7 @@ class TiedHeadLogProbs(torch.autograd.Function):
         width, padded = ctx.width, head.shape[0]
         grad = gradient.contiguous()
         dx = x.new_empty(rows, width) if need_x else None
-        one = rows <= (ctx.chunk_tokens or max_chunk(padded))
+        one = rows <= chunk_of(padded, width, ctx.chunk_tokens)
         dw = (torch.empty(padded, width, device=x.device,
                           dtype=head.dtype if one else torch.float32) if need_head else None)
         _logp_backward(_rows16(x, width), _rows16(head, width), ctx.vocab, labels, lse, grad, dx,
