@@ -456,8 +456,8 @@ int rv_adamw_step_clipped(int count, float* const* params, const float* const* g
  * per rv_adamw8_block() consecutive elements of a tensor (value = e4m3 *
  * 2^(b - 127); ceil(numel / block) bytes, all zero at the start).  p takes the fp32
  * moments; what is stored is rounded, the second moment at random (its expectation
- * kept), the first to nearest where 1 - beta1 >= 2^-4 and else at random too, with bits that follow from seed, the tensor's
- * ordinal, *step and the element's index alone.  Multiplies and adds are rounded
+ * kept), the first to nearest where 1 - beta1 >= 2^-4 and else at random too, with bits
+ * that follow from seed, the tensor's ordinal, *step and the element's index alone.  Multiplies and adds are rounded
  * one by one (no fused multiply-add). */
 int rv_adamw8_max_tensors(void);
 int rv_adamw8_block(void);

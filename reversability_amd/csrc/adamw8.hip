@@ -18,9 +18,9 @@
 // expectation.  m goes to the nearest value where 1 - b1 is at least 2^-4, the largest
 // half step (2^-4 of it: it is replaced within 1 / (1 - b1) steps, and a zero gradient
 // takes every value to a smaller one); with a slower b1 it would stand still like v, and is
-// rounded at random too (303 us where the nearest takes 293, below).  The random bits are MurmurHash3's 32-bit finalizer (A. Appleby) of
-// the element's index plus a key of seed, tensor and step: the same call gives the
-// same bits.  A v > 0 stays > 0: a zero v under an m that is not would make the next
+// rounded at random too (303 us where the nearest takes 293, below).  The random bits are
+// MurmurHash3's 32-bit finalizer (A. Appleby) of the element's index plus a key of seed,
+// tensor and step: the same call gives the same bits.  A v > 0 stays > 0: a zero v under an m that is not would make the next
 // update as large as 1 / eps.
 //
 // Memory-bound: 16.125 bytes a parameter (p 8, g 4, codes 4, scales 4 / 32; 28 with fp32

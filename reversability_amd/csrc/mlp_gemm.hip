@@ -2468,8 +2468,8 @@ int rv_head_logp_fwd(const void* x, const void* head, int64_t rows, int64_t d, i
   const hipStream_t s = (hipStream_t)stream;
   int st;
   if (stream_takes(d)) {
-    st = launch_stream<Stream::Logp>({a.a, a.b, rows, vocab, d, 0, 0, 0, 0, part, nullptr, a.head, 0}, dtype,
-                              s);
+    st = launch_stream<Stream::Logp>(
+        {a.a, a.b, rows, vocab, d, 0, 0, 0, 0, part, nullptr, a.head, 0}, dtype, s);
   } else {
     const int shape = logp_z_shape(rows, d, vocab);
     st = dtype == RV_BF16 ? launch_logp<false, false, Epi::LogProb, true>(shape, a, s)
@@ -2604,9 +2604,8 @@ int rv_head_logp_bwd(const void* x, const void* head, int64_t rows, int64_t d, i
     else if (!bf)
       hipLaunchKernelGGL(scaled_tokens<false>, grid, block, 0, s, from, grad, labels, vecs, d / 8,
                          ignore_index, reinterpret_cast<int*>(tops), wgs_x, to, scale + 1);
-    WgradJob j = plan_job(p, dlogits, padded, bf && !fine ? static_cast<const __half*>(x) : x2, d, k,
-                          dw_rows, d,
-                          static_cast<float*>(dw), accumulate, part);
+    WgradJob j = plan_job(p, dlogits, padded, bf && !fine ? static_cast<const __half*>(x) : x2, d,
+                          k, dw_rows, d, static_cast<float*>(dw), accumulate, part);
     j.g.panel = z.panel; j.g.panels = z.panels; j.g.head.scale = scale + 1;
     j.g.head.scale_step = 0;
     if (p.splits == 1) {

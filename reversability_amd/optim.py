@@ -55,8 +55,8 @@ class FusedAdamW(Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def _group_params(self, group):
-        """A group's parameters with elements and a gradient; raises for what the kernels do not take
-        (they read everything through its address) and changes nothing."""
+        """A group's parameters with elements and a gradient; raises for what the kernels do
+        not take (they read everything through its address) and changes nothing."""
         params = [p for p in group["params"] if p.grad is not None and p.numel()]
         if not params:
             return params

@@ -173,8 +173,9 @@ def tied_head_logprobs(x16: torch.Tensor, head16: torch.Tensor, vocab: int, labe
     -100 gives 0 and no gradient, another one outside [0, vocab) gives NaN (in its
     gradients too).  Products are summed in fp32 and the logits never rounded.  The
     backward holds ``chunk_tokens`` tokens' logit gradients in 16 bits at a time
-    (default: as many as fill GRADIENT_BYTES), in fp16 scaled by a power of two for each
-    token, so that a small gradient of x16 does not depend on larger ones of other tokens
+    (default: as many as fill GRADIENT_BYTES, 4 GiB; fewer take less memory), in fp16 scaled
+    by a power of two for each token, so that a small gradient of x16 does not depend on
+    larger ones of other tokens
     (up to 512 tokens as two 16-bit numbers each); gradients come in the operands' type.
     As in any product, a NaN or an infinity in an unscored token's row of ``x16`` reaches
     the gradient of the head.  A row whose largest logit is beyond 2^126 in magnitude has
