@@ -589,6 +589,90 @@ int rv_attn_bwd(const void* qkv, const void* out, const void* dout, const float*
                 void* dqkv, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Windowed attention and the attention over a paged cache (no counterpart in the
+ * reference, whose attention is causal over whole sequences).  dtype RV_F16 or
+ * RV_BF16; head_dim 32, 64 or 128; heads a multiple of kv_heads: query head h reads key
+ * and value head h / (heads / kv_heads).  A packed row (qkv) holds heads queries, kv_heads
+ * keys and kv_heads values of head_dim.  16-bit pointers, tables and workspaces 16-byte
+ * aligned.
+ */
+
+/* Causal attention with a sliding window (> 0) and `sinks` (>= 0) first tokens that
+ * stay visible: query i sees key j <= i where i - j < window or j < sinks.  qkv
+ * [batch, seq, (heads + 2 kv_heads) head_dim]; out [batch, seq, heads, head_dim]; lse
+ * fp32 [batch * heads, seq] (base 2). */
+int rv_window_attn_fwd(const void* qkv, int64_t batch, int64_t seq, int64_t heads,
+                       int64_t kv_heads, int64_t head_dim, int dtype, int64_t window,
+                       int64_t sinks, void* out, float* lse, void* stream);
+
+/* Workspace bytes of rv_window_attn_bwd (negative: -error). */
+int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
+                                           int64_t kv_heads, int64_t head_dim, int64_t window,
+                                           int64_t sinks);
+
+/* dqkv (qkv's type and layout) = gradient of out with respect to qkv, given dout and the
+ * forward's out and lse.  Deterministic. */
+int rv_window_attn_bwd(const void* qkv, const void* out, const void* dout, const float* lse,
+                       int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, int dtype, int64_t window, int64_t sinks, void* dqkv,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dst = the packed rows src [tokens] with every query and key head's pairs (a, b) of
+ * columns -- (i, i + head_dim / 2), or (2 i, 2 i + 1) if interleaved -- as (a cos - b sin,
+ * a sin + b cos); back: by the negative angle (the gradient).  table fp32 [table_rows,
+ * head_dim / 2, 2] (cosine, sine) by position; positions [tokens], NULL: the token's index
+ * modulo seq.  A position outside the table gives NaN queries and keys. */
+int rv_rotate_qkv(const void* src, void* dst, int64_t tokens, int64_t seq, int64_t heads,
+                  int64_t kv_heads, int64_t head_dim, int dtype, const float* table,
+                  int64_t table_rows, const int32_t* positions, int interleaved, int back,
+                  void* stream);
+
+/* A paged cache of one layer: keys and values [pages, kv_heads, page_size, head_dim],
+ * page_size a power of two in [16, 256]; slot page * page_size + row.  A batch of
+ * sequences: sequence b holds lengths[b] tokens in the pages page_table[b * ld_table + 0 ..
+ * table_pages - 1], the last starts[b + 1] - starts[b] of them new, rows starts[b] .. of the
+ * batch's `tokens` rows (starts [seqs + 1], not decreasing).  tree (nullable) [tokens]: the
+ * new tokens are a tree, bit i of a token's mask says that it sees the i-th new one of its
+ * sequence (at most 64, itself among them); its position is then that of the last token
+ * in front of the new ones plus the number of its bits. */
+
+/* slots [tokens] (-1: a row of no sequence, or a token that its pages do not hold) and
+ * positions [tokens] of the batch's rows. */
+int rv_cache_plan(const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                  const int32_t* lengths, const int32_t* starts, const int64_t* tree,
+                  int64_t seqs, int64_t tokens, int64_t page_size, int64_t* slots,
+                  int32_t* positions, void* stream);
+
+/* The packed rows' (row stride ld) keys and values into their slots (outside [0, pages *
+ * page_size): not stored), with a table rotated as rv_rotate_qkv does; q [tokens, heads,
+ * head_dim]: the queries (NULL without a table: they are not copied). */
+int rv_append_kv(const void* qkv, int64_t ld, void* q, void* keys, void* values,
+                 const int64_t* slots, int64_t tokens, int64_t heads, int64_t kv_heads,
+                 int64_t head_dim, int dtype, int64_t pages, int64_t page_size,
+                 const float* table, int64_t table_rows, const int32_t* positions,
+                 int interleaved, void* stream);
+
+/* Workspace bytes of rv_cached_attn (0: none; negative: -error). */
+int64_t rv_cached_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads,
+                                       int64_t kv_heads, int64_t head_dim, int64_t max_query,
+                                       int64_t max_length, int64_t window, int64_t sinks);
+
+/* out [tokens, heads, head_dim] = attention of the new tokens' q (row stride q_ld) over
+ * their sequences' caches: the slots up to a token's own, or with a tree the context and
+ * what its mask has; with a window (0: none) of these the tokens less than `window`
+ * positions before it and the first `sinks` positions.  A row that sees nothing is zeros;
+ * rows of no sequence, and those past a sequence's first max_query, are left as they
+ * were.  max_length: what a sequence holds at most (a longer one is still right, but
+ * slower).  Pages outside [0, pages) hold nothing.  Deterministic. */
+int rv_cached_attn(const void* q, int64_t q_ld, const void* keys, const void* values,
+                   const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                   const int32_t* lengths, const int32_t* starts, const int64_t* tree,
+                   int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                   int64_t head_dim, int dtype, int64_t pages, int64_t page_size,
+                   int64_t max_query, int64_t max_length, int64_t window, int64_t sinks,
+                   void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Token pipeline and token + position embedding (the steps in front of the
  * reversible stack).  Tables and activations fp32, d a multiple of 4, fp32
  * pointers 16-byte aligned.

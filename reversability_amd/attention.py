@@ -16,10 +16,18 @@ kernels do not cover (no fp16 ``qkv`` -- i.e. not under fp16 autocast --, head
 sizes other than 32/64/128, dropout in training mode, CPU tensors) keep the
 reference computation, recorded in ``paths.report()`` (or raising under
 ``paths.strict()``).
+
+Beside it, without a counterpart in the reference: ``window_attention``, causal
+attention with a sliding window and first tokens that stay visible (sinks), fp16 or
+bf16, with query heads that may share key and value heads; and ``rotate_qkv``, the
+rotation of queries and keys by position, from a ``Rotary`` table.
+``enable_attention(model, window=, sinks=, rotary=)`` trains a model with them, and
+``cache.decode`` answers with the same settings.
 """
 from __future__ import annotations
 
 import types
+from typing import Optional
 
 import torch
 import torch.nn.functional as F
@@ -27,7 +35,7 @@ from torch.autograd.function import once_differentiable
 
 from . import linear as _linear
 from . import paths
-from ._hip import RV_F16, RV_F32, _check, _stream, library
+from ._hip import RV_BF16, RV_F16, RV_F32, _check, _DeviceGuard, _stream, library
 from .mlp import cast_operands, splitk_workspace
 
 HEAD_DIMS = (32, 64, 128)
@@ -190,10 +198,255 @@ def reference_attention(qkv: torch.Tensor, heads: int, dropout: float = 0.0) -> 
     return mixed.transpose(1, 2).reshape(batch, length, d)
 
 
-def enable_attention(model: torch.nn.Module) -> None:
-    """Route every block's attention through the fused kernels where they apply."""
+# ---------------------------------------------------------------------------
+# windows, sinks and rotation
+# ---------------------------------------------------------------------------
+_CODES = {torch.float16: RV_F16, torch.bfloat16: RV_BF16}
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned, as the kernels read it."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def packed_heads(qkv: torch.Tensor, heads: int, kv_heads: Optional[int], what: str) -> tuple:
+    """(kv_heads, head size) of packed rows [..., (heads + 2 kv_heads) head size]; raises
+    on what the kernels do not cover."""
+    kv = heads if kv_heads is None else kv_heads
+    if heads < 1 or kv < 1 or heads % kv:
+        raise ValueError(f"{what} needs heads that are a multiple of kv_heads")
+    width = qkv.shape[-1] if qkv.ndim else 0
+    hd = width // (heads + 2 * kv)
+    if (not qkv.is_cuda or qkv.dtype not in _CODES or hd not in HEAD_DIMS
+            or hd * (heads + 2 * kv) != width):
+        raise ValueError(f"{what} needs CUDA (ROCm device) fp16 or bf16 rows of (heads + 2 "
+                         f"kv_heads) heads of size in {HEAD_DIMS}; no silent fallback")
+    return kv, hd
+
+
+class WindowAttention(torch.autograd.Function):
+    """See ``window_attention``."""
+
+    @staticmethod
+    def forward(ctx, qkv, heads, kv, window, sinks):
+        batch, seq, width = qkv.shape
+        hd = width // (heads + 2 * kv)
+        x = _dense(qkv)
+        out = torch.empty(batch, seq, heads * hd, device=x.device, dtype=x.dtype)
+        lse = torch.empty(batch * heads, seq, device=x.device, dtype=torch.float32)
+        if out.numel():
+            with _DeviceGuard(x):
+                _check(library().rv_window_attn_fwd(
+                    x.data_ptr(), batch, seq, heads, kv, hd, _CODES[x.dtype], window, sinks,
+                    out.data_ptr(), lse.data_ptr(), _stream(x)), "rv_window_attn_fwd")
+        ctx.save_for_backward(x, out, lse)
+        ctx.sizes = (batch, seq, heads, kv, hd)
+        ctx.span = (window, sinks)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, out, lse = ctx.saved_tensors
+        dqkv = torch.empty_like(x)
+        if out.numel():
+            lib, dout = library(), _dense(dout)
+            nbytes = lib.rv_window_attn_bwd_workspace_bytes(*ctx.sizes, *ctx.span)
+            if nbytes < 0:
+                _check(-nbytes, "rv_window_attn_bwd_workspace_bytes")
+            with _DeviceGuard(x):
+                ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+                _check(lib.rv_window_attn_bwd(
+                    x.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), *ctx.sizes,
+                    _CODES[x.dtype], *ctx.span, dqkv.data_ptr(), ws.data_ptr(), nbytes,
+                    _stream(x)), "rv_window_attn_bwd")
+        return dqkv, None, None, None, None
+
+
+def check_window(window: Optional[int], sinks: int, what: str) -> None:
+    if window is not None and window < 1:
+        raise ValueError(f"{what} needs a window of at least one token")
+    if sinks < 0:
+        raise ValueError(f"{what} needs sinks >= 0")
+
+
+def window_attention(qkv: torch.Tensor, heads: int, window: int, sinks: int = 0, *,
+                     kv_heads: Optional[int] = None) -> torch.Tensor:
+    """Causal attention with a sliding window and sinks, differentiable in ``qkv``.
+
+    ``qkv`` fp16 or bf16 [B, T, (heads + 2 kv_heads) hd], hd 32, 64 or 128: the query
+    heads, then the key heads, then the value heads (``kv_heads`` None: as many as
+    query heads); query head h reads key and value head h // (heads // kv_heads).  Query
+    i sees key j <= i where i - j < ``window`` or j < ``sinks``.  Returns [B, T, heads hd] in
+    qkv's type.  Scores, softmax statistics and sums are held in fp32; the weights are
+    rounded to qkv's type for the product with the values, as are the scores'
+    gradients.  Deterministic.  As in any product, a NaN or an infinity in a key or value
+    may reach queries that do not see it (and so may one in a query or gradient reach the
+    gradients of keys it does not see)."""
+    if qkv.ndim != 3:
+        raise ValueError("window_attention needs qkv [B, T, (heads + 2 kv_heads) hd]")
+    kv, _ = packed_heads(qkv, heads, kv_heads, "window_attention")
+    check_window(window, sinks, "window_attention")
+    return WindowAttention.apply(qkv, heads, kv, window, sinks)
+
+
+class Rotary:
+    """Cosines and sines by position for heads of size ``head_dim``: pair i of a head turns by
+    position * base^(-2 i / head_dim).  Pairs are the columns (i, i + head_dim / 2), or (2 i,
+    2 i + 1) if ``interleaved``.  ``table`` fp32 [positions, head_dim / 2, 2], made in 64
+    bits."""
+
+    def __init__(self, head_dim: int, positions: int, base: float = 10000.0,
+                 interleaved: bool = False, device="cuda"):
+        if head_dim not in HEAD_DIMS or positions < 1 or not base > 0.0:
+            raise ValueError(f"Rotary needs a head size in {HEAD_DIMS}, positions >= 1 and "
+                             "base > 0")
+        self.head_dim, self.positions = head_dim, positions
+        self.base, self.interleaved = float(base), bool(interleaved)
+        rate = self.base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
+        angle = torch.arange(positions, dtype=torch.float64).unsqueeze(1) * rate
+        self.table = torch.stack([angle.cos(), angle.sin()], -1).float().to(device)
+
+    def to(self, device) -> "Rotary":
+        """A copy with its table on ``device``."""
+        other = object.__new__(Rotary)
+        other.__dict__.update(self.__dict__, table=self.table.to(device))
+        return other
+
+    def check(self, like: torch.Tensor, head_dim: int, what: str) -> None:
+        if self.head_dim != head_dim or self.table.device != like.device:
+            raise ValueError(f"{what} needs a Rotary of its head size on its device")
+
+
+class RotateQKV(torch.autograd.Function):
+    """See ``rotate_qkv``."""
+
+    @staticmethod
+    def _turn(x, ctx, back):
+        y = torch.empty_like(x)
+        if y.numel():
+            rotary, (heads, kv, hd) = ctx.rotary, ctx.heads
+            with _DeviceGuard(x):
+                _check(library().rv_rotate_qkv(
+                    x.data_ptr(), y.data_ptr(), x.shape[0] * x.shape[1], x.shape[1], heads, kv, hd,
+                    _CODES[x.dtype], rotary.table.data_ptr(), rotary.positions,
+                    None if ctx.positions is None else ctx.positions.data_ptr(),
+                    rotary.interleaved, back, _stream(x)), "rv_rotate_qkv")
+        return y
+
+    @staticmethod
+    def forward(ctx, qkv, heads, kv, hd, rotary, positions):
+        ctx.rotary, ctx.heads = rotary, (heads, kv, hd)
+        ctx.save_for_backward(positions)
+        ctx.positions = positions
+        out = RotateQKV._turn(_dense(qkv), ctx, False)
+        del ctx.positions
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gradient):
+        ctx.positions, = ctx.saved_tensors
+        out = RotateQKV._turn(_dense(gradient), ctx, True)
+        del ctx.positions
+        return out, None, None, None, None, None
+
+
+def rotate_qkv(qkv: torch.Tensor, heads: int, rotary: Rotary,
+               positions: Optional[torch.Tensor] = None, *,
+               kv_heads: Optional[int] = None) -> torch.Tensor:
+    """``qkv`` [B, T, (heads + 2 kv_heads) hd], fp16 or bf16, with its queries and keys rotated
+    by their positions (int32 [B, T]; None: 0 .. T - 1), values as they are; differentiable in
+    ``qkv``.  Products in fp32, rounded once.  A position outside the table gives NaN
+    queries and keys."""
+    if qkv.ndim != 3:
+        raise ValueError("rotate_qkv needs qkv [B, T, (heads + 2 kv_heads) hd]")
+    kv, hd = packed_heads(qkv, heads, kv_heads, "rotate_qkv")
+    rotary.check(qkv, hd, "rotate_qkv")
+    if positions is None:
+        if qkv.shape[1] > rotary.positions:
+            raise ValueError("sequence exceeds the positions of the Rotary table")
+    elif (positions.dtype != torch.int32 or positions.shape != qkv.shape[:2]
+          or positions.device != qkv.device):
+        raise ValueError("positions must be int32 [B, T] on qkv's device")
+    else:
+        positions = positions.contiguous()
+    return RotateQKV.apply(qkv, heads, kv, hd, rotary, positions)
+
+
+def reference_rotation(qkv: torch.Tensor, heads: int, rotary: Rotary) -> torch.Tensor:
+    """``rotate_qkv`` of as many key heads as query heads in torch operations, for calls the
+    kernels do not cover."""
+    batch, length, width = qkv.shape
+    x = qkv.view(batch, length, 3, heads, -1)
+    turn = rotary.table[:length].to(qkv.device).unsqueeze(1).unsqueeze(1)  # [T, 1, 1, hd/2, 2]
+    cos, sin = turn.unbind(-1)
+    y, half = x[:, :, :2], rotary.head_dim // 2
+    a, b = (y[..., 0::2], y[..., 1::2]) if rotary.interleaved else (y[..., :half], y[..., half:])
+    pair = (a * cos - b * sin, a * sin + b * cos)
+    y = torch.stack(pair, -1).flatten(-2) if rotary.interleaved else torch.cat(pair, -1)
+    return torch.cat([y.to(qkv.dtype), x[:, :, 2:]], 2).reshape(batch, length, width)
+
+
+def reference_window_attention(qkv: torch.Tensor, heads: int, window: Optional[int], sinks: int,
+                               dropout: float = 0.0) -> torch.Tensor:
+    """``window_attention`` of as many key heads as query heads by torch's attention with a
+    mask, for calls the kernels do not cover."""
+    if window is None:
+        return reference_attention(qkv, heads, dropout)
+    batch, length, width = qkv.shape
+    d = width // 3
+    q, k, v = qkv.view(batch, length, 3, heads, d // heads).permute(2, 0, 3, 1, 4).unbind(0)
+    at = torch.arange(length, device=qkv.device)
+    gap = at.unsqueeze(1) - at
+    mask = (gap >= 0) & ((gap < window) | (at < sinks))
+    mixed = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, dropout_p=dropout)
+    return mixed.transpose(1, 2).reshape(batch, length, d)
+
+
+def _local_forward(attn, x, dropout):
+    """The attention of a layer with a window, a rotation, or both."""
+    qkv, heads, rotary = attn.qkv(x), attn.n_heads, attn._rv_rotary
+    window, sinks = attn._rv_window, attn._rv_sinks
+    hd = qkv.shape[-1] // (3 * heads)
+    if qkv.ndim == 3 and rotary is not None and qkv.shape[1] > rotary.positions:
+        raise ValueError("sequence exceeds the positions of the Rotary table")
+    if (qkv.is_cuda and qkv.dtype in _CODES and qkv.ndim == 3 and dropout == 0.0
+            and hd in HEAD_DIMS):
+        paths.took("attention", "hip")
+        if rotary is not None:
+            qkv = rotate_qkv(qkv, heads, rotary)
+        # (no window: one of the whole sequence)
+        mixed = window_attention(qkv, heads, window or max(1, qkv.shape[1]), sinks)
+    else:
+        paths.took("attention", "sdpa",
+                   f"windowed attention needs a CUDA fp16 or bf16 qkv, head size in {HEAD_DIMS} "
+                   f"and no dropout (got {qkv.dtype} on {qkv.device.type}, head size {hd}, "
+                   f"dropout {dropout})")
+        if rotary is not None:
+            qkv = reference_rotation(qkv, heads, rotary)
+        mixed = reference_window_attention(qkv, heads, window, sinks, dropout)
+    return attn.proj(mixed)
+
+
+def enable_attention(model: torch.nn.Module, window: Optional[int] = None, sinks: int = 0,
+                     rotary: Optional[Rotary] = None) -> None:
+    """Route every block's attention through the fused kernels where they apply.
+
+    ``window`` (None: all earlier tokens) and ``sinks`` limit what a token sees, as in
+    ``window_attention``; ``rotary`` rotates queries and keys by position
+    (``rotate_qkv``).  Calls that the kernels do not cover compute the same in torch."""
+    check_window(window, sinks, "enable_attention")
+    if rotary is not None:
+        sizes = {block.attn.head_dim for block in model.blocks}
+        if sizes - {rotary.head_dim}:
+            raise ValueError("enable_attention needs a Rotary of the model's head size")
+
     def forward(attn, x):
         dropout = attn.dropout if attn.training else 0.0
+        if attn._rv_window is not None or attn._rv_rotary is not None:
+            return _local_forward(attn, x, dropout)
         if _layer_supported(attn, x, dropout):
             paths.took("linear", "mfma")
             paths.took("attention", "hip")
@@ -211,4 +464,6 @@ def enable_attention(model: torch.nn.Module) -> None:
             mixed = reference_attention(qkv, attn.n_heads, dropout)
         return attn.proj(mixed)
     for block in model.blocks:
+        block.attn._rv_window, block.attn._rv_sinks = window, sinks
+        block.attn._rv_rotary = rotary
         block.attn.forward = types.MethodType(forward, block.attn)

@@ -1,0 +1,567 @@
+// Attention of new tokens over a paged cache of keys and values, for gfx950 on MFMA: one
+// token a sequence, a chunk of a prompt, or a tree of drafted tokens.
+//
+//   s_ij = q_i . k_j / sqrt(hd) where i sees j, p = softmax_j s, o = p v (0 where i sees nothing)
+//
+// A sequence holds lengths[b] tokens, the last n = starts[b + 1] - starts[b] of them new: token i
+// of the new ones is at slot context + i, context = lengths[b] - n.  It sees the slots up to its
+// own or, with a tree, all of the context and the new tokens whose bits its mask has; its position
+// is then context + (bits of its mask) - 1.  With a window it sees of these the tokens less
+// than `window` positions before it and the first `sinks` positions.
+//
+// Layouts: keys and values 16-bit [pages][KV][page][HD]; q [tokens][H][HD] with a row stride;
+// out [tokens][H][HD].  The rows that share a key head are the MFMA's columns: row r of a
+// sequence and key head is token r / G, head kvh G + r % G, G = H / KV.
+//
+// One workgroup takes 16 NR rows and a stretch of keys; its four waves take the tiles of
+// 32 keys in turn, each with a softmax of its own (no barrier in the loop), and are joined at
+// the end.  Long sequences are cut into stretches joined by cached_join_k.  Per tile a wave
+// loads K straight into MFMA operands (16 keys x 32 columns, 64-byte pieces; a page holds 16 keys
+// at least, so 16 keys share one table entry) and V through its own LDS tile, from which
+// ds_read_b64_tr_b16 gives the transposed operand; both are loaded a tile ahead.
+//
+//   S^T [32 keys][16 rows] = K Q^T (v_mfma 16x16x32: lane l has row l % 16 and keys (l/16)*4 + 0..3 of
+//   each 16), O^T [HD][16 rows] += V^T P^T, k index (l/16)*8 + i standing for key
+//   (i/4)*16 + (l/16)*4 + i%4, so that a lane's own P are its operand.
+//
+// Rows of V that no row of the workgroup sees (behind the last token, before the window, of a
+// page that does not exist) are taken as zeros and their scores as -inf, whatever the cache holds.
+
+#include <algorithm>
+#include <cmath>
+
+#include "attn_tile.h"
+
+namespace {
+
+using namespace rv_attn;
+
+constexpr int kKeys = 32;  // keys per tile of a wave
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 x, f16x8 y, f32x4 acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(b16x8 x, b16x8 y, f32x4 acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
+}
+
+struct Cached {
+  const void* q;
+  const void* keys;
+  const void* values;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const int64_t* tree;  // null: a chunk
+  void* out;
+  float* part;  // [tokens][H][splits][HD] sums, then [tokens][H][splits][2] their m and l
+  int64_t q_ld, table_ld, table_pages;
+  int tokens, seqs, H, KV, pages, page_shift, max_query;
+  int window, sinks;  // window 0: none
+  int row_blocks, splits, split_tiles;
+  float c;
+};
+
+// What a block of rows of a sequence sees: slots [lo, hi) and those below `sinks`, as tiles
+// [0, sink_tiles) and [first, first + count - sink_tiles).
+struct View {
+  int start, n, context;
+  int i0, i1;  // its tokens, both included
+  int lo, hi;
+  int sink_tiles, first, count;
+
+  __device__ __forceinline__ View(const Cached& a, int b, int rb, int rows) {
+    const int group = a.H / a.KV;
+    start = min(max(a.starts[b], 0), a.tokens);
+    const int end = min(max(a.starts[b + 1], start), a.tokens);
+    const int64_t held = a.table_pages << a.page_shift;
+    const int len = (int)min((int64_t)max(a.lengths[b], 0), min(held, (int64_t)1 << 30));
+    context = len - (end - start);
+    n = min(end - start, a.max_query);
+    i0 = rb * rows / group;
+    i1 = min(n - 1, (rb * rows + rows - 1) / group);
+    hi = min(len, a.tree ? context + n : context + i1 + 1);
+    lo = 0;
+    if (a.window) lo = max(0, (a.tree ? context : context + i0 + 1) - a.window);
+    count = sink_tiles = first = 0;
+    if (i0 < n && hi > 0) {
+      const int all = (hi + kKeys - 1) / kKeys;
+      first = min(lo / kKeys, all);
+      sink_tiles = min((a.sinks + kKeys - 1) / kKeys, first);
+      count = sink_tiles + all - first;
+    }
+  }
+  __device__ __forceinline__ int tile(int v) const {
+    return v < sink_tiles ? v : first + v - sink_tiles;
+  }
+};
+
+// Value of the lane's row over the four lanes that hold it (l % 16).
+__device__ __forceinline__ float row_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Half index of element (r, col) of a V tile [32][HD]: pairs of 16-byte chunks XOR-swizzled so that
+// eight rows' 32 bytes of one column block lie on different banks.
+template <int HD>
+__device__ __forceinline__ int v_at(int r, int col) {
+  const int turn = (r / (128 / HD)) & (HD / 16 - 1);
+  return r * HD + ((((col >> 4) ^ turn) << 4) | (col & 15));
+}
+
+// K operands and V rows of one tile on their way through registers.
+template <typename E, int HD>
+struct Tile {
+  static constexpr int KK = HD / 32, VC = HD / 16;
+  x8<E> k[2][KK];
+  x8<E> v[VC];
+  bool whole;  // both groups' pages exist and all rows lie in [lo, hi)
+
+  __device__ __forceinline__ void load(const Cached& a, const View& w, int b, int kvh, int k0,
+                                       int lane) {
+    const E* keys = static_cast<const E*>(a.keys);
+    const E* values = static_cast<const E*>(a.values);
+    int64_t at[2];
+    bool ok[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = k0 + 16 * g;
+      int page = -1;
+      if (key < w.hi) page = a.table[b * a.table_ld + (key >> a.page_shift)];
+      page = __builtin_amdgcn_readfirstlane(page);
+      ok[g] = page >= 0 && page < a.pages;
+      at[g] = ((((int64_t)(ok[g] ? page : 0) * a.KV + kvh) << a.page_shift) +
+               (key & ((1 << a.page_shift) - 1))) * HD;
+    }
+    whole = ok[0] && ok[1] && k0 + kKeys <= w.hi && (k0 >= w.lo || k0 + kKeys <= a.sinks);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const E* row = keys + at[g] + (lane & 15) * HD + (lane >> 4) * 8;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) k[g][kk] = *reinterpret_cast<const x8<E>*>(row + kk * 32);
+    }
+#pragma unroll
+    for (int it = 0; it < VC; ++it) {
+      const int ch = it * 64 + lane, r = ch / (HD / 8), col = (ch % (HD / 8)) * 8;
+      const int g = it / (VC / 2);  // the rows of one load lie in one group
+      v[it] = *reinterpret_cast<const x8<E>*>(values + at[g] + (r & 15) * HD + col);
+    }
+    if (!whole) {
+      seen[0] = ok[0], seen[1] = ok[1];
+#pragma unroll
+      for (int it = 0; it < VC; ++it) {
+        const int r = (it * 64 + lane) / (HD / 8), key = k0 + r;
+        if (!ok[it / (VC / 2)] || key >= w.hi || (key < w.lo && key >= a.sinks)) v[it] = x8<E>{};
+      }
+    }
+  }
+  bool seen[2];
+  __device__ __forceinline__ void store_v(E* t, int lane) const {
+#pragma unroll
+    for (int it = 0; it < VC; ++it) {
+      const int ch = it * 64 + lane, r = ch / (HD / 8), col = (ch % (HD / 8)) * 8;
+      *reinterpret_cast<x8<E>*>(t + v_at<HD>(r, col)) = v[it];
+    }
+  }
+};
+
+template <typename E, int HD, int NR>
+constexpr int kBlocks = HD * NR <= 128 ? 2 : 1;
+
+template <typename E, int HD, int NR>
+__global__ __launch_bounds__(kThreads, (kBlocks<E, HD, NR>))
+void cached_attn_k(Cached a) {
+  constexpr int KK = HD / 32, DT = HD / 16, R = 16 * NR;
+  constexpr int kVBytes = kWaves * kKeys * HD * 2, kOBytes = 2 * R * HD * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kVBytes > kOBytes ? kVBytes : kOBytes];
+  __shared__ float ml[2][kWaves][R];
+  int at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int rb = at % a.row_blocks;
+  at /= a.row_blocks;
+  const int kvh = at % a.KV, b = at / a.KV;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 4;
+  const View w(a, b, rb, R);
+  if (w.i0 >= w.n) return;  // no such rows
+  // (the last stretch takes what is left of a sequence that is longer than was said)
+  const int v_end = split + 1 == a.splits ? w.count : min(w.count, (split + 1) * a.split_tiles);
+  if (split && split * a.split_tiles >= w.count) return;  // (the first writes zeros if need be)
+  const int group = a.H / a.KV;
+
+  // the lane's rows: token and head, last slot seen (chunk) or mask (tree), position
+  x8<E> qf[NR][KK];
+  int token[NR], limit[NR], place[NR];
+  uint64_t mask[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int row = rb * R + r * 16 + (lane & 15);
+    token[r] = row / group;
+    const bool ok = token[r] < w.n;
+    const int head = kvh * group + row % group;
+    limit[r] = ok ? w.context + token[r] : -1;
+    place[r] = limit[r];
+    mask[r] = 0;
+    if (a.tree && ok) {
+      const uint64_t bits = w.n < 64 ? (uint64_t(1) << w.n) - 1 : ~uint64_t(0);
+      mask[r] = (uint64_t)a.tree[w.start + token[r]] & bits;
+      place[r] = w.context + __popcll(mask[r]) - 1;
+    }
+    const E* src = static_cast<const E*>(a.q) + (int64_t)(w.start + token[r]) * a.q_ld +
+                   (int64_t)head * HD + hl * 8;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[r][kk] = ok ? *reinterpret_cast<const x8<E>*>(src + kk * 32) : x8<E>{};
+  }
+  f32x4 o[DT][NR];
+  float m[NR], l[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // slots below `below` are seen by every row as far as order goes, from `from` on as far as the
+  // window goes
+  const int below = a.tree ? w.context : w.context + w.i0 + 1;
+  const int last = a.tree ? w.context + w.n - 1 : w.context + w.i1;
+  const int from = a.window ? last - a.window + 1 : 0;
+
+  E* vt = reinterpret_cast<E*>(lds) + wave * kKeys * HD;
+  const int i = lane & 15;
+  Tile<E, HD> next;
+  int v = split * a.split_tiles + wave;
+  if (v < v_end) next.load(a, w, b, kvh, w.tile(v) * kKeys, lane);
+  for (; v < v_end; v += kWaves) {
+    const int k0 = w.tile(v) * kKeys;
+    const Tile<E, HD> now = next;
+    // the wave's last reads of the tile come before these writes, the reads below behind
+    // them: one wave's LDS accesses keep their order, the fences keep the compiler's
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    now.store_v(vt, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (v + kWaves < v_end) next.load(a, w, b, kvh, w.tile(v + kWaves) * kKeys, lane);
+
+    f32x4 s[2][NR];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        s[g][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) s[g][r] = mfma16(now.k[g][kk], qf[r][kk], s[g][r]);
+      }
+    const bool plain = now.whole && k0 + kKeys <= below && (k0 >= from || k0 + kKeys <= a.sinks);
+    if (!plain) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = k0 + g * 16 + hl * 4 + j;
+          const bool there = now.whole || (now.seen[g] && key < w.hi);
+          int kp = key;  // the key's position
+          if (a.tree && a.window && key >= w.context && key - w.context < w.n) {
+            const uint64_t bits = w.n < 64 ? (uint64_t(1) << w.n) - 1 : ~uint64_t(0);
+            kp = w.context + __popcll((uint64_t)a.tree[w.start + key - w.context] & bits) - 1;
+          }
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            bool sees = there;
+            if (a.tree) {
+              if (key >= w.context) sees = sees && (mask[r] >> ((key - w.context) & 63) & 1);
+            } else {
+              sees = sees && key <= limit[r];
+            }
+            if (a.window) sees = sees && (place[r] - kp < a.window || kp < a.sinks);
+            if (!sees) s[g][r][j] = -INFINITY;
+          }
+        }
+    }
+    bool up = false;
+    float mx[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const f32x4 x = s[0][r], y = s[1][r];
+      mx[r] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                    fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * a.c;
+      up = up || mx[r] > m[r] + kLazy;
+    }
+    if (__any(up)) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float m_new = fmaxf(m[r], row_max(mx[r]));
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - m_new);
+        m[r] = m_new;
+        l[r] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt][r] *= alpha;
+      }
+    }
+    x8<E> pf[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float neg_m = m[r] == -INFINITY ? 0.f : -m[r];
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][r][e & 3], a.c, neg_m));
+        sum += p;
+        pf[r][e] = (E)p;
+      }
+      l[r] += sum;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (RV_LDS i16x4*)(vt + v_at<HD>(hl * 4 + (i >> 2), dt * 16 + 4 * (i & 3))));
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (RV_LDS i16x4*)(vt + v_at<HD>(16 + hl * 4 + (i >> 2), dt * 16 + 4 * (i & 3))));
+      const x4<E> p = __builtin_bit_cast(x4<E>, x), q = __builtin_bit_cast(x4<E>, y);
+      const x8<E> vf = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+#pragma unroll
+      for (int r = 0; r < NR; ++r) o[dt][r] = mfma16(vf, pf[r], o[dt][r]);
+    }
+  }
+
+  // the four waves' sums in one: scaled to the common maximum, then added in pairs
+  float all_m[NR], all_l[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    l[r] = row_sum(l[r]);
+    if (hl == 0) {
+      ml[0][wave][r * 16 + i] = m[r];
+      ml[1][wave][r * 16 + i] = l[r];
+    }
+  }
+  __syncthreads();  // (also: every wave is done with its V tile)
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    all_m[r] = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) all_m[r] = fmaxf(all_m[r], ml[0][x][r * 16 + i]);
+    const float top = all_m[r] == -INFINITY ? 0.f : all_m[r];
+    all_l[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x)
+      all_l[r] += ml[1][x][r * 16 + i] * __builtin_amdgcn_exp2f(ml[0][x][r * 16 + i] - top);
+    const float factor = __builtin_amdgcn_exp2f(m[r] - top);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][r] *= factor;
+  }
+  f32x4* swap = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+  for (int step = 2; step; step >>= 1) {
+    if (wave >= step && wave < 2 * step) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          swap[(((wave - step) * DT + dt) * NR + r) * 64 + lane] = o[dt][r];
+    }
+    __syncthreads();
+    if (wave < step) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) o[dt][r] += swap[((wave * DT + dt) * NR + r) * 64 + lane];
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+  const bool alone = a.splits == 1 || w.count <= a.split_tiles;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (token[r] >= w.n) continue;
+    const int row = rb * R + r * 16 + i;
+    const int64_t at = (int64_t)(w.start + token[r]) * a.H + kvh * group + row % group;
+    if (alone) {
+      const float inv = all_l[r] == 0.f ? 0.f : 1.f / all_l[r];
+      E* dst = static_cast<E*>(a.out) + at * HD + hl * 4;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        store4<E>(dst + dt * 16, o[dt][r][0] * inv, o[dt][r][1] * inv, o[dt][r][2] * inv,
+                  o[dt][r][3] * inv);
+    } else {
+      float* dst = a.part + (at * a.splits + split) * HD + hl * 4;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(dst + dt * 16) = o[dt][r];
+      if (hl == 0) {
+        float* stat = a.part + (int64_t)a.tokens * a.H * a.splits * HD + (at * a.splits + split) * 2;
+        stat[0] = all_m[r];
+        stat[1] = all_l[r];
+      }
+    }
+  }
+}
+
+// Joins the stretches of the rows that were cut: HD / 4 threads a row, rows of one sequence
+// numbered token by token.
+template <typename E, int HD>
+__global__ __launch_bounds__(kThreads)
+void cached_join_k(Cached a, int rows_per_block) {
+  constexpr int kPer = kThreads / (HD / 4);
+  const int blocks = (int)(((int64_t)a.max_query * a.H + kPer - 1) / kPer);
+  const int b = blockIdx.x / blocks;
+  const int64_t row = (int64_t)(blockIdx.x % blocks) * kPer + threadIdx.x / (HD / 4);
+  const int col = (threadIdx.x % (HD / 4)) * 4;
+  const int token = (int)(row / a.H), head = (int)(row % a.H), group = a.H / a.KV;
+  const View w(a, b, (token * group + head % group) / rows_per_block, rows_per_block);
+  if (token >= w.n || w.count <= a.split_tiles) return;
+  const int used = min((w.count + a.split_tiles - 1) / a.split_tiles, a.splits);
+  const int64_t at = ((int64_t)(w.start + token) * a.H + head) * a.splits;
+  const float* stat = a.part + (int64_t)a.tokens * a.H * a.splits * HD + at * 2;
+  float top = -INFINITY;
+  for (int s = 0; s < used; ++s) top = fmaxf(top, stat[2 * s]);
+  if (top == -INFINITY) top = 0.f;
+  float l = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < used; ++s) {
+    const float factor = __builtin_amdgcn_exp2f(stat[2 * s] - top);
+    l += stat[2 * s + 1] * factor;
+    sum += *reinterpret_cast<const f32x4*>(a.part + (at + s) * HD + col) * factor;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store4<E>(static_cast<E*>(a.out) + ((int64_t)(w.start + token) * a.H + head) * HD + col,
+            sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+}
+
+// Rows a workgroup takes (in sixteens), blocks of rows, stretches of keys.
+struct Plan {
+  int nr, row_blocks, splits, split_tiles;
+};
+
+constexpr int64_t kWanted = 1024;    // workgroups for the chip's 256 CUs
+constexpr int kLeastTiles = 8;       // tiles of a stretch: two for each wave
+constexpr int kMostTiles = 128;      // a longer one would keep a few workgroups busy alone
+constexpr int kMostSplits = 256;
+
+Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t max_length,
+             int64_t window, int64_t sinks) {
+  Plan p;
+  const int64_t rows = max_query * (heads / kv);
+  p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.row_blocks = (int)((rows + 16 * p.nr - 1) / (16 * p.nr));
+  int64_t seen = max_length;  // of one block of rows, at most (and the tiles' edges)
+  if (window) seen = std::min(seen, window + sinks + std::min<int64_t>(max_query, 64) + 3 * kKeys);
+  const int64_t tiles = std::max<int64_t>(1, (seen + kKeys - 1) / kKeys);
+  const int64_t blocks = seqs * kv * p.row_blocks;
+  int64_t splits = std::max((kWanted + blocks - 1) / blocks, (tiles + kMostTiles - 1) / kMostTiles);
+  splits = std::min<int64_t>(splits, (tiles + kLeastTiles - 1) / kLeastTiles);
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
+  p.split_tiles = (int)((tiles + splits - 1) / splits);
+  p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
+  return p;
+}
+
+int page_shift_of(int64_t page) {
+  if (page < 16 || page > 256 || (page & (page - 1))) return -1;
+  return __builtin_ctzll((unsigned long long)page);
+}
+
+bool args_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv, int64_t hd,
+             int64_t max_query, int64_t max_length, int64_t window, int64_t sinks) {
+  return tokens >= 0 && seqs > 0 && heads > 0 && kv > 0 && heads % kv == 0 && hd > 0 &&
+         max_query > 0 && max_length > 0 && window >= 0 && sinks >= 0;
+}
+
+bool sizes_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv, int64_t hd,
+              int64_t max_query, int64_t max_length, const Plan& p) {
+  return (hd == 32 || hd == 64 || hd == 128) && heads < (1 << 16) && tokens < (1 << 26) &&
+         max_query < (1 << 26) && max_length <= (1 << 30) && max_query * heads < (1 << 30) &&
+         seqs * kv * p.row_blocks * p.splits < (1 << 24) &&
+         seqs * ((max_query * heads * (hd / 4) + kThreads - 1) / kThreads) < (1 << 24);
+}
+
+int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t hd, const Plan& p) {
+  return p.splits == 1 ? 0 : tokens * heads * p.splits * (hd + 2) * 4;
+}
+
+template <typename E, int HD>
+int launch(const Cached& a, const Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.seqs * a.KV * p.row_blocks * p.splits)), block(kThreads);
+  if (p.nr == 1)
+    hipLaunchKernelGGL((cached_attn_k<E, HD, 1>), grid, block, 0, s, a);
+  else if (p.nr == 2)
+    hipLaunchKernelGGL((cached_attn_k<E, HD, 2>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((cached_attn_k<E, HD, 4>), grid, block, 0, s, a);
+  int rc = rv_host::check_launch();
+  if (rc != RV_OK || p.splits == 1) return rc;
+  constexpr int kPer = kThreads / (HD / 4);
+  const int64_t blocks = ((int64_t)a.max_query * a.H + kPer - 1) / kPer;
+  hipLaunchKernelGGL((cached_join_k<E, HD>), dim3((unsigned)(blocks * a.seqs)), block, 0, s, a,
+                     16 * p.nr);
+  return rv_host::check_launch();
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t rv_cached_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads,
+                                       int64_t kv_heads, int64_t head_dim, int64_t max_query,
+                                       int64_t max_length, int64_t window, int64_t sinks) {
+  if (!args_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, window, sinks))
+    return -RV_ERR_BAD_SIZE;
+  const Plan p = plan_of(seqs, heads, kv_heads, max_query, max_length, window, sinks);
+  if (!sizes_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, p))
+    return -RV_ERR_UNSUPPORTED;
+  return workspace_bytes(tokens, heads, head_dim, p);
+}
+
+int rv_cached_attn(const void* q, int64_t q_ld, const void* keys, const void* values,
+                   const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                   const int32_t* lengths, const int32_t* starts, const int64_t* tree,
+                   int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                   int64_t head_dim, int dtype, int64_t pages, int64_t page_size,
+                   int64_t max_query, int64_t max_length, int64_t window, int64_t sinks,
+                   void* out, void* workspace, int64_t workspace_bytes_given, void* stream) {
+  if (!q || !keys || !values || !page_table || !lengths || !starts || !out)
+    return RV_ERR_NULL_POINTER;
+  if (!args_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, window, sinks) ||
+      pages <= 0 || table_pages <= 0 || ld_table < table_pages || q_ld < heads * head_dim)
+    return RV_ERR_BAD_SIZE;
+  const Plan p = plan_of(seqs, heads, kv_heads, max_query, max_length, window, sinks);
+  const int shift = page_shift_of(page_size);
+  if (!sizes_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, p) ||
+      (dtype != RV_F16 && dtype != RV_BF16) || shift < 0 || (tree && max_query > 64) ||
+      pages >= (int64_t(1) << 31) || table_pages >= (int64_t(1) << 31) || q_ld % 8 ||
+      !rv_host::aligned16(q) || !rv_host::aligned16(keys) || !rv_host::aligned16(values) ||
+      !rv_host::aligned16(out) || !rv_host::aligned16(workspace))
+    return RV_ERR_UNSUPPORTED;
+  const int64_t need = workspace_bytes(tokens, heads, head_dim, p);
+  if (need && (!workspace || workspace_bytes_given < need)) return RV_ERR_WORKSPACE;
+  if (!tokens) return RV_OK;
+  Cached a{};
+  a.q = q, a.keys = keys, a.values = values, a.out = out;
+  a.table = page_table, a.lengths = lengths, a.starts = starts, a.tree = tree;
+  a.part = static_cast<float*>(workspace);
+  a.q_ld = q_ld, a.table_ld = ld_table, a.table_pages = table_pages;
+  a.tokens = (int)tokens, a.seqs = (int)seqs, a.H = (int)heads, a.KV = (int)kv_heads;
+  a.pages = (int)pages, a.page_shift = shift, a.max_query = (int)max_query;
+  // windows and sinks beyond what a cache holds see all of it
+  a.window = (int)std::min<int64_t>(window, 1 << 30);
+  a.sinks = window ? (int)std::min<int64_t>(sinks, 1 << 30) : 0;
+  a.row_blocks = p.row_blocks, a.splits = p.splits, a.split_tiles = p.split_tiles;
+  a.c = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype == RV_F16) {
+    if (head_dim == 32) return launch<_Float16, 32>(a, p, s);
+    if (head_dim == 64) return launch<_Float16, 64>(a, p, s);
+    return launch<_Float16, 128>(a, p, s);
+  }
+  if (head_dim == 32) return launch<__bf16, 32>(a, p, s);
+  if (head_dim == 64) return launch<__bf16, 64>(a, p, s);
+  return launch<__bf16, 128>(a, p, s);
+}
+
+}  // extern "C"
