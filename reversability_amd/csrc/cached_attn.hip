@@ -13,12 +13,13 @@
 // out [tokens][H][HD].  The rows that share a key head are the MFMA's columns: row r of a
 // sequence and key head is token r / G, head kvh G + r % G, G = H / KV.
 //
-// One workgroup takes 16 NR rows and a stretch of keys; its four waves take the tiles of
-// 32 keys in turn, each with a softmax of its own (no barrier in the loop), and are joined at
-// the end.  Long sequences are cut into stretches joined by cached_join_k.  Per tile a wave
+// Few rows (at most 32 of a sequence and key head; cached_few_k): one workgroup takes 16 NR rows
+// and a stretch of keys; its four waves take the tiles of 32 keys in turn, each with a softmax of
+// its own (no barrier in the loop), and are joined at the end.  Per tile a wave
 // loads K straight into MFMA operands (16 keys x 32 columns, 64-byte pieces; a page holds 16 keys
 // at least, so 16 keys share one table entry) and V through its own LDS tile, from which
-// ds_read_b64_tr_b16 gives the transposed operand; both are loaded a tile ahead.
+// ds_read_b64_tr_b16 gives the transposed operand; both are loaded a tile ahead, the table
+// entries of 32 tiles at once and 32 tiles ahead.
 //
 //   S^T [32 keys][16 rows] = K Q^T (v_mfma 16x16x32: lane l has row l % 16 and keys (l/16)*4 + 0..3 of
 //   each 16), O^T [HD][16 rows] += V^T P^T, k index (l/16)*8 + i standing for key
@@ -36,7 +37,7 @@ namespace {
 
 using namespace rv_attn;
 
-constexpr int kKeys = 32;  // keys per tile of a wave
+constexpr int kKeys = 32;  // keys per tile of a wave (few rows)
 constexpr int kWaves = 4;
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 x, f16x8 y, f32x4 acc) {
@@ -71,7 +72,7 @@ struct View {
   int lo, hi;
   int sink_tiles, first, count;
 
-  __device__ __forceinline__ View(const Cached& a, int b, int rb, int rows) {
+  __device__ __forceinline__ View(const Cached& a, int b, int rb, int rows, int keys) {
     const int group = a.H / a.KV;
     start = min(max(a.starts[b], 0), a.tokens);
     const int end = min(max(a.starts[b + 1], start), a.tokens);
@@ -86,14 +87,29 @@ struct View {
     if (a.window) lo = max(0, (a.tree ? context : context + i0 + 1) - a.window);
     count = sink_tiles = first = 0;
     if (i0 < n && hi > 0) {
-      const int all = (hi + kKeys - 1) / kKeys;
-      first = min(lo / kKeys, all);
-      sink_tiles = min((a.sinks + kKeys - 1) / kKeys, first);
+      const int all = (hi + keys - 1) / keys;
+      first = min(lo / keys, all);
+      sink_tiles = min((a.sinks + keys - 1) / keys, first);
       count = sink_tiles + all - first;
     }
   }
   __device__ __forceinline__ int tile(int v) const {
     return v < sink_tiles ? v : first + v - sink_tiles;
+  }
+};
+
+// A workgroup's stretch, block of rows, key head and sequence.  The stretches are numbered slowest:
+// those behind the shorter sequences' ends come last, and leave at once.
+struct Place {
+  int split, rb, kvh, b;
+  __device__ __forceinline__ explicit Place(const Cached& a) {
+    const int per = a.seqs * a.KV * a.row_blocks;
+    split = (int)blockIdx.x / per;
+    int at = (int)blockIdx.x % per;
+    rb = at % a.row_blocks;
+    at /= a.row_blocks;
+    kvh = at % a.KV;
+    b = at / a.KV;
   }
 };
 
@@ -117,6 +133,13 @@ __device__ __forceinline__ int v_at(int r, int col) {
   return r * HD + ((((col >> 4) ^ turn) << 4) | (col & 15));
 }
 
+// The page of the 16 keys from `key` on, -1 where there is none or none of them is needed.
+__device__ __forceinline__ int page_of(const Cached& a, const View& w, int b, int key) {
+  if (key >= w.hi) return -1;
+  const int page = a.table[b * a.table_ld + (key >> a.page_shift)];
+  return page >= 0 && page < a.pages ? page : -1;
+}
+
 // K operands and V rows of one tile on their way through registers.
 template <typename E, int HD>
 struct Tile {
@@ -125,8 +148,9 @@ struct Tile {
   x8<E> v[VC];
   bool whole;  // both groups' pages exist and all rows lie in [lo, hi)
 
-  __device__ __forceinline__ void load(const Cached& a, const View& w, int b, int kvh, int k0,
-                                       int lane) {
+  // ids: entry_of's of the block of tiles, this tile the it-th of them.
+  __device__ __forceinline__ void load(const Cached& a, const View& w, int kvh, int ids, int it,
+                                       int k0, int lane) {
     const E* keys = static_cast<const E*>(a.keys);
     const E* values = static_cast<const E*>(a.values);
     int64_t at[2];
@@ -134,10 +158,8 @@ struct Tile {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int key = k0 + 16 * g;
-      int page = -1;
-      if (key < w.hi) page = a.table[b * a.table_ld + (key >> a.page_shift)];
-      page = __builtin_amdgcn_readfirstlane(page);
-      ok[g] = page >= 0 && page < a.pages;
+      const int page = __builtin_amdgcn_readlane(ids, 2 * it + g);
+      ok[g] = page >= 0;
       at[g] = ((((int64_t)(ok[g] ? page : 0) * a.KV + kvh) << a.page_shift) +
                (key & ((1 << a.page_shift) - 1))) * HD;
     }
@@ -174,23 +196,16 @@ struct Tile {
 };
 
 template <typename E, int HD, int NR>
-constexpr int kBlocks = HD * NR <= 128 ? 2 : 1;
-
-template <typename E, int HD, int NR>
-__global__ __launch_bounds__(kThreads, (kBlocks<E, HD, NR>))
-void cached_attn_k(Cached a) {
+__global__ __launch_bounds__(kThreads, 2)
+void cached_few_k(Cached a) {
   constexpr int KK = HD / 32, DT = HD / 16, R = 16 * NR;
   constexpr int kVBytes = kWaves * kKeys * HD * 2, kOBytes = 2 * R * HD * 4;
   __shared__ __attribute__((aligned(16))) char lds[kVBytes > kOBytes ? kVBytes : kOBytes];
   __shared__ float ml[2][kWaves][R];
-  int at = blockIdx.x;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int rb = at % a.row_blocks;
-  at /= a.row_blocks;
-  const int kvh = at % a.KV, b = at / a.KV;
+  const Place at(a);
+  const int split = at.split, rb = at.rb, kvh = at.kvh, b = at.b;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 4;
-  const View w(a, b, rb, R);
+  const View w(a, b, rb, R, kKeys);
   if (w.i0 >= w.n) return;  // no such rows
   // (the last stretch takes what is left of a sequence that is longer than was said)
   const int v_end = split + 1 == a.splits ? w.count : min(w.count, (split + 1) * a.split_tiles);
@@ -240,16 +255,27 @@ void cached_attn_k(Cached a) {
   const int i = lane & 15;
   Tile<E, HD> next;
   int v = split * a.split_tiles + wave;
-  if (v < v_end) next.load(a, w, b, kvh, w.tile(v) * kKeys, lane);
+  // table entries of the wave's next 32 tiles, two a tile, in the lanes
+  auto entries = [&](int from_tile) {
+    const int x = from_tile + (lane >> 1) * kWaves;
+    return x < v_end ? page_of(a, w, b, w.tile(x) * kKeys + 16 * (lane & 1)) : -1;
+  };
+  int ids = entries(v), ids_next = entries(v + 32 * kWaves), it = 0;
+  if (v < v_end) next.load(a, w, kvh, ids, 0, w.tile(v) * kKeys, lane);
   for (; v < v_end; v += kWaves) {
     const int k0 = w.tile(v) * kKeys;
     const Tile<E, HD> now = next;
+    if (++it == 32) {
+      it = 0;
+      ids = ids_next;
+      ids_next = entries(v + 33 * kWaves);
+    }
     // the wave's last reads of the tile come before these writes, the reads below behind
     // them: one wave's LDS accesses keep their order, the fences keep the compiler's
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     now.store_v(vt, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (v + kWaves < v_end) next.load(a, w, b, kvh, w.tile(v + kWaves) * kKeys, lane);
+    if (v + kWaves < v_end) next.load(a, w, kvh, ids, it, w.tile(v + kWaves) * kKeys, lane);
 
     f32x4 s[2][NR];
 #pragma unroll
@@ -403,59 +429,349 @@ void cached_attn_k(Cached a) {
   }
 }
 
-// Joins the stretches of the rows that were cut: HD / 4 threads a row, rows of one sequence
-// numbered token by token.
+// ---------------------------------------------------------------------------
+// Many rows.
+// ---------------------------------------------------------------------------
+// A tile of 64 keys of K or V on its way into LDS.
+template <typename E, int HD>
+struct PagedCopy {
+  static constexpr int kPer = kTile * HD / 8 / kThreads, kRows = kTile / kPer;  // rows of one load
+  u32x4 v[kPer];
+
+  // ids: the pages of the tile's four groups of 16 keys in lanes 4 * it .. 4 * it + 3.
+  __device__ __forceinline__ void load(const E* cache, const Cached& a, const View& w, int kvh,
+                                       int ids, int it, int k0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int ch = i * kThreads + threadIdx.x;
+      const int r = ch / (HD / 8), c = ch % (HD / 8);
+      const int g = __builtin_amdgcn_readfirstlane(r >> 4);  // one group a wave
+      const int page = __builtin_amdgcn_readlane(ids, 4 * it + g), key = k0 + r;
+      const E* src = cache + ((((int64_t)max(page, 0) * a.KV + kvh) << a.page_shift) +
+                              ((k0 + 16 * g) & ((1 << a.page_shift) - 1)) + (r & 15)) * HD + c * 8;
+      v[i] = *reinterpret_cast<const u32x4*>(src);
+      if (page < 0 || key >= w.hi || (key < w.lo && key >= a.sinks)) v[i] = u32x4{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void store(E* t) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int ch = i * kThreads + threadIdx.x;
+      const int r = ch / (HD / 8), c = ch % (HD / 8);
+      *reinterpret_cast<u32x4*>(t + r * HD + (swz<HD>(r, c) << 3)) = v[i];
+    }
+  }
+};
+
+template <int HD>
+struct State {
+  f32x16 o[HD / 32];
+  float m, l;
+};
+
+// Halves of V's operands that are read ahead of the exponentials: at HD = 128 both do not fit beside
+// two workgroups per CU.
+template <int HD>
+constexpr int kAhead = HD == 128 ? 1 : HD == 64 ? 2 : 0;
+
+// 32 keys of a staged tile for one wave's 32 rows (lanes); sees(key) where MASK.
+template <typename E, int HD, bool MASK, typename Sees>
+__device__ __forceinline__ void many_rows(State<HD>& st, const E* Ks, const E* Vs,
+                                          const FragOffsets<HD, E>& fo,
+                                          const x8<E> (&qf)[HD / 16], int sub, float c,
+                                          const Sees& sees) {
+  constexpr int KK = HD / 16, DT = HD / 32;
+  prio_mfma();
+  x8<E> kf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) kf[kk] = fo.rowf(Ks, sub, kk);
+  if constexpr (kReadAhead<HD>) __builtin_amdgcn_sched_barrier(0);
+  f32x16 s = mfma(kf[0], qf[0], zero16());
+#pragma unroll
+  for (int kk = 1; kk < KK; ++kk) s = mfma(kf[kk], qf[kk], s);
+  prio_valu();
+  float mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if constexpr (MASK) {
+      if (!sees(acc_row(j))) s[j] = -INFINITY;
+    }
+    mx = fmaxf(mx, s[j]);
+  }
+  const float mxc = pair_max(mx) * c;
+  if (__any(mxc > st.m + kLazy)) {
+    const float m_new = fmaxf(st.m, mxc);
+    const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - m_new);
+    st.m = m_new;
+    st.l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st.o[dt][e] *= alpha;
+  }
+  const float neg_m = st.m == -INFINITY ? 0.f : -st.m;
+  x8<E> vf[2][DT];
+  if constexpr (kReadAhead<HD>) {
+#pragma unroll
+    for (int cc = 0; cc < kAhead<HD>; ++cc)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[cc][dt] = fo.trf(Vs, sub, cc, dt);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  float rowsum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, neg_m));
+    rowsum += p;
+    s[j] = p;
+  }
+  st.l += rowsum;
+  prio_mfma_tail();
+#pragma unroll
+  for (int cc = 0; cc < 2; ++cc) {
+    const x8<E> pf = pack8<E>(s, cc);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      if (cc >= kAhead<HD>) vf[cc][dt] = fo.trf(Vs, sub, cc, dt);
+      st.o[dt] = mfma(vf[cc][dt], pf, st.o[dt]);
+    }
+  }
+}
+
+template <typename E, int HD>
+__global__ __launch_bounds__(kThreads, 2)
+void cached_many_k(Cached a) {
+  constexpr int KK = HD / 16, DT = HD / 32, kBlock = 16;  // kBlock: tiles of one load of entries
+  __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];
+  const Place at(a);
+  const View w(a, at.b, at.rb, kBlockRows, kTile);
+  if (w.i0 >= w.n) return;
+  const int v0 = at.split * a.split_tiles;
+  const int v_end = at.split + 1 == a.splits ? w.count : min(w.count, v0 + a.split_tiles);
+  if (at.split && v0 >= w.count) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
+  const int group = a.H / a.KV;
+
+  // the lane's row; the wave's tokens [t0, t1]
+  const int row0 = at.rb * kBlockRows + wave * kWaveRows, row = row0 + (lane & 31);
+  const int t0 = row0 / group, t1 = min(w.n - 1, (row0 + kWaveRows - 1) / group);
+  const int token = row / group, head = at.kvh * group + row % group;
+  const bool ok = token < w.n, busy = t0 < w.n;
+  const uint64_t bits = w.n < 64 ? (uint64_t(1) << w.n) - 1 : ~uint64_t(0);
+  const int limit = ok ? w.context + token : -1;
+  int place = limit;
+  uint64_t mask = 0;
+  if (a.tree && ok) {
+    mask = (uint64_t)a.tree[w.start + token] & bits;
+    place = w.context + __popcll(mask) - 1;
+  }
+  x8<E> qf[KK];
+  const E* src = static_cast<const E*>(a.q) + (int64_t)(w.start + token) * a.q_ld +
+                 (int64_t)head * HD + hl * 8;
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)
+    qf[kk] = ok ? *reinterpret_cast<const x8<E>*>(src + kk * 16) : x8<E>{};
+  State<HD> st;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) st.o[dt] = zero16();
+  st.m = -INFINITY;
+  st.l = 0.f;
+  // for the wave: slots below `below` are seen by every row as far as order goes, from `from`
+  // on as far as the window goes; slots from `end` on, and between the sinks and `begin`, by none
+  const int below = a.tree ? w.context : w.context + t0 + 1;
+  const int from = a.window ? (a.tree ? w.context + w.n - 1 : w.context + t1) - a.window + 1 : 0;
+  const int end = a.tree ? w.hi : min(w.hi, w.context + t1 + 1);
+  const int begin = a.window && !a.tree ? w.context + t0 - a.window + 1 : w.lo;
+
+  const E* kc = static_cast<const E*>(a.keys);
+  const E* vc = static_cast<const E*>(a.values);
+  PagedCopy<E, HD> ck, cv;
+  auto entries = [&](int tile) {
+    const int x = tile + (lane >> 2);
+    return x < v_end ? page_of(a, w, at.b, w.tile(x) * kTile + 16 * (lane & 3)) : -1;
+  };
+  const FragOffsets<HD, E> fo(lane);
+  int ids = entries(v0), ids_next = entries(v0 + kBlock), it = 0;
+  unsigned missing = 0;  // tiles' groups without a page: of the staged tile, then of the next
+  auto gone = [&]() { return (unsigned)(__ballot(ids < 0) >> (4 * it)) & 15u; };
+  unsigned now = 0;
+  if (v0 < v_end) {
+    const int k0 = w.tile(v0) * kTile;
+    ck.load(kc, a, w, at.kvh, ids, 0, k0);
+    cv.load(vc, a, w, at.kvh, ids, 0, k0);
+    now = gone();
+    ck.store(lds[0][0]);
+    cv.store(lds[0][1]);
+  }
+  __syncthreads();
+#define RV_MANY_STEP(BUF)                                                                       \
+  {                                                                                             \
+    const int k0 = w.tile(v) * kTile;                                                           \
+    const bool more = v + 1 < v_end;                                                            \
+    if (more) {                                                                                 \
+      if (++it == kBlock) {                                                                     \
+        it = 0;                                                                                 \
+        ids = ids_next;                                                                         \
+        ids_next = entries(v + 1 + kBlock);                                                     \
+      }                                                                                         \
+      const int k1 = w.tile(v + 1) * kTile;                                                     \
+      ck.load(kc, a, w, at.kvh, ids, it, k1);                                                   \
+      cv.load(vc, a, w, at.kvh, ids, it, k1);                                                   \
+      missing = gone();                                                                         \
+    }                                                                                           \
+    _Pragma("unroll") for (int sub = 0; sub < 2; ++sub) {                                       \
+      const int ks = k0 + sub * 32;                                                             \
+      if (!busy || ks >= end || (ks + 32 <= begin && ks >= a.sinks)) continue;                  \
+      if (ks + 32 <= below && (ks >= from || ks + 32 <= a.sinks) && !(now >> (2 * sub) & 3u)) { \
+        many_rows<E, HD, false>(st, lds[BUF][0], lds[BUF][1], fo, qf, sub, a.c,                 \
+                                [](int) { return true; });                                      \
+      } else {                                                                                  \
+        const unsigned lost = now >> (2 * sub);                                                 \
+        many_rows<E, HD, true>(st, lds[BUF][0], lds[BUF][1], fo, qf, sub, a.c, [&](int r) {     \
+          return sees(ks + r + hl * 4, !(lost >> (r >> 4) & 1u));                               \
+        });                                                                                     \
+      }                                                                                         \
+    }                                                                                           \
+    now = missing;                                                                              \
+    if (more) {                                                                                 \
+      ck.store(lds[1 - (BUF)][0]);                                                              \
+      cv.store(lds[1 - (BUF)][1]);                                                              \
+    }                                                                                           \
+    __syncthreads();                                                                            \
+  }
+  auto sees = [&](int key, bool there) {
+    bool yes = there && key < w.hi;
+    int kp = key;
+    if (a.tree) {
+      if (key >= w.context) {
+        yes = yes && (mask >> ((key - w.context) & 63) & 1);
+        if (a.window && key - w.context < w.n)
+          kp = w.context + __popcll((uint64_t)a.tree[w.start + key - w.context] & bits) - 1;
+      }
+    } else {
+      yes = yes && key <= limit;
+    }
+    if (a.window) yes = yes && (place - kp < a.window || kp < a.sinks);
+    return yes;
+  };
+  for (int v = v0; v < v_end; ++v) {
+    RV_MANY_STEP(0)
+    if (++v >= v_end) break;
+    RV_MANY_STEP(1)
+  }
+#undef RV_MANY_STEP
+  const float l = pair_sum(st.l);
+  if (!ok) return;
+  const int64_t to = (int64_t)(w.start + token) * a.H + head;
+  if (a.splits == 1 || w.count <= a.split_tiles) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    E* dst = static_cast<E*>(a.out) + to * HD + hl * 4;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int jg = 0; jg < 4; ++jg)
+        store4<E>(dst + dt * 32 + jg * 8, st.o[dt][4 * jg] * inv, st.o[dt][4 * jg + 1] * inv,
+                  st.o[dt][4 * jg + 2] * inv, st.o[dt][4 * jg + 3] * inv);
+    return;
+  }
+  float* dst = a.part + (to * a.splits + at.split) * HD + hl * 4;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int jg = 0; jg < 4; ++jg)
+      rv::st_f4(dst + dt * 32 + jg * 8, make_float4(st.o[dt][4 * jg], st.o[dt][4 * jg + 1],
+                                                    st.o[dt][4 * jg + 2], st.o[dt][4 * jg + 3]));
+  if (hl == 0) {
+    float* stat = a.part + (int64_t)a.tokens * a.H * a.splits * HD + (to * a.splits + at.split) * 2;
+    stat[0] = st.m;
+    stat[1] = l;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the stretches of the rows that were cut: one wave a row of HD columns, rows of
+// one sequence numbered token by token.  The lanes hold the stretches' factors, 64 at a time;
+// then HD / 4 of them take four columns each and the others the next stretches.
+// ---------------------------------------------------------------------------
 template <typename E, int HD>
 __global__ __launch_bounds__(kThreads)
-void cached_join_k(Cached a, int rows_per_block) {
-  constexpr int kPer = kThreads / (HD / 4);
-  const int blocks = (int)(((int64_t)a.max_query * a.H + kPer - 1) / kPer);
-  const int b = blockIdx.x / blocks;
-  const int64_t row = (int64_t)(blockIdx.x % blocks) * kPer + threadIdx.x / (HD / 4);
-  const int col = (threadIdx.x % (HD / 4)) * 4;
+void cached_join_k(Cached a, int rows_per_block, int keys) {
+  constexpr int kCols = HD / 4, kSide = 64 / kCols;  // stretches at once
+  const int64_t per = ((int64_t)a.max_query * a.H + kWaves - 1) / kWaves;
+  const int b = (int)(blockIdx.x / per), lane = threadIdx.x & 63;
+  const int64_t row = blockIdx.x % per * kWaves + (threadIdx.x >> 6);
   const int token = (int)(row / a.H), head = (int)(row % a.H), group = a.H / a.KV;
-  const View w(a, b, (token * group + head % group) / rows_per_block, rows_per_block);
+  const View w(a, b, (token * group + head % group) / rows_per_block, rows_per_block, keys);
   if (token >= w.n || w.count <= a.split_tiles) return;
   const int used = min((w.count + a.split_tiles - 1) / a.split_tiles, a.splits);
-  const int64_t at = ((int64_t)(w.start + token) * a.H + head) * a.splits;
+  const int64_t to = (int64_t)(w.start + token) * a.H + head, at = to * a.splits;
   const float* stat = a.part + (int64_t)a.tokens * a.H * a.splits * HD + at * 2;
   float top = -INFINITY;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, stat[2 * s]);
+  for (int s = lane; s < used; s += 64) top = fmaxf(top, stat[2 * s]);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
   if (top == -INFINITY) top = 0.f;
   float l = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < used; ++s) {
-    const float factor = __builtin_amdgcn_exp2f(stat[2 * s] - top);
-    l += stat[2 * s + 1] * factor;
-    sum += *reinterpret_cast<const f32x4*>(a.part + (at + s) * HD + col) * factor;
+  const int side = lane / kCols, col = lane % kCols * 4;
+  for (int s0 = 0; s0 < used; s0 += 64) {
+    const int s = s0 + lane;
+    const float factor = s < used ? __builtin_amdgcn_exp2f(stat[2 * s] - top) : 0.f;
+    if (s < used) l += stat[2 * s + 1] * factor;
+    const int n = min(64, used - s0);
+    for (int x = 0; x < n; x += 4 * kSide) {  // four loads under way
+      f32x4 v[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int mine = min(x + y * kSide + side, n - 1);
+        v[y] = *reinterpret_cast<const f32x4*>(a.part + (at + s0 + mine) * HD + col);
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int mine = x + y * kSide + side;
+        const float f = __shfl(factor, mine & 63);
+        if (mine < n) sum += v[y] * f;
+      }
+    }
   }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
+#pragma unroll
+  for (int x = 32; x >= kCols; x >>= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], x);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  store4<E>(static_cast<E*>(a.out) + ((int64_t)(w.start + token) * a.H + head) * HD + col,
-            sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+  if (side == 0)
+    store4<E>(static_cast<E*>(a.out) + to * HD + col, sum[0] * inv, sum[1] * inv, sum[2] * inv,
+              sum[3] * inv);
 }
 
-// Rows a workgroup takes (in sixteens), blocks of rows, stretches of keys.
+// Rows and keys a tile, blocks of rows, stretches of keys.
 struct Plan {
-  int nr, row_blocks, splits, split_tiles;
+  int rows, keys, row_blocks, splits, split_tiles;
 };
 
-constexpr int64_t kWanted = 1024;    // workgroups for the chip's 256 CUs
-constexpr int kLeastTiles = 8;       // tiles of a stretch: two for each wave
-constexpr int kMostTiles = 128;      // a longer one would keep a few workgroups busy alone
+constexpr int64_t kFewWanted = 1024;   // workgroups for the chip's 256 CUs
+constexpr int64_t kManyWanted = 512;
+constexpr int kLeastKeys = 256;        // of a stretch
+constexpr int kMostKeys = 1024;        // a longer one would keep a few workgroups busy alone
 constexpr int kMostSplits = 256;
 
 Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t max_length,
              int64_t window, int64_t sinks) {
   Plan p;
   const int64_t rows = max_query * (heads / kv);
-  p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p.row_blocks = (int)((rows + 16 * p.nr - 1) / (16 * p.nr));
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kBlockRows;
+  const bool many = p.rows == kBlockRows;
+  p.keys = many ? kTile : kKeys;
+  p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
   int64_t seen = max_length;  // of one block of rows, at most (and the tiles' edges)
-  if (window) seen = std::min(seen, window + sinks + std::min<int64_t>(max_query, 64) + 3 * kKeys);
-  const int64_t tiles = std::max<int64_t>(1, (seen + kKeys - 1) / kKeys);
-  const int64_t blocks = seqs * kv * p.row_blocks;
-  int64_t splits = std::max((kWanted + blocks - 1) / blocks, (tiles + kMostTiles - 1) / kMostTiles);
-  splits = std::min<int64_t>(splits, (tiles + kLeastTiles - 1) / kLeastTiles);
+  if (window) seen = std::min(seen, window + sinks + std::min<int64_t>(max_query, 128) + 3 * p.keys);
+  const int64_t tiles = std::max<int64_t>(1, (seen + p.keys - 1) / p.keys);
+  const int64_t blocks = seqs * kv * p.row_blocks, wanted = many ? kManyWanted : kFewWanted;
+  const int64_t least = kLeastKeys / p.keys, most = (many ? 4 : 1) * kMostKeys / p.keys;
+  int64_t splits = std::max((wanted + blocks - 1) / blocks, (tiles + most - 1) / most);
+  splits = std::min<int64_t>(splits, (tiles + least - 1) / least);
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
@@ -478,7 +794,7 @@ bool sizes_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv, int64_t h
   return (hd == 32 || hd == 64 || hd == 128) && heads < (1 << 16) && tokens < (1 << 26) &&
          max_query < (1 << 26) && max_length <= (1 << 30) && max_query * heads < (1 << 30) &&
          seqs * kv * p.row_blocks * p.splits < (1 << 24) &&
-         seqs * ((max_query * heads * (hd / 4) + kThreads - 1) / kThreads) < (1 << 24);
+         seqs * ((max_query * heads + kWaves - 1) / kWaves) < (1 << 24);
 }
 
 int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t hd, const Plan& p) {
@@ -488,18 +804,17 @@ int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t hd, const Plan& p
 template <typename E, int HD>
 int launch(const Cached& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.seqs * a.KV * p.row_blocks * p.splits)), block(kThreads);
-  if (p.nr == 1)
-    hipLaunchKernelGGL((cached_attn_k<E, HD, 1>), grid, block, 0, s, a);
-  else if (p.nr == 2)
-    hipLaunchKernelGGL((cached_attn_k<E, HD, 2>), grid, block, 0, s, a);
+  if (p.rows == 16)
+    hipLaunchKernelGGL((cached_few_k<E, HD, 1>), grid, block, 0, s, a);
+  else if (p.rows == 32)
+    hipLaunchKernelGGL((cached_few_k<E, HD, 2>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((cached_attn_k<E, HD, 4>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((cached_many_k<E, HD>), grid, block, 0, s, a);
   int rc = rv_host::check_launch();
   if (rc != RV_OK || p.splits == 1) return rc;
-  constexpr int kPer = kThreads / (HD / 4);
-  const int64_t blocks = ((int64_t)a.max_query * a.H + kPer - 1) / kPer;
+  const int64_t blocks = ((int64_t)a.max_query * a.H + kWaves - 1) / kWaves;
   hipLaunchKernelGGL((cached_join_k<E, HD>), dim3((unsigned)(blocks * a.seqs)), block, 0, s, a,
-                     16 * p.nr);
+                     p.rows, p.keys);
   return rv_host::check_launch();
 }
 

@@ -37,7 +37,7 @@ struct Geometry {
 
 // Workgroups per CU the register budget is sized for (attention.hip's figures).
 template <int HD>
-constexpr int kFwdMinBlocks = HD == 128 ? 1 : (HD == 64 ? 3 : 2);
+constexpr int kFwdMinBlocks = HD == 128 ? 2 : (HD == 64 ? 3 : 2);
 template <int HD>
 constexpr int kQMinBlocks = HD == 128 ? 1 : (HD == 64 ? 3 : 2);
 template <int HD>
