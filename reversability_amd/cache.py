@@ -26,10 +26,11 @@ Nothing here is differentiable, and there is no CPU fallback.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import paths
 from ._hip import _check, _DeviceGuard, _stream, library
@@ -42,11 +43,17 @@ from .residual import euler_step, midpoint_step
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
+# These operators run once a layer and token, on calls of a few microseconds: what is checked is
+# checked without building anything.
 def _no_graph(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError(f"{what} is not differentiable: call it under torch.no_grad()")
-    if any(unpack_dual(t).tangent is not None for t in tensors):
-        raise NotImplementedError(f"{what} has no forward-mode derivative")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ValueError(f"{what} is not differentiable: call it under torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (no dual tensors outside a level)
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _check_cache(keys: torch.Tensor, values: torch.Tensor, what: str) -> None:
@@ -119,16 +126,17 @@ def append_kv(qkv: torch.Tensor, heads: int, keys: torch.Tensor, values: torch.T
     kv, hd = packed_heads(qkv, heads, keys.shape[1], "append_kv")
     if qkv.dtype != keys.dtype or qkv.device != keys.device or hd != keys.shape[3]:
         raise ValueError("append_kv needs qkv of the cache's type, head size and device")
-    rows = qkv.reshape(-1, qkv.shape[-1])
+    rows = qkv if qkv.ndim == 2 else qkv.reshape(-1, qkv.shape[-1])
     if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.stride(0) < rows.shape[1]:
         rows = rows.contiguous()
     if rows.data_ptr() % 16:
         rows = rows.clone()
     n = rows.shape[0]
     slots = _ints(slots, (n,), keys, "slots", torch.int64)
-    q = rows[:, :heads * hd].unflatten(1, (heads, hd))
     turn = (None, 0, None, False)
-    if rotary is not None:
+    if rotary is None:
+        q = rows[:, :heads * hd].view(n, heads, hd)
+    else:
         rotary.check(qkv, hd, "append_kv")
         if positions is None:
             raise ValueError("append_kv needs positions to rotate by")
@@ -145,6 +153,14 @@ def append_kv(qkv: torch.Tensor, heads: int, keys: torch.Tensor, values: torch.T
                 _CODES[keys.dtype], keys.shape[0], keys.shape[2], *turn, _stream(keys)),
                 "rv_append_kv")
     return q
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(*sizes) -> int:
+    nbytes = library().rv_cached_attn_workspace_bytes(*sizes)
+    if nbytes < 0:
+        _check(-nbytes, "rv_cached_attn_workspace_bytes")
+    return nbytes
 
 
 def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
@@ -191,7 +207,8 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
         q = q.contiguous()
         q = q if q.data_ptr() % 16 == 0 else q.clone()
     if out is None:
-        out = torch.empty(tokens, heads, hd, device=q.device, dtype=q.dtype)
+        out = (torch.empty_like(q) if q.is_contiguous() else
+               torch.empty(tokens, heads, hd, device=q.device, dtype=q.dtype))
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned tensor like q")
@@ -200,9 +217,7 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
         return out
     lib, span = library(), (window or 0, sinks if window else 0)
     sizes = (tokens, table.shape[0], heads, kv, hd)
-    nbytes = lib.rv_cached_attn_workspace_bytes(*sizes, max_query, max_length, *span)
-    if nbytes < 0:
-        _check(-nbytes, "rv_cached_attn_workspace_bytes")
+    nbytes = _workspace_bytes(*sizes, max_query, max_length, *span)
     with _DeviceGuard(q):
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
         _check(lib.rv_cached_attn(

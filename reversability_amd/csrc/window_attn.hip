@@ -65,6 +65,27 @@ __device__ __forceinline__ bool all_seen(const Geometry& g, int q0, int k0, int 
   return k0 + n - 1 <= q0 && (k0 > q0 + kWaveRows - 1 - g.window || k0 + n <= g.sinks);
 }
 
+// What a lane with one query sees of keys k0 + r, r the lane's row of a tile of keys (no
+// branches: two comparisons an element): the window, or the sinks among the keys up to its own.
+struct QuerySight {
+  int at, sinks;  // query - k0, and sinks up to the query - k0
+  unsigned window;
+  __device__ __forceinline__ QuerySight(const Geometry& g, int q, int k0)
+      : at(q - k0), sinks(min(g.sinks, q + 1) - k0), window((unsigned)g.window) {}
+  __device__ __forceinline__ bool operator()(int r) const {
+    return ((unsigned)(at - r) < window) | (r < sinks);
+  }
+};
+
+// Which queries q0 + r a lane with one key is seen by.
+struct KeySight {
+  int at;  // q0 - key
+  unsigned reach;
+  __device__ __forceinline__ KeySight(const Geometry& g, int key, int q0)
+      : at(q0 - key), reach(key < g.sinks ? 0x80000000u : (unsigned)g.window) {}
+  __device__ __forceinline__ bool operator()(int r) const { return (unsigned)(at + r) < reach; }
+};
+
 template <int HD>
 struct FwdState {
   f32x16 o[HD / 32];
@@ -90,12 +111,10 @@ __device__ __forceinline__ void fwd_rows(FwdState<HD>& st, const E* Ks, const E*
   for (int kk = 1; kk < KK; ++kk) s = mfma(kf[kk], qf[kk], s);
   prio_valu();
   float mx = -INFINITY;
+  const QuerySight sees(g, q, k0 + hl * 4);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    if constexpr (MASK) {
-      const int k = k0 + acc_row(j) + hl * 4;
-      if (k > q || (q - k >= g.window && k >= g.sinks)) s[j] = -INFINITY;
-    }
+    if constexpr (MASK) s[j] = sees(acc_row(j)) ? s[j] : -INFINITY;
     mx = fmaxf(mx, s[j]);
   }
   const float mxc = pair_max(mx) * c;
@@ -258,15 +277,12 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
   }
   const float neg_l = -Lq;
   prio_valu();
+  const QuerySight sees(g, q, k0 + hl * 4);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, neg_l));
-    float d = p * (dp[j] - Dq);
-    if constexpr (MASK) {
-      const int k = k0 + acc_row(j) + hl * 4;
-      if (k > q || (q - k >= g.window && k >= g.sinks)) d = 0.f;
-    }
-    dp[j] = d;
+    const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, neg_l));
+    dp[j] = p * (dp[j] - Dq);
+    if constexpr (MASK) dp[j] = sees(acc_row(j)) ? dp[j] : 0.f;
   }
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc) {
@@ -409,6 +425,7 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
     __builtin_amdgcn_sched_barrier(0);
   }
   prio_valu();
+  const KeySight seen(g, key, q0 + hl * 4);
 #pragma unroll
   for (int jg = 0; jg < 4; ++jg) {
     const int r4 = sub * 32 + jg * 8 + hl * 4;
@@ -419,14 +436,11 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int j = 4 * jg + e;
-      float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, -Lr[e]));
-      float d = p * (dp[j] - Dr[e]);
-      if constexpr (MASK) {
-        const int q = q0 + jg * 8 + hl * 4 + e;
-        if (key > q || (q - key >= g.window && key >= g.sinks)) p = d = 0.f;
-      }
-      s[j] = p;
-      dp[j] = d;
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, -Lr[e]));
+      const float d = p * (dp[j] - Dr[e]);
+      const bool on = !MASK || seen(acc_row(j));
+      s[j] = on ? p : 0.f;
+      dp[j] = on ? d : 0.f;
     }
   }
 #pragma unroll
