@@ -57,6 +57,13 @@ struct KeyTiles {
   __device__ __forceinline__ int at(int t) const { return t < ns ? t : first + t - ns; }
 };
 
+// Workgroups are dealt to the eight XCDs in turn, each with an L2 of its own: the number that gives
+// each XCD a stretch of neighbours, which read the same keys or queries.
+__device__ __forceinline__ int near_index() {
+  const int n = (int)gridDim.x, x = (int)blockIdx.x % 8, per = n / 8, more = n % 8;
+  return x * per + min(x, more) + (int)blockIdx.x / 8;
+}
+
 // Whether no / every query of [q0, q0 + 31] sees any / all of the keys [k0, k0 + n).
 __device__ __forceinline__ bool none_seen(const Geometry& g, int q0, int k0, int n) {
   return k0 > q0 + kWaveRows - 1 || (k0 + n - 1 <= q0 - g.window && k0 >= g.sinks);
@@ -164,7 +171,7 @@ void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, float* __restri
                  Geometry g, int n_qt, float c) {
   constexpr int KK = HD / 16, DT = HD / 32;
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];
-  const int bh = (int)(blockIdx.x / n_qt), qt = (int)(blockIdx.x % n_qt);
+  const int at = near_index(), bh = at / n_qt, qt = at % n_qt;
   const int b = bh / g.H, h = bh % g.H, kvh = h / (g.H / g.KV);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
   const int64_t rs = (int64_t)(g.H + 2 * g.KV) * HD;
@@ -303,7 +310,7 @@ void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
                    float scale) {
   constexpr int KK = HD / 16, DT = HD / 32;
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][K / V]
-  const int bh = (int)(blockIdx.x / n_qt), qt = (int)(blockIdx.x % n_qt);
+  const int at = near_index(), bh = at / n_qt, qt = at % n_qt;
   const int b = bh / g.H, h = bh % g.H, kvh = h / (g.H / g.KV);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
   const int64_t rs = (int64_t)(g.H + 2 * g.KV) * HD, os = (int64_t)g.H * HD;
@@ -488,7 +495,7 @@ void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][Q / dO]
   __shared__ __attribute__((aligned(16))) float rowv[2][2][kTile];  // [buf][lse / delta]
   const int units = plan.units();
-  const int bkv = (int)(blockIdx.x / units), unit = (int)(blockIdx.x % units);
+  const int number = near_index(), bkv = number / units, unit = number % units;
   const int sink_units = plan.sink_blocks * plan.sink_chunks;
   const bool sink = unit < sink_units;
   const int chunks = sink ? plan.sink_chunks : plan.near_chunks;
@@ -581,7 +588,7 @@ void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
 #undef RV_KV_STEP
   if (key >= g.T) return;
   if (chunks > 1) {  // [unit][K / V][128][HD] fp32
-    float* row = part + (((int64_t)blockIdx.x * 2) * kBlockRows + key - kbase) * HD;
+    float* row = part + (((int64_t)number * 2) * kBlockRows + key - kbase) * HD;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
