@@ -600,10 +600,12 @@ int rv_attn_bwd(const void* qkv, const void* out, const void* dout, const float*
 /* Causal attention with a sliding window (> 0) and `sinks` (>= 0) first tokens that
  * stay visible: query i sees key j <= i where i - j < window or j < sinks.  qkv
  * [batch, seq, (heads + 2 kv_heads) head_dim]; out [batch, seq, heads, head_dim]; lse
- * fp32 [batch * heads, seq] (base 2). */
+ * fp32 [batch * heads, seq] (base 2); rest (nullable, like out): what out's rounding left
+ * (the backward's rows of dO . O need the digits).  The weights' roundings for the product
+ * with the values are made up for. */
 int rv_window_attn_fwd(const void* qkv, int64_t batch, int64_t seq, int64_t heads,
                        int64_t kv_heads, int64_t head_dim, int dtype, int64_t window,
-                       int64_t sinks, void* out, float* lse, void* stream);
+                       int64_t sinks, void* out, void* rest, float* lse, void* stream);
 
 /* Workspace bytes of rv_window_attn_bwd (negative: -error). */
 int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
@@ -611,9 +613,9 @@ int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t h
                                            int64_t sinks);
 
 /* dqkv (qkv's type and layout) = gradient of out with respect to qkv, given dout and the
- * forward's out and lse.  Deterministic. */
-int rv_window_attn_bwd(const void* qkv, const void* out, const void* dout, const float* lse,
-                       int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
+ * forward's out, rest (nullable) and lse.  Deterministic. */
+int rv_window_attn_bwd(const void* qkv, const void* out, const void* rest, const void* dout,
+                       const float* lse, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
                        int64_t head_dim, int dtype, int64_t window, int64_t sinks, void* dqkv,
                        void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -115,9 +115,9 @@ SIGNATURES = {
     "rv_attn_fwd": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P]),
     "rv_attn_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "rv_attn_bwd": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
-    "rv_window_attn_fwd": (_I, [_P, *[_I64] * 5, _I, _I64, _I64, _P, _P, _P]),
+    "rv_window_attn_fwd": (_I, [_P, *[_I64] * 5, _I, _I64, _I64, _P, _P, _P, _P]),
     "rv_window_attn_bwd_workspace_bytes": (_I64, [_I64] * 7),
-    "rv_window_attn_bwd": (_I, [_P, _P, _P, _P, *[_I64] * 5, _I, _I64, _I64, _P, _P, _I64, _P]),
+    "rv_window_attn_bwd": (_I, [_P, _P, _P, _P, _P, *[_I64] * 5, _I, _I64, _I64, _P, _P, _I64, _P]),
     "rv_rotate_qkv": (_I, [_P, _P, *[_I64] * 5, _I, _P, _I64, _P, _I, _I, _P]),
     "rv_cache_plan": (_I, [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P]),
     "rv_append_kv": (_I, [_P, _I64, _P, _P, _P, _P, *[_I64] * 4, _I, _I64, _I64, _P, _I64, _P, _I,

@@ -234,13 +234,15 @@ class WindowAttention(torch.autograd.Function):
         hd = width // (heads + 2 * kv)
         x = _dense(qkv)
         out = torch.empty(batch, seq, heads * hd, device=x.device, dtype=x.dtype)
+        rest = torch.empty_like(out) if ctx.needs_input_grad[0] else None
         lse = torch.empty(batch * heads, seq, device=x.device, dtype=torch.float32)
         if out.numel():
             with _DeviceGuard(x):
                 _check(library().rv_window_attn_fwd(
                     x.data_ptr(), batch, seq, heads, kv, hd, _CODES[x.dtype], window, sinks,
-                    out.data_ptr(), lse.data_ptr(), _stream(x)), "rv_window_attn_fwd")
-        ctx.save_for_backward(x, out, lse)
+                    out.data_ptr(), None if rest is None else rest.data_ptr(), lse.data_ptr(),
+                    _stream(x)), "rv_window_attn_fwd")
+        ctx.save_for_backward(x, out, rest, lse)
         ctx.sizes = (batch, seq, heads, kv, hd)
         ctx.span = (window, sinks)
         return out
@@ -248,7 +250,7 @@ class WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        x, out, lse = ctx.saved_tensors
+        x, out, rest, lse = ctx.saved_tensors
         dqkv = torch.empty_like(x)
         if out.numel():
             lib, dout = library(), _dense(dout)
@@ -258,7 +260,8 @@ class WindowAttention(torch.autograd.Function):
             with _DeviceGuard(x):
                 ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
                 _check(lib.rv_window_attn_bwd(
-                    x.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), *ctx.sizes,
+                    x.data_ptr(), out.data_ptr(), rest.data_ptr(), dout.data_ptr(),
+                    lse.data_ptr(), *ctx.sizes,
                     _CODES[x.dtype], *ctx.span, dqkv.data_ptr(), ws.data_ptr(), nbytes,
                     _stream(x)), "rv_window_attn_bwd")
         return dqkv, None, None, None, None

@@ -20,7 +20,9 @@
 // dK/dV: a key block's work is (heads that share it) x (tiles of queries).  It is cut into
 // chunks where a block alone would take much longer than the rest (the sinks' block
 // sees the whole sequence) or where there are few blocks; a chunk writes fp32 partials
-// and wattn_reduce_k adds them in order.
+// and wattn_reduce_k adds them in order.  The sinks' sums are long and their terms large: there
+// P and dS are taken with what their roundings left, by twice the products (of 16384 queries'
+// terms the roundings alone were half as large as the other keys' gradients are).
 
 #include <algorithm>
 #include <cmath>
@@ -37,9 +39,9 @@ struct Geometry {
 
 // Workgroups per CU the register budget is sized for (attention.hip's figures).
 template <int HD>
-constexpr int kFwdMinBlocks = HD == 128 ? 2 : (HD == 64 ? 3 : 2);
+constexpr int kFwdMinBlocks = HD == 128 ? 2 : (HD == 64 ? 4 : 2);
 template <int HD>
-constexpr int kQMinBlocks = HD == 128 ? 1 : (HD == 64 ? 3 : 2);
+constexpr int kQMinBlocks = HD == 128 ? 2 : (HD == 64 ? 3 : 2);
 template <int HD>
 constexpr int kKvMinBlocks = HD == 128 ? 1 : 2;
 
@@ -101,6 +103,8 @@ struct FwdState {
 
 // 32 keys (rows sub * 32 .. of the tile) for one wave's 32 queries.  MASK: some of them are not
 // seen by some query; q, k0: the lane's query and the first of the keys.
+// P's roundings are made up for by a second product with what they left: the output is then known to
+// more digits than its type has, which the backward's dO . O needs (rest).
 template <typename E, int HD, bool MASK>
 __device__ __forceinline__ void fwd_rows(FwdState<HD>& st, const E* Ks, const E* Vs,
                                          const FragOffsets<HD, E>& fo, const x8<E> (&qf)[HD / 16],
@@ -157,18 +161,22 @@ __device__ __forceinline__ void fwd_rows(FwdState<HD>& st, const E* Ks, const E*
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc) {
     const x8<E> pf = pack8<E>(s, cc);
+    x8<E> left;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) left[i] = (E)(s[8 * cc + i] - (float)pf[i]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (!kReadAhead<HD>) vf[cc][dt] = fo.trf(Vs, sub, cc, dt);
       st.o[dt] = mfma(vf[cc][dt], pf, st.o[dt]);
+      st.o[dt] = mfma(vf[cc][dt], left, st.o[dt]);
     }
   }
 }
 
 template <typename E, int HD>
 __global__ __launch_bounds__(kThreads, kFwdMinBlocks<HD>)
-void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, float* __restrict__ lse,
-                 Geometry g, int n_qt, float c) {
+void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__ rest,
+                 float* __restrict__ lse, Geometry g, int n_qt, float c) {
   constexpr int KK = HD / 16, DT = HD / 32;
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];
   const int at = near_index(), bh = at / n_qt, qt = at % n_qt;
@@ -236,14 +244,22 @@ void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, float* __restri
   const float l = pair_sum(st.l);
   if (q < g.T) {
     const float inv = 1.0f / l;
-    E* orow = out + ((int64_t)b * g.T + q) * g.H * HD + (int64_t)h * HD;
+    const int64_t row = (((int64_t)b * g.T + q) * g.H + h) * HD;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int jg = 0; jg < 4; ++jg)
-        store4<E>(orow + dt * 32 + jg * 8 + hl * 4, st.o[dt][4 * jg] * inv,
-                  st.o[dt][4 * jg + 1] * inv, st.o[dt][4 * jg + 2] * inv,
-                  st.o[dt][4 * jg + 3] * inv);
+      for (int jg = 0; jg < 4; ++jg) {
+        const int64_t at = row + dt * 32 + jg * 8 + hl * 4;
+        x4<E> v, r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = st.o[dt][4 * jg + e] * inv;
+          v[e] = (E)x;
+          r[e] = (E)(x - (float)v[e]);
+        }
+        *reinterpret_cast<x4<E>*>(out + at) = v;
+        if (rest) *reinterpret_cast<x4<E>*>(rest + at) = r;
+      }
     if (hl == 0) lse[(int64_t)bh * g.T + q] = st.m + __log2f(l);
   }
 }
@@ -260,28 +276,24 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
   constexpr int KK = HD / 16, DT = HD / 32;
   const int hl = lane >> 5;
   prio_mfma();
-  x8<E> kf[KK], vf[KK];
+  // half of the row operands at a time: all of them do not fit in the registers
+  constexpr int KH = KK > 4 ? 4 : KK > 2 ? 2 : KK;
+  f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    kf[kk] = fo.rowf(Ks, sub, kk);
-    vf[kk] = fo.rowf(Vs, sub, kk);
-  }
-  if constexpr (kReadAhead<HD>) __builtin_amdgcn_sched_barrier(0);
-  f32x16 s = mfma(kf[0], qf[0], zero16());
-  f32x16 dp = mfma(vf[0], gf[0], zero16());
+  for (int k0h = 0; k0h < KK; k0h += KH) {
+    x8<E> kf[KH], vf[KH];
 #pragma unroll
-  for (int kk = 1; kk < KK; ++kk) {
-    s = mfma(kf[kk], qf[kk], s);
-    dp = mfma(vf[kk], gf[kk], dp);
+    for (int kk = 0; kk < KH; ++kk) {
+      kf[kk] = fo.rowf(Ks, sub, k0h + kk);
+      vf[kk] = fo.rowf(Vs, sub, k0h + kk);
+    }
+#pragma unroll
+    for (int kk = 0; kk < KH; ++kk) {
+      s = mfma(kf[kk], qf[k0h + kk], s);
+      dp = mfma(vf[kk], gf[k0h + kk], dp);
+    }
   }
   x8<E> kt[2][DT];
-  if constexpr (kReadAhead<HD>) {
-#pragma unroll
-    for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) kt[cc][dt] = fo.trf(Ks, sub, cc, dt);
-    __builtin_amdgcn_sched_barrier(0);
-  }
   const float neg_l = -Lq;
   prio_valu();
   const QuerySight sees(g, q, k0 + hl * 4);
@@ -296,7 +308,7 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
     const x8<E> dsf = pack8<E>(dp, cc);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      if constexpr (!kReadAhead<HD>) kt[cc][dt] = fo.trf(Ks, sub, cc, dt);
+      kt[cc][dt] = fo.trf(Ks, sub, cc, dt);
       dq[dt] = mfma(kt[cc][dt], dsf, dq[dt]);
     }
   }
@@ -305,7 +317,7 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
 template <typename E, int HD>
 __global__ __launch_bounds__(kThreads, kQMinBlocks<HD>)
 void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
-                   const E* __restrict__ dout, const float* __restrict__ lse,
+                   const E* __restrict__ rest, const E* __restrict__ dout, const float* __restrict__ lse,
                    float* __restrict__ delta, E* __restrict__ dqkv, Geometry g, int n_qt, float c,
                    float scale) {
   constexpr int KK = HD / 16, DT = HD / 32;
@@ -319,23 +331,26 @@ void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
   const E* kb = base + (int64_t)(g.H + kvh) * HD;
   const E* vb = kb + (int64_t)g.KV * HD;
   const E* gb = dout + (int64_t)b * g.T * os + (int64_t)h * HD;
-  const E* ob = out + (int64_t)b * g.T * os + (int64_t)h * HD;
+  const int64_t o0 = (int64_t)b * g.T * os + (int64_t)h * HD;
   const int q0 = qt * kBlockRows + wave * kWaveRows;
   const int q = q0 + (lane & 31);
   const bool qok = q < g.T;
 
   x8<E> qf[KK], gf[KK];
-  // delta = sum_d dO O over the query's row: this lane's HD / 2 columns (the
-  // fragments' layout), then the other half from lane l ^ 32
+  // delta = sum_d dO O over the query's row (O with what its rounding left): this lane's
+  // HD / 2 columns (the fragments' layout), then the other half from lane l ^ 32
   float dsum = 0.f;
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     const int64_t col = kk * 16 + hl * 8;
     qf[kk] = qok ? *reinterpret_cast<const x8<E>*>(qb + (int64_t)q * rs + col) : x8<E>{};
     gf[kk] = qok ? *reinterpret_cast<const x8<E>*>(gb + (int64_t)q * os + col) : x8<E>{};
-    const x8<E> of = qok ? *reinterpret_cast<const x8<E>*>(ob + (int64_t)q * os + col) : x8<E>{};
+    const int64_t at = o0 + (int64_t)q * os + col;
+    const x8<E> of = qok ? *reinterpret_cast<const x8<E>*>(out + at) : x8<E>{};
+    const x8<E> ol = qok && rest ? *reinterpret_cast<const x8<E>*>(rest + at) : x8<E>{};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dsum = fmaf((float)gf[kk][i], (float)of[i], dsum);
+    for (int i = 0; i < 8; ++i)
+      dsum = fmaf((float)gf[kk][i], (float)of[i] + (float)ol[i], dsum);
   }
   const float Lq = qok ? lse[(int64_t)bh * g.T + q] : 0.f;
   const float Dq = pair_sum(dsum);
@@ -398,8 +413,9 @@ void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
 
 // dK/dV contribution of 32 staged queries (tile rows sub * 32 ..) to one wave's 32 keys
 // (lanes).  Query rows past the sequence hold zeros (Q, dO, lse, delta): their
-// P is 1 but dS = 0 and dO = 0, so they add nothing.
-template <typename E, int HD, bool MASK>
+// P is 1 but dS = 0 and dO = 0, so they add nothing.  REST: what the roundings of P and dS left is
+// added by products of its own.
+template <typename E, int HD, bool MASK, bool REST>
 __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD / 32], const E* Qs,
                                         const E* Gs, const float* Ls, const float* Ds,
                                         const FragOffsets<HD, E>& fo, const x8<E> (&kf)[HD / 16],
@@ -453,6 +469,14 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc) {
     const x8<E> pf = pack8<E>(s, cc), dsf = pack8<E>(dp, cc);
+    x8<E> pl, dsl;
+    if constexpr (REST) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pl[i] = (E)(s[8 * cc + i] - (float)pf[i]);
+        dsl[i] = (E)(dp[8 * cc + i] - (float)dsf[i]);
+      }
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if (cc == 1 || !kReadAhead<HD>) {
@@ -461,6 +485,10 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
       }
       dv[dt] = mfma(gt[cc][dt], pf, dv[dt]);
       dk[dt] = mfma(qt[cc][dt], dsf, dk[dt]);
+      if constexpr (REST) {
+        dv[dt] = mfma(gt[cc][dt], pl, dv[dt]);
+        dk[dt] = mfma(qt[cc][dt], dsl, dk[dt]);
+      }
     }
   }
 }
@@ -563,12 +591,15 @@ void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
     _Pragma("unroll") for (int sub = 0; sub < 2; ++sub) {                                     \
       const int qs = qt0 + sub * 32;                                                          \
       if (none_seen(g, qs, k0w, kWaveRows)) continue;                                         \
-      if (all_seen(g, qs, k0w, kWaveRows))                                                    \
-        kv_rows<E, HD, false>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0], rowv[BUF][1],   \
-                              fo, kf, vf, g, sub, qs, key, c, lane);                          \
-      else                                                                                    \
-        kv_rows<E, HD, true>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0], rowv[BUF][1],    \
-                             fo, kf, vf, g, sub, qs, key, c, lane);                           \
+      if (sink)                                                                                \
+        kv_rows<E, HD, true, true>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],             \
+                                   rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);        \
+      else if (all_seen(g, qs, k0w, kWaveRows))                                                \
+        kv_rows<E, HD, false, false>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],           \
+                                     rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);      \
+      else                                                                                     \
+        kv_rows<E, HD, true, false>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],            \
+                                    rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);       \
     }                                                                                         \
     if (more) {                                                                               \
       cq.store(lds[1 - (BUF)][0]);                                                            \
@@ -640,6 +671,7 @@ void wattn_reduce_k(const float* __restrict__ part, E* __restrict__ dqkv, Geomet
     if (key >= g.T) continue;
     const float* src = part + ((unit * 2 + side) * kBlockRows + r) * HD + col;
     float4 sum = rv::ld_f4(src);
+#pragma unroll 8
     for (int j = 1; j < chunks; ++j) {
       const float4 v = rv::ld_f4(src + (int64_t)j * 2 * kBlockRows * HD);
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
@@ -650,36 +682,53 @@ void wattn_reduce_k(const float* __restrict__ part, E* __restrict__ dqkv, Geomet
   }
 }
 
-// Steps that a chunk has at least, workgroups wanted on the chip's 256 CUs, and the most that
-// the sinks' blocks are cut into (their partials' memory).
+// Steps that a chunk has at least, and the most that the sinks' blocks are cut into (their
+// partials' memory).
 constexpr int kLeastSteps = 8;
-constexpr int kWanted = 512;
 constexpr int kMostUnits = 4096;
 
-KvPlan kv_plan(const Geometry& g, int64_t batch) {
-  KvPlan p;
+// Chunks that the other blocks are cut into: of the plans with 1, 2, 3 .. the one that takes the fewest
+// steps in a row, where `slots` chunks run at once (a workgroup's start and end count
+// as three steps, the partials by their bytes at 4 TB/s and a launch, a step as 2 us).
+// 3 x 1999 tokens, 20 heads of 64 over 4, window 500: 3 chunks of 17 steps in two rounds
+// 77 + 11.7 us (sums, then partials), 2 of 25 in one 68 + 8.9.
+KvPlan kv_plan(const Geometry& g, int64_t batch, int64_t hd) {
   const int group = g.H / g.KV;
-  p.blocks = (g.T + kBlockRows - 1) / kBlockRows;
-  p.sink_blocks = std::min((g.sinks + kBlockRows - 1) / kBlockRows, p.blocks);
-  const int64_t outer = batch * g.KV;
-  // steps of the first block without sinks: no later one has more
-  const int near = p.sink_blocks < p.blocks ? group * query_tiles(g, p.sink_blocks * kBlockRows)
-                                            : 0;
-  const int64_t blocks = outer * p.blocks;
-  int chunks = 1;
-  if (blocks < kWanted) chunks = (int)((kWanted + blocks - 1) / blocks);
-  chunks = std::max(1, std::min(chunks, near / kLeastSteps));
-  p.near_len = (near + chunks - 1) / chunks;
-  p.near_chunks = near ? (near + p.near_len - 1) / p.near_len : 1;
-  p.sink_len = p.sink_chunks = 1;
-  if (p.sink_blocks) {
-    const int most = group * query_tiles(g, 0);
-    int64_t len = std::max(p.near_len, kLeastSteps);
-    len = std::max(len, (outer * p.sink_blocks * most + kMostUnits - 1) / kMostUnits);
-    p.sink_len = (int)std::min<int64_t>(len, most);
-    p.sink_chunks = (most + p.sink_len - 1) / p.sink_len;
+  const int64_t outer = batch * g.KV, slots = 256 * (hd == 32 ? 3 : hd == 64 ? 2 : 1);
+  KvPlan best{};
+  best.blocks = (g.T + kBlockRows - 1) / kBlockRows;
+  best.sink_blocks = std::min((g.sinks + kBlockRows - 1) / kBlockRows, best.blocks);
+  // steps of the first block without sinks (no later one has more), and of the very first
+  const int near = best.sink_blocks < best.blocks
+                       ? group * query_tiles(g, best.sink_blocks * kBlockRows) : 0;
+  const int most = group * query_tiles(g, 0);
+  double least = 0;
+  for (int chunks = 1; chunks == 1 || (chunks <= 64 && chunks <= std::max(near, most) / kLeastSteps);
+       ++chunks) {
+    KvPlan p = best;
+    p.near_len = near ? (near + chunks - 1) / chunks : 1;
+    p.near_chunks = near ? (near + p.near_len - 1) / p.near_len : 1;
+    p.sink_len = p.sink_chunks = 1;
+    if (p.sink_blocks) {
+      int64_t len = std::max(near ? p.near_len : (most + chunks - 1) / chunks, kLeastSteps);
+      len = std::max(len, (outer * p.sink_blocks * most + kMostUnits - 1) / kMostUnits);
+      p.sink_len = (int)std::min<int64_t>(len, most);
+      p.sink_chunks = (most + p.sink_len - 1) / p.sink_len;
+    }
+    const int64_t rounds = (outer * p.units() + slots - 1) / slots;
+    double steps = (double)rounds * (std::max(near ? p.near_len : 0, p.sink_blocks ? p.sink_len : 0) + 3);
+    if (p.near_chunks > 1 || p.sink_chunks > 1) {
+      const int64_t cut = (p.near_chunks > 1 ? (p.blocks - p.sink_blocks) * p.near_chunks : 0) +
+                          (p.sink_chunks > 1 ? p.sink_blocks * p.sink_chunks : 0);
+      steps += 2 + (double)(outer * cut) * 2 * kBlockRows * hd * 4 * 2 / 4e12 / 2e-6;
+    }
+    if (chunks == 1 || steps < least) {
+      least = steps;
+      best.near_len = p.near_len, best.near_chunks = p.near_chunks;
+      best.sink_len = p.sink_len, best.sink_chunks = p.sink_chunks;
+    }
   }
-  return p;
+  return best;
 }
 
 int64_t partial_bytes(const KvPlan& p, int64_t outer, int64_t hd) {
@@ -709,22 +758,24 @@ Geometry geometry(int64_t seq, int64_t heads, int64_t kv, int64_t window, int64_
 }
 
 template <typename E, int HD>
-int launch_fwd(const void* qkv, int64_t batch, const Geometry& g, void* out, float* lse,
-               hipStream_t s) {
+int launch_fwd(const void* qkv, int64_t batch, const Geometry& g, void* out, void* rest,
+               float* lse, hipStream_t s) {
   const int n_qt = (g.T + kBlockRows - 1) / kBlockRows;
   const float c = (float)(1.4426950408889634 / std::sqrt((double)HD));
-  hipLaunchKernelGGL((wattn_fwd_k<E, HD>), dim3((unsigned)(n_qt * batch * g.H)), dim3(kThreads), 0,
-                     s, static_cast<const E*>(qkv), static_cast<E*>(out), lse, g, n_qt, c);
+  const dim3 grid((unsigned)(n_qt * batch * g.H)), block(kThreads);
+  const E* x = static_cast<const E*>(qkv);
+  E *o = static_cast<E*>(out), *r = static_cast<E*>(rest);
+  hipLaunchKernelGGL((wattn_fwd_k<E, HD>), grid, block, 0, s, x, o, r, lse, g, n_qt, c);
   return rv_host::check_launch();
 }
 
 template <typename E, int HD>
-int launch_bwd(const void* qkv, const void* out, const void* dout, const float* lse,
-               int64_t batch, const Geometry& g, void* dqkv, float* ws, hipStream_t s) {
+int launch_bwd(const void* qkv, const void* out, const void* rest, const void* dout,
+               const float* lse, int64_t batch, const Geometry& g, void* dqkv, float* ws, hipStream_t s) {
   const int n_qt = (g.T + kBlockRows - 1) / kBlockRows;
   const double scale = 1.0 / std::sqrt((double)HD);
   const float c = (float)(1.4426950408889634 * scale);
-  const KvPlan plan = kv_plan(g, batch);
+  const KvPlan plan = kv_plan(g, batch, HD);
   const int64_t rows = batch * g.H * g.T;
   float* delta = ws;
   float* part = ws + (rows + 3) / 4 * 4;
@@ -733,8 +784,8 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
   E* dx = static_cast<E*>(dqkv);
   // the dQ kernel writes delta, which the dK/dV kernel reads
   hipLaunchKernelGGL((wattn_bwd_q_k<E, HD>), dim3((unsigned)(n_qt * batch * g.H)), dim3(kThreads),
-                     0, s, x, static_cast<const E*>(out), go, lse, delta, dx, g, n_qt, c,
-                     (float)scale);
+                     0, s, x, static_cast<const E*>(out), static_cast<const E*>(rest), go, lse,
+                     delta, dx, g, n_qt, c, (float)scale);
   int rc = rv_host::check_launch();
   if (rc != RV_OK) return rc;
   hipLaunchKernelGGL((wattn_bwd_kv_k<E, HD>), dim3((unsigned)(plan.units() * batch * g.KV)),
@@ -758,21 +809,22 @@ extern "C" {
 
 int rv_window_attn_fwd(const void* qkv, int64_t batch, int64_t seq, int64_t heads,
                        int64_t kv_heads, int64_t head_dim, int dtype, int64_t window,
-                       int64_t sinks, void* out, float* lse, void* stream) {
+                       int64_t sinks, void* out, void* rest, float* lse, void* stream) {
   if (!qkv || !out || !lse) return RV_ERR_NULL_POINTER;
   if (!args_ok(batch, seq, heads, kv_heads, head_dim, window, sinks)) return RV_ERR_BAD_SIZE;
   if (!sizes_ok(batch, seq, heads, kv_heads, head_dim, dtype)) return RV_ERR_UNSUPPORTED;
-  if (!rv_host::aligned16(qkv) || !rv_host::aligned16(out)) return RV_ERR_UNSUPPORTED;
+  if (!rv_host::aligned16(qkv) || !rv_host::aligned16(out) || !rv_host::aligned16(rest))
+    return RV_ERR_UNSUPPORTED;
   const Geometry g = geometry(seq, heads, kv_heads, window, sinks);
   const hipStream_t s = (hipStream_t)stream;
   if (dtype == RV_F16) {
-    if (head_dim == 32) return launch_fwd<_Float16, 32>(qkv, batch, g, out, lse, s);
-    if (head_dim == 64) return launch_fwd<_Float16, 64>(qkv, batch, g, out, lse, s);
-    return launch_fwd<_Float16, 128>(qkv, batch, g, out, lse, s);
+    if (head_dim == 32) return launch_fwd<_Float16, 32>(qkv, batch, g, out, rest, lse, s);
+    if (head_dim == 64) return launch_fwd<_Float16, 64>(qkv, batch, g, out, rest, lse, s);
+    return launch_fwd<_Float16, 128>(qkv, batch, g, out, rest, lse, s);
   }
-  if (head_dim == 32) return launch_fwd<__bf16, 32>(qkv, batch, g, out, lse, s);
-  if (head_dim == 64) return launch_fwd<__bf16, 64>(qkv, batch, g, out, lse, s);
-  return launch_fwd<__bf16, 128>(qkv, batch, g, out, lse, s);
+  if (head_dim == 32) return launch_fwd<__bf16, 32>(qkv, batch, g, out, rest, lse, s);
+  if (head_dim == 64) return launch_fwd<__bf16, 64>(qkv, batch, g, out, rest, lse, s);
+  return launch_fwd<__bf16, 128>(qkv, batch, g, out, rest, lse, s);
 }
 
 int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
@@ -780,19 +832,19 @@ int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t h
                                            int64_t sinks) {
   if (!args_ok(batch, seq, heads, kv_heads, head_dim, window, sinks)) return -RV_ERR_BAD_SIZE;
   if (!sizes_ok(batch, seq, heads, kv_heads, head_dim, RV_F16)) return -RV_ERR_UNSUPPORTED;
-  const KvPlan p = kv_plan(geometry(seq, heads, kv_heads, window, sinks), batch);
+  const KvPlan p = kv_plan(geometry(seq, heads, kv_heads, window, sinks), batch, head_dim);
   return (batch * heads * seq + 3) / 4 * 16 + partial_bytes(p, batch * kv_heads, head_dim);
 }
 
-int rv_window_attn_bwd(const void* qkv, const void* out, const void* dout, const float* lse,
-                       int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
+int rv_window_attn_bwd(const void* qkv, const void* out, const void* rest, const void* dout,
+                       const float* lse, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
                        int64_t head_dim, int dtype, int64_t window, int64_t sinks, void* dqkv,
                        void* workspace, int64_t workspace_bytes, void* stream) {
   if (!qkv || !out || !dout || !lse || !dqkv) return RV_ERR_NULL_POINTER;
   if (!args_ok(batch, seq, heads, kv_heads, head_dim, window, sinks)) return RV_ERR_BAD_SIZE;
   if (!sizes_ok(batch, seq, heads, kv_heads, head_dim, dtype)) return RV_ERR_UNSUPPORTED;
   if (!rv_host::aligned16(qkv) || !rv_host::aligned16(out) || !rv_host::aligned16(dout) ||
-      !rv_host::aligned16(dqkv) || !rv_host::aligned16(workspace))
+      !rv_host::aligned16(dqkv) || !rv_host::aligned16(rest) || !rv_host::aligned16(workspace))
     return RV_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < rv_window_attn_bwd_workspace_bytes(
                                           batch, seq, heads, kv_heads, head_dim, window, sinks))
@@ -801,13 +853,13 @@ int rv_window_attn_bwd(const void* qkv, const void* out, const void* dout, const
   const hipStream_t s = (hipStream_t)stream;
   float* ws = static_cast<float*>(workspace);
   if (dtype == RV_F16) {
-    if (head_dim == 32) return launch_bwd<_Float16, 32>(qkv, out, dout, lse, batch, g, dqkv, ws, s);
-    if (head_dim == 64) return launch_bwd<_Float16, 64>(qkv, out, dout, lse, batch, g, dqkv, ws, s);
-    return launch_bwd<_Float16, 128>(qkv, out, dout, lse, batch, g, dqkv, ws, s);
+    if (head_dim == 32) return launch_bwd<_Float16, 32>(qkv, out, rest, dout, lse, batch, g, dqkv, ws, s);
+    if (head_dim == 64) return launch_bwd<_Float16, 64>(qkv, out, rest, dout, lse, batch, g, dqkv, ws, s);
+    return launch_bwd<_Float16, 128>(qkv, out, rest, dout, lse, batch, g, dqkv, ws, s);
   }
-  if (head_dim == 32) return launch_bwd<__bf16, 32>(qkv, out, dout, lse, batch, g, dqkv, ws, s);
-  if (head_dim == 64) return launch_bwd<__bf16, 64>(qkv, out, dout, lse, batch, g, dqkv, ws, s);
-  return launch_bwd<__bf16, 128>(qkv, out, dout, lse, batch, g, dqkv, ws, s);
+  if (head_dim == 32) return launch_bwd<__bf16, 32>(qkv, out, rest, dout, lse, batch, g, dqkv, ws, s);
+  if (head_dim == 64) return launch_bwd<__bf16, 64>(qkv, out, rest, dout, lse, batch, g, dqkv, ws, s);
+  return launch_bwd<__bf16, 128>(qkv, out, rest, dout, lse, batch, g, dqkv, ws, s);
 }
 
 }  // extern "C"

@@ -150,7 +150,7 @@ def test_entry_points_validate_without_device():
     lib = _hip.library()
     fake, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
     half, f32 = _hip.RV_F16, _hip.RV_F32
-    fwd = lambda *a: lib.rv_window_attn_fwd(*a, None)
+    fwd = lambda *a: lib.rv_window_attn_fwd(*a[:-1], None, a[-1], None)
     assert fwd(None, 1, 8, 2, 1, 32, half, 4, 0, fake, fake) == 1
     assert fwd(fake, 1, 0, 2, 1, 32, half, 4, 0, fake, fake) == 2
     assert fwd(fake, 1, 8, 2, 1, 32, half, 0, 0, fake, fake) == 2
@@ -164,7 +164,7 @@ def test_entry_points_validate_without_device():
     assert need >= 300 * 4 * 4
     assert lib.rv_window_attn_bwd_workspace_bytes(1, 300, 4, 2, 64, 0, 4) == -2
     assert lib.rv_window_attn_bwd_workspace_bytes(1, 300, 4, 3, 64, 8, 4) == -3
-    bwd = lambda ws, n: lib.rv_window_attn_bwd(fake, fake, fake, fake, 1, 300, 4, 2, 64, half, 32,
+    bwd = lambda ws, n: lib.rv_window_attn_bwd(fake, fake, None, fake, fake, 1, 300, 4, 2, 64, half, 32,
                                                4, fake, ws, n, None)
     assert bwd(None, need) == 4 and bwd(fake, need - 1) == 4 and bwd(odd, need) == 3
     turn = lambda src, tokens, rows, table: lib.rv_rotate_qkv(
