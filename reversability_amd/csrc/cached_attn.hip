@@ -29,6 +29,7 @@
 // page that does not exist) are taken as zeros and their scores as -inf, whatever the cache holds.
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "attn_tile.h"
@@ -123,6 +124,21 @@ __device__ __forceinline__ float row_sum(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
                                                   false);
   return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// The position of the token at slot `key`: a drafted one's goes by its mask.
+__device__ __forceinline__ int position_of(const Cached& a, const View& w, int key) {
+  if (key < w.context || key - w.context >= w.n) return key;
+  const uint64_t bits = w.n < 64 ? (uint64_t(1) << w.n) - 1 : ~uint64_t(0);
+  return w.context + __popcll((uint64_t)a.tree[w.start + key - w.context] & bits) - 1;
+}
+
+// Whether a row sees the slot `key` as far as order goes: up to its own (limit), or the context and what
+// its mask has.  Without branches: it is asked for every element of a tile at an edge.
+__device__ __forceinline__ bool in_order(bool tree, int context, int key, int limit,
+                                         uint64_t mask) {
+  if (!tree) return key <= limit;
+  return (key < context) | ((mask >> ((key - context) & 63) & 1) != 0);
 }
 
 // Half index of element (r, col) of a V tile [32][HD]: pairs of 16-byte chunks XOR-swizzled so that
@@ -245,6 +261,7 @@ void cached_few_k(Cached a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  const int reach = a.window ? a.window : INT_MAX;
   // slots below `below` are seen by every row as far as order goes, from `from` on as far as the
   // window goes
   const int below = a.tree ? w.context : w.context + w.i0 + 1;
@@ -293,22 +310,13 @@ void cached_few_k(Cached a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int key = k0 + g * 16 + hl * 4 + j;
-          const bool there = now.whole || (now.seen[g] && key < w.hi);
-          int kp = key;  // the key's position
-          if (a.tree && a.window && key >= w.context && key - w.context < w.n) {
-            const uint64_t bits = w.n < 64 ? (uint64_t(1) << w.n) - 1 : ~uint64_t(0);
-            kp = w.context + __popcll((uint64_t)a.tree[w.start + key - w.context] & bits) - 1;
-          }
+          const bool there = (now.seen[g] | now.whole) & (key < w.hi);
+          const int kp = a.tree && a.window ? position_of(a, w, key) : key;
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
-            bool sees = there;
-            if (a.tree) {
-              if (key >= w.context) sees = sees && (mask[r] >> ((key - w.context) & 63) & 1);
-            } else {
-              sees = sees && key <= limit[r];
-            }
-            if (a.window) sees = sees && (place[r] - kp < a.window || kp < a.sinks);
-            if (!sees) s[g][r][j] = -INFINITY;
+            const bool sees = there & in_order(a.tree != nullptr, w.context, key, limit[r], mask[r]) &
+                              ((place[r] - kp < reach) | (kp < a.sinks));
+            s[g][r][j] = sees ? s[g][r][j] : -INFINITY;
           }
         }
     }
@@ -494,7 +502,7 @@ __device__ __forceinline__ void many_rows(State<HD>& st, const E* Ks, const E* V
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     if constexpr (MASK) {
-      if (!sees(acc_row(j))) s[j] = -INFINITY;
+      s[j] = sees(acc_row(j)) ? s[j] : -INFINITY;
     }
     mx = fmaxf(mx, s[j]);
   }
@@ -639,20 +647,11 @@ void cached_many_k(Cached a) {
     }                                                                                           \
     __syncthreads();                                                                            \
   }
+  const int reach = a.window ? a.window : INT_MAX;
   auto sees = [&](int key, bool there) {
-    bool yes = there && key < w.hi;
-    int kp = key;
-    if (a.tree) {
-      if (key >= w.context) {
-        yes = yes && (mask >> ((key - w.context) & 63) & 1);
-        if (a.window && key - w.context < w.n)
-          kp = w.context + __popcll((uint64_t)a.tree[w.start + key - w.context] & bits) - 1;
-      }
-    } else {
-      yes = yes && key <= limit;
-    }
-    if (a.window) yes = yes && (place - kp < a.window || kp < a.sinks);
-    return yes;
+    const int kp = a.tree && a.window ? position_of(a, w, key) : key;
+    return there & (key < w.hi) & in_order(a.tree != nullptr, w.context, key, limit, mask) &
+           ((place - kp < reach) | (kp < a.sinks));
   };
   for (int v = v0; v < v_end; ++v) {
     RV_MANY_STEP(0)

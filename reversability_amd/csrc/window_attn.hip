@@ -20,9 +20,15 @@
 // dK/dV: a key block's work is (heads that share it) x (tiles of queries).  It is cut into
 // chunks where a block alone would take much longer than the rest (the sinks' block
 // sees the whole sequence) or where there are few blocks; a chunk writes fp32 partials
-// and wattn_reduce_k adds them in order.  The sinks' sums are long and their terms large: there
-// P and dS are taken with what their roundings left, by twice the products (of 16384 queries'
-// terms the roundings alone were half as large as the other keys' gradients are).
+// and wattn_reduce_k adds them in order.
+//
+// P and dS are rounded to the type for the products they enter.  Where that shows it is made up
+// for by a second product with what the rounding left (REST): for the first 128 queries, which see
+// few keys with large weights, and the keys of the first block and of the sinks, whose sums are
+// long and of large terms (16384 queries' roundings were half as large as other keys' gradients).
+// Of every output the forward also keeps what its rounding left (rest), for D = rowsum(dO O).
+// Error of the gradients relative to that of the final rounding alone: without all this 1.5
+// to 2.1, with it 1.0 to 1.3, at a few percent of the time.
 
 #include <algorithm>
 #include <cmath>
@@ -95,6 +101,15 @@ struct KeySight {
   __device__ __forceinline__ bool operator()(int r) const { return (unsigned)(at + r) < reach; }
 };
 
+// What the rounding of values 8 h .. 8 h + 7 of an accumulator to `r` left, rounded in its turn.
+template <typename E>
+__device__ __forceinline__ x8<E> rest8(const f32x16& v, const x8<E>& r, int h) {
+  x8<E> left;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) left[i] = (E)(v[8 * h + i] - (float)r[i]);
+  return left;
+}
+
 template <int HD>
 struct FwdState {
   f32x16 o[HD / 32];
@@ -103,9 +118,8 @@ struct FwdState {
 
 // 32 keys (rows sub * 32 .. of the tile) for one wave's 32 queries.  MASK: some of them are not
 // seen by some query; q, k0: the lane's query and the first of the keys.
-// P's roundings are made up for by a second product with what they left: the output is then known to
-// more digits than its type has, which the backward's dO . O needs (rest).
-template <typename E, int HD, bool MASK>
+// REST: what P's roundings left is added by a product of its own.
+template <typename E, int HD, bool MASK, bool REST>
 __device__ __forceinline__ void fwd_rows(FwdState<HD>& st, const E* Ks, const E* Vs,
                                          const FragOffsets<HD, E>& fo, const x8<E> (&qf)[HD / 16],
                                          const Geometry& g, int sub, int q, int k0, float c,
@@ -162,24 +176,22 @@ __device__ __forceinline__ void fwd_rows(FwdState<HD>& st, const E* Ks, const E*
   for (int cc = 0; cc < 2; ++cc) {
     const x8<E> pf = pack8<E>(s, cc);
     x8<E> left;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) left[i] = (E)(s[8 * cc + i] - (float)pf[i]);
+    if constexpr (REST) left = rest8<E>(s, pf, cc);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (!kReadAhead<HD>) vf[cc][dt] = fo.trf(Vs, sub, cc, dt);
       st.o[dt] = mfma(vf[cc][dt], pf, st.o[dt]);
-      st.o[dt] = mfma(vf[cc][dt], left, st.o[dt]);
+      if constexpr (REST) st.o[dt] = mfma(vf[cc][dt], left, st.o[dt]);
     }
   }
 }
 
-template <typename E, int HD>
-__global__ __launch_bounds__(kThreads, kFwdMinBlocks<HD>)
-void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__ rest,
-                 float* __restrict__ lse, Geometry g, int n_qt, float c) {
+template <typename E, int HD, bool REST>
+__device__ __forceinline__ void fwd_block(const E* __restrict__ qkv, E* __restrict__ out,
+                                          E* __restrict__ rest, float* __restrict__ lse,
+                                          const Geometry& g, int bh, int qt, float c,
+                                          E (&lds)[2][2][kTile * HD]) {
   constexpr int KK = HD / 16, DT = HD / 32;
-  __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];
-  const int at = near_index(), bh = at / n_qt, qt = at % n_qt;
   const int b = bh / g.H, h = bh % g.H, kvh = h / (g.H / g.KV);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
   const int64_t rs = (int64_t)(g.H + 2 * g.KV) * HD;
@@ -225,9 +237,11 @@ void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__
       const int ks = k0 + sub * 32;                                                          \
       if (none_seen(g, q0, ks, 32)) continue;                                                \
       if (all_seen(g, q0, ks, 32))                                                           \
-        fwd_rows<E, HD, false>(st, lds[BUF][0], lds[BUF][1], fo, qf, g, sub, q, ks, c, lane); \
+        fwd_rows<E, HD, false, REST>(st, lds[BUF][0], lds[BUF][1], fo, qf, g, sub, q, ks, c, \
+                                     lane);                                                  \
       else                                                                                   \
-        fwd_rows<E, HD, true>(st, lds[BUF][0], lds[BUF][1], fo, qf, g, sub, q, ks, c, lane); \
+        fwd_rows<E, HD, true, REST>(st, lds[BUF][0], lds[BUF][1], fo, qf, g, sub, q, ks, c,  \
+                                    lane);                                                   \
     }                                                                                        \
     if (more) {                                                                              \
       ck.store(lds[1 - (BUF)][0]);                                                           \
@@ -264,11 +278,22 @@ void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__
   }
 }
 
+template <typename E, int HD>
+__global__ __launch_bounds__(kThreads, kFwdMinBlocks<HD>)
+void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__ rest,
+                 float* __restrict__ lse, Geometry g, int n_qt, float c) {
+  __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];
+  const int at = near_index(), bh = at / n_qt, qt = at % n_qt;
+  if (qt == 0) fwd_block<E, HD, true>(qkv, out, rest, lse, g, bh, qt, c, lds);
+  else fwd_block<E, HD, false>(qkv, out, rest, lse, g, bh, qt, c, lds);
+}
+
 // ---------------------------------------------------------------------------
 // Backward.
 // ---------------------------------------------------------------------------
-// dQ contribution of 32 staged keys to one wave's 32 queries (lanes).
-template <typename E, int HD, bool MASK>
+// dQ contribution of 32 staged keys to one wave's 32 queries (lanes).  REST: what the roundings of dS
+// left is added by a product of its own.
+template <typename E, int HD, bool MASK, bool REST>
 __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const E* Vs,
                                        const FragOffsets<HD, E>& fo, const x8<E> (&qf)[HD / 16],
                                        const x8<E> (&gf)[HD / 16], const Geometry& g, float Lq,
@@ -306,23 +331,32 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc) {
     const x8<E> dsf = pack8<E>(dp, cc);
+    x8<E> left;
+    if constexpr (REST) left = rest8<E>(dp, dsf, cc);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       kt[cc][dt] = fo.trf(Ks, sub, cc, dt);
       dq[dt] = mfma(kt[cc][dt], dsf, dq[dt]);
+      if constexpr (REST) dq[dt] = mfma(kt[cc][dt], left, dq[dt]);
     }
   }
 }
 
-template <typename E, int HD>
+// The first blocks of queries and the others in one launch or, at HD >= 64, where the first ones' products
+// cost the others registers, in two (at HD = 128 559 us against 1170 in one).
+enum Part { kAll, kFirst, kOthers };
+
+template <typename E, int HD, Part PART>
 __global__ __launch_bounds__(kThreads, kQMinBlocks<HD>)
 void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
-                   const E* __restrict__ rest, const E* __restrict__ dout, const float* __restrict__ lse,
-                   float* __restrict__ delta, E* __restrict__ dqkv, Geometry g, int n_qt, float c,
-                   float scale) {
+                   const E* __restrict__ rest, const E* __restrict__ dout,
+                   const float* __restrict__ lse, float* __restrict__ delta, E* __restrict__ dqkv,
+                   Geometry g, int n_qt, float c, float scale) {
   constexpr int KK = HD / 16, DT = HD / 32;
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][K / V]
-  const int at = near_index(), bh = at / n_qt, qt = at % n_qt;
+  const int per = PART == kFirst ? 1 : PART == kOthers ? n_qt - 1 : n_qt;
+  const int number = near_index(), bh = number / per, qt = number % per + (PART == kOthers);
+  const bool first = PART == kFirst || (PART == kAll && qt == 0);
   const int b = bh / g.H, h = bh % g.H, kvh = h / (g.H / g.KV);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
   const int64_t rs = (int64_t)(g.H + 2 * g.KV) * HD, os = (int64_t)g.H * HD;
@@ -380,12 +414,15 @@ void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
     _Pragma("unroll") for (int sub = 0; sub < 2; ++sub) {                                     \
       const int ks = k0 + sub * 32;                                                           \
       if (none_seen(g, q0, ks, 32)) continue;                                                 \
-      if (all_seen(g, q0, ks, 32))                                                            \
-        q_rows<E, HD, false>(dq, lds[BUF][0], lds[BUF][1], fo, qf, gf, g, Lq, Dq, sub, q, ks, \
-                             c, lane);                                                        \
-      else                                                                                    \
-        q_rows<E, HD, true>(dq, lds[BUF][0], lds[BUF][1], fo, qf, gf, g, Lq, Dq, sub, q, ks,  \
-                            c, lane);                                                         \
+      if (first)                                                                               \
+        q_rows<E, HD, true, PART != kOthers>(dq, lds[BUF][0], lds[BUF][1], fo, qf, gf, g, Lq,  \
+                                             Dq, sub, q, ks, c, lane);                         \
+      else if (all_seen(g, q0, ks, 32))                                                        \
+        q_rows<E, HD, false, false>(dq, lds[BUF][0], lds[BUF][1], fo, qf, gf, g, Lq, Dq, sub,  \
+                                    q, ks, c, lane);                                           \
+      else                                                                                     \
+        q_rows<E, HD, true, false>(dq, lds[BUF][0], lds[BUF][1], fo, qf, gf, g, Lq, Dq, sub,   \
+                                   q, ks, c, lane);                                            \
     }                                                                                         \
     if (more) {                                                                               \
       ck.store(lds[1 - (BUF)][0]);                                                            \
@@ -471,11 +508,8 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
     const x8<E> pf = pack8<E>(s, cc), dsf = pack8<E>(dp, cc);
     x8<E> pl, dsl;
     if constexpr (REST) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        pl[i] = (E)(s[8 * cc + i] - (float)pf[i]);
-        dsl[i] = (E)(dp[8 * cc + i] - (float)dsf[i]);
-      }
+      pl = rest8<E>(s, pf, cc);
+      dsl = rest8<E>(dp, dsf, cc);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
@@ -494,7 +528,7 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
 }
 
 // How the dK/dV work of one (sequence, key head) is cut into chunks: key blocks
-// [0, sink_blocks) hold sinks and take sink_chunks of sink_len steps each, the rest
+// [0, sink_blocks), the first and those that hold sinks, take sink_chunks of sink_len steps each, the rest
 // near_chunks of near_len.  A step is one tile of queries of one head that shares the keys.
 struct KvPlan {
   int blocks, sink_blocks;
@@ -513,23 +547,21 @@ __host__ __device__ inline int query_tiles(const Geometry& g, int kbase) {
   return (int)((end - kbase + kTile - 1) / kTile);
 }
 
-template <typename E, int HD>
-__global__ __launch_bounds__(kThreads, kKvMinBlocks<HD>)
-void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
-                    const float* __restrict__ lse, const float* __restrict__ delta,
-                    E* __restrict__ dqkv, float* __restrict__ part, Geometry g, KvPlan plan,
-                    float c, float scale) {
+// One unit of the plan, of the sinks' blocks (SINK) or of the others.
+template <typename E, int HD, bool SINK>
+__device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __restrict__ dout,
+                                        const float* __restrict__ lse,
+                                        const float* __restrict__ delta, E* __restrict__ dqkv,
+                                        float* __restrict__ part, const Geometry& g,
+                                        const KvPlan& plan, int number, float c, float scale,
+                                        E (&lds)[2][2][kTile * HD], float (&rowv)[2][2][kTile]) {
   constexpr int KK = HD / 16, DT = HD / 32;
-  __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][Q / dO]
-  __shared__ __attribute__((aligned(16))) float rowv[2][2][kTile];  // [buf][lse / delta]
   const int units = plan.units();
-  const int number = near_index(), bkv = number / units, unit = number % units;
-  const int sink_units = plan.sink_blocks * plan.sink_chunks;
-  const bool sink = unit < sink_units;
-  const int chunks = sink ? plan.sink_chunks : plan.near_chunks;
-  const int len = sink ? plan.sink_len : plan.near_len;
-  const int at = sink ? unit : unit - sink_units;
-  const int kt = at / chunks + (sink ? 0 : plan.sink_blocks), chunk = at % chunks;
+  const int bkv = number / units, unit = number % units;
+  const int chunks = SINK ? plan.sink_chunks : plan.near_chunks;
+  const int len = SINK ? plan.sink_len : plan.near_len;
+  const int at = SINK ? unit : unit - plan.sink_blocks * plan.sink_chunks;
+  const int kt = at / chunks + (SINK ? 0 : plan.sink_blocks), chunk = at % chunks;
   const int b = bkv / g.KV, kvh = bkv % g.KV, group = g.H / g.KV;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
   const int64_t rs = (int64_t)(g.H + 2 * g.KV) * HD, os = (int64_t)g.H * HD;
@@ -591,7 +623,7 @@ void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
     _Pragma("unroll") for (int sub = 0; sub < 2; ++sub) {                                     \
       const int qs = qt0 + sub * 32;                                                          \
       if (none_seen(g, qs, k0w, kWaveRows)) continue;                                         \
-      if (sink)                                                                                \
+      if constexpr (SINK)                                                                      \
         kv_rows<E, HD, true, true>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],             \
                                    rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);        \
       else if (all_seen(g, qs, k0w, kWaveRows))                                                \
@@ -647,6 +679,22 @@ void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
     }
 }
 
+template <typename E, int HD>
+__global__ __launch_bounds__(kThreads, kKvMinBlocks<HD>)
+void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
+                    const float* __restrict__ lse, const float* __restrict__ delta,
+                    E* __restrict__ dqkv, float* __restrict__ part, Geometry g, KvPlan plan,
+                    float c, float scale) {
+  __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][Q / dO]
+  __shared__ __attribute__((aligned(16))) float rowv[2][2][kTile];  // [buf][lse / delta]
+  const int number = near_index();
+  if (number % plan.units() < plan.sink_blocks * plan.sink_chunks)
+    kv_unit<E, HD, true>(qkv, dout, lse, delta, dqkv, part, g, plan, number, c, scale, lds, rowv);
+  else
+    kv_unit<E, HD, false>(qkv, dout, lse, delta, dqkv, part, g, plan, number, c, scale, lds,
+                          rowv);
+}
+
 // Sums of the chunks' partials, in order.  One workgroup = 32 rows of one cut key
 // block and side (K / V); grid (8 * cut blocks, B * KV), the cut blocks being the sinks', the
 // others, or all.
@@ -684,7 +732,8 @@ void wattn_reduce_k(const float* __restrict__ part, E* __restrict__ dqkv, Geomet
 
 // Steps that a chunk has at least, and the most that the sinks' blocks are cut into (their
 // partials' memory).
-constexpr int kLeastSteps = 8;
+constexpr int kLeastSteps = 4;
+constexpr double kSinkStep = 1.6;  // steps of other blocks that one of the sinks' takes as long as
 constexpr int kMostUnits = 4096;
 
 // Chunks that the other blocks are cut into: of the plans with 1, 2, 3 .. the one that takes the fewest
@@ -697,32 +746,36 @@ KvPlan kv_plan(const Geometry& g, int64_t batch, int64_t hd) {
   const int64_t outer = batch * g.KV, slots = 256 * (hd == 32 ? 3 : hd == 64 ? 2 : 1);
   KvPlan best{};
   best.blocks = (g.T + kBlockRows - 1) / kBlockRows;
-  best.sink_blocks = std::min((g.sinks + kBlockRows - 1) / kBlockRows, best.blocks);
+  best.sink_blocks = std::min(std::max(1, (g.sinks + kBlockRows - 1) / kBlockRows), best.blocks);
   // steps of the first block without sinks (no later one has more), and of the very first
   const int near = best.sink_blocks < best.blocks
                        ? group * query_tiles(g, best.sink_blocks * kBlockRows) : 0;
   const int most = group * query_tiles(g, 0);
   double least = 0;
-  for (int chunks = 1; chunks == 1 || (chunks <= 64 && chunks <= std::max(near, most) / kLeastSteps);
-       ++chunks) {
+  // (odd: the sinks' chunks shorter by the time that a step of theirs takes longer)
+  for (int i = 2; i < 4 || (i < 130 && i / 2 <= std::max(near, most) / kLeastSteps); ++i) {
+    const int chunks = i / 2;
     KvPlan p = best;
     p.near_len = near ? (near + chunks - 1) / chunks : 1;
     p.near_chunks = near ? (near + p.near_len - 1) / p.near_len : 1;
     p.sink_len = p.sink_chunks = 1;
     if (p.sink_blocks) {
-      int64_t len = std::max(near ? p.near_len : (most + chunks - 1) / chunks, kLeastSteps);
+      int64_t len = near ? p.near_len : (most + chunks - 1) / chunks;
+      if (i & 1) len = (int64_t)(len / kSinkStep);
+      len = std::max<int64_t>(len, kLeastSteps);
       len = std::max(len, (outer * p.sink_blocks * most + kMostUnits - 1) / kMostUnits);
       p.sink_len = (int)std::min<int64_t>(len, most);
       p.sink_chunks = (most + p.sink_len - 1) / p.sink_len;
     }
     const int64_t rounds = (outer * p.units() + slots - 1) / slots;
-    double steps = (double)rounds * (std::max(near ? p.near_len : 0, p.sink_blocks ? p.sink_len : 0) + 3);
+    double steps = (double)rounds * (std::max(near ? (double)p.near_len : 0.0,
+                                              p.sink_blocks ? kSinkStep * p.sink_len : 0.0) + 3);
     if (p.near_chunks > 1 || p.sink_chunks > 1) {
       const int64_t cut = (p.near_chunks > 1 ? (p.blocks - p.sink_blocks) * p.near_chunks : 0) +
                           (p.sink_chunks > 1 ? p.sink_blocks * p.sink_chunks : 0);
       steps += 2 + (double)(outer * cut) * 2 * kBlockRows * hd * 4 * 2 / 4e12 / 2e-6;
     }
-    if (chunks == 1 || steps < least) {
+    if (i == 2 || steps < least) {
       least = steps;
       best.near_len = p.near_len, best.near_chunks = p.near_chunks;
       best.sink_len = p.sink_len, best.sink_chunks = p.sink_chunks;
@@ -783,9 +836,19 @@ int launch_bwd(const void* qkv, const void* out, const void* rest, const void* d
   const E* go = static_cast<const E*>(dout);
   E* dx = static_cast<E*>(dqkv);
   // the dQ kernel writes delta, which the dK/dV kernel reads
-  hipLaunchKernelGGL((wattn_bwd_q_k<E, HD>), dim3((unsigned)(n_qt * batch * g.H)), dim3(kThreads),
-                     0, s, x, static_cast<const E*>(out), static_cast<const E*>(rest), go, lse,
-                     delta, dx, g, n_qt, c, (float)scale);
+  const int64_t bh = batch * g.H;
+  auto queries = [&](auto kernel, int blocks) {
+    if (blocks)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * bh)), dim3(kThreads), 0, s, x,
+                         static_cast<const E*>(out), static_cast<const E*>(rest), go, lse, delta,
+                         dx, g, n_qt, c, (float)scale);
+  };
+  if constexpr (HD >= 64) {
+    queries(wattn_bwd_q_k<E, HD, kFirst>, 1);
+    queries(wattn_bwd_q_k<E, HD, kOthers>, n_qt - 1);
+  } else {
+    queries(wattn_bwd_q_k<E, HD, kAll>, n_qt);
+  }
   int rc = rv_host::check_launch();
   if (rc != RV_OK) return rc;
   hipLaunchKernelGGL((wattn_bwd_kv_k<E, HD>), dim3((unsigned)(plan.units() * batch * g.KV)),
