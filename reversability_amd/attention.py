@@ -307,9 +307,11 @@ class Rotary:
                              "base > 0")
         self.head_dim, self.positions = head_dim, positions
         self.base, self.interleaved = float(base), bool(interleaved)
-        rate = self.base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
-        angle = torch.arange(positions, dtype=torch.float64).unsqueeze(1) * rate
-        self.table = torch.stack([angle.cos(), angle.sin()], -1).float().to(device)
+        rate = self.base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64, device=device)
+                             / head_dim)
+        at = torch.arange(positions, dtype=torch.float64, device=device)
+        angle = at.unsqueeze(1) * rate
+        self.table = torch.stack([angle.cos(), angle.sin()], -1).float()
 
     def to(self, device) -> "Rotary":
         """A copy with its table on ``device``."""
