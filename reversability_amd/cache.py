@@ -257,14 +257,26 @@ class PagedCache:
 
     @torch.no_grad()
     def move(self, source: torch.Tensor, target: torch.Tensor) -> None:
-        """Copies the tokens at the slots ``source`` to the slots ``target`` (int64 [n], all of
-        the cache's slots; all are read before any is written) in every layer: what is kept of
-        a checked tree goes behind its context."""
-        size = self.page_size
-        if source.dtype != torch.int64 or source.shape != target.shape or source.ndim != 1:
-            raise ValueError("move needs two int64 lists of slots of one length")
-        for side in (self.keys, self.values):
-            side[:, target // size, :, target % size] = side[:, source // size, :, source % size]
+        """Copies the tokens at the slots ``source`` to the slots ``target`` (int64 [n]) in every
+        layer, all read before any is written: what is kept of a checked tree goes behind its
+        context.  A pair with a slot outside the cache (as ``cache_plan``'s -1) is passed over;
+        the others' targets must differ."""
+        layers, pages, kv, size, hd = self.keys.shape
+        n = _ints(source, tuple(source.shape), self.keys, "source", torch.int64).numel()
+        if source.ndim != 1:
+            raise ValueError("move needs lists of slots")
+        target = _ints(target, (n,), self.keys, "target", torch.int64)
+        _check_cache(self.keys[0], self.values[0], "move")
+        inside = (source >= 0) & (source < pages * size)
+        target = torch.where(inside, target, -1)
+        at = source.clamp(0, pages * size - 1)
+        page, row = at // size, at % size
+        # packed rows of kv heads each: queries (not read), keys, values
+        rows = torch.empty(layers, n, 3, kv, hd, device=self.keys.device, dtype=self.keys.dtype)
+        for i, side in ((1, self.keys), (2, self.values)):
+            rows[:, :, i] = side[:, page, :, row].transpose(0, 1)
+        for layer in range(layers if n else 0):
+            append_kv(rows[layer].view(n, -1), kv, self.keys[layer], self.values[layer], target)
 
 
 class CacheBatch(NamedTuple):

@@ -34,11 +34,13 @@ template <typename E>
 struct Vec;
 template <>
 struct Vec<_Float16> {
+  static constexpr unsigned kExponent = 0x7c00u;  // its bits
   typedef f16x8 x8;
   typedef f16x4 x4;
 };
 template <>
 struct Vec<__bf16> {
+  static constexpr unsigned kExponent = 0x7f80u;
   typedef b16x8 x8;
   typedef b16x4 x4;
 };

@@ -27,6 +27,7 @@
 //
 // Rows of V that no row of the workgroup sees (behind the last token, before the window, of a
 // page that does not exist) are taken as zeros and their scores as -inf, whatever the cache holds.
+// A token that only some rows see reaches those alone, also where it is not a number (exact_rows).
 
 #include <algorithm>
 #include <climits>
@@ -160,6 +161,98 @@ __device__ __forceinline__ int page_of(const Cached& a, const View& w, int b, in
   return page >= 0 && page < a.pages ? page : -1;
 }
 
+// Values that are not numbers, or infinite, in V of keys that some rows see and others do not: 0 times
+// them is NaN, and would reach rows that do not see them.  They are looked for in the tiles at an edge
+// alone, where masks are; a workgroup that meets one makes its rows again key by key (exact_rows).
+template <typename E>
+__device__ __forceinline__ bool finite(const x8<E>& v) {
+  constexpr unsigned kExp = Vec<E>::kExponent;
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  bool yes = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    yes = yes & ((w[i] & kExp) != kExp) & ((w[i] & (kExp << 16)) != (kExp << 16));
+  return yes;
+}
+
+// Where K and V of the token at slot `key` lie in the caches, -1 where there is none.
+template <int HD>
+__device__ __forceinline__ int64_t row_of(const Cached& a, const View& w, int b, int kvh, int key) {
+  const int page = page_of(a, w, b, key);
+  return page < 0 ? -1
+                  : ((((int64_t)page * a.KV + kvh) << a.page_shift) +
+                     (key & ((1 << a.page_shift) - 1))) * HD;
+}
+
+// The rows of a workgroup over its stretch [v0, v_end) of tiles of `keys` keys, one row a wave at a time:
+// lanes are keys for the scores, columns for the sums.  Slow, and seldom called.
+template <typename E, int HD>
+__device__ __forceinline__ void exact_rows(const Cached& a, const View& w, int b,
+                                                     int kvh, int row0, int rows, int split,
+                                                     int v0, int v_end, int keys) {
+  const int lane = threadIdx.x & 63, group = a.H / a.KV;
+  const uint64_t bits = w.n < 64 ? (uint64_t(1) << w.n) - 1 : ~uint64_t(0);
+  const int reach = a.window ? a.window : INT_MAX;
+  for (int row = row0 + (int)(threadIdx.x >> 6); row < row0 + rows; row += kWaves) {
+    const int token = row / group, head = kvh * group + row % group;
+    if (token >= w.n) return;
+    const uint64_t mask = a.tree ? (uint64_t)a.tree[w.start + token] & bits : 0;
+    const int limit = w.context + token;
+    const int place = a.tree ? w.context + __popcll(mask) - 1 : limit;
+    const E* q = static_cast<const E*>(a.q) + (int64_t)(w.start + token) * a.q_ld + head * HD;
+    float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
+    for (int v = v0; v < v_end; ++v) {
+      const int k0 = w.tile(v) * keys, key = k0 + lane;
+      int64_t at = -1;
+      if (lane < keys && key < w.hi && in_order(a.tree != nullptr, w.context, key, limit, mask)) {
+        const int kp = a.tree && a.window ? position_of(a, w, key) : key;
+        if (place - kp < reach || kp < a.sinks) at = row_of<HD>(a, w, b, kvh, key);
+      }
+      uint64_t seen = __ballot(at >= 0);
+      if (!seen) continue;
+      float s = 0.f;
+      for (int i = 0; i < HD; i += 8) {
+        const x8<E> x = *reinterpret_cast<const x8<E>*>(q + i);
+        const x8<E> y = *reinterpret_cast<const x8<E>*>(static_cast<const E*>(a.keys) +
+                                                        (at < 0 ? 0 : at) + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf((float)x[e], (float)y[e], s);
+      }
+      s = at < 0 ? -INFINITY : s * a.c;
+      float top = s;
+#pragma unroll
+      for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+      const float m_new = fmaxf(m, top);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+      const float p = at < 0 ? 0.f : __builtin_amdgcn_exp2f(s - m_new);
+      m = m_new;
+      l = l * alpha + rv::wave_sum(p);
+      o[0] *= alpha, o[1] *= alpha;
+      while (seen) {
+        const int k = __builtin_ctzll(seen);
+        seen &= seen - 1;
+        const float pk = (float)(E)__shfl(p, k);
+        const E* vr = static_cast<const E*>(a.values) + __shfl(at, k);
+        o[0] += pk * (float)vr[lane % HD];
+        if (HD == 128) o[1] += pk * (float)vr[64 + lane];
+      }
+    }
+    const int64_t to = (int64_t)(w.start + token) * a.H + head;
+    if (a.splits == 1 || w.count <= a.split_tiles) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      E* dst = static_cast<E*>(a.out) + to * HD;
+      if (lane < HD) dst[lane] = (E)(o[0] * inv);
+      if (HD == 128) dst[64 + lane] = (E)(o[1] * inv);
+    } else {
+      float* dst = a.part + (to * a.splits + split) * HD;
+      if (lane < HD) dst[lane] = o[0];
+      if (HD == 128) dst[64 + lane] = o[1];
+      float* stat = a.part + (int64_t)a.tokens * a.H * a.splits * HD + (to * a.splits + split) * 2;
+      if (lane == 0) stat[0] = m, stat[1] = l;
+    }
+  }
+}
+
 // K operands and V rows of one tile on their way through registers.
 template <typename E, int HD>
 struct Tile {
@@ -206,6 +299,12 @@ struct Tile {
     }
   }
   bool seen[2];
+  __device__ __forceinline__ bool odd() const {  // of the wave: some V is not finite
+    bool yes = true;
+#pragma unroll
+    for (int it = 0; it < VC; ++it) yes = yes & finite<E>(v[it]);
+    return __any(!yes);
+  }
   __device__ __forceinline__ void store_v(E* t, int lane) const {
 #pragma unroll
     for (int it = 0; it < VC; ++it) {
@@ -222,6 +321,7 @@ void cached_few_k(Cached a) {
   constexpr int kVBytes = kWaves * kKeys * HD * 2, kOBytes = 2 * R * HD * 4;
   __shared__ __attribute__((aligned(16))) char lds[kVBytes > kOBytes ? kVBytes : kOBytes];
   __shared__ float ml[2][kWaves][R];
+  __shared__ int odds[kWaves];
   const Place at(a);
   if (at.split >= a.splits) return;
   const int split = at.split, rb = at.rb, kvh = at.kvh, b = at.b;
@@ -274,6 +374,12 @@ void cached_few_k(Cached a) {
   const int last = a.tree ? w.context + w.n - 1 : w.context + w.i1;
   const int from = a.window ? last - a.window + 1 : 0;
 
+  auto sees = [&](int key, int r) {
+    const int kp = a.tree && a.window ? position_of(a, w, key) : key;
+    return (key < w.hi) & in_order(a.tree != nullptr, w.context, key, limit[r], mask[r]) &
+           ((place[r] - kp < reach) | (kp < a.sinks));
+  };
+
   E* vt = reinterpret_cast<E*>(lds) + wave * kKeys * HD;
   const int i = lane & 15;
   Tile<E, HD> next;
@@ -283,11 +389,13 @@ void cached_few_k(Cached a) {
     const int x = from_tile + (lane >> 1) * kWaves;
     return x < v_end ? page_of(a, w, b, w.tile(x) * kKeys + 16 * (lane & 1)) : -1;
   };
-  int ids = entries(v), ids_next = entries(v + 32 * kWaves), it = 0;
+  int ids = entries(v), ids_next = entries(v + 32 * kWaves), it = 0, odd = 0;
   if (v < v_end) next.load(a, w, kvh, ids, 0, w.tile(v) * kKeys, lane);
   for (; v < v_end; v += kWaves) {
     const int k0 = w.tile(v) * kKeys;
     const Tile<E, HD> now = next;
+    const bool plain = now.whole && k0 + kKeys <= below && (k0 >= from || k0 + kKeys <= a.sinks);
+    if (!plain && now.odd()) odd = 1;
     if (++it == 32) {
       it = 0;
       ids = ids_next;
@@ -309,21 +417,16 @@ void cached_few_k(Cached a) {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) s[g][r] = mfma16(now.k[g][kk], qf[r][kk], s[g][r]);
       }
-    const bool plain = now.whole && k0 + kKeys <= below && (k0 >= from || k0 + kKeys <= a.sinks);
     if (!plain) {
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int key = k0 + g * 16 + hl * 4 + j;
-          const bool there = (now.seen[g] | now.whole) & (key < w.hi);
-          const int kp = a.tree && a.window ? position_of(a, w, key) : key;
+          const bool there = now.seen[g] | now.whole;
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const bool sees = there & in_order(a.tree != nullptr, w.context, key, limit[r], mask[r]) &
-                              ((place[r] - kp < reach) | (kp < a.sinks));
-            s[g][r][j] = sees ? s[g][r][j] : -INFINITY;
-          }
+          for (int r = 0; r < NR; ++r)
+            s[g][r][j] = there & sees(key, r) ? s[g][r][j] : -INFINITY;
         }
     }
     bool up = false;
@@ -382,7 +485,12 @@ void cached_few_k(Cached a) {
       ml[1][wave][r * 16 + i] = l[r];
     }
   }
+  if (lane == 0) odds[wave] = odd;
   __syncthreads();  // (also: every wave is done with its V tile)
+  if (odds[0] | odds[1] | odds[2] | odds[3]) {
+    exact_rows<E, HD>(a, w, b, kvh, rb * R, R, split, split * a.split_tiles, v_end, kKeys);
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     all_m[r] = -INFINITY;
@@ -471,8 +579,9 @@ struct PagedCopy {
     }
   }
   // missing: the groups without a page; rows of V that no row of the workgroup sees become zeros.
-  __device__ __forceinline__ void store(E* ks, E* vs, const Cached& a, const View& w, int k0,
-                                        unsigned missing) {
+  // Returns whether at an edge some V that the thread holds is not finite.
+  __device__ __forceinline__ bool store(E* ks, E* vs, const Cached& a, const View& w, int k0,
+                                        unsigned missing, bool edge) {
     if (missing || k0 + kTile > w.hi || (k0 < w.lo && k0 + kTile > a.sinks)) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -481,12 +590,18 @@ struct PagedCopy {
           v[i] = u32x4{0, 0, 0, 0};
       }
     }
+    bool odd = false;
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) odd = odd | !finite<E>(__builtin_bit_cast(x8<E>, v[i]));
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = row(i), to = r * HD + (swz<HD>(r, chunk()) << 3);
       *reinterpret_cast<u32x4*>(ks + to) = k[i];
       *reinterpret_cast<u32x4*>(vs + to) = v[i];
     }
+    return odd;
   }
 };
 
@@ -574,6 +689,7 @@ __global__ __launch_bounds__(kThreads, 2)
 void cached_many_k(Cached a) {
   constexpr int KK = HD / 16, DT = HD / 32, kBlock = 16;  // kBlock: tiles of one load of entries
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];
+  __shared__ int odds[kWaves];
   const Place at(a);
   if (at.split >= a.splits) return;
   const View w(a, at.b, at.rb, kBlockRows, kTile);
@@ -630,9 +746,20 @@ void cached_many_k(Cached a) {
     missing = (unsigned)(__ballot(ids < 0) >> (4 * it)) & 15u;
     copy.load(kc, vc, a, at.kvh, ids, it, k0);
   };
+  // whether some row of the workgroup does not see some key of a tile, though another may
+  const int all_below = TREE ? w.context : w.context + w.i0 + 1;
+  const int all_from =
+      a.window ? (TREE ? w.context + w.n - 1 : w.context + w.i1) - a.window + 1 : 0;
+  auto edge = [&](int k0) {
+    return k0 + kTile > all_below || (k0 < all_from && k0 + kTile > a.sinks);
+  };
+  int odd = 0;
+  auto store = [&](int buf, int k0) {
+    if (__any(copy.store(lds[buf][0], lds[buf][1], a, w, k0, missing, edge(k0)))) odd = 1;
+  };
   if (v0 < v_end) {
     load(w.tile(v0) * kTile);
-    copy.store(lds[0][0], lds[0][1], a, w, w.tile(v0) * kTile, missing);
+    store(0, w.tile(v0) * kTile);
   }
   unsigned now = missing;
   __syncthreads();
@@ -652,24 +779,23 @@ void cached_many_k(Cached a) {
       const int ks = k0 + sub * 32;                                                             \
       if (!busy || ks >= end || (ks + 32 <= begin && ks >= a.sinks)) continue;                  \
       if (ks + 32 <= below && (ks >= from || ks + 32 <= a.sinks) && !(now >> (2 * sub) & 3u)) { \
-        many_rows<E, HD, false>(st, lds[BUF][0], lds[BUF][1], fo, qf, sub, a.c,                 \
-                                [](int) { return true; });                                      \
-      } else {                                                                                  \
-        const unsigned lost = now >> (2 * sub);                                                 \
-        many_rows<E, HD, true>(st, lds[BUF][0], lds[BUF][1], fo, qf, sub, a.c, [&](int r) {     \
-          return sees(ks + r + hl * 4, !(lost >> (r >> 4) & 1u));                               \
-        });                                                                                     \
-      }                                                                                         \
-    }                                                                                           \
+        many_rows<E, HD, false>(st, lds[BUF][0], lds[BUF][1], fo, qf, sub, a.c,                \
+                                [](int) { return true; });                                     \
+      } else {                                                                                 \
+        const unsigned lost = now >> (2 * sub);                                                \
+        many_rows<E, HD, true>(st, lds[BUF][0], lds[BUF][1], fo, qf, sub, a.c, [&](int r) {    \
+          return ((lost >> (r >> 4) & 1u) == 0) & sees(ks + r + hl * 4);                       \
+        });                                                                                    \
+      }                                                                                        \
+    }                                                                                          \
     now = missing;                                                                              \
-    if (more)                                                                                  \
-      copy.store(lds[1 - (BUF)][0], lds[1 - (BUF)][1], a, w, w.tile(v + 1) * kTile, missing);  \
+    if (more) store(1 - (BUF), w.tile(v + 1) * kTile);                                         \
     __syncthreads();                                                                            \
   }
   const int reach = a.window ? a.window : INT_MAX;
-  auto sees = [&](int key, bool there) {
+  auto sees = [&](int key) {
     const int kp = TREE && a.window ? position_of(a, w, key) : key;
-    return there & (key < w.hi) & in_order(TREE, w.context, key, limit, mask) &
+    return (key < w.hi) & in_order(TREE, w.context, key, limit, mask) &
            ((place - kp < reach) | (kp < a.sinks));
   };
   for (int v = v0; v < v_end; ++v) {
@@ -678,6 +804,13 @@ void cached_many_k(Cached a) {
     RV_MANY_STEP(1)
   }
 #undef RV_MANY_STEP
+  if (lane == 0) odds[wave] = odd;
+  __syncthreads();
+  if (odds[0] | odds[1] | odds[2] | odds[3]) {
+    exact_rows<E, HD>(a, w, at.b, at.kvh, at.rb * kBlockRows, kBlockRows, at.split, v0, v_end,
+                      kTile);
+    return;
+  }
   const float l = pair_sum(st.l);
   if (!ok) return;
   const int64_t to = (int64_t)(w.start + token) * a.H + head;

@@ -366,6 +366,65 @@ def test_append(cuda_device, heads, kv, hd, page, style, dtype):
     assert none.shape == (0, heads, hd)
 
 
+def test_move(cuda_device):
+    """All read before any is written; slots outside the cache are passed over."""
+    from reversability_amd.cache import PagedCache
+    held = PagedCache(2, 3, 16, 2, 32, torch.bfloat16, cuda_device)
+    held.keys.normal_()
+    held.values.normal_()
+    before = [t.clone().transpose(2, 3).reshape(2, 48, 2, 32) for t in (held.keys, held.values)]
+    as_slots = lambda *v: torch.tensor(v, dtype=torch.int64, device=cuda_device)
+    held.move(as_slots(0, 17, 40, 5, -1, 48), as_slots(17, 40, 3, -1, 6, 7))
+    for side, was in zip((held.keys, held.values), before):
+        now = side.transpose(2, 3).reshape(2, 48, 2, 32)
+        want = was.clone()
+        want[:, [17, 40, 3]] = was[:, [0, 17, 40]]
+        assert torch.equal(now, want)
+    held.move(as_slots(), as_slots())
+
+
+@pytest.mark.parametrize("heads,kv,hd,page", [(2, 2, 32, 16), (8, 2, 64, 32), (4, 1, 128, 16)])
+@pytest.mark.parametrize("new,held", [([1], [90]), ([3], [90]), ([14], [75]), ([50, 2], [333, 40])])
+@pytest.mark.parametrize("kind", ["chunk", "tree", "window"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_values_that_are_not_finite(cuda_device, heads, kv, hd, page, new, held, kind, bad):
+    """A key or value that is not finite reaches the rows that see it, and in V the columns where
+    it stands, and nothing else."""
+    dtype = torch.bfloat16
+    table, lengths, starts, pages = batch_of(new, held, page, cuda_device)
+    keys, values = filled(table, held, pages, kv, page, hd, dtype, cuda_device, spread=0.5)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(sum(new), heads, hd, generator=g).to(dtype).to(cuda_device)
+    masks = trees(new) if kind == "tree" else None
+    span = dict(window=20, sinks=2) if kind == "window" else {}
+    slots = slots_of(table, held, page)
+    for which, (n, total) in enumerate(zip(new, held)):
+        # in front of the window, at its edge and among the new tokens
+        spots = {5: (0, 3), max(0, total - n - 19): (0, 7), total - n // 2 - 1: (kv - 1, hd - 1)}
+        for t, (head, column) in spots.items():
+            slot = slots[which][t]
+            values[slot // page, head, slot % page, column] = bad
+        slot = slots[which][max(0, total - n - 21)]
+        if kind == "window":  # outside every window
+            keys[slot // page, :, slot % page] = bad
+    out = cached_attention(q, keys, values, table, lengths, starts, max(new),
+                           tree=None if masks is None else signed(masks, cuda_device), **span)
+    clean = [c.nan_to_num(0.0, 0.0, 0.0) for c in (keys, values)]
+    ref, tol = reference(q, *clean, table, new, held, masks, **span)
+    # the same with the bad values marked: a row of ones where a row and column sees one
+    mark = (~torch.isfinite(values)).to(dtype)
+    for slot in set(range(pages * page)) - set(sum(slots, [])):
+        mark[slot // page, :, slot % page] = 0
+    hit, _ = reference(q, clean[0], mark, table, new, held, masks, **span)
+    touched = hit > 0
+    assert touched.any() and not touched.all()
+    assert not torch.isfinite(out[touched]).any()
+    if bad == math.inf:
+        assert (out[touched] == math.inf).all()
+    assert torch.isfinite(out[~touched]).all()
+    check(out[~touched], ref[~touched], tol[~touched])
+
+
 def test_captured_step(cuda_device):
     """Plan, append and attention in two graphs that are alive together, replayed with other
     tokens, lengths and pages than they were captured with."""
