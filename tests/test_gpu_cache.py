@@ -488,8 +488,8 @@ def _model(method, device, window, sinks, rotated, precision_fused):
                         "d_model": 128, "d_ff": 256}, "method": method}
     torch.manual_seed(9)
     model = build_model(config).to(device)
-    if precision_fused and method != "baseline":
-        install_v3(model, core_mode="split" if method == "midpoint" else "inverse",
+    if precision_fused:
+        install_v3(model, core_mode="split" if method == "midpoint" else "reference",
                    mlp_tokens=64, swiglu=True, rmsnorm=True)
         enable_linear(model)
     rotary = Rotary(32, 256, device=device) if rotated else None
@@ -498,7 +498,8 @@ def _model(method, device, window, sinks, rotated, precision_fused):
 
 
 @pytest.mark.parametrize("method,fused", [("baseline", False), ("midpoint", False),
-                                          ("midpoint", True), ("euler", False)])
+                                          ("midpoint", True), ("euler", False),
+                                          ("euler", True), ("baseline", True)])
 @pytest.mark.parametrize("window,sinks,rotated", [(None, 0, False), (20, 2, True)])
 @pytest.mark.parametrize("precision", ["fp16", "bf16"])
 def test_decode_matches_whole_sequences(cuda_device, method, fused, window, sinks, rotated,
@@ -544,13 +545,12 @@ def test_decode_matches_whole_sequences(cuda_device, method, fused, window, sink
         outs, done = feed(parts, done, pad=2)
         for a, o in zip(got, outs):
             a.append(o)
-    for _ in range(1):
-        outs, done = feed([t[d:d + 1] for t, d in zip(text, done)], done)
-        for a, o in zip(got, outs):
-            a.append(o)
+    outs, done = feed([t[d:d + 1] for t, d in zip(text, done)], done)
+    for a, o in zip(got, outs):
+        a.append(o)
     assert done == lens
     for ids, parts in zip(text, got):
-        assert (torch.cat(parts) - whole(ids)).abs().max() <= limit * 1.0
+        assert (torch.cat(parts) - whole(ids)).abs().max() <= limit
     # a tree behind each text: two branches, and the second's path kept
     tree = torch.tensor([0b1, 0b11, 0b101, 0b1101] * 3, dtype=torch.int64, device=cuda_device)
     drafts = [torch.randint(0, 97, (4,), generator=g).to(cuda_device) for _ in range(3)]
@@ -568,3 +568,95 @@ def test_decode_matches_whole_sequences(cuda_device, method, fused, window, sink
     for ids, draft, end, o in zip(text, drafts, last, outs):
         want = whole(torch.cat([ids, draft[[0, 2, 3]], end]))[-1]
         assert (o[0] - want).abs().max() <= limit
+
+
+def test_decode_of_chosen_rows_and_refusals(cuda_device):
+    from reversability_amd.cache import CacheBatch, PagedCache, decode
+    model = _model("midpoint", cuda_device, 20, 2, True, False)
+    cache = PagedCache.for_model(model, pages=4, page_size=16)
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    batch = CacheBatch(as_int([[0, 1], [2, 3]]), as_int([5, 3]), as_int([0, 5, 8]), 5, 32)
+    ids = torch.randint(0, 97, (8,), device=cuda_device)
+    whole = decode(model, ids, cache, batch)
+    rows = torch.tensor([4, 7], device=cuda_device)
+    # (the head's product over fewer rows may round otherwise)
+    assert torch.allclose(decode(model, ids, cache, batch, rows=rows), whole[rows], atol=2e-3)
+    with pytest.raises(ValueError, match="ids"):
+        decode(model, ids.view(2, 4), cache, batch)
+    with pytest.raises(ValueError, match="type"):
+        append_kv(torch.zeros(8, 384, device=cuda_device, dtype=torch.bfloat16), 4,
+                  cache.keys[0], cache.values[0], torch.zeros(8, dtype=torch.int64,
+                                                             device=cuda_device))
+
+
+def test_captured_decode(cuda_device):
+    """decode in a graph, replayed for other sequences, against eager calls on a cache of their
+    own."""
+    from reversability_amd.cache import CacheBatch, PagedCache, decode
+    from reversability_amd.graph import CapturedStep
+    model = _model("midpoint", cuda_device, 20, 2, True, True)
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    table = as_int([[3, 0, 5], [1, 4, 2]])
+    caches = [PagedCache.for_model(model, pages=6, page_size=16) for _ in range(2)]
+    prompt = torch.randint(0, 97, (30,), device=cuda_device)
+    first = CacheBatch(table, as_int([20, 10]), as_int([0, 20, 30]), 20, 48)
+    for cache in caches:
+        decode(model, prompt, cache, first)
+    ids, lengths = torch.zeros(2, dtype=torch.int64, device=cuda_device), as_int([21, 11])
+    batch = CacheBatch(table, lengths, as_int([0, 1, 2]), 1, 48)
+    step = CapturedStep(lambda: decode(model, ids, caches[0], batch))
+    torch.cuda.synchronize()
+    caches[0].keys.copy_(caches[1].keys)  # (the warm-up calls wrote the first token)
+    caches[0].values.copy_(caches[1].values)
+    for at in range(4):
+        ids.copy_(torch.randint(0, 97, (2,), device=cuda_device))
+        lengths.copy_(as_int([21 + at, 11 + at]))
+        torch.cuda.synchronize()
+        got = step().clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, decode(model, ids, caches[1], batch))
+        assert torch.equal(caches[0].keys, caches[1].keys)
+
+
+def test_refusals(cuda_device):
+    """Arguments that the operators do not take, on the device and before any launch."""
+    table, lengths, starts, pages = batch_of([1, 1], [20, 5], 16, cuda_device)
+    keys, values = filled(table, [20, 5], pages, 2, 16, 32, torch.float16, cuda_device)
+    q = torch.zeros(2, 4, 32, device=cuda_device, dtype=torch.float16)
+    good = dict(q=q, keys=keys, values=values, page_table=table, lengths=lengths, starts=starts,
+                max_query=1)
+    cached_attention(**good)
+    wide = torch.zeros(2, 4, 32, device=cuda_device, dtype=torch.int64)
+    for bad in (dict(q=q.float()), dict(q=q.bfloat16()), dict(q=q[:, :3]), dict(q=q[..., :16]),
+                dict(q=q[0]), dict(values=values[1:]), dict(values=values.bfloat16()),
+                dict(keys=keys.transpose(2, 3)), dict(keys=keys[:, :, :8], values=values[:, :, :8]),
+                dict(page_table=table.long()), dict(page_table=table[0]), dict(page_table=table[:1]),
+                dict(lengths=lengths.long()), dict(starts=starts[1:]), dict(max_query=0),
+                dict(max_length=0), dict(window=0), dict(sinks=-1), dict(tree=lengths),
+                dict(max_query=65, tree=torch.zeros(100, dtype=torch.int64, device=cuda_device),
+                     q=q.new_zeros(100, 4, 32)),
+                dict(out=q.float()), dict(out=torch.empty_like(q).transpose(0, 1)),
+                dict(lengths=lengths.cpu())):
+        with pytest.raises(ValueError):
+            cached_attention(**{**good, **bad})
+    with pytest.raises(ValueError, match="no_grad"):
+        cached_attention(**{**good, "q": q.clone().requires_grad_(True)})
+    with torch.no_grad():
+        cached_attention(**{**good, "q": q.clone().requires_grad_(True)})
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError):
+            cached_attention(**{**good, "q": dual})
+    qkv = torch.zeros(2, 8 * 32, device=cuda_device, dtype=torch.float16)
+    slots = torch.tensor([3, 4], device=cuda_device)
+    rotary = Rotary(32, 8, device=cuda_device)
+    for bad in (dict(heads=3), dict(heads=5), dict(slots=slots[:1]), dict(slots=slots.int()),
+                dict(rotary=rotary), dict(rotary=Rotary(64, 8, device=cuda_device),
+                                          positions=slots.int()),
+                dict(rotary=rotary, positions=slots), dict(qkv=qkv[:, :-32])):
+        with pytest.raises(ValueError):
+            append_kv(**{**dict(qkv=qkv, heads=4, keys=keys, values=values, slots=slots), **bad})
+    for bad in (dict(page_size=24), dict(tokens=-1), dict(tree=wide[0, 0, :3])):
+        with pytest.raises(ValueError):
+            cache_plan(**{**dict(page_table=table, lengths=lengths, starts=starts, tokens=2,
+                                 page_size=16), **bad})

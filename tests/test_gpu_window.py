@@ -222,6 +222,63 @@ def test_captured(cuda_device):
         assert torch.equal(held[0], out) and torch.equal(held[1], grad)
 
 
+def test_refusals(cuda_device):
+    qkv, _ = make(1, 8, 4, 2, 32, torch.float16, cuda_device)
+    for bad in (dict(qkv=qkv.float()), dict(qkv=qkv[0]), dict(heads=3), dict(kv_heads=3),
+                dict(qkv=qkv[..., :-32]), dict(window=0), dict(sinks=-1)):
+        with pytest.raises(ValueError):
+            window_attention(**{**dict(qkv=qkv, heads=4, window=3, sinks=1, kv_heads=2), **bad})
+    x = qkv.clone().requires_grad_(True)
+    grad, = torch.autograd.grad(window_attention(x, 4, 3, kv_heads=2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivative
+        grad.sum().backward()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(qkv, torch.ones_like(qkv))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            window_attention(dual, 4, 3, kv_heads=2)
+    rotary = Rotary(32, 8, device=cuda_device)
+    positions = torch.zeros(1, 8, device=cuda_device, dtype=torch.int32)
+    for bad in (dict(rotary=Rotary(64, 8, device=cuda_device)), dict(positions=positions.long()),
+                dict(positions=positions[0]), dict(positions=positions.cpu()),
+                dict(rotary=Rotary(32, 8, device="cpu")), dict(rotary=Rotary(
+                    32, 7, device=cuda_device))):
+        with pytest.raises(ValueError):
+            rotate_qkv(**{**dict(qkv=qkv, heads=4, rotary=rotary, kv_heads=2), **bad})
+
+
+def test_gradients_of_a_frozen_input_and_twice(cuda_device):
+    """Without gradients the same values; two backward passes through one graph agree."""
+    qkv, dout = make(2, 200, 4, 2, 64, torch.float16, cuda_device)
+    with torch.no_grad():
+        frozen = window_attention(qkv, 4, 30, 2, kv_heads=2)
+    x = qkv.clone().requires_grad_(True)
+    out = window_attention(x, 4, 30, 2, kv_heads=2)
+    assert torch.equal(out, frozen)
+    first, = torch.autograd.grad(out, x, dout, retain_graph=True)
+    second, = torch.autograd.grad(out, x, dout)
+    assert torch.equal(first, second)
+
+
+def test_long_sequences_and_sinks(cuda_device):
+    """Sinks summed over many queries keep their digits: errors as on short sequences."""
+    heads, kv, hd, window, sinks = 2, 1, 64, 128, 3
+    qkv, dout = make(1, 9000, heads, kv, hd, torch.bfloat16, cuda_device, seed=5)
+    x = qkv.requires_grad_(True)
+    out = window_attention(x, heads, window, sinks, kv_heads=kv)
+    got, = torch.autograd.grad(out, x, dout)
+    out_ref, out_tol, ref, tol = reference(qkv.detach(), dout, heads, kv, window, sinks)
+    assert worst(out, out_ref, out_tol) <= 1.0
+    assert worst(got, ref, tol) <= 1.0
+    # of the sinks' keys and values the roundings of P and dS are made up for: what is left is the
+    # final rounding, D's (its output kept twice: 2^-16 of it) and fp32 sums of 9000 terms
+    u = torch.finfo(torch.bfloat16).eps / 2
+    part = slice(heads * hd, None)
+    left = (got[0, :sinks, part].double() - ref[0, :sinks, part]).abs()
+    loose = tol[0, :sinks, part]  # 2 (u of every term + u of the sum): u^2 of the terms stay
+    bound = u * ref[0, :sinks, part].abs() + 4 * u * loose + 2 ** -14 * loose
+    assert float((left / bound).max()) <= 1.0
+
+
 # ---------------------------------------------------------------------------
 # rotation
 # ---------------------------------------------------------------------------
