@@ -122,7 +122,7 @@ def append_kv(qkv: torch.Tensor, heads: int, keys: torch.Tensor, values: torch.T
     ``rotate_qkv`` does; without, the queries are a view of ``qkv``.  A slot outside the cache
     is not written; the slots of one call must differ.  All of one type, fp16 or bf16."""
     _check_cache(keys, values, "append_kv")
-    _no_graph("append_kv", qkv)
+    _no_graph("append_kv", qkv, keys, values)
     kv, hd = packed_heads(qkv, heads, keys.shape[1], "append_kv")
     if qkv.dtype != keys.dtype or qkv.device != keys.device or hd != keys.shape[3]:
         raise ValueError("append_kv needs qkv of the cache's type, head size and device")
@@ -179,7 +179,7 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
     ``tree`` its context and what its mask has; with ``window`` of these the tokens less than
     ``window`` positions before it and the first ``sinks`` positions.  A token that sees
     nothing gets zeros.  Returns ``out`` (contiguous, q's shape and type; None: a new
-    tensor), whose rows of no sequence are left as they were.
+    tensor; not q's memory), whose rows of no sequence are left as they were.
 
     Slots that no sequence's tokens hold are never used, whatever they contain.  Scores,
     statistics and sums in fp32, the weights rounded to the cache's type for the product with
@@ -212,6 +212,9 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned tensor like q")
+    elif tokens and (out.data_ptr() < q.data_ptr() + q.stride(0) * (tokens - 1) * 2 + heads * hd * 2
+                     and q.data_ptr() < out.data_ptr() + out.numel() * 2):
+        raise ValueError("out must not overlap q")
     paths.took("cached_attention", "hip")
     if not tokens:
         return out
@@ -298,9 +301,12 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
     The model is a ``BaselineLM`` or ``ReversibleLM`` with what was enabled on it; a window,
     sinks and a rotation are those of ``enable_attention``.  Logits are what the model's own
     forward pass gives for the whole sequences, but for roundings; dropout is not applied.
-    Logits of rows of no sequence have no meaning.  ``batch.max_length`` must not exceed the
-    model's ``max_sequence_length`` (positions past it, which only a wrong max_length lets
-    through, are taken as its last)."""
+    Logits of rows of no sequence have no meaning (their ids must be of the vocabulary all the
+    same); no sequence may have more than ``batch.max_query`` of them.  ``batch.max_length`` must
+    not exceed the model's ``max_sequence_length``, nor the positions of its ``Rotary``
+    (positions past the former, which only a wrong max_length lets through, are taken as its
+    last).  The keys and values of one call's tokens need slots of their own: sequences may
+    share pages of tokens that all of them hold, not those that new tokens go to."""
     from .optimized_v3 import castable_weights
     if precision not in _AMP_DTYPES or _AMP_DTYPES[precision] != cache.keys.dtype:
         raise ValueError("decode needs fp16 or bf16 precision, that of its cache")
@@ -311,6 +317,12 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
         raise ValueError("sequence exceeds max_sequence_length")
     if len(model.blocks) != cache.keys.shape[0]:
         raise ValueError("decode needs a cache of the model's layers")
+    rotary = getattr(model.blocks[0].attn, "_rv_rotary", None)
+    if rotary is not None and batch.max_length > rotary.positions:
+        raise ValueError("sequence exceeds the positions of the Rotary table")
+    if not ids.shape[0]:
+        return torch.empty(0, model.lm_head.weight.shape[0], device=ids.device,
+                           dtype=cache.keys.dtype)
     slots, positions = cache_plan(batch.page_table, batch.lengths, batch.starts, ids.shape[0],
                                   cache.page_size, batch.tree)
 

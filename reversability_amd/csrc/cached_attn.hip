@@ -222,9 +222,9 @@ __device__ __forceinline__ void exact_rows(const Cached& a, const View& w, int b
       float top = s;
 #pragma unroll
       for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-      const float m_new = fmaxf(m, top);
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-      const float p = at < 0 ? 0.f : __builtin_amdgcn_exp2f(s - m_new);
+      const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      const float p = __builtin_amdgcn_exp2f(s - base);
       m = m_new;
       l = l * alpha + rv::wave_sum(p);
       o[0] *= alpha, o[1] *= alpha;
@@ -923,6 +923,7 @@ constexpr int kMostSplits = 256;
 Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t max_length,
              int64_t window, int64_t sinks) {
   Plan p;
+  window = std::min<int64_t>(window, 1 << 30), sinks = std::min<int64_t>(sinks, 1 << 30);
   const int64_t rows = max_query * (heads / kv);
   p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kBlockRows;
   const bool many = p.rows == kBlockRows;
@@ -933,7 +934,11 @@ Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t
   const int64_t tiles = std::max<int64_t>(1, (seen + p.keys - 1) / p.keys);
   const int64_t blocks = seqs * kv * p.row_blocks, wanted = many ? kManyWanted : kFewWanted;
   const int64_t least = (many ? 2 : 1) * kLeastKeys / p.keys, most = (many ? 4 : 1) * kMostKeys / p.keys;
-  int64_t splits = std::max((wanted + blocks - 1) / blocks, (tiles + most - 1) / most);
+  // (what one sequence alone fills the chip with is enough for the longest: 8 chunks of 65536
+  // tokens, 32 heads of 128, want no partials, where 16 stretches have 136 GB of them)
+  const int64_t alone = kv * p.row_blocks;
+  const int64_t shorter = std::min((tiles + most - 1) / most, (wanted + alone - 1) / alone);
+  int64_t splits = std::max((wanted + blocks - 1) / blocks, shorter);
   splits = std::min<int64_t>(splits, (tiles + least - 1) / least);
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, kMostSplits));
   p.split_tiles = (int)((tiles + splits - 1) / splits);
@@ -952,12 +957,26 @@ bool args_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv, int64_t hd
          max_query > 0 && max_length > 0 && window >= 0 && sinks >= 0;
 }
 
-bool sizes_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv, int64_t hd,
-              int64_t max_query, int64_t max_length, const Plan& p) {
+// Rows that a workgroup joins: a few stretches take a wave a row, many the whole workgroup (33 sequences of
+// up to 65536 tokens in 64 stretches 11.5 -> 7.8 us).
+int join_rows(const Plan& p) { return p.splits > 16 ? 1 : kWaves; }
+
+int64_t join_blocks(int64_t seqs, int64_t heads, int64_t max_query, const Plan& p) {
+  return p.splits == 1 ? 0 : (max_query * heads + join_rows(p) - 1) / join_rows(p) * seqs;
+}
+
+// Sizes that the kernels take (and whose products plan_of forms).
+bool sizes_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t hd, int64_t max_query,
+              int64_t max_length) {
   return (hd == 32 || hd == 64 || hd == 128) && heads < (1 << 16) && tokens < (1 << 26) &&
-         max_query < (1 << 26) && max_length <= (1 << 30) && max_query * heads < (1 << 30) &&
-         (seqs * kv * p.splits + 7) * p.row_blocks < (1 << 24) &&
-         seqs * max_query * heads < (1 << 24);
+         seqs < (1 << 24) && max_query < (1 << 26) && max_length <= (1 << 30) &&
+         max_query * heads < (1 << 30);
+}
+
+// A launch has fewer than 2^32 threads.
+bool launch_ok(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, const Plan& p) {
+  return (seqs * kv * p.splits + 7) * p.row_blocks < (1 << 24) &&
+         join_blocks(seqs, heads, max_query, p) < (1 << 24);
 }
 
 int64_t workspace_bytes(int64_t tokens, int64_t heads, int64_t hd, const Plan& p) {
@@ -977,12 +996,9 @@ int launch(const Cached& a, const Plan& p, hipStream_t s) {
                        block, 0, s, a);
   int rc = rv_host::check_launch();
   if (rc != RV_OK || p.splits == 1) return rc;
-  // a few stretches: a wave a row, many: the whole workgroup
-  // (33 sequences of up to 65536 tokens in 64 stretches 11.5 -> 7.8 us)
-  const int rows = p.splits > 16 ? 1 : kWaves;
-  const int64_t blocks = ((int64_t)a.max_query * a.H + rows - 1) / rows;
-  hipLaunchKernelGGL((p.splits > 16 ? cached_join_k<E, HD, kWaves> : cached_join_k<E, HD, 1>),
-                     dim3((unsigned)(blocks * a.seqs)), block, 0, s, a, p.rows, p.keys);
+  const int64_t blocks = join_blocks(a.seqs, a.H, a.max_query, p);
+  hipLaunchKernelGGL((join_rows(p) == 1 ? cached_join_k<E, HD, kWaves> : cached_join_k<E, HD, 1>),
+                     dim3((unsigned)blocks), block, 0, s, a, p.rows, p.keys);
   return rv_host::check_launch();
 }
 
@@ -995,9 +1011,9 @@ int64_t rv_cached_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hea
                                        int64_t max_length, int64_t window, int64_t sinks) {
   if (!args_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, window, sinks))
     return -RV_ERR_BAD_SIZE;
+  if (!sizes_ok(tokens, seqs, heads, head_dim, max_query, max_length)) return -RV_ERR_UNSUPPORTED;
   const Plan p = plan_of(seqs, heads, kv_heads, max_query, max_length, window, sinks);
-  if (!sizes_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, p))
-    return -RV_ERR_UNSUPPORTED;
+  if (!launch_ok(seqs, heads, kv_heads, max_query, p)) return -RV_ERR_UNSUPPORTED;
   return workspace_bytes(tokens, heads, head_dim, p);
 }
 
@@ -1013,14 +1029,15 @@ int rv_cached_attn(const void* q, int64_t q_ld, const void* keys, const void* va
   if (!args_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, window, sinks) ||
       pages <= 0 || table_pages <= 0 || ld_table < table_pages || q_ld < heads * head_dim)
     return RV_ERR_BAD_SIZE;
-  const Plan p = plan_of(seqs, heads, kv_heads, max_query, max_length, window, sinks);
   const int shift = page_shift_of(page_size);
-  if (!sizes_ok(tokens, seqs, heads, kv_heads, head_dim, max_query, max_length, p) ||
+  if (!sizes_ok(tokens, seqs, heads, head_dim, max_query, max_length) ||
       (dtype != RV_F16 && dtype != RV_BF16) || shift < 0 || (tree && max_query > 64) ||
       pages >= (int64_t(1) << 31) || table_pages >= (int64_t(1) << 31) || q_ld % 8 ||
       !rv_host::aligned16(q) || !rv_host::aligned16(keys) || !rv_host::aligned16(values) ||
       !rv_host::aligned16(out) || !rv_host::aligned16(workspace))
     return RV_ERR_UNSUPPORTED;
+  const Plan p = plan_of(seqs, heads, kv_heads, max_query, max_length, window, sinks);
+  if (!launch_ok(seqs, heads, kv_heads, max_query, p)) return RV_ERR_UNSUPPORTED;
   const int64_t need = workspace_bytes(tokens, heads, head_dim, p);
   if (need && (!workspace || workspace_bytes_given < need)) return RV_ERR_WORKSPACE;
   if (!tokens) return RV_OK;

@@ -140,6 +140,9 @@ def test_decode_refuses():
         cache.decode(model, ids, held, batch._replace(max_length=41))
     with pytest.raises(ValueError, match="layers"):
         cache.decode(model, ids, cache.PagedCache(1, 3, 16, 2, 32, device="cpu"), batch)
+    attention.enable_attention(model, rotary=attention.Rotary(32, 39, device="cpu"))
+    with pytest.raises(ValueError, match="Rotary"):
+        cache.decode(model, ids, held, batch)
 
 
 def test_entry_points_validate_without_device():
@@ -187,3 +190,37 @@ def test_entry_points_validate_without_device():
     assert see(length=100_000, ws=fake, n=size - 1) == 4 and see(length=100_000, ws=odd, n=size) == 3
     assert lib.rv_cached_attn_workspace_bytes(5, 2, 3, 2, 32, 1, 64, 0, 0) == -2
     assert lib.rv_cached_attn_workspace_bytes(5, 2, 2, 1, 48, 1, 64, 0, 0) == -3
+
+
+def test_entry_points_refuse_sizes_whose_products_pass_64_bits():
+    lib = _hip.library()
+    fake, huge = ctypes.c_void_p(4096), 1 << 62
+    names = ("tokens", "seqs", "heads", "kv", "hd", "query", "length", "window", "sinks")
+    good = dict(zip(names, (5, 2, 4, 2, 64, 3, 100_000, 7, 4)))
+    assert lib.rv_cached_attn_workspace_bytes(*good.values()) >= 0
+    for name in names[:4] + names[5:7]:
+        assert lib.rv_cached_attn_workspace_bytes(*{**good, name: huge}.values()) < 0, name
+    for name in ("window", "sinks"):  # all of what a cache holds
+        assert lib.rv_cached_attn_workspace_bytes(*{**good, name: huge}.values()) > 0, name
+    sizes = dict(batch=2, seq=300, heads=4, kv=2, hd=64, window=32, sinks=4)
+    for name in ("batch", "seq", "heads"):
+        args = {**sizes, name: huge}.values()
+        assert lib.rv_window_attn_bwd_workspace_bytes(*args) == -3, name
+    for name in ("window", "sinks"):
+        args = {**sizes, name: huge}.values()
+        assert lib.rv_window_attn_bwd_workspace_bytes(*args) > 0, name
+    assert lib.rv_cache_plan(fake, 4, 4, fake, fake, None, huge, 5, 16, fake, fake, None) == 3
+    assert lib.rv_append_kv(fake, 1 << 30, None, fake, fake, fake, 4, huge, 1, 32, _hip.RV_F16, 3, 16,
+                            None, 0, None, 0, None) == 2
+
+
+def test_partials_of_long_chunks_are_bounded():
+    """Chunks that fill the chip by themselves are not cut: partials of every row would be larger
+    than the cache."""
+    size = _hip.library().rv_cached_attn_workspace_bytes
+    assert size(8 * 65536, 8, 32, 8, 128, 65536, 65536, 0, 0) == 0
+    for seqs in (1, 4, 32):
+        for query in (1, 7, 64, 512, 4096):
+            for length in (512, 12000, 1 << 20):
+                nbytes = size(seqs * query, seqs, 32, 8, 128, query, length, 0, 0)
+                assert 0 <= nbytes <= seqs * (150 << 20), (seqs, query, length, nbytes)

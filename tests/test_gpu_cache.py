@@ -425,6 +425,42 @@ def test_values_that_are_not_finite(cuda_device, heads, kv, hd, page, new, held,
     check(out[~touched], ref[~touched], tol[~touched])
 
 
+def test_infinite_scores_beside_a_value_that_is_not_finite(cuda_device):
+    """Keys that no weight is left for, in front of a value that is made up for key by key."""
+    table, lengths, starts, pages = batch_of([2], [100], 16, cuda_device)
+    keys, values = filled(table, [100], pages, 1, 16, 32, torch.float16, cuda_device)
+    slots = slots_of(table, [100], 16)[0]
+    for j in range(70):
+        keys[slots[j] // 16, 0, slots[j] % 16, 0] = -math.inf
+    q = torch.zeros(2, 1, 32, device=cuda_device, dtype=torch.float16)
+    q[:, 0, 0] = 1.0
+    ref, tol = reference(q, keys, values, table, [2], [100])
+    values[slots[99] // 16, 0, slots[99] % 16, 3] = math.nan  # the second token's own
+    out = cached_attention(q, keys, values, table, lengths, starts, 2)
+    check(out[:1], ref[:1], tol[:1])
+    assert out[1, 0, 3].isnan() and out[1, 0, :3].isfinite().all()
+
+
+def test_two_calls_at_once(cuda_device):
+    """Calls on two streams, each with stretches of its own to join, and one after the other."""
+    new, held = [1, 1, 1], [3000, 700, 1999]
+    table, lengths, starts, pages = batch_of(new, held, 16, cuda_device)
+    keys, values = filled(table, held, pages, 2, 16, 64, torch.float16, cuda_device)
+    g = torch.Generator().manual_seed(5)
+    qs = [torch.randn(3, 8, 64, generator=g).half().to(cuda_device) for _ in range(8)]
+    call = lambda q: cached_attention(q, keys, values, table, lengths, starts, 1)
+    want = [call(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, q in enumerate(qs):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(call(q))
+    torch.cuda.synchronize()
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
 def test_captured_step(cuda_device):
     """Plan, append and attention in two graphs that are alive together, replayed with other
     tokens, lengths and pages than they were captured with."""
@@ -589,6 +625,27 @@ def test_decode_of_chosen_rows_and_refusals(cuda_device):
                                                              device=cuda_device))
 
 
+def test_decode_of_a_padded_batch_and_of_nothing(cuda_device):
+    """Rows of no sequence in front of and behind the others change neither those nor the cache."""
+    from reversability_amd.cache import CacheBatch, PagedCache, decode
+    model = _model("euler", cuda_device, 20, 2, True, False)
+    caches = [PagedCache.for_model(model, pages=4, page_size=16) for _ in range(2)]
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    table, lengths = as_int([[0, 1], [2, 3]]), as_int([5, 3])
+    ids = torch.randint(0, 97, (14,), device=cuda_device)
+    want = decode(model, ids[2:10].clone(), caches[0],
+                  CacheBatch(table, lengths, as_int([0, 5, 8]), 5, 32))
+    got = decode(model, ids, caches[1], CacheBatch(table, lengths, as_int([2, 7, 10]), 5, 32))
+    # (products over more rows may round otherwise)
+    assert torch.allclose(got[2:10], want, atol=4e-3)
+    assert torch.allclose(caches[0].keys, caches[1].keys, atol=4e-3)
+    assert torch.allclose(caches[0].values, caches[1].values, atol=4e-3)
+    before = caches[0].keys.clone()
+    none = decode(model, ids[:0], caches[0], CacheBatch(table, lengths, as_int([0, 0, 0]), 1, 32))
+    assert none.shape == (0, 97) and none.dtype == torch.float16
+    assert torch.equal(caches[0].keys, before)
+
+
 def test_captured_decode(cuda_device):
     """decode in a graph, replayed for other sequences, against eager calls on a cache of their
     own."""
@@ -635,7 +692,7 @@ def test_refusals(cuda_device):
                 dict(max_length=0), dict(window=0), dict(sinks=-1), dict(tree=lengths),
                 dict(max_query=65, tree=torch.zeros(100, dtype=torch.int64, device=cuda_device),
                      q=q.new_zeros(100, 4, 32)),
-                dict(out=q.float()), dict(out=torch.empty_like(q).transpose(0, 1)),
+                dict(out=q.float()), dict(out=torch.empty_like(q).transpose(0, 1)), dict(out=q),
                 dict(lengths=lengths.cpu())):
         with pytest.raises(ValueError):
             cached_attention(**{**good, **bad})
