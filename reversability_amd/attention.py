@@ -26,6 +26,7 @@ rotation of queries and keys by position, from a ``Rotary`` table.
 """
 from __future__ import annotations
 
+import math
 import types
 from typing import Optional
 
@@ -307,11 +308,13 @@ class Rotary:
                              "base > 0")
         self.head_dim, self.positions = head_dim, positions
         self.base, self.interleaved = float(base), bool(interleaved)
-        rate = self.base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64, device=device)
-                             / head_dim)
+        rate = torch.arange(0, head_dim, 2, dtype=torch.float64, device=device)
+        rate = rate.mul_(-math.log(self.base) / head_dim).exp_()
         at = torch.arange(positions, dtype=torch.float64, device=device)
         angle = at.unsqueeze(1) * rate
-        self.table = torch.stack([angle.cos(), angle.sin()], -1).float()
+        self.table = torch.empty(*angle.shape, 2, dtype=torch.float32, device=device)
+        torch.cos(angle, out=self.table[..., 0])  # rounded on the way
+        torch.sin(angle, out=self.table[..., 1])
 
     def to(self, device) -> "Rotary":
         """A copy with its table on ``device``."""

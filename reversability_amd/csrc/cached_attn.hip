@@ -28,6 +28,13 @@
 // Rows of V that no row of the workgroup sees (behind the last token, before the window, of a
 // page that does not exist) are taken as zeros and their scores as -inf, whatever the cache holds.
 // A token that only some rows see reaches those alone, also where it is not a number (exact_rows).
+//
+// Measured: 33 sequences of 100 to 65536 tokens, a token each, 8 key heads of 128, 312 + 8 us (the stretches,
+// their joining), 5.5 TB/s of keys and values, past a large copy's rate; one sequence of 200 tokens 6 us,
+// the chain of its loads; 8 trees over 4000 tokens 23 + 7 us and four chunks of up to 512 tokens over
+// 12000, 128 wide, 76 + 15 us: there the matrix cores are 4-12% busy, the stretches being short (the rest
+// is their start, softmax and partials).  Looking for values that are not finite costs 0.4 us of the
+// single sequence's 6, 1.5 of the trees' 23 and 2 of the chunks' 87.
 
 #include <algorithm>
 #include <climits>
@@ -914,10 +921,18 @@ struct Plan {
   int rows, keys, row_blocks, splits, split_tiles;
 };
 
-constexpr int64_t kFewWanted = 1024;   // workgroups for the chip's 256 CUs
-constexpr int64_t kManyWanted = 1024;
-constexpr int kLeastKeys = 256;        // of a stretch; twice as many with many rows
-constexpr int kMostKeys = 1024;        // a longer one would keep a few workgroups busy alone
+// Workgroups for the chip's 256 CUs.  Few rows: half as many 318 us, twice as many 319, 1024 318 (33 sequences
+// of 100 to 65536 tokens, a token each; one of 65536 48, 51, 49).  Many rows, where sequences of unlike
+// lengths share the chip: 512 113 us, 1024 94, 2048 87, 4096 96 (four chunks of up to 512 tokens over
+// 12000), 811, 620, 488, 489 (two of 2048 over 30000); one sequence's stretches are alike and gain
+// nothing from more (700 tokens over 20000, heads of 32: 58 us with 1024, 64 with 2048).
+constexpr int64_t kFewWanted = 1024, kManyWanted = 2048, kAloneWanted = 1024;
+// Keys of a stretch at least, twice as many with many rows: 128 19.4 us, 256 15.5, 512 15.5 (a sequence
+// of 200 tokens), 29, 30, 41 (8 trees of up to 64 tokens over 4000).
+constexpr int kLeastKeys = 256;
+// And at most, twice as many with many rows; a longer one keeps a few workgroups busy alone: 512 339 us,
+// 1024 318, 2048 313 (the 33 sequences), many rows 2048 499, 4096 488 (the two chunks).
+constexpr int kMostKeys = 2048;
 constexpr int kMostSplits = 256;
 
 Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t max_length,
@@ -925,6 +940,8 @@ Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t
   Plan p;
   window = std::min<int64_t>(window, 1 << 30), sinks = std::min<int64_t>(sinks, 1 << 30);
   const int64_t rows = max_query * (heads / kv);
+  // 32 rows of 8 sequences over 4000 tokens: 10.3 us as few, 15.6 as many; 4 of 64 over 2000 (or one over
+  // 65536) 41 and 57
   p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kBlockRows;
   const bool many = p.rows == kBlockRows;
   p.keys = many ? kTile : kKeys;
@@ -932,8 +949,10 @@ Plan plan_of(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, int64_t
   int64_t seen = max_length;  // of one block of rows, at most (and the tiles' edges)
   if (window) seen = std::min(seen, window + sinks + std::min<int64_t>(max_query, 128) + 3 * p.keys);
   const int64_t tiles = std::max<int64_t>(1, (seen + p.keys - 1) / p.keys);
-  const int64_t blocks = seqs * kv * p.row_blocks, wanted = many ? kManyWanted : kFewWanted;
-  const int64_t least = (many ? 2 : 1) * kLeastKeys / p.keys, most = (many ? 4 : 1) * kMostKeys / p.keys;
+  const int64_t blocks = seqs * kv * p.row_blocks;
+  const int64_t wanted = !many ? kFewWanted : seqs > 1 ? kManyWanted : kAloneWanted;
+  const int64_t least = (many ? 2 : 1) * kLeastKeys / p.keys;
+  const int64_t most = (many ? 2 : 1) * kMostKeys / p.keys;
   // (what one sequence alone fills the chip with is enough for the longest: 8 chunks of 65536
   // tokens, 32 heads of 128, want no partials, where 16 stretches have 136 GB of them)
   const int64_t alone = kv * p.row_blocks;

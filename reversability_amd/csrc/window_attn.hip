@@ -29,6 +29,15 @@
 // Of every output the forward also keeps what its rounding left (rest), for D = rowsum(dO O).
 // Error of the gradients relative to that of the final rounding alone: without all this 1.5
 // to 2.1, with it 1.0 to 1.3, at a few percent of the time.
+//
+// Measured (us; forward, dQ, dK/dV, sums; window and sinks behind the comma), with the rate over the
+// visible pairs' 4 + 10 HD flops:
+//   33 x 512, 8 heads of 32, 128 + 4, fp16          22   25        31   4.5    71 TFLOP/s
+//   3 x 1999, 20 heads of 64 over 4, 500 + 3, bf16  41   10 + 57   67  11     280
+//   2 x 16384, 10 heads of 128, 2048 + 4, bf16     440   17 + 565  990  14    600
+// Short windows are bound by the exponentials and masks (VALU 25-35% busy with the waits between, matrix
+// cores 14-20%), long ones by the matrix cores' feeding: 35% busy in the forward, 42% in dQ, 29% in
+// dK/dV, whose 128 accumulators and 64 operands leave one wave per SIMD (two spill: 1500 us).
 
 #include <algorithm>
 #include <cmath>
@@ -739,8 +748,8 @@ constexpr int kMostUnits = 4096;
 // Chunks that the other blocks are cut into: of the plans with 1, 2, 3 .. the one that takes the fewest
 // steps in a row, where `slots` chunks run at once (a workgroup's start and end count
 // as three steps, the partials by their bytes at 4 TB/s and a launch, a step as 2 us).
-// 3 x 1999 tokens, 20 heads of 64 over 4, window 500: 3 chunks of 17 steps in two rounds
-// 77 + 11.7 us (sums, then partials), 2 of 25 in one 68 + 8.9.
+// 3 x 1999 tokens, 20 heads of 64 over 4, window 500 (492 chunks): 3 of 17 steps a block in two
+// rounds 77 + 11.7 us (sums, then partials), 2 of 25 in one 67 + 10.9.
 KvPlan kv_plan(const Geometry& g, int64_t batch, int64_t hd) {
   const int group = g.H / g.KV;
   const int64_t outer = batch * g.KV, slots = 256 * (hd == 32 ? 3 : hd == 64 ? 2 : 1);
