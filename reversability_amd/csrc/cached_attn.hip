@@ -29,10 +29,10 @@
 // page that does not exist) are taken as zeros and their scores as -inf, whatever the cache holds.
 // A token that only some rows see reaches those alone, also where it is not a number (exact_rows).
 //
-// Measured: 33 sequences of 100 to 65536 tokens, a token each, 8 key heads of 128, 312 + 8 us (the stretches,
-// their joining), 5.5 TB/s of keys and values, past a large copy's rate; one sequence of 200 tokens 6 us,
+// Measured: 33 sequences of 100 to 65536 tokens, a token each, 8 key heads of 128, 310 + 7 us (the stretches,
+// their joining), 5.6 TB/s of keys and values, past a large copy's rate; one sequence of 200 tokens 6 us,
 // the chain of its loads; 8 trees over 4000 tokens 23 + 7 us and four chunks of up to 512 tokens over
-// 12000, 128 wide, 76 + 15 us: there the matrix cores are 4-12% busy, the stretches being short (the rest
+// 12000, 16 heads of 128 over 2 with a window of 4096, 74 + 18 us: there the matrix cores are 4-12% busy, the stretches being short (the rest
 // is their start, softmax and partials).  Looking for values that are not finite costs 0.4 us of the
 // single sequence's 6, 1.5 of the trees' 23 and 2 of the chunks' 87.
 
