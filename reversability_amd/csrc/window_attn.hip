@@ -33,7 +33,7 @@
 // Measured (us; forward, dQ, dK/dV, sums; window and sinks behind the comma), with the rate over the
 // visible pairs' 4 + 10 HD flops:
 //   33 x 512, 8 heads of 32, 128 + 4, fp16          22   25        31   4.5    71 TFLOP/s
-//   3 x 1999, 20 heads of 64 over 4, 500 + 3, bf16  41   10 + 57   67  11     280
+//   3 x 1999, 20 heads of 64 over 4, 500 + 3, bf16  41   65        67  11     285
 //   2 x 16384, 10 heads of 128, 2048 + 4, bf16     440   17 + 565  990  14    600
 // Short windows are bound by the exponentials and masks (VALU 25-35% busy with the waits between, matrix
 // cores 14-20%), long ones by the matrix cores' feeding: 35% busy in the forward, 42% in dQ, 29% in
@@ -55,8 +55,6 @@ struct Geometry {
 // Workgroups per CU the register budget is sized for (attention.hip's figures).
 template <int HD>
 constexpr int kFwdMinBlocks = HD == 128 ? 2 : (HD == 64 ? 4 : 2);
-template <int HD>
-constexpr int kQMinBlocks = HD == 128 ? 2 : (HD == 64 ? 3 : 2);
 template <int HD>
 constexpr int kKvMinBlocks = HD == 128 ? 1 : 2;
 
@@ -351,12 +349,18 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
   }
 }
 
-// The first blocks of queries and the others in one launch or, at HD >= 64, where the first ones' products
-// cost the others registers, in two (at HD = 128 559 us against 1170 in one).
+// The first blocks of queries and the others in one launch or, where the first ones' products cost the
+// others registers, in two: at HD = 128 (559 us against 1170 in one), and at HD = 64 with more blocks than
+// the chip runs in a few rounds (16 x 2048, 16 heads 586 us forward and backward against 627, 2 x 16384,
+// 8 heads 723 against 762; 3 x 1999, 20 heads 184 against 179, 8 x 700, 8 heads 113 against 108).
 enum Part { kAll, kFirst, kOthers };
+constexpr int64_t kOneLaunch = 1024;  // blocks, at HD = 64
+
+template <int HD, Part PART>
+constexpr int kQMinBlocks = HD == 64 && PART != kAll ? 3 : 2;
 
 template <typename E, int HD, Part PART>
-__global__ __launch_bounds__(kThreads, kQMinBlocks<HD>)
+__global__ __launch_bounds__(kThreads, (kQMinBlocks<HD, PART>))
 void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
                    const E* __restrict__ rest, const E* __restrict__ dout,
                    const float* __restrict__ lse, float* __restrict__ delta, E* __restrict__ dqkv,
@@ -852,11 +856,16 @@ int launch_bwd(const void* qkv, const void* out, const void* rest, const void* d
                          static_cast<const E*>(out), static_cast<const E*>(rest), go, lse, delta,
                          dx, g, n_qt, c, (float)scale);
   };
+  bool two = HD >= 64;
+  if constexpr (HD < 128) {
+    two = HD == 64 && n_qt * bh > kOneLaunch;
+    if (!two) queries(wattn_bwd_q_k<E, HD, kAll>, n_qt);
+  }
   if constexpr (HD >= 64) {
-    queries(wattn_bwd_q_k<E, HD, kFirst>, 1);
-    queries(wattn_bwd_q_k<E, HD, kOthers>, n_qt - 1);
-  } else {
-    queries(wattn_bwd_q_k<E, HD, kAll>, n_qt);
+    if (two) {
+      queries(wattn_bwd_q_k<E, HD, kFirst>, 1);
+      queries(wattn_bwd_q_k<E, HD, kOthers>, n_qt - 1);
+    }
   }
   int rc = rv_host::check_launch();
   if (rc != RV_OK) return rc;

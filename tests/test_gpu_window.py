@@ -259,6 +259,28 @@ def test_gradients_of_a_frozen_input_and_twice(cuda_device):
     assert torch.equal(first, second)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_sequences_are_as_few(cuda_device, hd):
+    """A batch whose queries are launched in two parts: each sequence as in a smaller batch."""
+    heads, kv, seq, window, sinks = 6, 2, 300, 70, 3
+    qkv, dout = make(80, seq, heads, kv, hd, torch.float16, cuda_device, seed=3)
+
+    def grads(first, last):
+        x = qkv[first:last].detach().clone().requires_grad_(True)
+        out = window_attention(x, heads, window, sinks, kv_heads=kv)
+        return out.detach(), torch.autograd.grad(out, x, dout[first:last].contiguous())[0]
+    out, got = grads(0, 80)
+    own = slice(0, heads * hd)
+    for first in range(0, 80, 20):
+        few, part = grads(first, first + 20)
+        assert torch.equal(out[first:first + 20], few)
+        assert torch.equal(got[first:first + 20, :, own], part[:, :, own])
+    rows = torch.tensor([0, 41, 79], device=cuda_device)
+    out_ref, out_tol, ref, tol = reference(qkv.detach()[rows], dout[rows], heads, kv, window, sinks)
+    assert worst(out[rows], out_ref, out_tol) <= 1.0
+    assert worst(got[rows], ref, tol) <= 1.0
+
+
 def test_long_sequences_and_sinks(cuda_device):
     """Sinks summed over many queries keep their digits: errors as on short sequences."""
     heads, kv, hd, window, sinks = 2, 1, 64, 128, 3
