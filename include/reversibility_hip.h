@@ -665,7 +665,9 @@ int64_t rv_cached_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hea
  * positions before it and the first `sinks` positions.  A row that sees nothing is zeros;
  * rows of no sequence, and those past a sequence's first max_query, are left as they
  * were.  max_length: what a sequence holds at most (a longer one is still right, but
- * slower).  Pages outside [0, pages) hold nothing.  Deterministic. */
+ * slower).  Pages outside [0, pages) hold nothing; of new tokens that the page table has no
+ * room for the others are where rv_cache_plan puts them, and these see what is held (a sequence
+ * that has no room for its first new token is cut to what it has).  Deterministic. */
 int rv_cached_attn(const void* q, int64_t q_ld, const void* keys, const void* values,
                    const int32_t* page_table, int64_t ld_table, int64_t table_pages,
                    const int32_t* lengths, const int32_t* starts, const int64_t* tree,

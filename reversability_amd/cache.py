@@ -181,6 +181,9 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
     nothing gets zeros.  Returns ``out`` (contiguous, q's shape and type; None: a new
     tensor; not q's memory), whose rows of no sequence are left as they were.
 
+    New tokens that their sequence's pages have no room for see what the pages hold, the others
+    are where ``cache_plan`` puts them (a sequence without room for its first new token is
+    cut to its pages).
     Slots that no sequence's tokens hold are never used, whatever they contain.  Scores,
     statistics and sums in fp32, the weights rounded to the cache's type for the product with
     the values.  Deterministic."""

@@ -85,13 +85,17 @@ struct View {
     const int group = a.H / a.KV;
     start = min(max(a.starts[b], 0), a.tokens);
     const int end = min(max(a.starts[b + 1], start), a.tokens);
-    const int64_t held = a.table_pages << a.page_shift;
-    const int len = (int)min((int64_t)max(a.lengths[b], 0), min(held, (int64_t)1 << 30));
+    // The new tokens are where the plan puts them, also where the pages hold only some of them: what is
+    // cut to the pages is what can be read.  (A sequence whose pages do not even hold its first new
+    // token is cut as a whole: none of its new tokens was stored.)
+    const int held = (int)min(a.table_pages << a.page_shift, (int64_t)1 << 30);
+    int len = max(a.lengths[b], 0);
+    if (len - (end - start) >= held) len = held;
     context = len - (end - start);
     n = min(end - start, a.max_query);
     i0 = rb * rows / group;
     i1 = min(n - 1, (rb * rows + rows - 1) / group);
-    hi = min(len, a.tree ? context + n : context + i1 + 1);
+    hi = min(min(len, held), a.tree ? context + n : context + i1 + 1);
     lo = 0;
     if (a.window) lo = max(0, (a.tree ? context : context + i0 + 1) - a.window);
     count = sink_tiles = first = 0;

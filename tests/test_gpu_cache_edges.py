@@ -1,0 +1,76 @@
+"""Calls at the edges of the paged cache: pages that hold only some of a sequence's new tokens.
+Bounds are test_gpu_cache.py's."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from reversability_amd.cache import append_kv, cache_plan, cached_attention
+from test_gpu_cache import batch_of, check, filled, signed, slots_of, trees
+
+pytestmark = pytest.mark.gpu
+
+
+def seen_by(new, total, kept, masks, window, sinks):
+    """[new, kept]: which of the ``kept`` slots the last ``new`` of ``total`` tokens see."""
+    context, low = total - new, (1 << new) - 1
+    place = list(range(total))
+    if masks is not None:
+        for i in range(new):
+            place[context + i] = context + bin(masks[i] & low).count("1") - 1
+    seen = torch.zeros(new, kept, dtype=torch.bool)
+    for i in range(new):
+        for j in range(kept):
+            order = j <= context + i if masks is None else (
+                j < context or bool(masks[i] >> (j - context) & 1))
+            seen[i, j] = order and (window is None or place[context + i] - place[j] < window
+                                    or place[j] < sinks)
+    return seen
+
+
+def attend(q, k, v, seen):
+    """fp64 outputs of q [n, heads, hd] over k, v [kept, kv, hd], and their bounds."""
+    heads, hd = q.shape[1:]
+    u = torch.finfo(q.dtype).eps / 2
+    sub = torch.finfo(q.dtype).smallest_normal * u
+    k, v = (t.double().transpose(0, 1).repeat_interleave(heads // k.shape[1], 0).contiguous()
+            for t in (k, v))
+    seen = seen.to(q.device)
+    score = q.double().transpose(0, 1).contiguous() @ k.transpose(1, 2).contiguous() / math.sqrt(hd)
+    p = torch.softmax(score.masked_fill(~seen, -math.inf), -1).nan_to_num(0.0)
+    out = p @ v
+    few = seen.sum(1).view(1, -1, 1)
+    tol = 2 * (u * (p @ v.abs()) + u * out.abs() + sub * (1 + few * v.abs().max()))
+    return out.transpose(0, 1), tol.transpose(0, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,hd", [(2, 2, 32), (8, 2, 64), (12, 1, 128)])
+@pytest.mark.parametrize("new,over", [(4, 2), (1, 0), (30, 29), (30, 5), (64, 1)])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (9, 3)])
+def test_pages_that_hold_some_of_the_new_tokens(cuda_device, new, over, heads, kv, hd, dtype, tree,
+                                                window, sinks):
+    """Plan, append and attention agree on where the new tokens are: those that the pages hold see
+    themselves and what is in front of them, the ``over`` others what is held."""
+    page, kept = 16, 80
+    total = kept + over
+    table, _, starts, pages = batch_of([new], [kept], page, cuda_device, wide=0)
+    lengths = torch.tensor([total], dtype=torch.int32, device=cuda_device)
+    held = total - new  # the context
+    keys, values = filled(table, [held], pages, kv, page, hd, dtype, cuda_device)
+    g = torch.Generator().manual_seed(4)
+    qkv = (1.5 * torch.randn(new, (heads + 2 * kv) * hd, generator=g)).to(dtype).to(cuda_device)
+    masks = trees([new]) if tree else None
+    bits = signed(masks, cuda_device) if tree else None
+    slots, _ = cache_plan(table, lengths, starts, new, page, tree=bits)
+    every = slots_of(table, [kept], page)[0]
+    assert slots.tolist() == every[held:] + [-1] * over
+    q = append_kv(qkv, heads, keys, values, slots)
+    out = cached_attention(q, keys, values, table, lengths, starts, new, tree=bits, window=window,
+                           sinks=sinks)
+    at = torch.tensor(every, device=cuda_device)
+    k, v = (c.transpose(1, 2).reshape(-1, kv, hd)[at] for c in (keys, values))
+    check(out, *attend(q, k, v, seen_by(new, total, kept, masks, window, sinks)))
