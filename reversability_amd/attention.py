@@ -285,7 +285,8 @@ def window_attention(qkv: torch.Tensor, heads: int, window: int, sinks: int = 0,
     i sees key j <= i where i - j < ``window`` or j < ``sinks``.  Returns [B, T, heads hd] in
     qkv's type.  Scores, softmax statistics and sums are held in fp32; the weights are
     rounded to qkv's type for the product with the values, as are the scores'
-    gradients.  Deterministic.  As in any product, a NaN or an infinity in a key or value
+    gradients (in fp16 times a power of two that goes by the size of the gradient that
+    comes in: they keep their digits however small it is).  Deterministic.  As in any product, a NaN or an infinity in a key or value
     may reach queries that do not see it (and so may one in a query or gradient reach the
     gradients of keys it does not see)."""
     if qkv.ndim != 3:

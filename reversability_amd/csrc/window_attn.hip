@@ -298,6 +298,31 @@ void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__
 // ---------------------------------------------------------------------------
 // Backward.
 // ---------------------------------------------------------------------------
+// fp16's dS loses digits below 2^-14 and vanishes below 2^-25, where dK and dQ are sums of thousands
+// of such terms: gradients of 2^-10 came out three times as far off as their own rounding, those of
+// 2^-12 over 6000 tokens ten times.  Everything behind dO is linear in it, so dS is made of dO times
+// a power of two that brings its largest element into [1/4, 1/2) -- a query's own in dQ, that of a
+// tile of 64 queries in dK/dV, where the sums are moved from one power to the next -- and the sums
+// are divided by it: exact.  Never a smaller power than 1: gradients of 1/4 and more keep their bits.
+// (|dS| <= max |dO v| / 2: it overflows where values above 2000 agree with dO in sign in
+// every column.)  us of dQ and dK/dV in fp16, without and with: 33 x 512, heads of 32, 25.1 -> 27.1
+// and 31.3 -> 31.1; 3 x 1999, heads of 64, 64.7 -> 66.6 and 68.3 -> 70.4; 2 x 16384, heads of 128,
+// 600 -> 605 and 1058 -> 1120 (a power for each 32 queries 1240: the moves cut the loop's code).
+template <typename E>
+constexpr bool kScaled = false;
+template <>
+constexpr bool kScaled<_Float16> = true;
+
+// The power of two for gradients of at most `top`, itself a fp16 number.
+__device__ __forceinline__ float grad_scale(float top) {
+  const int exponent = (int)(__float_as_uint(top) >> 23 & 255u) - 127;  // top is in [2^e, 2^(e + 1))
+  return __uint_as_float((unsigned)(127 + min(max(-2 - exponent, 0), 15)) << 23);
+}
+// 1 / x of a power of two.
+__device__ __forceinline__ float inverse_power(float x) {
+  return __uint_as_float((254u << 23) - __float_as_uint(x));
+}
+
 // dQ contribution of 32 staged keys to one wave's 32 queries (lanes).  REST: what the roundings of dS
 // left is added by a product of its own.
 template <typename E, int HD, bool MASK, bool REST>
@@ -363,8 +388,9 @@ template <typename E, int HD, Part PART>
 __global__ __launch_bounds__(kThreads, (kQMinBlocks<HD, PART>))
 void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
                    const E* __restrict__ rest, const E* __restrict__ dout,
-                   const float* __restrict__ lse, float* __restrict__ delta, E* __restrict__ dqkv,
-                   Geometry g, int n_qt, float c, float scale) {
+                   const float* __restrict__ lse, float* __restrict__ delta,
+                   float* __restrict__ tops, E* __restrict__ dqkv, Geometry g, int n_qt, float c,
+                   float scale) {
   constexpr int KK = HD / 16, DT = HD / 32;
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][K / V]
   const int per = PART == kFirst ? 1 : PART == kOthers ? n_qt - 1 : n_qt;
@@ -400,8 +426,24 @@ void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
       dsum = fmaf((float)gf[kk][i], (float)of[i] + (float)ol[i], dsum);
   }
   const float Lq = qok ? lse[(int64_t)bh * g.T + q] : 0.f;
-  const float Dq = pair_sum(dsum);
+  float Dq = pair_sum(dsum);
   if (qok && hl == 0) delta[(int64_t)bh * g.T + q] = Dq;
+  if constexpr (kScaled<E>) {
+    float top = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf((float)gf[kk][i]));
+    top = pair_max(top);
+    const float power = grad_scale(top);
+    scale *= inverse_power(power);
+    Dq *= power;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) gf[kk] *= (E)power;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    if (lane == 0 && qok) tops[(int64_t)bh * ((g.T + 31) / 32) + q0 / 32] = top;
+  }
   f32x16 dq[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
@@ -464,13 +506,13 @@ void wattn_bwd_q_k(const E* __restrict__ qkv, const E* __restrict__ out,
 // dK/dV contribution of 32 staged queries (tile rows sub * 32 ..) to one wave's 32 keys
 // (lanes).  Query rows past the sequence hold zeros (Q, dO, lse, delta): their
 // P is 1 but dS = 0 and dO = 0, so they add nothing.  REST: what the roundings of P and dS left is
-// added by products of its own.
+// added by products of its own.  power: what dS is multiplied by (and Ds already is).
 template <typename E, int HD, bool MASK, bool REST>
 __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD / 32], const E* Qs,
                                         const E* Gs, const float* Ls, const float* Ds,
                                         const FragOffsets<HD, E>& fo, const x8<E> (&kf)[HD / 16],
                                         const x8<E> (&vf)[HD / 16], const Geometry& g, int sub,
-                                        int q0, int key, float c, int lane) {
+                                        int q0, int key, float c, float power, int lane) {
   constexpr int KK = HD / 16, DT = HD / 32;
   const int hl = lane >> 5;
   prio_mfma();
@@ -510,7 +552,7 @@ __device__ __forceinline__ void kv_rows(f32x16 (&dk)[HD / 32], f32x16 (&dv)[HD /
     for (int e = 0; e < 4; ++e) {
       const int j = 4 * jg + e;
       const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, -Lr[e]));
-      const float d = p * (dp[j] - Dr[e]);
+      const float d = p * (kScaled<E> ? fmaf(dp[j], power, -Dr[e]) : dp[j] - Dr[e]);
       const bool on = !MASK || seen(acc_row(j));
       s[j] = on ? p : 0.f;
       dp[j] = on ? d : 0.f;
@@ -564,7 +606,8 @@ __host__ __device__ inline int query_tiles(const Geometry& g, int kbase) {
 template <typename E, int HD, bool SINK>
 __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __restrict__ dout,
                                         const float* __restrict__ lse,
-                                        const float* __restrict__ delta, E* __restrict__ dqkv,
+                                        const float* __restrict__ delta,
+                                        const float* __restrict__ tops, E* __restrict__ dqkv,
                                         float* __restrict__ part, const Geometry& g,
                                         const KvPlan& plan, int number, float c, float scale,
                                         E (&lds)[2][2][kTile * HD], float (&rowv)[2][2][kTile]) {
@@ -605,6 +648,8 @@ __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __re
   const int first = chunk * len, last = min(first + len, group * per);
   TileCopy<HD> cq(rs), cg(os);
   float lv = 0.f, dvv = 0.f;
+  float top[2] = {0.f, 0.f};  // the largest |dO| of the halves of the tile under way
+  float power = 1.f;          // of the staged tile: what dk holds its sums times
   int head = first / per, tile = first % per;
   auto load = [&]() {  // the tile at (head, tile), then on to the next
     const int h = kvh * group + head, q0 = kbase + tile * kTile;
@@ -613,7 +658,29 @@ __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __re
     const int64_t row = ((int64_t)b * g.H + h) * g.T;
     lv = load_rowval(lse + row, q0, g.T);
     dvv = load_rowval(delta + row, q0, g.T);
+    if constexpr (kScaled<E>) {
+      const int groups = (g.T + 31) / 32;
+      const float* of_head = tops + ((int64_t)b * g.H + h) * groups;
+      top[0] = of_head[q0 / 32];
+      top[1] = of_head[min(q0 / 32 + 1, groups - 1)];
+    }
     if (++tile == per) tile = 0, ++head;
+  };
+  auto store_rows = [&](int buf) {
+    if constexpr (kScaled<E>) {
+      const float next = grad_scale(fmaxf(top[0], top[1]));
+      dvv *= next;
+      if (__float_as_uint(next) != __float_as_uint(power)) {  // (scalars)
+        const float turn = next * inverse_power(power);
+        power = next;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dk[dt] *= turn;
+      }
+    }
+    if (threadIdx.x < kTile) {
+      rowv[buf][0][threadIdx.x] = lv;
+      rowv[buf][1][threadIdx.x] = dvv;
+    }
   };
   const FragOffsets<HD, E> fo(lane);
   int now = first % per;  // the staged tile
@@ -621,11 +688,11 @@ __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __re
     load();
     cq.store(lds[0][0]);
     cg.store(lds[0][1]);
-    if (threadIdx.x < kTile) {
-      rowv[0][0][threadIdx.x] = lv;
-      rowv[0][1][threadIdx.x] = dvv;
-    }
+    store_rows(0);
   }
+  // vmcnt(0): K and V are there.  The compiler does not know it where no tile was loaded, and would
+  // wait for the tile under way in every step.
+  __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 #define RV_KV_STEP(BUF)                                                                       \
   {                                                                                           \
@@ -638,21 +705,20 @@ __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __re
       if (none_seen(g, qs, k0w, kWaveRows)) continue;                                         \
       if constexpr (SINK)                                                                      \
         kv_rows<E, HD, true, true>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],             \
-                                   rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);        \
+                                   rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, power, lane); \
       else if (all_seen(g, qs, k0w, kWaveRows))                                                \
         kv_rows<E, HD, false, false>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],           \
-                                     rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);      \
+                                     rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, power,      \
+                                     lane);                                                    \
       else                                                                                     \
         kv_rows<E, HD, true, false>(dk, dv, lds[BUF][0], lds[BUF][1], rowv[BUF][0],            \
-                                    rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, lane);       \
+                                    rowv[BUF][1], fo, kf, vf, g, sub, qs, key, c, power,       \
+                                    lane);                                                     \
     }                                                                                         \
     if (more) {                                                                               \
       cq.store(lds[1 - (BUF)][0]);                                                            \
       cg.store(lds[1 - (BUF)][1]);                                                            \
-      if (threadIdx.x < kTile) {                                                              \
-        rowv[1 - (BUF)][0][threadIdx.x] = lv;                                                 \
-        rowv[1 - (BUF)][1][threadIdx.x] = dvv;                                                \
-      }                                                                                       \
+      store_rows(1 - (BUF));                                                                  \
     }                                                                                         \
     __syncthreads();                                                                          \
   }
@@ -663,6 +729,11 @@ __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __re
   }
 #undef RV_KV_STEP
   if (key >= g.T) return;
+  if constexpr (kScaled<E>) {
+    const float back = inverse_power(power);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dk[dt] *= back;
+  }
   if (chunks > 1) {  // [unit][K / V][128][HD] fp32
     float* row = part + (((int64_t)number * 2) * kBlockRows + key - kbase) * HD;
 #pragma unroll
@@ -696,15 +767,16 @@ template <typename E, int HD>
 __global__ __launch_bounds__(kThreads, kKvMinBlocks<HD>)
 void wattn_bwd_kv_k(const E* __restrict__ qkv, const E* __restrict__ dout,
                     const float* __restrict__ lse, const float* __restrict__ delta,
-                    E* __restrict__ dqkv, float* __restrict__ part, Geometry g, KvPlan plan,
-                    float c, float scale) {
+                    const float* __restrict__ tops, E* __restrict__ dqkv,
+                    float* __restrict__ part, Geometry g, KvPlan plan, float c, float scale) {
   __shared__ __attribute__((aligned(16))) E lds[2][2][kTile * HD];  // [buf][Q / dO]
   __shared__ __attribute__((aligned(16))) float rowv[2][2][kTile];  // [buf][lse / delta]
   const int number = near_index();
   if (number % plan.units() < plan.sink_blocks * plan.sink_chunks)
-    kv_unit<E, HD, true>(qkv, dout, lse, delta, dqkv, part, g, plan, number, c, scale, lds, rowv);
+    kv_unit<E, HD, true>(qkv, dout, lse, delta, tops, dqkv, part, g, plan, number, c, scale, lds,
+                         rowv);
   else
-    kv_unit<E, HD, false>(qkv, dout, lse, delta, dqkv, part, g, plan, number, c, scale, lds,
+    kv_unit<E, HD, false>(qkv, dout, lse, delta, tops, dqkv, part, g, plan, number, c, scale, lds,
                           rowv);
 }
 
@@ -797,6 +869,15 @@ KvPlan kv_plan(const Geometry& g, int64_t batch, int64_t hd) {
   return best;
 }
 
+// The workspace: delta, one fp32 a query and head, the largest |dO| of every 32 of them, and the
+// partials, each from a multiple of four values on.
+int64_t delta_values(int64_t batch, int64_t heads, int64_t seq) {
+  return (batch * heads * seq + 3) / 4 * 4;
+}
+int64_t top_values(int64_t batch, int64_t heads, int64_t seq) {
+  return (batch * heads * ((seq + 31) / 32) + 3) / 4 * 4;
+}
+
 int64_t partial_bytes(const KvPlan& p, int64_t outer, int64_t hd) {
   if (p.near_chunks == 1 && p.sink_chunks == 1) return 0;
   return outer * p.units() * 2 * kBlockRows * hd * 4;
@@ -842,19 +923,19 @@ int launch_bwd(const void* qkv, const void* out, const void* rest, const void* d
   const double scale = 1.0 / std::sqrt((double)HD);
   const float c = (float)(1.4426950408889634 * scale);
   const KvPlan plan = kv_plan(g, batch, HD);
-  const int64_t rows = batch * g.H * g.T;
   float* delta = ws;
-  float* part = ws + (rows + 3) / 4 * 4;
+  float* tops = delta + delta_values(batch, g.H, g.T);
+  float* part = tops + top_values(batch, g.H, g.T);
   const E* x = static_cast<const E*>(qkv);
   const E* go = static_cast<const E*>(dout);
   E* dx = static_cast<E*>(dqkv);
-  // the dQ kernel writes delta, which the dK/dV kernel reads
+  // the dQ kernel writes delta and tops, which the dK/dV kernel reads
   const int64_t bh = batch * g.H;
   auto queries = [&](auto kernel, int blocks) {
     if (blocks)
       hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * bh)), dim3(kThreads), 0, s, x,
                          static_cast<const E*>(out), static_cast<const E*>(rest), go, lse, delta,
-                         dx, g, n_qt, c, (float)scale);
+                         tops, dx, g, n_qt, c, (float)scale);
   };
   bool two = HD >= 64;
   if constexpr (HD < 128) {
@@ -870,7 +951,8 @@ int launch_bwd(const void* qkv, const void* out, const void* rest, const void* d
   int rc = rv_host::check_launch();
   if (rc != RV_OK) return rc;
   hipLaunchKernelGGL((wattn_bwd_kv_k<E, HD>), dim3((unsigned)(plan.units() * batch * g.KV)),
-                     dim3(kThreads), 0, s, x, go, lse, delta, dx, part, g, plan, c, (float)scale);
+                     dim3(kThreads), 0, s, x, go, lse, delta, tops, dx, part, g, plan, c,
+                     (float)scale);
   rc = rv_host::check_launch();
   if (rc != RV_OK) return rc;
   const int cut = (plan.sink_chunks > 1 ? plan.sink_blocks : 0) +
@@ -914,7 +996,8 @@ int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t h
   if (!args_ok(batch, seq, heads, kv_heads, head_dim, window, sinks)) return -RV_ERR_BAD_SIZE;
   if (!sizes_ok(batch, seq, heads, kv_heads, head_dim, RV_F16)) return -RV_ERR_UNSUPPORTED;
   const KvPlan p = kv_plan(geometry(seq, heads, kv_heads, window, sinks), batch, head_dim);
-  return (batch * heads * seq + 3) / 4 * 16 + partial_bytes(p, batch * kv_heads, head_dim);
+  return (delta_values(batch, heads, seq) + top_values(batch, heads, seq)) * 4 +
+         partial_bytes(p, batch * kv_heads, head_dim);
 }
 
 int rv_window_attn_bwd(const void* qkv, const void* out, const void* rest, const void* dout,
