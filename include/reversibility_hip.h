@@ -664,7 +664,7 @@ int64_t rv_cached_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t hea
  * what its mask has; with a window (0: none) of these the tokens less than `window`
  * positions before it and the first `sinks` positions.  A row that sees nothing is zeros;
  * rows of no sequence, and those past a sequence's first max_query, are left as they
- * were.  max_length: what a sequence holds at most (a longer one is still right, but
+ * were.  out must not overlap q, keys or values (RV_ERR_UNSUPPORTED).  max_length: what a sequence holds at most (a longer one is still right, but
  * slower).  Pages outside [0, pages) hold nothing; of new tokens that the page table has no
  * room for the others are where rv_cache_plan puts them, and these see what is held (a sequence
  * that has no room for its first new token is cut to what it has).  Deterministic. */

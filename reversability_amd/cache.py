@@ -179,7 +179,7 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
     ``tree`` its context and what its mask has; with ``window`` of these the tokens less than
     ``window`` positions before it and the first ``sinks`` positions.  A token that sees
     nothing gets zeros.  Returns ``out`` (contiguous, q's shape and type; None: a new
-    tensor; not q's memory), whose rows of no sequence are left as they were.
+    tensor; memory of its own), whose rows of no sequence are left as they were.
 
     New tokens that their sequence's pages have no room for see what the pages hold, the others
     are where ``cache_plan`` puts them (a sequence without room for its first new token is
@@ -215,9 +215,12 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned tensor like q")
-    elif tokens and (out.data_ptr() < q.data_ptr() + q.stride(0) * (tokens - 1) * 2 + heads * hd * 2
-                     and q.data_ptr() < out.data_ptr() + out.numel() * 2):
-        raise ValueError("out must not overlap q")
+    else:
+        first, last = out.data_ptr(), out.data_ptr() + out.numel() * 2
+        for t, values_of in ((q, q.stride(0) * (tokens - 1) + heads * hd), (keys, keys.numel()),
+                             (values, keys.numel())):
+            if tokens and first < t.data_ptr() + values_of * 2 and t.data_ptr() < last:
+                raise ValueError("out must not overlap q, keys or values")
     paths.took("cached_attention", "hip")
     if not tokens:
         return out

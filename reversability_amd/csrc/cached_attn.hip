@@ -996,6 +996,11 @@ bool sizes_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t hd, int64_t m
          max_query * heads < (1 << 30);
 }
 
+bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  const uint64_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
 // A launch has fewer than 2^32 threads.
 bool launch_ok(int64_t seqs, int64_t heads, int64_t kv, int64_t max_query, const Plan& p) {
   return (seqs * kv * p.splits + 7) * p.row_blocks < (1 << 24) &&
@@ -1064,6 +1069,12 @@ int rv_cached_attn(const void* q, int64_t q_ld, const void* keys, const void* va
   const int64_t need = workspace_bytes(tokens, heads, head_dim, p);
   if (need && (!workspace || workspace_bytes_given < need)) return RV_ERR_WORKSPACE;
   if (!tokens) return RV_OK;
+  // other workgroups still read what one has written over
+  const uint64_t row = heads * head_dim * 2, size = tokens * row;
+  const uint64_t cache = (uint64_t)pages * kv_heads * page_size * head_dim * 2;
+  if (overlap(out, size, q, (tokens - 1) * (uint64_t)q_ld * 2 + row) ||
+      overlap(out, size, keys, cache) || overlap(out, size, values, cache))
+    return RV_ERR_UNSUPPORTED;
   Cached a{};
   a.q = q, a.keys = keys, a.values = values, a.out = out;
   a.table = page_table, a.lengths = lengths, a.starts = starts, a.tree = tree;

@@ -226,3 +226,20 @@ def test_partials_of_long_chunks_are_bounded():
                 # 2048 blocks of 128 rows and one more for each row, of 130 fp32 values
                 most = (2048 * 128 + max(query * 32, 2048 * 128)) * 130 * 4
                 assert 0 <= nbytes <= seqs * most, (seqs, query, length, nbytes)
+
+
+def test_cached_attention_refuses_an_output_in_its_operands():
+    """Three tokens of 64 values (384 bytes) and caches of 9216: one byte more on either side of an
+    operand is refused, also where the rows of q are strided."""
+    lib = _hip.library()
+    at = ctypes.c_void_p
+    q, keys, values = 1 << 20, 2 << 20, 3 << 20
+
+    def call(out, ld=64):
+        return lib.rv_cached_attn(at(q), ld, at(keys), at(values), at(4096), 8, 8, at(4096), at(4096),
+                                  None, 3, 2, 2, 1, 32, _hip.RV_F16, 9, 16, 1, 64, 0, 0, at(out),
+                                  None, 0, None)
+    for first, size in ((q, 384), (keys, 9216), (values, 9216)):
+        for out in (first, first - 368, first + size - 16):
+            assert call(out) == 3
+    assert call(q + 2048 + 112, ld=512) == 3  # (rows at 0, 1024 and 2048 bytes)

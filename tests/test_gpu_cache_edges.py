@@ -74,3 +74,16 @@ def test_pages_that_hold_some_of_the_new_tokens(cuda_device, new, over, heads, k
     at = torch.tensor(every, device=cuda_device)
     k, v = (c.transpose(1, 2).reshape(-1, kv, hd)[at] for c in (keys, values))
     check(out, *attend(q, k, v, seen_by(new, total, kept, masks, window, sinks)))
+
+
+def test_outputs_in_the_cache_are_refused(cuda_device):
+    table, lengths, starts, pages = batch_of([1, 1], [20, 5], 16, cuda_device)
+    keys, values = filled(table, [20, 5], pages, 2, 16, 32, torch.float16, cuda_device)
+    q = torch.randn(2, 4, 32, device=cuda_device).half()
+    for side in (keys, values):
+        before = side.clone()
+        for first in (0, side.numel() - 256):
+            out = side.view(-1)[first:first + 256].view(2, 4, 32)
+            with pytest.raises(ValueError, match="overlap"):
+                cached_attention(q, keys, values, table, lengths, starts, 1, out=out)
+        assert torch.equal(side.nan_to_num(9), before.nan_to_num(9))
