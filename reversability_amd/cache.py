@@ -75,15 +75,23 @@ def _ints(t: torch.Tensor, shape: tuple, like: torch.Tensor, what: str,
     return t.contiguous()
 
 
+def _row_stride(t: torch.Tensor, width: int) -> int:
+    """The stride of rows of ``width``.  That of a lone row may be anything (torch ignores it, and
+    ``contiguous()`` leaves it): it has no next row, and gets its width."""
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
 def _sequences(page_table, lengths, starts, like, what):
-    """The batch's description, checked; the page table keeps its row stride."""
+    """The batch's description, checked; the page table keeps its row stride, which is returned
+    behind it."""
     if (page_table.dtype != torch.int32 or page_table.ndim != 2 or not page_table.numel()
             or page_table.device != like.device):
         raise ValueError(f"{what} needs an int32 page_table [sequences, pages] on its device")
     seqs = page_table.shape[0]
-    if page_table.stride(1) != 1 or page_table.stride(0) < page_table.shape[1]:
+    columns = page_table.shape[1]
+    if page_table.stride(1) != 1 or _row_stride(page_table, columns) < columns:
         page_table = page_table.contiguous()
-    return (page_table, _ints(lengths, (seqs,), like, "lengths"),
+    return (page_table, _row_stride(page_table, columns), _ints(lengths, (seqs,), like, "lengths"),
             _ints(starts, (seqs + 1,), like, "starts"))
 
 
@@ -97,7 +105,7 @@ def cache_plan(page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Te
     if not page_table.is_cuda or page_size not in PAGE_SIZES or tokens < 0:
         raise ValueError(f"cache_plan needs CUDA (ROCm device) tensors, a page size in "
                          f"{PAGE_SIZES} and tokens >= 0")
-    table, lengths, starts = _sequences(page_table, lengths, starts, page_table, "cache_plan")
+    table, ld, lengths, starts = _sequences(page_table, lengths, starts, page_table, "cache_plan")
     if tree is not None:
         tree = _ints(tree, (tokens,), table, "tree", torch.int64)
     slots = torch.empty(tokens, device=table.device, dtype=torch.int64)
@@ -105,7 +113,7 @@ def cache_plan(page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Te
     with _DeviceGuard(table):
         if tokens:
             _check(library().rv_cache_plan(
-                table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+                table.data_ptr(), ld, table.shape[1], lengths.data_ptr(),
                 starts.data_ptr(), None if tree is None else tree.data_ptr(), table.shape[0],
                 tokens, page_size, slots.data_ptr(), positions.data_ptr(), _stream(table)),
                 "rv_cache_plan")
@@ -127,11 +135,12 @@ def append_kv(qkv: torch.Tensor, heads: int, keys: torch.Tensor, values: torch.T
     if qkv.dtype != keys.dtype or qkv.device != keys.device or hd != keys.shape[3]:
         raise ValueError("append_kv needs qkv of the cache's type, head size and device")
     rows = qkv if qkv.ndim == 2 else qkv.reshape(-1, qkv.shape[-1])
-    if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.stride(0) < rows.shape[1]:
-        rows = rows.contiguous()
+    n, width = rows.shape
+    ld = _row_stride(rows, width)
+    if rows.stride(1) != 1 or ld % 8 or ld < width:
+        rows, ld = rows.contiguous(), width
     if rows.data_ptr() % 16:
-        rows = rows.clone()
-    n = rows.shape[0]
+        rows, ld = rows.clone(memory_format=torch.contiguous_format), width
     slots = _ints(slots, (n,), keys, "slots", torch.int64)
     turn = (None, 0, None, False)
     if rotary is None:
@@ -148,7 +157,7 @@ def append_kv(qkv: torch.Tensor, heads: int, keys: torch.Tensor, values: torch.T
     if n:
         with _DeviceGuard(keys):
             _check(library().rv_append_kv(
-                rows.data_ptr(), rows.stride(0), q.data_ptr() if rotary is not None else None,
+                rows.data_ptr(), ld, q.data_ptr() if rotary is not None else None,
                 keys.data_ptr(), values.data_ptr(), slots.data_ptr(), n, heads, kv, hd,
                 _CODES[keys.dtype], keys.shape[0], keys.shape[2], *turn, _stream(keys)),
                 "rv_append_kv")
@@ -196,7 +205,8 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
                          "size and device, heads a multiple of its kv_heads")
     check_window(window, sinks, "cached_attention")
     tokens, heads = q.shape[:2]
-    table, lengths, starts = _sequences(page_table, lengths, starts, keys, "cached_attention")
+    table, table_ld, lengths, starts = _sequences(page_table, lengths, starts, keys,
+                                                  "cached_attention")
     held = table.shape[1] * page
     if max_query < 1 or (max_length is not None and max_length < 1):
         raise ValueError("cached_attention needs max_query and max_length >= 1")
@@ -205,9 +215,10 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
         tree = _ints(tree, (tokens,), keys, "tree", torch.int64)
         if max_query > 64:
             raise ValueError("cached_attention takes trees of at most 64 tokens a sequence")
-    if (q.stride(2) != 1 or q.stride(1) != hd or q.stride(0) % 8 or q.stride(0) < heads * hd
+    q_ld = _row_stride(q, heads * hd)
+    if (q.stride(2) != 1 or q.stride(1) != hd or q_ld % 8 or q_ld < heads * hd
             or q.data_ptr() % 16):
-        q = q.contiguous()
+        q, q_ld = q.contiguous(), heads * hd
         q = q if q.data_ptr() % 16 == 0 else q.clone()
     if out is None:
         out = (torch.empty_like(q) if q.is_contiguous() else
@@ -217,7 +228,7 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
         raise ValueError("out must be a contiguous, 16-byte aligned tensor like q")
     else:
         first, last = out.data_ptr(), out.data_ptr() + out.numel() * 2
-        for t, values_of in ((q, q.stride(0) * (tokens - 1) + heads * hd), (keys, keys.numel()),
+        for t, values_of in ((q, q_ld * (tokens - 1) + heads * hd), (keys, keys.numel()),
                              (values, keys.numel())):
             if tokens and first < t.data_ptr() + values_of * 2 and t.data_ptr() < last:
                 raise ValueError("out must not overlap q, keys or values")
@@ -230,8 +241,8 @@ def cached_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
     with _DeviceGuard(q):
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
         _check(lib.rv_cached_attn(
-            q.data_ptr(), q.stride(0), keys.data_ptr(), values.data_ptr(), table.data_ptr(),
-            table.stride(0), table.shape[1], lengths.data_ptr(), starts.data_ptr(),
+            q.data_ptr(), q_ld, keys.data_ptr(), values.data_ptr(), table.data_ptr(),
+            table_ld, table.shape[1], lengths.data_ptr(), starts.data_ptr(),
             None if tree is None else tree.data_ptr(), *sizes, _CODES[q.dtype], pages, page,
             max_query, max_length, *span, out.data_ptr(), None if ws is None else ws.data_ptr(),
             nbytes, _stream(q)), "rv_cached_attn")

@@ -87,3 +87,54 @@ def test_outputs_in_the_cache_are_refused(cuda_device):
             with pytest.raises(ValueError, match="overlap"):
                 cached_attention(q, keys, values, table, lengths, starts, 1, out=out)
         assert torch.equal(side.nan_to_num(9), before.nan_to_num(9))
+
+
+def test_lone_rows_of_any_stride(cuda_device):
+    """One token, one sequence, one head, one page: torch lets the stride of a size of one be
+    anything, and calls it contiguous."""
+    table, lengths, starts, pages = batch_of([1], [40], 16, cuda_device)
+    keys, values = filled(table, [40], pages, 2, 16, 64, torch.float16, cuda_device)
+    plain = torch.randn(1, 4, 64, device=cuda_device).half()
+    want = cached_attention(plain, keys, values, table, lengths, starts, 1)
+    wide = torch.zeros(1, 515, device=cuda_device, dtype=torch.float16)
+    wide[:, :256] = plain.view(1, 256)
+    shifted = torch.zeros(1, 515, device=cuda_device, dtype=torch.float16)
+    shifted[:, 1:257] = plain.view(1, 256)
+    for q in (plain.transpose(0, 1).contiguous().transpose(0, 1), wide[:, :256].view(1, 4, 64),
+              shifted[:, 1:257].view(1, 4, 64), plain.as_strided(plain.shape, (0, 64, 1)),
+              plain.as_strided(plain.shape, (3, 64, 1))):
+        out = torch.empty_like(want)
+        assert torch.equal(cached_attention(q, keys, values, table, lengths, starts, 1), want)
+        assert cached_attention(q, keys, values, table, lengths, starts, 1, out=out) is out
+        assert torch.equal(out, want)
+    turned = table.reshape(-1, 1).clone().t()  # one sequence: strides (1, 1)
+    assert turned.stride() == (1, 1) and torch.equal(turned, table)
+    assert torch.equal(cached_attention(plain, keys, values, turned, lengths, starts, 1), want)
+    slots, positions = cache_plan(table, lengths, starts, 1, 16)
+    for got, ref in zip(cache_plan(turned, lengths, starts, 1, 16), (slots, positions)):
+        assert torch.equal(got, ref)
+    lone = table[:, :1]  # one page, of every stride
+    few = torch.tensor([9], dtype=torch.int32, device=cuda_device)
+    first = cached_attention(plain, keys, values, lone.contiguous(), few, starts, 1)
+    for strides in ((1, 1), (0, 7), (7, 0), (1, 5)):
+        odd = lone.as_strided((1, 1), strides)
+        assert torch.equal(cached_attention(plain, keys, values, odd, few, starts, 1), first)
+    # one row to append, from rows of a stride that no two rows could have
+    qkv = torch.randn(1, 512, device=cuda_device).half()
+    after = []
+    for rows in (qkv, torch.cat([qkv, qkv[:, :3]], 1)[:, :512], qkv.as_strided((1, 512), (5, 1)),
+                 torch.cat([qkv[:, :1], qkv], 1)[:, 1:], qkv.as_strided((1, 1, 512), (7, 3, 1))):
+        kept = [c.clone() for c in (keys, values)]
+        q = append_kv(rows, 4, *kept, slots)
+        assert torch.equal(q, qkv[:, :256].view(1, 4, 64))
+        # (q, a view of such rows, goes on to the attention)
+        after.append([cached_attention(q, *kept, table, lengths, starts, 1), *kept])
+    for other in after[1:]:
+        assert all(torch.equal(a.nan_to_num(9), b.nan_to_num(9)) for a, b in zip(after[0], other))
+    # one head
+    table, lengths, starts, pages = batch_of([2], [20], 16, cuda_device)
+    keys, values = filled(table, [20], pages, 1, 16, 32, torch.float16, cuda_device)
+    q = torch.randn(2, 1, 32, device=cuda_device).half()
+    want = cached_attention(q, keys, values, table, lengths, starts, 2)
+    odd = q.as_strided((2, 1, 32), (32, 5, 1))
+    assert torch.equal(cached_attention(odd, keys, values, table, lengths, starts, 2), want)
