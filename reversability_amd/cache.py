@@ -319,7 +319,8 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
     sinks and a rotation are those of ``enable_attention``.  Logits are what the model's own
     forward pass gives for the whole sequences, but for roundings; dropout is not applied.
     Logits of rows of no sequence have no meaning (their ids must be of the vocabulary all the
-    same); no sequence may have more than ``batch.max_query`` of them.  ``batch.max_length`` must
+    same); no sequence may have more than ``batch.max_query`` of them (those past it attend to
+    nothing).  ``batch.max_length`` must
     not exceed the model's ``max_sequence_length``, nor the positions of its ``Rotary``
     (positions past the former, which only a wrong max_length lets through, are taken as its
     last).  The keys and values of one call's tokens need slots of their own: sequences may
@@ -343,6 +344,12 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
     slots, positions = cache_plan(batch.page_table, batch.lengths, batch.starts, ids.shape[0],
                                   cache.page_size, batch.tree)
 
+    # what the attention does not write (rows of no sequence or past max_query) are zeros, not what the
+    # memory held: the layers behind it append keys made from them
+    first = model.blocks[0].attn
+    seen = torch.zeros(ids.shape[0], first.n_heads, first.head_dim, device=ids.device,
+                       dtype=cache.keys.dtype)
+
     def attend(layer, x):
         attn = model.blocks[layer].attn
         keys, values = cache.keys[layer], cache.values[layer]
@@ -351,7 +358,7 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
         mixed = cached_attention(q, keys, values, batch.page_table, batch.lengths, batch.starts,
                                  batch.max_query, max_length=batch.max_length, tree=batch.tree,
                                  window=getattr(attn, "_rv_window", None),
-                                 sinks=getattr(attn, "_rv_sinks", 0))
+                                 sinks=getattr(attn, "_rv_sinks", 0), out=seen)
         return attn.proj(mixed.flatten(1).unsqueeze(0))
 
     with weight_cast_cache(), amp_context(ids.device, precision):

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from reversability_amd.cache import append_kv, cache_plan, cached_attention
-from test_gpu_cache import batch_of, check, filled, signed, slots_of, trees
+from test_gpu_cache import _model, batch_of, check, filled, signed, slots_of, trees
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,34 @@ def test_lone_rows_of_any_stride(cuda_device):
     want = cached_attention(q, keys, values, table, lengths, starts, 2)
     odd = q.as_strided((2, 1, 32), (32, 5, 1))
     assert torch.equal(cached_attention(odd, keys, values, table, lengths, starts, 2), want)
+
+
+@pytest.fixture
+def marked_memory():
+    """New tensors that nothing is written to hold NaN."""
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    assert torch.utils.deterministic.fill_uninitialized_memory
+    yield
+    torch.use_deterministic_algorithms(False)
+
+
+@pytest.mark.parametrize("method,fused", [("baseline", False), ("midpoint", True), ("euler", False)])
+def test_decode_appends_nothing_that_was_not_computed(cuda_device, marked_memory, method, fused):
+    """Rows of no sequence, and tokens past ``max_query``: finite logits, keys and values, and the
+    other sequence's as without them."""
+    from reversability_amd.cache import CacheBatch, PagedCache, decode
+    model = _model(method, cuda_device, 20, 2, True, fused)
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    table = as_int([[0, 1], [2, 3]])
+    ids = torch.randint(0, 97, (12,), device=cuda_device)
+    caches = [PagedCache.for_model(model, pages=4, page_size=16) for _ in range(2)]
+    # five new tokens and two where two are allowed; three rows of no sequence
+    logits = decode(model, ids, caches[0], CacheBatch(table, as_int([5, 2]), as_int([1, 6, 8]), 2, 32))
+    assert torch.isfinite(logits).all()
+    assert all(torch.isfinite(t).all() for t in (caches[0].keys, caches[0].values))
+    want = decode(model, ids[6:8].clone(), caches[1],
+                  CacheBatch(table[1:], as_int([2]), as_int([0, 2]), 2, 32))
+    # (products over more rows may round otherwise)
+    assert torch.allclose(logits[6:8], want, atol=4e-3)
+    for a, b in ((caches[0].keys, caches[1].keys), (caches[0].values, caches[1].values)):
+        assert torch.allclose(a[:, 2:], b[:, 2:], atol=4e-3)
