@@ -303,7 +303,7 @@ void wattn_fwd_k(const E* __restrict__ qkv, E* __restrict__ out, E* __restrict__
 // 2^-12 over 6000 tokens ten times.  Everything behind dO is linear in it, so dS is made of dO times
 // a power of two that brings its largest element into [1/4, 1/2) -- a query's own in dQ, that of a
 // tile of 64 queries in dK/dV, where the sums are moved from one power to the next -- and the sums
-// are divided by it: exact.  Never a smaller power than 1: gradients of 1/4 and more keep their bits.
+// are divided by it: exact.  Never a smaller power than 1: gradients of 1/4 and more are as they are.
 // (|dS| <= max |dO v| / 2: it overflows where values above 2000 agree with dO in sign in
 // every column.)  us of dQ and dK/dV in fp16, without and with: 33 x 512, heads of 32, 25.1 -> 27.1
 // and 31.3 -> 31.1; 3 x 1999, heads of 64, 64.7 -> 66.6 and 68.3 -> 70.4; 2 x 16384, heads of 128,
@@ -591,6 +591,11 @@ struct KvPlan {
   __host__ __device__ int units() const {
     return sink_blocks * sink_chunks + (blocks - sink_blocks) * near_chunks;
   }
+  // Only units of blocks that are cut write partials: the sinks', then the others'.
+  __host__ __device__ int cut_sinks() const { return sink_chunks > 1 ? sink_blocks * sink_chunks : 0; }
+  __host__ __device__ int cut_units() const {
+    return cut_sinks() + (near_chunks > 1 ? (blocks - sink_blocks) * near_chunks : 0);
+  }
 };
 
 // Tiles of queries that see a key of the block at kbase, the first of them kbase / kTile.
@@ -734,8 +739,9 @@ __device__ __forceinline__ void kv_unit(const E* __restrict__ qkv, const E* __re
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dk[dt] *= back;
   }
-  if (chunks > 1) {  // [unit][K / V][128][HD] fp32
-    float* row = part + (((int64_t)number * 2) * kBlockRows + key - kbase) * HD;
+  if (chunks > 1) {  // [cut unit][K / V][128][HD] fp32
+    const int64_t place = (int64_t)bkv * plan.cut_units() + at + (SINK ? 0 : plan.cut_sinks());
+    float* row = part + (place * 2 * kBlockRows + key - kbase) * HD;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -792,10 +798,8 @@ void wattn_reduce_k(const float* __restrict__ part, E* __restrict__ dqkv, Geomet
   if (plan.sink_chunks == 1) kt += plan.sink_blocks;  // only the others are cut
   const bool sink = kt < plan.sink_blocks;
   const int chunks = sink ? plan.sink_chunks : plan.near_chunks;
-  const int64_t unit = (int64_t)blockIdx.y * plan.units() +
-                       (sink ? kt * chunks
-                             : plan.sink_blocks * plan.sink_chunks +
-                                   (kt - plan.sink_blocks) * chunks);
+  const int64_t unit = (int64_t)blockIdx.y * plan.cut_units() +
+                       (sink ? kt * chunks : plan.cut_sinks() + (kt - plan.sink_blocks) * chunks);
   const int b = (int)blockIdx.y / g.KV, kvh = (int)blockIdx.y % g.KV;
   const float factor = side ? 1.f : scale;
   for (int i = threadIdx.x; i < 32 * HD / 4; i += kThreads) {
@@ -856,9 +860,7 @@ KvPlan kv_plan(const Geometry& g, int64_t batch, int64_t hd) {
     double steps = (double)rounds * (std::max(near ? (double)p.near_len : 0.0,
                                               p.sink_blocks ? kSinkStep * p.sink_len : 0.0) + 3);
     if (p.near_chunks > 1 || p.sink_chunks > 1) {
-      const int64_t cut = (p.near_chunks > 1 ? (p.blocks - p.sink_blocks) * p.near_chunks : 0) +
-                          (p.sink_chunks > 1 ? p.sink_blocks * p.sink_chunks : 0);
-      steps += 2 + (double)(outer * cut) * 2 * kBlockRows * hd * 4 * 2 / 4e12 / 2e-6;
+      steps += 2 + (double)(outer * p.cut_units()) * 2 * kBlockRows * hd * 4 * 2 / 4e12 / 2e-6;
     }
     if (i == 2 || steps < least) {
       least = steps;
@@ -879,8 +881,7 @@ int64_t top_values(int64_t batch, int64_t heads, int64_t seq) {
 }
 
 int64_t partial_bytes(const KvPlan& p, int64_t outer, int64_t hd) {
-  if (p.near_chunks == 1 && p.sink_chunks == 1) return 0;
-  return outer * p.units() * 2 * kBlockRows * hd * 4;
+  return outer * p.cut_units() * 2 * kBlockRows * hd * 4;
 }
 
 // Sizes the kernels take: a kTile-row tile of qkv spans less than 2 GiB, so a tile's

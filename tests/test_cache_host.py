@@ -243,3 +243,21 @@ def test_cached_attention_refuses_an_output_in_its_operands():
         for out in (first, first - 368, first + size - 16):
             assert call(out) == 3
     assert call(q + 2048 + 112, ld=512) == 3  # (rows at 0, 1024 and 2048 bytes)
+
+
+def test_partials_of_windows_are_those_of_cut_blocks():
+    """The backward's workspace: D and the largest |dO| of 32 queries a head, and fp32 partials of
+    the keys' gradients.  At sizes where the keys behind the sinks' fill the chip uncut, only the
+    sinks' blocks have them: at most 4096 chunks and one more a block, 128 keys and values each, and
+    less than qkv itself."""
+    size = _hip.library().rv_window_attn_bwd_workspace_bytes
+    for batch, seq, heads, kv, hd, window, sinks in (
+            (2, 16384, 10, 10, 128, 2048, 4), (1, 65536, 32, 32, 128, 4096, 4),
+            (1, 1 << 20, 16, 16, 128, 2048, 4), (16, 2048, 16, 16, 64, 512, 4),
+            (64, 2048, 8, 8, 32, 128, 200)):
+        rows = 4 * (batch * heads * seq + 4) + 4 * (batch * heads * (seq // 32 + 1) + 4)
+        blocks = batch * kv * -(-sinks // 128)
+        most = rows + (4096 + blocks) * 2 * 128 * hd * 4
+        nbytes = size(batch, seq, heads, kv, hd, window, sinks)
+        assert 0 < nbytes <= most, (seq, nbytes, most)
+        assert nbytes < batch * seq * (heads + 2 * kv) * hd * 2  # qkv's
