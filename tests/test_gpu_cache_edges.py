@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from reversability_amd.cache import append_kv, cache_plan, cached_attention
-from test_gpu_cache import _model, batch_of, check, filled, signed, slots_of, trees
+from test_gpu_cache import (_model, batch_of, check, filled, reference, signed, slots_of,
+                            trees)
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +170,47 @@ def test_decode_appends_nothing_that_was_not_computed(cuda_device, marked_memory
     assert torch.allclose(logits[6:8], want, atol=4e-3)
     for a, b in ((caches[0].keys, caches[1].keys), (caches[0].values, caches[1].values)):
         assert torch.allclose(a[:, 2:], b[:, 2:], atol=4e-3)
+
+
+@pytest.mark.parametrize("heads,kv,hd,page", [(4, 4, 32, 16), (10, 2, 64, 32), (8, 1, 128, 64)])
+@pytest.mark.parametrize("new,held", [([64], [64]), ([5, 0, 23, 64], [5, 0, 500, 1000]),
+                                      ([33, 2], [2081, 34])])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2, 0), (300, 40)])
+def test_trees_in_fp16(cuda_device, new, held, heads, kv, hd, page, window, sinks):
+    """Up to 512 rows that share a key head, at every head size."""
+    table, lengths, starts, pages = batch_of(new, held, page, cuda_device)
+    keys, values = filled(table, held, pages, kv, page, hd, torch.float16, cuda_device)
+    g = torch.Generator().manual_seed(2)
+    q = (2 * torch.randn(sum(new), heads, hd, generator=g)).half().to(cuda_device)
+    masks = trees(new)
+    out = cached_attention(q, keys, values, table, lengths, starts, 64,
+                           tree=signed(masks, cuda_device), window=window, sinks=sinks)
+    check(out, *reference(q, keys, values, table, new, held, masks, window, sinks))
+
+
+@pytest.mark.parametrize("method", ["baseline", "midpoint", "euler"])
+def test_decode_of_fused_models_in_bf16(cuda_device, method):
+    """install_v3 without its fp16 MLP: the logits are the model's own on the whole sequence, within
+    twice bf16's roundings of values of order 1 (3 layers of 8)."""
+    from reversability_amd import build_model
+    from reversability_amd.attention import enable_attention
+    from reversability_amd.cache import CacheBatch, PagedCache, decode
+    from reversability_amd.optimized import amp_context
+    from reversability_amd.optimized_v3 import install_v3
+    config = {"model": {"vocab_size": 97, "max_sequence_length": 256, "n_layers": 3, "n_heads": 4,
+                        "d_model": 128, "d_ff": 256}, "method": method}
+    torch.manual_seed(9)
+    model = build_model(config).to(cuda_device)
+    install_v3(model, core_mode="split" if method == "midpoint" else "reference", rmsnorm=True)
+    enable_attention(model, window=20, sinks=2)
+    ids = torch.randint(0, 97, (50,), device=cuda_device)
+    with torch.no_grad(), amp_context(cuda_device, "bf16"):
+        want = model(ids.unsqueeze(0))[0].float()
+    cache = PagedCache.for_model(model, pages=4, page_size=16, dtype=torch.bfloat16)
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    got = []
+    for first, last in ((0, 30), (30, 49), (49, 50)):
+        batch = CacheBatch(as_int([[2, 0, 3, 1]]), as_int([last]), as_int([0, last - first]),
+                           last - first, 64)
+        got.append(decode(model, ids[first:last], cache, batch, precision="bf16").float())
+    assert (torch.cat(got) - want).abs().max() <= 24 * torch.finfo(torch.bfloat16).eps

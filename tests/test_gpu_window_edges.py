@@ -117,3 +117,30 @@ def test_fp16_gradients_of_unlike_sizes(cuda_device, batch, seq, heads, kv, hd, 
         bad = max(bad, worst(heads_of(got[b], hd), grad, tol))
     print(f"  {bad:.3f} of the bound", flush=True)
     assert bad <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_large_scores_by_their_roundings(cuda_device, dtype):
+    """Scores of up to +-10^3, where single tokens take whole rows.  Beside the roundings of P and of the
+    output: a score is a sum in fp32 of hd products, off by d = (hd + 1) 2^-24 sum |q k| s, then of
+    2^-22 of its size (times log2 e, less the maximum); weights move with it, and the output by
+    sum P (d + its mean) |v - out| in the first order (twice for the rest)."""
+    seq, heads, hd, window, sinks = 400, 2, 64, 50, 3
+    qkv, _ = make(1, seq, heads, heads, hd, dtype, cuda_device, spread=6.0)
+    qkv[..., :2 * heads * hd] *= 4
+    out = window_attention(qkv, heads, window, sinks)[0].view(seq, heads, hd).transpose(0, 1).double()
+    q, k, v, _, p, _ = parts(qkv[0], torch.zeros_like(qkv[0, :, :heads * hd]), heads, heads, window,
+                             sinks)
+    s, u = 1 / math.sqrt(hd), torch.finfo(dtype).eps / 2
+    sub = torch.finfo(dtype).smallest_normal * u
+    score = (q @ turn(k)).abs() * s
+    off = (hd + 1) * 2.0 ** -24 * (q.abs() @ turn(k.abs())) * s + 2.0 ** -22 * score
+    off = off + (p * off).sum(-1, keepdim=True)
+    ref = p @ v
+    few = (p > 0).sum(-1, keepdim=True)
+    tol = 2 * (u * (p @ v.abs()) + u * ref.abs() + sub * (1 + few * v.abs().amax()))
+    for h in range(heads):  # [seq, seq, hd] at a time
+        tol[h] += 2 * ((p[h] * off[h]).unsqueeze(-1) * (v[h] - ref[h].unsqueeze(1)).abs()).sum(1)
+    print(f"  {worst(out, ref, tol):.3f} of the bound; tolerance at most {float(tol.max()):.4f}",
+          flush=True)
+    assert worst(out, ref, tol) <= 1.0
