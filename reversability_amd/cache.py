@@ -361,7 +361,8 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
                                  sinks=getattr(attn, "_rv_sinks", 0), out=seen)
         return attn.proj(mixed.flatten(1).unsqueeze(0))
 
-    with weight_cast_cache(), amp_context(ids.device, precision):
+    # (the fused layers launch on the current device)
+    with _DeviceGuard(ids), weight_cast_cache(), amp_context(ids.device, precision):
         if precision == "fp16":
             prefetch_casts(castable_weights(model))
         where = positions.clamp(max=limit - 1)

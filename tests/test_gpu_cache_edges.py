@@ -214,3 +214,30 @@ def test_decode_of_fused_models_in_bf16(cuda_device, method):
                            last - first, 64)
         got.append(decode(model, ids[first:last], cache, batch, precision="bf16").float())
     assert (torch.cat(got) - want).abs().max() <= 24 * torch.finfo(torch.bfloat16).eps
+
+
+def test_decode_runs_on_its_tensors_device(cuda_device, monkeypatch):
+    """Every module of the model runs while the cache's device is the current one."""
+    from reversability_amd import cache as module
+    depth, seen = [0], []
+
+    class Guard(module._DeviceGuard):
+        def __enter__(self):
+            assert self.index == cuda_device.index
+            depth[0] += 1
+            return super().__enter__()
+
+        def __exit__(self, *exc):
+            depth[0] -= 1
+            return super().__exit__(*exc)
+    monkeypatch.setattr(module, "_DeviceGuard", Guard)
+    model = _model("midpoint", cuda_device, 20, 2, True, True)
+    for name, part in model.named_modules():
+        part.register_forward_pre_hook(lambda *_, name=name: seen.append((name, depth[0])))
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    held = module.PagedCache.for_model(model, pages=2, page_size=16)
+    batch = module.CacheBatch(as_int([[0, 1]]), as_int([3]), as_int([0, 3]), 3, 32)
+    module.decode(model, torch.randint(0, 97, (3,), device=cuda_device), held, batch)
+    names = {name for name, _ in seen}
+    assert {"token_embedding", "blocks.0.attn.qkv", "blocks.2.mlp", "lm_head"} <= names
+    assert all(inside for _, inside in seen) and depth[0] == 0
