@@ -601,8 +601,8 @@ int rv_attn_bwd(const void* qkv, const void* out, const void* dout, const float*
  * stay visible: query i sees key j <= i where i - j < window or j < sinks.  qkv
  * [batch, seq, (heads + 2 kv_heads) head_dim]; out [batch, seq, heads, head_dim]; lse
  * fp32 [batch * heads, seq] (base 2); rest (nullable, like out): what out's rounding left
- * (the backward's rows of dO . O need the digits).  The weights' roundings for the product
- * with the values are made up for. */
+ * (the backward's rows of dO . O need the digits).  The weights are rounded to dtype for the
+ * product with the values; for the first 128 queries of a sequence what that left is added. */
 int rv_window_attn_fwd(const void* qkv, int64_t batch, int64_t seq, int64_t heads,
                        int64_t kv_heads, int64_t head_dim, int dtype, int64_t window,
                        int64_t sinks, void* out, void* rest, float* lse, void* stream);
@@ -613,7 +613,9 @@ int64_t rv_window_attn_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t h
                                            int64_t sinks);
 
 /* dqkv (qkv's type and layout) = gradient of out with respect to qkv, given dout and the
- * forward's out, rest (nullable) and lse.  Deterministic. */
+ * forward's out, rest (nullable) and lse.  The weights and the scores' gradients are rounded to
+ * dtype for their products, the latter in RV_F16 times a power of two that goes by dout's size (a
+ * query's, and that of 64 queries): small gradients keep their digits.  Deterministic. */
 int rv_window_attn_bwd(const void* qkv, const void* out, const void* rest, const void* dout,
                        const float* lse, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
                        int64_t head_dim, int dtype, int64_t window, int64_t sinks, void* dqkv,

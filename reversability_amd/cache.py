@@ -324,7 +324,11 @@ def decode(model, ids: torch.Tensor, cache: PagedCache, batch: CacheBatch,
     not exceed the model's ``max_sequence_length``, nor the positions of its ``Rotary``
     (positions past the former, which only a wrong max_length lets through, are taken as its
     last).  The keys and values of one call's tokens need slots of their own: sequences may
-    share pages of tokens that all of them hold, not those that new tokens go to."""
+    share pages of tokens that all of them hold, not those that new tokens go to; tokens that the
+    page table has no room for are not kept.
+
+    The modules' weights are read, their parts called one by one: forward hooks on the model, a
+    block or its ``attn`` do not run (and on the fused path those of ``mlp_norm`` do not)."""
     from .optimized_v3 import castable_weights
     if precision not in _AMP_DTYPES or _AMP_DTYPES[precision] != cache.keys.dtype:
         raise ValueError("decode needs fp16 or bf16 precision, that of its cache")

@@ -29,12 +29,20 @@
 // page that does not exist) are taken as zeros and their scores as -inf, whatever the cache holds.
 // A token that only some rows see reaches those alone, also where it is not a number (exact_rows).
 //
-// Measured: 33 sequences of 100 to 65536 tokens, a token each, 8 key heads of 128, 310 + 7 us (the stretches,
-// their joining), 5.6 TB/s of keys and values, past a large copy's rate; one sequence of 200 tokens 6 us,
-// the chain of its loads; 8 trees over 4000 tokens 23 + 7 us and four chunks of up to 512 tokens over
-// 12000, 16 heads of 128 over 2 with a window of 4096, 74 + 18 us: there the matrix cores are 4-12% busy, the stretches being short (the rest
-// is their start, softmax and partials).  Looking for values that are not finite costs 0.4 us of the
-// single sequence's 6, 1.5 of the trees' 23 and 2 of the chunks' 87.
+// Measured (the stretches + their joining, each by itself under the profiler): 33 sequences of 100 to
+// 65536 tokens, a token each, 8 key heads of 128, 306 + 6 us, 5.6 TB/s of keys and values, past a large
+// copy's rate; one sequence of 200 tokens 6 us, the chain of its loads; 8 trees over 4000 tokens 24 + 7 us
+// (29 the whole call in a row of them) and four chunks of up to 512 tokens over 12000, 16 heads of 128
+// over 2 with a window of 4096, 76 + 18 us (84 the call): there the matrix cores are 4 and 14% busy and
+// the VALU 14 and 27, the stretches being short (the rest is their start, a single tile in flight, softmax
+// and partials).  Looking for values that are not finite costs 0.4 us of the single sequence's 6, 1.5 of
+// the trees' 23 and 2 of the chunks (of 87 at that time).  At HD = 128 registers spill to scratch: 8 of
+// cached_few_k's 256 with 17 to 32 rows, 15 of cached_many_k's for a chunk and 30 for a tree (HD = 32 and
+// 64: none); exact_rows accounts for one or two of them.
+//
+// The weights are rounded to the type for the product with V, and nothing is made up for: errors against
+// 64 bits are 1.1 to 1.4 times those of the output's own rounding (fp16 2.4e-4 to 2.9e-4, 2.1e-4; bf16
+// 2.1e-3 to 2.3e-3, 1.7e-3).
 
 #include <algorithm>
 #include <climits>

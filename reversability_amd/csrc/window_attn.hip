@@ -30,14 +30,18 @@
 // Error of the gradients relative to that of the final rounding alone: without all this 1.5
 // to 2.1, with it 1.0 to 1.3, at a few percent of the time.
 //
-// Measured (us; forward, dQ, dK/dV, sums; window and sinks behind the comma), with the rate over the
-// visible pairs' 4 + 10 HD flops:
-//   33 x 512, 8 heads of 32, 128 + 4, fp16          22   25        31   4.5    71 TFLOP/s
-//   3 x 1999, 20 heads of 64 over 4, 500 + 3, bf16  41   65        67  11     285
-//   2 x 16384, 10 heads of 128, 2048 + 4, bf16     440   17 + 565  990  14    600
-// Short windows are bound by the exponentials and masks (VALU 25-35% busy with the waits between, matrix
-// cores 14-20%), long ones by the matrix cores' feeding: 35% busy in the forward, 42% in dQ, 29% in
-// dK/dV, whose 128 accumulators and 64 operands leave one wave per SIMD (two spill: 1500 us).
+// Measured (us; forward, dQ, dK/dV, sums, each by itself under the profiler, where they run up to 10%
+// longer; the whole pass in a row of them; window and sinks behind the comma), with the whole pass's
+// rate over the visible pairs' 4 + 10 HD flops:
+//   33 x 512, 8 heads of 32, 128 + 4, fp16          23   28        32    5     103   69 TFLOP/s
+//   3 x 1999, 20 heads of 64 over 4, 500 + 3, bf16  42   65        65   11     164   288
+//   2 x 16384, 10 heads of 128, 2048 + 4, bf16     453   18 + 570  998  14    1840   614
+// Short windows are bound by waits: a workgroup has four to eleven tiles, so that its start, the loads
+// of its first tiles and its end show; VALU 27-38% busy (an exponential counted as four other
+// instructions), matrix cores 4-7% at head size 32 and 14-20% at 64.  Long ones by products and
+// softmax that overlap in part: matrix cores 35% and VALU 39% busy in the forward, 42 and 32 in
+// dQ, 31 and 22 in dK/dV, whose 128 accumulators and 64 operands leave one wave per SIMD (two spill:
+// 1500 us).  The forward at head size 64 spills 11 of its 128 registers to scratch.
 
 #include <algorithm>
 #include <cmath>
@@ -376,8 +380,9 @@ __device__ __forceinline__ void q_rows(f32x16 (&dq)[HD / 32], const E* Ks, const
 
 // The first blocks of queries and the others in one launch or, where the first ones' products cost the
 // others registers, in two: at HD = 128 (559 us against 1170 in one), and at HD = 64 with more blocks than
-// the chip runs in a few rounds (16 x 2048, 16 heads 586 us forward and backward against 627, 2 x 16384,
-// 8 heads 723 against 762; 3 x 1999, 20 heads 184 against 179, 8 x 700, 8 heads 113 against 108).
+// the chip runs in a few rounds (forward and backward, ten in a row from the host: 16 x 2048, 16 heads
+// 572 us against 603, 2 x 16384, 8 heads 733 against 769; 3 x 1999, 20 heads 182 against 179, 8 x 700,
+// 8 heads 113 against 110).
 enum Part { kAll, kFirst, kOthers };
 constexpr int64_t kOneLaunch = 1024;  // blocks, at HD = 64
 
