@@ -121,7 +121,9 @@ def weight_cast_cache():
     (what autocast's own cast cache does within one autocast region).  The
     weights must not be modified inside the block; the trainers open it
     around one forward + backward, before the optimizer step.  Nested blocks
-    share the outer cache.
+    share the outer cache, and so do other threads (autograd's runs the
+    backward); a cast is handed out on the stream it was made on alone: another
+    thread's stream has not waited for it, nor has its memory for that stream.
     """
     global _weight_cache
     if _weight_cache is not None:
@@ -139,11 +141,12 @@ def cast_weight(w: torch.Tensor) -> torch.Tensor:
     cache = _weight_cache
     if cache is None:
         return cast_f16(w)
+    stream = _stream(w) if w.is_cuda else None
     hit = cache.get(id(w))
     if hit is not None and hit[0] is w:
-        return hit[1]
+        return hit[1] if hit[2] == stream else cast_f16(w)
     w16 = cast_f16(w)
-    cache[id(w)] = (w, w16)  # the strong reference keeps id(w) unique in the block
+    cache[id(w)] = (w, w16, stream)  # the strong reference keeps id(w) unique in the block
     return w16
 
 
@@ -176,7 +179,7 @@ def prefetch_casts(weights) -> None:
             offset += size
         _cast_group(group, outs)
         for w, o in zip(group, outs):
-            cache[id(w)] = (w, o)
+            cache[id(w)] = (w, o, _stream(w))
 
 
 def _f16(t: torch.Tensor, what: str) -> None:

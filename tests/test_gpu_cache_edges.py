@@ -241,3 +241,57 @@ def test_decode_runs_on_its_tensors_device(cuda_device, monkeypatch):
     names = {name for name, _ in seen}
     assert {"token_embedding", "blocks.0.attn.qkv", "blocks.2.mlp", "lm_head"} <= names
     assert all(inside for _, inside in seen) and depth[0] == 0
+
+
+def test_weight_casts_stay_on_their_stream(cuda_device):
+    """Two threads that answer at once, each on a stream of its own: a cast that one of them made is
+    not handed to the other, whose stream does not wait for it."""
+    from reversability_amd import mlp
+    w = torch.randn(64, 64, device=cuda_device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with mlp.weight_cast_cache():
+        for make in (lambda: mlp.prefetch_casts([w]), lambda: None):
+            make()
+            own = mlp.cast_weight(w)
+            assert mlp.cast_weight(w) is own
+            with torch.cuda.stream(side):
+                other = mlp.cast_weight(w)
+                assert other is not own and other.data_ptr() != own.data_ptr()
+            side.synchronize()
+            assert torch.equal(own, other) and mlp.cast_weight(w) is own
+
+
+def test_decode_on_two_threads(cuda_device):
+    """Two threads, streams and caches, one model: each thread's logits and cache are those of its
+    calls one after the other."""
+    import threading
+
+    from reversability_amd.cache import CacheBatch, PagedCache, decode
+    model = _model("midpoint", cuda_device, 20, 2, True, True)
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    ids = torch.randint(0, 97, (2, 24), device=cuda_device)
+
+    def answer(which):
+        cache = PagedCache.for_model(model, pages=2, page_size=16)
+        out = []
+        for n in range(8):
+            batch = CacheBatch(as_int([[1, 0]]), as_int([3 * n + 3]), as_int([0, 3]), 3, 32)
+            out.append(decode(model, ids[which, 3 * n:3 * n + 3], cache, batch))
+        torch.cuda.current_stream().synchronize()
+        return torch.cat(out), cache.keys, cache.values
+    want = [answer(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(which):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[which] = answer(which)
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
